@@ -37,7 +37,8 @@ HIP_FLAGS = [
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
     "-Wall", "-Wno-unused-function",
 ]
-HIP_SOURCES = ["dc_runtime.hip", "dc_streaming.hip", "dc_linq.hip", "dc_linq_jit.hip", "dc_gemm.hip", "dc_spmv.hip"]
+HIP_SOURCES = ["dc_runtime.hip", "dc_streaming.hip", "dc_linq.hip", "dc_linq_jit.hip", "dc_gemm.hip", "dc_spmv.hip",
+               "dc_norm.hip", "dc_linear.hip", "dc_adamw.hip"]
 # Headers the run-time LINQ compiler (dc_linq_jit.hip) hands to hipRTC, by the names the sources
 # include them under there.
 JIT_HEADERS = [("dotcompute_hip.h", os.path.join(ROOT, "include", "dotcompute_hip.h")),

@@ -21,10 +21,7 @@
 // the 8 consecutive k's [8h, 8h+8) of each 16-wide k step; fp32 (one k per lane per MFMA): the
 // kernels choose k orders that make each lane's LDS reads contiguous.
 //
-// Tile order: consecutive workgroups are dispatched round-robin over the 8 XCDs (each with its own
-// L2). Block b is mapped to tile (b % 8) * (T / 8) + b / 8, so each XCD works on a contiguous
-// range of tiles, and within it tiles are walked in groups of 8 tile-rows, column by column, so
-// the blocks resident on one XCD share A row-panels and B column-panels in that XCD's L2.
+// (The order of the tiles over the chip: dc_gemm_tile.hpp.)
 #include <algorithm>
 
 #include <cstddef>
@@ -33,6 +30,7 @@
 
 #include "dc_device.hpp"
 #include "dc_gemm_route.hpp"
+#include "dc_gemm_tile.hpp"
 #include "dc_internal.hpp"
 
 namespace {
@@ -43,25 +41,11 @@ typedef unsigned short u16x8 __attribute__((ext_vector_type(8)));
 typedef unsigned short u16x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
-constexpr int kGroupM = 8;
-
-struct TileCoord {
-  int tm, tn;
-};
-
-__device__ inline TileCoord map_tile(int tiles_m, int tiles_n) {
-  const int total = tiles_m * tiles_n;
-  // (dc::gemm_grid's rows; workgroups past the last tile form that one too: an early exit here costs
-  // every launch 0.1-0.2 us)
-  const int b = min((int)(blockIdx.x + (blockIdx.y << dc::kGemmGridRowBits)), total - 1);
-  const int t = (total % 8 == 0) ? (b % 8) * (total / 8) + b / 8 : b;
-  const int group = kGroupM * tiles_n;
-  const int g = t / group;
-  const int first_m = g * kGroupM;
-  const int gm = min(tiles_m - first_m, kGroupM);
-  const int in_g = t - g * group;
-  return TileCoord{first_m + in_g % gm, in_g / gm};
-}
+using dc::dma_barrier;
+using dc::lds_ptr_t;
+using dc::map_tile;
+using dc::tile_grid;
+using dc::TileCoord;
 
 // ---------------------------------------------------------------------------------------------
 // fp32, full 64×64 tiles (m, n multiples of 64, k of 32): direct-to-LDS loads, no staging registers and
@@ -89,15 +73,6 @@ struct F32DmaSmem {
   float* a[2];
   float* b[2];
 };
-
-typedef __attribute__((address_space(3))) void* lds_ptr_t;
-
-// Waits until this wave's direct-to-LDS loads have landed (vmcnt(0); expcnt and lgkmcnt left
-// alone), then the workgroup barrier: after it every wave's loads issued before are visible.
-__device__ inline void dma_barrier() {
-  __builtin_amdgcn_s_waitcnt(0x0F70);  // gfx9 encoding: vmcnt = 0, expcnt = 7, lgkmcnt = 15
-  __syncthreads();
-}
 
 template <int BUF>
 __device__ inline void f32_tile_to_lds(const F32DmaSmem& sm, __amdgpu_buffer_rsrc_t ra, const float* __restrict__ B, int N,
@@ -1200,11 +1175,6 @@ __global__ __launch_bounds__(256) void f32_to_bf16_kernel(const float* __restric
     }
     y[i] = h;
   }
-}
-
-dim3 tile_grid(int tiles_m, int tiles_n, int threads) {
-  const dc::GemmGrid g = dc::gemm_grid((int64_t)tiles_m * tiles_n, threads);
-  return dim3((unsigned)g.x, (unsigned)g.rows);
 }
 
 template <int TM, int TN, int WM, int WN, int KS, bool kDma>

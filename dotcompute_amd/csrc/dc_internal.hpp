@@ -159,6 +159,8 @@ int32_t ensure_spmv_plan_mem(dc_hip_ctx* ctx, size_t bytes);
 int32_t launch_reduce_sum_f32(dc_hip_ctx* ctx, const float* input, int64_t n, double* sum_out);
 // *sum_out = partials[0] + ... + partials[count-1] (float64, fixed order; one workgroup).
 int32_t launch_reduce_partials_f64(dc_hip_ctx* ctx, const double* partials, int count, double* sum_out);
+// out[c] = parts[0][c] + ... + parts[count - 1][c] for float32 rows of `cols`, in a fixed order.
+int32_t launch_column_sums(dc_hip_ctx* ctx, const float* parts, float* out, int64_t count, int64_t cols);
 // Fills device memory with zero bytes using a kernel (capture-safe).
 int32_t zero_async(dc_hip_ctx* ctx, void* dst, size_t bytes);
 inline int32_t last_launch_status() { return (int32_t)hipGetLastError(); }

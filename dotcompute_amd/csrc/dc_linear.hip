@@ -1,0 +1,811 @@
+// dc_linear.hip — matrix products with bias, activation and residual in their epilogue, and their gradients.
+//
+// Forward: z = x w^T (x_scales w_scales) + bias, y = act(z) + residual, with x [m][k] and w [n][k] in bf16 or e4m3 and
+// sums in fp32. Backward: dz = dy act'(pre); dx = dz w, dw = dz^T x, dbias = column sums of dz.
+//
+// Kernels:
+//   - product_kernel: D[i][j] = sum_c A(i, c) B(j, c) in tiles on the matrix cores. A's rows run along c. B's do too
+//     (forward), or are the rows c of a row-major [c][j] matrix (the gradients).
+//   - few_rows_kernel: forward with few rows of x. Bound by reading w, which goes from memory to the matrix
+//     cores' operands without a stop in LDS.
+//   - slope_kernel: dz and its transpose in bf16 (what the two gradients' products run along), and dbias's parts.
+//   - pack_kernel: rows that the direct-to-LDS loads cannot take (not 16-byte aligned, or no whole number of
+//     16 bytes) copied to ones padded with zeros.
+#include <algorithm>
+
+#include <cstddef>
+#include <type_traits>
+
+#include "dc_gemm_tile.hpp"
+#include "dc_internal.hpp"
+#include "dc_linear_route.hpp"
+#include "dc_numeric.hpp"
+
+namespace {
+
+using dc::bf16;
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4* lds_s16x4_ptr;
+
+// ---- activations -----------------------------------------------------------------------------------
+// exp and the reciprocal are the hardware's (about an ulp): the results are rounded to bf16, or are float32
+// values whose sums carry more error than that.
+__device__ inline float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.0f + __expf(-v)); }
+constexpr float kTanhArg = 2.0f * 0.7978845608f;  // 2 sqrt(2 / pi)
+constexpr float kTanhCube = 0.044715f;
+
+__device__ inline float act_value(int act, float z) {
+  switch (act) {
+    case DC_ACT_RELU: return z < 0.0f ? 0.0f : z;
+    case DC_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678f));
+    case DC_ACT_GELU_TANH: return z * sigmoid(kTanhArg * (z + kTanhCube * z * z * z));
+    case DC_ACT_SILU: return z * sigmoid(z);
+    default: return z;
+  }
+}
+
+__device__ inline float act_slope(int act, float z) {
+  switch (act) {
+    case DC_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
+    case DC_ACT_GELU:
+      return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * (__expf(-0.5f * z * z) * 0.3989422804f);
+    case DC_ACT_GELU_TANH: {
+      const float zz = fminf(z * z, 1e4f);  // (past |z| = 100 the slope is 0 or 1, and z^2 may not be finite)
+      const float s = sigmoid(kTanhArg * z * (1.0f + kTanhCube * zz));
+      return s + z * s * (1.0f - s) * (kTanhArg * (1.0f + 3.0f * kTanhCube * zz));
+    }
+    case DC_ACT_SILU: {
+      const float s = sigmoid(z);
+      return s * (1.0f + z * (1.0f - s));
+    }
+    default: return 1.0f;
+  }
+}
+
+// ---- epilogue --------------------------------------------------------------------------------------
+struct Epilogue {
+  const float *a_scales, *b_scales;  // both or neither
+  const bf16 *bias, *residual;
+  bf16* pre;
+  void* y;
+  int64_t residual_stride, pre_stride, y_stride;
+  int32_t act;
+  int32_t y_f32;
+};
+
+// The E neighbouring results (i, j..) from their sums; `left`: how many columns there are from j on (at least one).
+template <int E>
+__device__ inline void finish(const Epilogue& p, int64_t i, int64_t j, int64_t left, float (&z)[E]) {
+  auto load = [&](const bf16* q, float (&v)[E]) __attribute__((always_inline)) {
+    if constexpr (E == 8) {
+      dc::load_some(q, left, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = e < left ? dc::to_f32(q[e]) : 0.0f;
+    }
+  };
+  auto store = [&](bf16* q, const float (&v)[E]) __attribute__((always_inline)) {
+    if constexpr (E == 8) {
+      dc::store_some(q, left, v);
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (e < left) q[e] = dc::from_f32<bf16>(v[e]);
+    }
+  };
+  if (p.a_scales) {
+    const float s = p.a_scales[i];
+    float b[E];
+#pragma unroll
+    for (int e = 0; e < E; e += 4) {
+      float (&q)[4] = *reinterpret_cast<float (*)[4]>(b + e);
+      dc::load_some(p.b_scales + j + e, left - e, q);
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) z[e] = z[e] * s * b[e];
+  }
+  float u[E];
+  if (p.bias) {
+    load(p.bias + j, u);
+#pragma unroll
+    for (int e = 0; e < E; ++e) z[e] += u[e];
+  }
+  if (p.pre) store(p.pre + i * p.pre_stride + j, z);
+  if (p.act != DC_ACT_NONE) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) z[e] = act_value(p.act, z[e]);
+  }
+  if (p.residual) {
+    load(p.residual + i * p.residual_stride + j, u);
+#pragma unroll
+    for (int e = 0; e < E; ++e) z[e] += u[e];
+  }
+  if (p.y_f32) {
+    float* q = static_cast<float*>(p.y) + i * p.y_stride + j;
+#pragma unroll
+    for (int e = 0; e < E; e += 4) dc::store_some(q + e, left - e, *reinterpret_cast<const float (*)[4]>(z + e));
+  } else {
+    store(static_cast<bf16*>(p.y) + i * p.y_stride + j, z);
+  }
+}
+
+// ---- tiles -----------------------------------------------------------------------------------------
+// Macro tile TM×TN, 128 bytes of c at a time (64 bf16 or 128 e4m3), double-buffered LDS, WM×WN waves of
+// 32·kMT × 32·kNT results on v_mfma_f32_32x32x16_bf16 / v_mfma_f32_32x32x64_f8f6f4; KS > 1: KS such groups of waves take the
+// tiles along c in turn, and their sums are added in group order at the end.
+//
+// LDS image of an operand whose rows run along c: T rows of 128 bytes; the 16-byte piece q of row R sits at
+// q ^ ((R >> 1) & 7), so a fragment read (rows R0..R0+15 at one piece for each 16 lanes) touches 16 distinct 16-byte
+// bank groups. Of an operand with rows c: 64 rows of 2·T bytes, the 64-byte block b of row c at b ^ (c & 3) (T = 64:
+// b ^ ((c >> 1) & 1)), read through ds_read_b64_tr_b16, which hands a lane four c of one column. The swizzles are
+// applied where the direct-to-LDS loads fetch: lane L of a load fills LDS bytes 16·L of a 1 KiB block.
+//
+// The instructions get B's fragment first and A's second, so a lane ends up with four neighbouring j of one i: the
+// sums go through LDS once more, a wave at a time in its own part, and the epilogue reads and writes rows of 8 results
+// a lane, 64 or 128 bytes a row, whatever the activation, in one short loop.
+constexpr int kTileBytes = 128;  // of c
+constexpr int kRange = dc::kLinearRange;
+constexpr uint32_t kPast = 0x80000000u;  // a byte offset past every range: loads zeros
+
+struct Operands {
+  const unsigned char *a, *b;
+  int64_t a_pitch, b_pitch;  // bytes from row to row
+  int32_t m, n;              // results
+  int32_t c_bytes;           // A's row length; B's too, or c_rows of them
+  int32_t c_rows;
+  int32_t b_cols;            // B's columns with their padding, a multiple of 8 (rows c only)
+};
+
+template <int TM, int TN>
+struct TileSmem {
+  unsigned char a[2][TM * kTileBytes];
+  unsigned char b[2][TN * kTileBytes];
+};
+
+template <bool kFp8>
+struct Frag;
+template <>
+struct Frag<false> {
+  bf16x8 v;
+};
+template <>
+struct Frag<true> {
+  i32x8 v;
+};
+
+// 16 bytes a lane to 1 KiB of LDS, from `voff` (the lane's, kPast for zeros) + `soff` bytes past `base`.
+__device__ inline void load_block(const unsigned char* base, unsigned char* to, uint32_t voff, int soff) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(dc::range_rsrc(base, kRange), (dc::lds_ptr_t)to, 16, voff, soff, 0, 0);
+}
+
+template <int TM, int TN, int WM, int WN, int KS, bool kFp8, bool kRowsC>
+__global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void product_kernel(Operands o, Epilogue ep,
+                                                                                           int tiles_m, int tiles_n) {
+  static_assert(!(kFp8 && kRowsC), "8-bit operands run along c");
+  constexpr int kWaves = WM * WN;
+  constexpr int kMT = TM / WM / 32, kNT = TN / WN / 32;
+  constexpr int kABlocks = TM / 8 / kWaves, kBBlocks = TN / 8 / kWaves;  // 1 KiB blocks of a wave and tile
+  constexpr int kSteps = kFp8 ? 2 : 4;                                   // instructions along c of a tile
+  using Smem = TileSmem<TM, TN>;
+  __shared__ __align__(16) Smem sms[KS];
+  const dc::TileCoord tc = dc::map_tile(tiles_m, tiles_n);
+  const int m0 = tc.tm * TM, n0 = tc.tn * TN;
+  const int tid = threadIdx.x, lane = tid & 63, gwave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int group = gwave / kWaves, wave = gwave % kWaves;
+  Smem& sm = sms[group];
+  const int wm = wave / WN, wn = wave % WN;
+  const int r = lane & 31, h = lane >> 5;
+  const int tiles_c = (o.c_bytes + kTileBytes - 1) / kTileBytes;
+  const int kt_count = (tiles_c + KS - 1) / KS;  // of a group
+
+  // ---- load side. Rows along c: lane -> row lane / 8 of a block, slot lane % 8, which holds the piece of the swizzle.
+  const int lrow = lane >> 3;
+  const int piece = 16 * ((lane & 7) ^ ((4 * wave + (lrow >> 1)) & 7));  // byte offset in the row's 128
+  // Rows c: lane -> row of the block and 16-byte chunk of it.
+  constexpr int kRowChunks = TN / 8, kRows = 64 / kRowChunks;
+  auto bswz = [](int c) __attribute__((always_inline)) { return TN == 64 ? (c >> 1) & 1 : c & 3; };
+  const int brow = lane / kRowChunks, bc = lane % kRowChunks;
+  const int bchunk = 4 * ((bc >> 2) ^ bswz(kRows * wave + brow)) + (bc & 3);
+  uint32_t avoff[kABlocks], bvoff[kRowsC ? 1 : kBBlocks];
+#pragma unroll
+  for (int i = 0; i < kABlocks; ++i)
+    avoff[i] = (uint32_t)min(8 * (i * kWaves + wave) + lrow, o.m - 1 - m0) * (uint32_t)o.a_pitch + (uint32_t)piece;
+  if constexpr (kRowsC) {
+    bvoff[0] = (uint32_t)brow * (uint32_t)o.b_pitch + (uint32_t)(2 * min(8 * bchunk, o.b_cols - 8 - n0));
+  } else {
+#pragma unroll
+    for (int i = 0; i < kBBlocks; ++i)
+      bvoff[i] = (uint32_t)min(8 * (i * kWaves + wave) + lrow, o.n - 1 - n0) * (uint32_t)o.b_pitch + (uint32_t)piece;
+  }
+  const unsigned char* abase = o.a + (int64_t)m0 * o.a_pitch;
+  const unsigned char* bbase = kRowsC ? o.b + (int64_t)n0 * 2 : o.b + (int64_t)n0 * o.b_pitch;
+  auto load_tile = [&](auto BUF, int KT) __attribute__((always_inline)) {
+    constexpr int kBuf = decltype(BUF)::value;
+    const int t = KT * KS + group;
+    const int at = t * kTileBytes;  // bytes into A's rows (past the last: every load is past the range)
+    const int left = o.c_bytes - at;
+#pragma unroll
+    for (int i = 0; i < kABlocks; ++i)
+      load_block(abase + at, sm.a[kBuf] + (i * kWaves + wave) * 1024, piece < left ? avoff[i] : kPast, 0);
+    if constexpr (kRowsC) {
+      const int c0 = t * (kTileBytes / 2);
+#pragma unroll
+      for (int i = 0; i < kBBlocks; ++i) {
+        const int row = kRows * (i * kWaves + wave);
+        load_block(bbase + (int64_t)c0 * o.b_pitch, sm.b[kBuf] + (i * kWaves + wave) * 1024,
+                   c0 + row + brow < o.c_rows ? bvoff[0] : kPast, row * (int)o.b_pitch);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < kBBlocks; ++i)
+        load_block(bbase + at, sm.b[kBuf] + (i * kWaves + wave) * 1024, piece < left ? bvoff[i] : kPast, 0);
+    }
+  };
+
+  // ---- read side: byte offsets in buffer 0 of a step's pieces, for rows 32·t + r (so the swizzle is (r >> 1) & 7).
+  // bf16: piece 2·step + h; e4m3: pieces 4·step + 2h and + 1 (any split of c over the lanes' halves will do, as both
+  // operands use the same).
+  const int rswz = (r >> 1) & 7;
+  uint32_t poff[8 / 2];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    poff[i] = 16u * (uint32_t)((kFp8 ? 4 * (i >> 1) + 2 * h + (i & 1) : 2 * i + h) ^ rswz);
+  const uint32_t arow = (uint32_t)((wm * 32 * kMT + r) * kTileBytes);
+  const uint32_t brow_l = (uint32_t)offsetof(Smem, b) + (uint32_t)((wn * 32 * kNT + r) * kTileBytes);
+  uint32_t boff[kNT];
+  if constexpr (kRowsC) {
+    const int j = (lane & 15) >> 2, p4 = lane & 3, cg = (lane >> 4) & 1;
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt)
+      boff[nt] = (uint32_t)offsetof(Smem, b) + (uint32_t)((8 * h + j) * 2 * TN) +
+                 64u * (uint32_t)((kNT * wn + nt) ^ bswz(j)) + (uint32_t)(32 * cg + 8 * p4);
+  }
+  const unsigned char* lds = reinterpret_cast<const unsigned char*>(&sm);
+
+  f32x16 acc[kMT][kNT];
+#pragma unroll
+  for (int i = 0; i < kMT; ++i)
+#pragma unroll
+    for (int j = 0; j < kNT; ++j)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.0f;
+
+  typedef Frag<kFp8> F;
+  auto read_row = [&](uint32_t at, int step) __attribute__((always_inline)) {
+    F f;
+    if constexpr (kFp8) {
+      const dc::u32x4 lo = *reinterpret_cast<const dc::u32x4*>(lds + at + poff[2 * step]);
+      const dc::u32x4 hi = *reinterpret_cast<const dc::u32x4*>(lds + at + poff[2 * step + 1]);
+      f.v = __builtin_bit_cast(i32x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    } else {
+      f.v = __builtin_bit_cast(bf16x8, *reinterpret_cast<const dc::u32x4*>(lds + at + poff[step]));
+    }
+    return f;
+  };
+  auto read_a = [&](auto BUF, int step, F* a) __attribute__((always_inline)) {
+    constexpr uint32_t kBufA = (uint32_t)decltype(BUF)::value * TM * kTileBytes;
+#pragma unroll
+    for (int mt = 0; mt < kMT; ++mt) a[mt] = read_row(arow + kBufA + mt * 32 * kTileBytes, step);
+  };
+  auto read_b = [&](auto BUF, int step, F* b) __attribute__((always_inline)) {
+    constexpr uint32_t kBufB = (uint32_t)decltype(BUF)::value * TN * kTileBytes;
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt) b[nt] = read_row(brow_l + kBufB + nt * 32 * kTileBytes, step);
+  };
+  // Rows c: the fragments of a whole tile in one burst. The compiler cannot tell these reads apart from the LDS that the
+  // direct-to-LDS loads write, and waits for every load in flight before each of them: they go out while none is.
+  auto read_b_tile = [&](auto BUF, F (*b)[kNT]) __attribute__((always_inline)) {
+    if constexpr (kRowsC) {
+      constexpr uint32_t kBufB = (uint32_t)decltype(BUF)::value * TN * kTileBytes;
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st)
+#pragma unroll
+        for (int nt = 0; nt < kNT; ++nt) {
+          const unsigned char* q = lds + boff[nt] + kBufB + st * 16 * 2 * TN;
+          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(q));
+          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4_ptr)(q + 4 * 2 * TN));
+          b[st][nt].v = __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+        }
+    }
+  };
+  auto mfmas = [&](const F* a, const F* b) __attribute__((always_inline)) {
+#pragma unroll
+    for (int mt = 0; mt < kMT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt) {
+        if constexpr (kFp8)
+          acc[mt][nt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[nt].v, a[mt].v, acc[mt][nt], 0, 0, 0, 0x7f7f7f7f, 0,
+                                                                       0x7f7f7f7f);
+        else
+          acc[mt][nt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[nt].v, a[mt].v, acc[mt][nt], 0, 0, 0);
+      }
+  };
+  // LDS reads between the products: as many as there are of each.
+  constexpr int kReads = (kMT + (kRowsC ? 0 : kNT)) * (kFp8 ? 2 : 1), kProducts = kMT * kNT;
+  auto interleave = []() __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < kProducts; ++i) {
+      constexpr int kPer = (kReads + kProducts - 1) / kProducts;
+      __builtin_amdgcn_sched_group_barrier(0x100, kPer, 0);
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    }
+  };
+
+  // Tile kt in buffer kt & 1: its steps run their products with the next step's reads between them; before the last
+  // step comes the tile's one barrier, which also waits for tile kt+1's loads, issued a tile earlier; then tile
+  // kt+2's loads go out into the buffer that tile kt is done with.
+  F fa[2][kMT], fb[2][kRowsC ? kSteps : 1][kNT];
+  constexpr std::integral_constant<int, 0> kBuf0{};
+  constexpr std::integral_constant<int, 1> kBuf1{};
+  load_tile(kBuf0, 0);
+  dc::dma_barrier();
+  if constexpr (kRowsC) read_b_tile(kBuf0, fb[0]);
+  else read_b(kBuf0, 0, fb[0][0]);
+  read_a(kBuf0, 0, fa[0]);
+  if (kt_count > 1) load_tile(kBuf1, 1);
+  // (a macro, so that the fragment arrays stay plain registers)
+#define DC_TILE(BUF, KT)                                                                            \
+  {                                                                                                 \
+    _Pragma("unroll") for (int step = 0; step + 1 < kSteps; ++step) {                               \
+      const int cur = step & 1;                                                                     \
+      __builtin_amdgcn_sched_barrier(0);                                                            \
+      read_a(kBuf##BUF, step + 1, fa[cur ^ 1]);                                                     \
+      if constexpr (!kRowsC) read_b(kBuf##BUF, step + 1, fb[cur ^ 1][0]);                           \
+      mfmas(fa[cur], kRowsC ? fb[BUF][kRowsC ? step : 0] : fb[cur][0]);                             \
+      interleave();                                                                                 \
+      __builtin_amdgcn_sched_barrier(0);                                                            \
+    }                                                                                               \
+    dc::dma_barrier();                                                                              \
+    if constexpr (kRowsC) read_b_tile(kBuf##BUF##Other, fb[1 - (BUF)]);                             \
+    if ((KT) + 2 < kt_count) load_tile(kBuf##BUF, (KT) + 2);                                        \
+    __builtin_amdgcn_sched_barrier(0);                                                              \
+    read_a(kBuf##BUF##Other, 0, fa[0]);                                                             \
+    if constexpr (!kRowsC) read_b(kBuf##BUF##Other, 0, fb[0][0]);                                   \
+    mfmas(fa[1], kRowsC ? fb[BUF][kRowsC ? kSteps - 1 : 0] : fb[1][0]);                             \
+    interleave();                                                                                   \
+    __builtin_amdgcn_sched_barrier(0);                                                              \
+  }
+  constexpr auto kBuf0Other = kBuf1;
+  constexpr auto kBuf1Other = kBuf0;
+  __builtin_assume(kt_count > 0);
+  int kt = 0;
+  do {
+    DC_TILE(0, kt);
+    if (kt + 1 < kt_count) DC_TILE(1, kt + 1);
+    kt += 2;
+  } while (kt < kt_count);
+#undef DC_TILE
+
+  // (after the last tile: reads of the other buffer that nobody uses; every wave is past them beyond this barrier)
+  __syncthreads();
+  if constexpr (KS > 1) {  // the groups' sums, added in group order by group 0
+    static_assert(sizeof(Smem) >= kWaves * 64 * kMT * kNT * 16 * sizeof(float), "a group's sums fit in its buffers");
+    float* part = reinterpret_cast<float*>(&sm) + tid % (64 * kWaves);
+    if (group > 0)
+#pragma unroll
+      for (int i = 0; i < kMT * kNT * 16; ++i) part[i * 64 * kWaves] = acc[i / 16 / kNT][i / 16 % kNT][i % 16];
+    __syncthreads();
+    if (group > 0) return;
+#pragma unroll
+    for (int g = 1; g < KS; ++g) {
+      const float* other = reinterpret_cast<const float*>(&sms[g]) + tid;
+#pragma unroll
+      for (int i = 0; i < kMT * kNT * 16; ++i) acc[i / 16 / kNT][i / 16 % kNT][i % 16] += other[i * 64 * kWaves];
+    }
+  }
+
+  // acc[mt][nt][v]: i = r, j = 8·(v / 4) + 4·h + v % 4 of the 32×32 block. A wave's 32 rows of 32·kNT sums at a time.
+  constexpr int kCols = 32 * kNT, kPitch = kCols + 4, kLanes = kCols / 8;
+  static_assert(sizeof(Smem) >= kWaves * 32 * kPitch * sizeof(float), "the waves' blocks fit in the buffers");
+  float* own = reinterpret_cast<float*>(&sms[0]) + wave * 32 * kPitch;
+  const int64_t j = n0 + wn * kCols + 8 * (lane % kLanes), left = o.n - j;
+#pragma unroll
+  for (int mt = 0; mt < kMT; ++mt) {
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const f32x4 v = {acc[mt][nt][4 * q], acc[mt][nt][4 * q + 1], acc[mt][nt][4 * q + 2], acc[mt][nt][4 * q + 3]};
+        *reinterpret_cast<f32x4*>(own + r * kPitch + 32 * nt + 8 * q + 4 * h) = v;
+      }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+#pragma unroll 1
+    for (int r0 = 0; r0 < 32; r0 += 64 / kLanes) {
+      const int row = r0 + lane / kLanes;
+      const int64_t i = m0 + (wm * kMT + mt) * 32 + row;
+      float z[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) z[e] = own[row * kPitch + 8 * (lane % kLanes) + e];
+      if (i < o.m && left > 0) finish(ep, i, j, left, z);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  }
+}
+
+// ---- few rows ----------------------------------------------------------------------------------------
+// 16·NB outputs (rows of w) and 16·MT rows of x per workgroup, whose W waves take the 128-byte steps along c in turn:
+// lane l of a wave holds pieces l / 16 and 4 + l / 16 of row l % 16, of w (the instruction's first operand) and of x
+// (its second), straight from memory at any alignment. A wave's sums go to LDS, and each lane adds the waves' in
+// order for four neighbouring outputs of one row of x.
+__device__ inline dc::u32x4 load_piece(const unsigned char* row, int64_t at, int64_t bytes) {
+  dc::u32x4 w = {0, 0, 0, 0};
+  if (at + 16 <= bytes) {
+    w = *reinterpret_cast<const dc::u32x4_at1*>(row + at);
+  } else if (at < bytes) {
+    unsigned char* p = reinterpret_cast<unsigned char*>(&w);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      if (at + i < bytes) p[i] = row[at + i];
+  }
+  return w;
+}
+
+template <bool kFp8, int MT, int NB, int W, int U>
+__global__ __launch_bounds__(64 * W) void few_rows_kernel(Operands o, Epilogue ep) {
+  __shared__ f32x4 sums[W][NB * MT][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int r = lane & 15, g = lane >> 4;
+  const int64_t n0 = (int64_t)blockIdx.x * 16 * NB;
+  const unsigned char* wrow[NB];
+#pragma unroll
+  for (int i = 0; i < NB; ++i) wrow[i] = o.b + std::min<int64_t>(n0 + 16 * i + r, o.n - 1) * o.b_pitch;
+  const int64_t bytes = o.c_bytes;
+  const int64_t steps = (bytes + kTileBytes - 1) / kTileBytes;
+  for (int64_t m0 = (int64_t)blockIdx.y * 16 * MT; m0 < o.m; m0 += (int64_t)gridDim.y * 16 * MT) {
+    const unsigned char* xrow[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) xrow[i] = o.a + std::min<int64_t>(m0 + 16 * i + r, o.m - 1) * o.a_pitch;
+    f32x4 acc[NB][MT];
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int64_t s0 = wave; s0 < steps; s0 += W * U) {
+      dc::u32x4 wv[U][NB][2], xv[U][MT][2];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int64_t at = (s0 + u * W) * kTileBytes + 16 * g;
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+#pragma unroll
+          for (int i = 0; i < NB; ++i) wv[u][i][p] = load_piece(wrow[i], at + 64 * p, bytes);
+#pragma unroll
+          for (int i = 0; i < MT; ++i) xv[u][i][p] = load_piece(xrow[i], at + 64 * p, bytes);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+#pragma unroll
+        for (int i = 0; i < NB; ++i)
+#pragma unroll
+          for (int j = 0; j < MT; ++j) {
+            if constexpr (kFp8) {
+              const i32x8 a = __builtin_bit_cast(i32x8, __builtin_shufflevector(wv[u][i][0], wv[u][i][1], 0, 1, 2, 3, 4, 5, 6, 7));
+              const i32x8 b = __builtin_bit_cast(i32x8, __builtin_shufflevector(xv[u][j][0], xv[u][j][1], 0, 1, 2, 3, 4, 5, 6, 7));
+              acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[i][j], 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+            } else {
+#pragma unroll
+              for (int p = 0; p < 2; ++p)
+                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wv[u][i][p]),
+                                                                   __builtin_bit_cast(bf16x8, xv[u][j][p]), acc[i][j], 0, 0, 0);
+            }
+          }
+    }
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) sums[wave][i * MT + j][lane] = acc[i][j];
+    __syncthreads();
+    // acc[i][j][v]: output 16·i + 4·g + v of row 16·j + r of x
+    for (int t = threadIdx.x; t < NB * MT * 64; t += 64 * W) {
+      const int b = t >> 6, l = t & 63;
+      f32x4 v = sums[0][b][l];
+#pragma unroll
+      for (int w = 1; w < W; ++w) v += sums[w][b][l];
+      const int64_t i = m0 + 16 * (b % MT) + (l & 15), j = n0 + 16 * (b / MT) + 4 * (l >> 4);
+      float z[4] = {v.x, v.y, v.z, v.w};
+      if (i < o.m && j < o.n) finish(ep, i, j, o.n - j, z);
+    }
+    __syncthreads();
+  }
+}
+
+// ---- what the gradients' products run along ---------------------------------------------------------------
+// dz = dy act'(pre) over 64×64 pieces: dz itself (pitch dz_pitch, columns from n to there zero), its transpose (pitch
+// t_pitch, columns from m to there zero) through LDS, and the piece's column sums, unrounded. A thread holds two
+// neighbouring rows of 8 columns, so the transpose's LDS words are pairs of rows.
+struct SlopeArgs {
+  const bf16 *dy, *pre;
+  bf16 *dz, *dzt;  // either may be NULL
+  float* parts;    // [pieces of rows][n], or NULL
+  int64_t m, n, dy_stride, pre_stride, dz_pitch, t_pitch;
+  int32_t act;
+};
+__global__ __launch_bounds__(256) void slope_kernel(SlopeArgs a) {
+  __shared__ uint32_t turned[64][33];
+  __shared__ float sums[32][65];
+  const int t = threadIdx.x, c8 = t & 7, pair = t >> 3;
+  const int64_t across = (a.n + 63) / 64, total = across * ((a.m + 63) / 64);
+  for (int64_t at = blockIdx.x; at < total; at += gridDim.x) {
+  const int64_t m0 = at / across * 64, n0 = at % across * 64;
+  const int64_t j = n0 + 8 * c8;
+  float dz[2][8];
+#pragma unroll
+  for (int q = 0; q < 2; ++q) {
+    const int64_t i = m0 + 2 * pair + q;
+    if (i < a.m && j < a.n) {
+      dc::load_some(a.dy + i * a.dy_stride + j, a.n - j, dz[q]);
+      if (a.act != DC_ACT_NONE) {
+        float z[8];
+        dc::load_some(a.pre + i * a.pre_stride + j, a.n - j, z);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dz[q][e] *= j + e < a.n ? act_slope(a.act, z[e]) : 0.0f;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) dz[q][e] = 0.0f;
+    }
+    if (a.dz && i < a.m && j < a.dz_pitch) dc::store_chunk(a.dz + i * a.dz_pitch + j, dz[q]);
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    turned[8 * c8 + e][pair] = dc::pack_bf16(dz[0][e], dz[1][e]);
+    sums[pair][8 * c8 + e] = dz[0][e] + dz[1][e];
+  }
+  __syncthreads();
+  if (a.dzt) {
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {  // 64 rows of 8 16-byte chunks
+      const int row = (t >> 3) + 32 * q, chunk = t & 7;
+      const int64_t c = m0 + 8 * chunk;
+      if (n0 + row < a.n && c < a.t_pitch) {
+        const dc::u32x4 w = {turned[row][4 * chunk], turned[row][4 * chunk + 1], turned[row][4 * chunk + 2],
+                             turned[row][4 * chunk + 3]};
+        *reinterpret_cast<dc::u32x4*>(a.dzt + (n0 + row) * a.t_pitch + c) = w;
+      }
+    }
+  }
+  if (a.parts && t < 64 && n0 + t < a.n) {
+    float s = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) s += sums[i][t];
+    a.parts[m0 / 64 * a.n + n0 + t] = s;
+  }
+  __syncthreads();
+  }
+}
+
+// Rows of `bytes` bytes at any alignment to rows of `to_pitch` (a multiple of 16), padded with zeros.
+struct PackArgs {
+  const unsigned char* from;
+  unsigned char* to;
+  int64_t rows, bytes, from_pitch, to_pitch;
+};
+__global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
+  const int64_t pieces = a.to_pitch / 16, total = a.rows * pieces, step = (int64_t)gridDim.x * 256;
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += step) {
+    const int64_t row = t / pieces, at = 16 * (t - row * pieces);
+    *reinterpret_cast<dc::u32x4*>(a.to + row * a.to_pitch + at) = load_piece(a.from + row * a.from_pitch, at, a.bytes);
+  }
+}
+
+// ---- host ------------------------------------------------------------------------------------------------
+template <int TM, int TN, int WM, int WN, int KS, bool kFp8, bool kRowsC>
+int32_t launch_product(dc_hip_ctx* ctx, const Operands& o, const Epilogue& ep) {
+  constexpr int kThr = 64 * WM * WN * KS;
+  const int tiles_m = (o.m + TM - 1) / TM, tiles_n = (o.n + TN - 1) / TN;
+  product_kernel<TM, TN, WM, WN, KS, kFp8, kRowsC>
+      <<<dc::tile_grid(tiles_m, tiles_n, kThr), kThr, 0, ctx->stream>>>(o, ep, tiles_m, tiles_n);
+  return dc::last_launch_status();
+}
+
+template <bool kFp8, bool kRowsC>
+int32_t product(dc_hip_ctx* ctx, const Operands& o, const Epilogue& ep) {
+  using dc::LinearTile;
+  switch (dc::linear_tile(o.m, o.n, o.c_bytes, o.a_pitch, o.b_pitch, kRowsC, std::max(1, ctx->cu_count))) {
+    case LinearTile::k256: return launch_product<256, 256, 2, 4, 1, kFp8, kRowsC>(ctx, o, ep);
+    case LinearTile::k128: return launch_product<128, 128, 2, 2, 1, kFp8, kRowsC>(ctx, o, ep);
+    case LinearTile::k128x2: return launch_product<128, 128, 2, 2, 2, kFp8, kRowsC>(ctx, o, ep);
+    case LinearTile::k64: return launch_product<64, 64, 2, 2, 1, kFp8, kRowsC>(ctx, o, ep);
+    case LinearTile::k64x2: return launch_product<64, 64, 2, 2, 2, kFp8, kRowsC>(ctx, o, ep);
+    case LinearTile::k64x4: return launch_product<64, 64, 2, 2, 4, kFp8, kRowsC>(ctx, o, ep);
+  }
+  return DC_ERR_INVALID_ARGUMENT;
+}
+
+template <bool kFp8, int MT>
+int32_t launch_few_rows(dc_hip_ctx* ctx, const Operands& o, const Epilogue& ep) {
+  const unsigned gy = (unsigned)std::min((o.m + 16 * MT - 1) / (16 * MT), 32768);
+  few_rows_kernel<kFp8, MT, 1, 8, 4><<<dim3((unsigned)((o.n + 15) / 16), gy), 512, 0, ctx->stream>>>(o, ep);
+  return dc::last_launch_status();
+}
+
+template <bool kFp8>
+int32_t few_rows(dc_hip_ctx* ctx, const Operands& o, const Epilogue& ep) {
+  return o.m <= 16 ? launch_few_rows<kFp8, 1>(ctx, o, ep) : launch_few_rows<kFp8, 2>(ctx, o, ep);
+}
+
+bool aligned_to(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+int64_t padded(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// Scratch of one call: pieces of ctx->partials, each at a multiple of 256 bytes.
+struct Scratch {
+  size_t bytes = 0;
+  size_t take(int64_t n) {
+    const size_t at = bytes;
+    bytes += (size_t)padded(n, 256);
+    return at;
+  }
+};
+
+// An operand as the direct-to-LDS loads take it: 16-byte aligned rows of whole 16-byte pieces, with a pitch that keeps
+// a tile's rows in range; else a copy that is.
+struct Rows {
+  const unsigned char* p;
+  int64_t pitch, rows, bytes;
+  bool copied = false;
+  size_t at = 0;
+  void plan(Scratch& s) {
+    copied = !aligned_to(p, 16) || pitch % 16 != 0 || bytes % 16 != 0 || pitch > dc::kLinearPitch;
+    if (copied) at = s.take(rows * padded(bytes, 16));
+  }
+  int32_t lay_out(dc_hip_ctx* ctx) {
+    if (!copied) return DC_OK;
+    unsigned char* to = static_cast<unsigned char*>(ctx->partials) + at;
+    const PackArgs a{p, to, rows, bytes, pitch, padded(bytes, 16)};
+    const int64_t groups = (rows * (a.to_pitch / 16) + 255) / 256;
+    pack_kernel<<<(unsigned)std::min<int64_t>(groups, 65536), 256, 0, ctx->stream>>>(a);
+    p = to;
+    pitch = a.to_pitch;
+    return dc::last_launch_status();
+  }
+};
+
+int32_t check_rows(const void* p, int64_t size, int64_t stride, int64_t rows, int64_t cols) {
+  if (!p) return DC_ERR_INVALID_ARGUMENT;
+  if (!aligned_to(p, (uintptr_t)size)) return DC_ERR_MISALIGNED;
+  return rows > 1 && stride < cols ? DC_ERR_DIMENSION : DC_OK;
+}
+
+int32_t check_dims(int64_t m, int64_t n, int64_t k, int32_t act) {
+  if (m < 0 || n < 0 || k < 0 || act < DC_ACT_NONE || act > DC_ACT_SILU) return DC_ERR_INVALID_ARGUMENT;
+  if (m > INT32_MAX / 2) return DC_ERR_INVALID_ARGUMENT;
+  return n > dc::kLinearWidth || k > dc::kLinearWidth ? DC_ERR_UNSUPPORTED : DC_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+DC_HIP_API int32_t dc_hip_linear(dc_hip_ctx* ctx, const dc_linear* args) {
+  if (!args) return DC_ERR_INVALID_ARGUMENT;
+  const dc_linear& p = *args;
+  DC_RETURN_IF(check_dims(p.m, p.n, p.k, p.activation));
+  const bool fp8 = p.dtype == DC_DTYPE_FP8, y_f32 = p.y_dtype == DC_DTYPE_F32;
+  if ((!fp8 && p.dtype != DC_DTYPE_BF16) || (!y_f32 && p.y_dtype != DC_DTYPE_BF16) || p.reserved != 0)
+    return DC_ERR_INVALID_ARGUMENT;
+  if (fp8 != (p.x_scales != nullptr) || fp8 != (p.w_scales != nullptr)) return DC_ERR_INVALID_ARGUMENT;
+  const int64_t size = fp8 ? 1 : 2;
+  if (p.m > 0 && p.n > 0) {
+    if (p.k > 0) {
+      DC_RETURN_IF(check_rows(p.x, size, p.x_stride, p.m, p.k));
+      DC_RETURN_IF(check_rows(p.w, size, p.w_stride, p.n, p.k));
+    }
+    DC_RETURN_IF(check_rows(p.y, y_f32 ? 4 : 2, p.y_stride, p.m, p.n));
+    if (p.residual) DC_RETURN_IF(check_rows(p.residual, 2, p.residual_stride, p.m, p.n));
+    if (p.pre) DC_RETURN_IF(check_rows(p.pre, 2, p.pre_stride, p.m, p.n));
+    if (!aligned_to(p.bias, 2) || !aligned_to(p.x_scales, 4) || !aligned_to(p.w_scales, 4)) return DC_ERR_MISALIGNED;
+  }
+  DC_CTX_ENTER(ctx);
+  if (p.m == 0 || p.n == 0) return DC_OK;
+  const Epilogue ep{p.x_scales,
+                    p.w_scales,
+                    reinterpret_cast<const bf16*>(p.bias),
+                    reinterpret_cast<const bf16*>(p.residual),
+                    reinterpret_cast<bf16*>(p.pre),
+                    p.y,
+                    p.residual_stride,
+                    p.pre_stride,
+                    p.y_stride,
+                    p.activation,
+                    y_f32};
+  Operands o{static_cast<const unsigned char*>(p.x),
+             static_cast<const unsigned char*>(p.w),
+             p.x_stride * size,
+             p.w_stride * size,
+             (int32_t)p.m,
+             (int32_t)p.n,
+             (int32_t)(p.k * size),
+             0};
+  if (p.k == 0 || dc::linear_few_rows(p.m, p.n, p.k * size)) return fp8 ? few_rows<true>(ctx, o, ep) : few_rows<false>(ctx, o, ep);
+  Scratch scratch;
+  Rows x{o.a, o.a_pitch, p.m, o.c_bytes}, w{o.b, o.b_pitch, p.n, o.c_bytes};
+  x.plan(scratch);
+  w.plan(scratch);
+  if (scratch.bytes) DC_RETURN_IF(dc::ensure_partials(ctx, scratch.bytes));
+  DC_RETURN_IF(x.lay_out(ctx));
+  DC_RETURN_IF(w.lay_out(ctx));
+  o.a = x.p, o.b = w.p, o.a_pitch = x.pitch, o.b_pitch = w.pitch;
+  return fp8 ? product<true, false>(ctx, o, ep) : product<false, false>(ctx, o, ep);
+}
+
+DC_HIP_API int32_t dc_hip_linear_backward(dc_hip_ctx* ctx, const dc_linear_grad* args) {
+  if (!args) return DC_ERR_INVALID_ARGUMENT;
+  const dc_linear_grad& p = *args;
+  DC_RETURN_IF(check_dims(p.m, p.n, p.k, p.activation));
+  if (p.reserved != 0) return DC_ERR_INVALID_ARGUMENT;
+  if (p.m > dc::kLinearWidth) return DC_ERR_UNSUPPORTED;  // dw's sums run along m
+  const bool act = p.activation != DC_ACT_NONE;
+  const bool dx = p.dx && p.m > 0 && p.k > 0, dw = p.dw && p.n > 0 && p.k > 0, dbias = p.dbias && p.n > 0;
+  const bool inputs = p.m > 0 && p.n > 0 && (dx || dw || dbias);
+  if (inputs) {
+    DC_RETURN_IF(check_rows(p.dy, 2, p.dy_stride, p.m, p.n));
+    if (act) DC_RETURN_IF(check_rows(p.pre, 2, p.pre_stride, p.m, p.n));
+    if (dx) DC_RETURN_IF(check_rows(p.w, 2, p.w_stride, p.n, p.k));
+    if (dw) DC_RETURN_IF(check_rows(p.x, 2, p.x_stride, p.m, p.k));
+  }
+  if (dx) DC_RETURN_IF(check_rows(p.dx, 2, p.dx_stride, p.m, p.k));
+  if (dw) DC_RETURN_IF(check_rows(p.dw, 2, p.dw_stride, p.n, p.k));
+  if (!aligned_to(p.dbias, 4)) return DC_ERR_MISALIGNED;
+  DC_CTX_ENTER(ctx);
+  if (!dx && !dw && !dbias) return DC_OK;
+  // dz runs along n in dx and along m in dw: a copy of each, padded to whole 16-byte pieces, in scratch; dy itself where
+  // it serves as dz. (Without rows, or columns, of dz the sums are empty: few_rows with no steps writes the zeros.)
+  Scratch scratch;
+  Rows dz{reinterpret_cast<const unsigned char*>(p.dy), 2 * p.dy_stride, p.m, 2 * p.n};
+  Rows w{reinterpret_cast<const unsigned char*>(p.w), 2 * p.w_stride, p.n, 2 * p.k};
+  Rows x{reinterpret_cast<const unsigned char*>(p.x), 2 * p.x_stride, p.m, 2 * p.k};
+  SlopeArgs s{reinterpret_cast<const bf16*>(p.dy), reinterpret_cast<const bf16*>(p.pre), nullptr, nullptr, nullptr, p.m, p.n,
+              p.dy_stride, p.pre_stride, padded(p.n, 8), padded(p.m, 8), p.activation};
+  size_t at_dz = 0, at_dzt = 0, at_parts = 0;
+  bool own_dz = false;
+  const int64_t pieces = (p.m + 63) / 64;
+  if (inputs) {
+    if (dx) {
+      dz.plan(scratch);
+      own_dz = act || dz.copied;
+      if (own_dz) at_dz = dz.copied ? dz.at : scratch.take(p.m * 2 * s.dz_pitch);
+      w.plan(scratch);
+    }
+    if (dw) {
+      at_dzt = scratch.take(p.n * 2 * s.t_pitch);
+      x.plan(scratch);
+    }
+    if (dbias) at_parts = scratch.take(pieces * p.n * (int64_t)sizeof(float));
+    if (scratch.bytes) DC_RETURN_IF(dc::ensure_partials(ctx, scratch.bytes));
+    unsigned char* base = static_cast<unsigned char*>(ctx->partials);
+    if (own_dz) s.dz = reinterpret_cast<bf16*>(base + at_dz);
+    if (dw) s.dzt = reinterpret_cast<bf16*>(base + at_dzt);
+    if (dbias) s.parts = reinterpret_cast<float*>(base + at_parts);
+    if (s.dz || s.dzt || s.parts) {
+      const int64_t grid = std::min<int64_t>((p.n + 63) / 64 * pieces, 1 << 20);
+      slope_kernel<<<(unsigned)grid, 256, 0, ctx->stream>>>(s);
+      DC_RETURN_IF(dc::last_launch_status());
+    }
+  }
+  Epilogue ep{};
+  // One gradient: the product of `rows` (m of them, along c) and `b` (c rows of k), or zeros where c is empty.
+  auto gradient = [&](const unsigned char* rows, int64_t pitch, int64_t m, int64_t c, Rows& b, void* out, int64_t stride) -> int32_t {
+    ep.y = out, ep.y_stride = stride;
+    if (!inputs) return few_rows<false>(ctx, Operands{nullptr, nullptr, 0, 0, (int32_t)m, (int32_t)p.k, 0, 0, 0}, ep);
+    DC_RETURN_IF(b.lay_out(ctx));
+    const Operands o{rows, b.p, pitch, b.pitch, (int32_t)m, (int32_t)p.k, (int32_t)(2 * c), (int32_t)c, (int32_t)padded(p.k, 8)};
+    return product<false, true>(ctx, o, ep);
+  };
+  if (dx) {
+    const unsigned char* rows = s.dz ? reinterpret_cast<const unsigned char*>(s.dz) : dz.p;
+    DC_RETURN_IF(gradient(rows, s.dz ? 2 * s.dz_pitch : dz.pitch, p.m, p.n, w, p.dx, p.dx_stride));
+  }
+  if (dw)
+    DC_RETURN_IF(gradient(reinterpret_cast<const unsigned char*>(s.dzt), 2 * s.t_pitch, p.n, p.m, x, p.dw, p.dw_stride));
+  if (!dbias) return DC_OK;
+  if (!inputs) return dc::zero_async(ctx, p.dbias, (size_t)p.n * sizeof(float));
+  return dc::launch_column_sums(ctx, s.parts, p.dbias, pieces, p.n);
+}
+
+}  // extern "C"

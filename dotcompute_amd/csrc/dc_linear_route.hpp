@@ -1,0 +1,35 @@
+// dc_linear_route.hpp — which kernel of dc_linear.hip takes a shape: pure functions of the sizes and the number of
+// CUs, checked on the CPU by tests/cpp/host_tests.cpp.
+#pragma once
+
+#include <cstdint>
+
+namespace dc {
+
+// Bytes that a direct-to-LDS load can be away from its tile's first, and the pitch with which the rows of the smallest
+// tiles stay below that; rows are at most kLinearWidth elements.
+constexpr int32_t kLinearRange = INT32_MAX;
+constexpr int64_t kLinearPitch = (int64_t(1) << 25) - 16;
+constexpr int64_t kLinearWidth = int64_t(1) << 23;
+static_assert(64 * kLinearPitch < kLinearRange && 2 * kLinearWidth <= kLinearPitch);
+
+// Tiles, square, and groups of waves that take the steps along c in turn.
+enum class LinearTile { k256, k128, k128x2, k64, k64x2, k64x4 };
+
+inline LinearTile linear_tile(int64_t m, int64_t n, int64_t c_bytes, int64_t a_pitch, int64_t b_pitch, bool rows_c, int64_t cus) {
+  auto tiles = [&](int64_t t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
+  auto fits = [&](int64_t t) { return t * a_pitch < kLinearRange && (rows_c || t * b_pitch < kLinearRange); };
+  const int64_t t256 = tiles(256), t128 = tiles(128), t64 = tiles(64), k = c_bytes / 2;
+  const bool brief = (k <= 64 && (t256 > cus || 4 * t256 <= 3 * cus)) || (k <= 128 && t256 > 2 * cus);
+  if (fits(256) && 2 * t256 > cus && (t256 <= cus || 10 * t256 > 13 * cus) && !brief) return LinearTile::k256;
+  if (fits(128) && t128 > cus && !brief) return LinearTile::k128;
+  if (fits(128) && 4 * t128 > 3 * cus && k > 128) return LinearTile::k128x2;
+  if (t64 > 2 * cus || k < 512) return LinearTile::k64;
+  if (2 * t64 > cus || k < 2048) return LinearTile::k64x2;
+  return LinearTile::k64x4;
+}
+
+// Few rows of x.
+inline bool linear_few_rows(int64_t m, int64_t n, int64_t c_bytes) { return m <= 32; }
+
+}  // namespace dc

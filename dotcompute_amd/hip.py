@@ -47,6 +47,11 @@ LINQ_FOLD_MAX = 3
 
 DC_LINQ_MAX_INSTR = 48
 
+# dc_dtype, dc_activation: element types and activations of the feed-forward block's operators
+DTYPE_F32, DTYPE_BF16, DTYPE_FP8 = range(3)
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+ADAMW_BLOCK = 256  # elements of an 8-bit state that share a scale
+
 # dc_linq_op
 NOP, LOAD, ADD, SUB, RSUB, MUL, DIV, RDIV, MIN, MAX, NEG, ABS, SQRT, STORE_S0, STORE_S1 = range(15)
 REM, RREM, FLOOR, CEIL, ROUND = range(15, 20)
@@ -122,6 +127,186 @@ class LinqChain(C.Structure):
                 ins.imm = float(imm)
             ch.code[i] = ins
         return ch
+
+
+def dtype_of(a: "DeviceArray") -> int:
+    """dc_dtype of an array: float32, bf16 bit patterns (uint16) or e4m3 bytes (uint8)."""
+    try:
+        return {np.dtype(np.float32): DTYPE_F32, np.dtype(np.uint16): DTYPE_BF16,
+                np.dtype(np.uint8): DTYPE_FP8}[np.dtype(a.dtype)]
+    except KeyError:
+        raise ValueError(f"no operator takes elements of type {a.dtype}") from None
+
+
+def _matrix(a: "DeviceArray", name: str) -> tuple:
+    if len(a.shape) != 2:
+        raise ValueError(f"{name} is a matrix (got shape {a.shape})")
+    return a.shape
+
+
+def _expect(a: "DeviceArray | None", name: str, dtypes: tuple, shape: tuple) -> None:
+    """The structures below carry addresses only, so that what a kernel will read is checked here."""
+    if a is None:
+        return
+    if tuple(a.shape) != tuple(shape) or dtype_of(a) not in dtypes:
+        raise ValueError(f"{name}: shape {tuple(shape)} expected, of type {dtypes} (got {tuple(a.shape)}, {a.dtype})")
+
+
+class _Arguments(C.Structure):
+    """An argument block of arrays by name; it keeps them alive as long as it lives."""
+
+    def _put(self, strides: dict, **arrays) -> None:
+        self._arrays = arrays
+        for name, a in arrays.items():
+            if a is None:
+                continue
+            setattr(self, name, a.ptr)
+            if len(a.shape) == 2:
+                setattr(self, name + "_stride", strides.pop(name + "_stride", a.shape[1]))
+        if strides:
+            raise ValueError(f"no such strides: {sorted(strides)}")
+
+
+class RmsNorm(_Arguments):
+    """dc_rms_norm: h = x + residual, y = h * weight / sqrt(mean(h^2) + eps)."""
+    _fields_ = ([("rows", C.c_int64), ("cols", C.c_int64), ("dtype", C.c_int32), ("y_dtype", C.c_int32), ("eps", C.c_float),
+                 ("reserved", C.c_int32)] + [(n, C.c_void_p) for n in ("x", "residual", "weight", "sum", "y", "scales")] +
+                [(n, C.c_int64) for n in ("x_stride", "residual_stride", "sum_stride", "y_stride")])
+
+    @classmethod
+    def of(cls, x: "DeviceArray", weight: "DeviceArray", y: "DeviceArray", residual: "DeviceArray | None" = None,
+           sum: "DeviceArray | None" = None, scales: "DeviceArray | None" = None, eps: float = 1e-6, **strides) -> "RmsNorm":
+        """y in x's type, or uint8 (e4m3) with `scales`. Row strides in elements by name (x_stride=...), else dense."""
+        rows, cols = _matrix(x, "x")
+        same = (dtype_of(x),)
+        _expect(weight, "weight", same, (cols,))
+        _expect(y, "y", same + (DTYPE_FP8,), (rows, cols))
+        _expect(residual, "residual", same, (rows, cols))
+        _expect(sum, "sum", same, (rows, cols))
+        _expect(scales, "scales", (DTYPE_F32,), (rows,))
+        a = cls(rows=rows, cols=cols, dtype=dtype_of(x), y_dtype=dtype_of(y), eps=eps)
+        a._put(strides, x=x, residual=residual, weight=weight, sum=sum, y=y, scales=scales)
+        return a
+
+
+class RmsNormGrad(_Arguments):
+    """dc_rms_norm_grad: the gradients of RmsNorm's y by h and by the weight."""
+    _fields_ = ([("rows", C.c_int64), ("cols", C.c_int64), ("dtype", C.c_int32), ("eps", C.c_float)] +
+                [(n, C.c_void_p) for n in ("dy", "h", "weight", "dh", "dx", "dweight")] +
+                [(n, C.c_int64) for n in ("dy_stride", "h_stride", "dh_stride", "dx_stride")])
+
+    @classmethod
+    def of(cls, dy: "DeviceArray", h: "DeviceArray", weight: "DeviceArray", dx: "DeviceArray | None" = None,
+           dweight: "DeviceArray | None" = None, dh: "DeviceArray | None" = None, eps: float = 1e-6, **strides) -> "RmsNormGrad":
+        """dx in h's type (plus dh, where given), dweight in float32."""
+        rows, cols = _matrix(h, "h")
+        same = (dtype_of(h),)
+        _expect(weight, "weight", same, (cols,))
+        _expect(dy, "dy", same, (rows, cols))
+        _expect(dh, "dh", same, (rows, cols))
+        _expect(dx, "dx", same, (rows, cols))
+        _expect(dweight, "dweight", (DTYPE_F32,), (cols,))
+        a = cls(rows=rows, cols=cols, dtype=dtype_of(h), eps=eps)
+        a._put(strides, dy=dy, h=h, weight=weight, dh=dh, dx=dx, dweight=dweight)
+        return a
+
+
+class Linear(_Arguments):
+    """dc_linear: z = x w^T + bias, y = act(z) + residual."""
+    _fields_ = ([("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64), ("dtype", C.c_int32), ("y_dtype", C.c_int32),
+                 ("activation", C.c_int32), ("reserved", C.c_int32)] +
+                [(n, C.c_void_p) for n in ("x", "w", "x_scales", "w_scales", "bias", "residual", "pre", "y")] +
+                [(n, C.c_int64) for n in ("x_stride", "w_stride", "residual_stride", "pre_stride", "y_stride")])
+
+    @classmethod
+    def of(cls, x: "DeviceArray", w: "DeviceArray", y: "DeviceArray", bias: "DeviceArray | None" = None,
+           residual: "DeviceArray | None" = None, pre: "DeviceArray | None" = None, x_scales: "DeviceArray | None" = None,
+           w_scales: "DeviceArray | None" = None, activation: str = "none", **strides) -> "Linear":
+        """x [m, k] and w [n, k] in bf16, or in e4m3 with x_scales [m] and w_scales [n]; bias [n], residual and pre
+        (receives z) [m, n] in bf16; y [m, n] in bf16 or float32."""
+        (m, k), (n, _) = _matrix(x, "x"), _matrix(w, "w")
+        _expect(x, "x", (DTYPE_BF16, DTYPE_FP8), (m, k))
+        _expect(w, "w", (dtype_of(x),), (n, k))
+        _expect(x_scales, "x_scales", (DTYPE_F32,), (m,))
+        _expect(w_scales, "w_scales", (DTYPE_F32,), (n,))
+        _expect(bias, "bias", (DTYPE_BF16,), (n,))
+        _expect(residual, "residual", (DTYPE_BF16,), (m, n))
+        _expect(pre, "pre", (DTYPE_BF16,), (m, n))
+        _expect(y, "y", (DTYPE_BF16, DTYPE_F32), (m, n))
+        a = cls(m=m, n=n, k=k, dtype=dtype_of(x), y_dtype=dtype_of(y), activation=ACTIVATIONS[activation])
+        a._put(strides, x=x, w=w, x_scales=x_scales, w_scales=w_scales, bias=bias, residual=residual, pre=pre, y=y)
+        return a
+
+
+class LinearGrad(_Arguments):
+    """dc_linear_grad: the gradients of Linear's y by x, w and bias."""
+    _fields_ = ([("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64), ("activation", C.c_int32), ("reserved", C.c_int32)] +
+                [(n, C.c_void_p) for n in ("dy", "x", "w", "pre", "dx", "dw", "dbias")] +
+                [(n, C.c_int64) for n in ("dy_stride", "x_stride", "w_stride", "pre_stride", "dx_stride", "dw_stride")])
+
+    @classmethod
+    def of(cls, dy: "DeviceArray", x: "DeviceArray", w: "DeviceArray", pre: "DeviceArray | None" = None,
+           dx: "DeviceArray | None" = None, dw: "DeviceArray | None" = None, dbias: "DeviceArray | None" = None,
+           activation: str = "none", **strides) -> "LinearGrad":
+        """All bf16 but dbias (float32); pre: what Linear wrote there (may be left out where activation is none)."""
+        (m, k), (n, _) = _matrix(x, "x"), _matrix(w, "w")
+        for name, a, shape in (("dy", dy, (m, n)), ("x", x, (m, k)), ("w", w, (n, k)), ("pre", pre, (m, n)), ("dx", dx, (m, k)),
+                               ("dw", dw, (n, k))):
+            _expect(a, name, (DTYPE_BF16,), shape)
+        _expect(dbias, "dbias", (DTYPE_F32,), (n,))
+        a = cls(m=m, n=n, k=k, activation=ACTIVATIONS[activation])
+        a._put(strides, dy=dy, x=x, w=w, pre=pre, dx=dx, dw=dw, dbias=dbias)
+        return a
+
+
+class AdamW(C.Structure):
+    """dc_adamw: the numbers of one step (`step` counts from 1). The states' type comes with the tensors."""
+    _fields_ = ([(n, C.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay", "grad_scale")] +
+                [("step", C.c_int64), ("state_dtype", C.c_int32), ("reserved", C.c_int32)])
+
+    @classmethod
+    def of(cls, lr: float, step: int = 1, beta1: float = 0.9, beta2: float = 0.999, eps: float = 1e-8,
+           weight_decay: float = 0.01, grad_scale: float = 1.0) -> "AdamW":
+        return cls(lr=lr, beta1=beta1, beta2=beta2, eps=eps, weight_decay=weight_decay, grad_scale=grad_scale, step=step)
+
+
+class AdamWTensor(C.Structure):
+    """dc_adamw_tensor: one tensor of a step."""
+    _fields_ = ([(n, C.c_void_p) for n in ("param", "grad", "m", "v", "m_scales", "v_scales", "copy")] +
+                [("n", C.c_int64), ("grad_dtype", C.c_int32), ("reserved", C.c_int32)])
+
+
+class AdamWTensors:
+    """The tensors of a step: an array of dc_adamw_tensor, and the type of their states."""
+
+    def __init__(self, items, state_dtype: int, arrays: list):
+        self.items, self.state_dtype, self.arrays = items, state_dtype, arrays
+
+    @classmethod
+    def of(cls, parts: list) -> "AdamWTensors":
+        """`parts`: a dict of arrays per tensor: param (float32), grad (float32 or bf16), m and v (float32; or uint8, with
+        m_scales and v_scales, one for every 256 elements) and, optionally, copy (bf16)."""
+        items, states = (AdamWTensor * len(parts))(), set()
+        for t, part in zip(items, parts):
+            n = part["param"].size
+            state = dtype_of(part["m"])
+            flat = {name: tuple(a.shape) for name, a in part.items()}
+            for name, a in part.items():
+                if name not in AdamWTensor.__dict__:
+                    raise ValueError(f"a step takes no array called {name}")
+                want = -(-n // ADAMW_BLOCK) if name.endswith("scales") else n
+                if a.size != want:
+                    raise ValueError(f"{name}: {want} elements expected (got {flat[name]})")
+                setattr(t, name, a.ptr)
+            types = {name: dtype_of(a) for name, a in part.items()}
+            if types["param"] != DTYPE_F32 or types["grad"] == DTYPE_FP8 or state == DTYPE_BF16 or types["v"] != state \
+                    or types.get("copy", DTYPE_BF16) != DTYPE_BF16:
+                raise ValueError(f"no such types: {types}")
+            t.n, t.grad_dtype = n, types["grad"]
+            states.add(state)
+        if len(states) > 1:
+            raise ValueError("the states of one step are of one type")
+        return cls(items, states.pop() if states else DTYPE_F32, parts)
 
 
 def compile_chain(chain: LinqChain, element: int = LINQ_ELEMENT_F32, arch: str = "gfx950") -> int:
@@ -221,6 +406,12 @@ SIGNATURES: dict[str, list] = {
     "dc_hip_spmv_plan_power_iterate_f32": [_P, _P, _P, _P, _i32, _P],
     "dc_hip_spmv_plan_info": [_P, C.POINTER(_i32), C.POINTER(_i64), C.POINTER(_i64)],
     "dc_hip_spmv_plan_destroy": [_P],
+    "dc_hip_rms_norm": [_P, C.POINTER(RmsNorm)],
+    "dc_hip_rms_norm_backward": [_P, C.POINTER(RmsNormGrad)],
+    "dc_hip_quantize_fp8": [_P, _P, _i32, _i64, _P, _i64, _P, _i64, _i64],
+    "dc_hip_linear": [_P, C.POINTER(Linear)],
+    "dc_hip_linear_backward": [_P, C.POINTER(LinearGrad)],
+    "dc_hip_adamw_step": [_P, C.POINTER(AdamW), C.POINTER(AdamWTensor), _i32],
 }
 _RESTYPES = {"dc_hip_error_string": C.c_char_p, "dc_hip_default_module_path": C.c_char_p}
 
@@ -497,6 +688,31 @@ class Context:
     def convert_f32_to_bf16(self, x: DeviceArray, out: DeviceArray, n: int | None = None) -> None:
         n = x.size if n is None else n
         check(load().dc_hip_convert_f32_to_bf16(self.handle, x.ptr, out.ptr, n), "dc_hip_convert_f32_to_bf16")
+
+    # ---- operators of a feed-forward block: argument blocks built once, run any number of times ----
+    def rms_norm(self, args: RmsNorm) -> None:
+        check(load().dc_hip_rms_norm(self.handle, args), "dc_hip_rms_norm")
+
+    def rms_norm_backward(self, args: RmsNormGrad) -> None:
+        check(load().dc_hip_rms_norm_backward(self.handle, args), "dc_hip_rms_norm_backward")
+
+    def quantize_fp8(self, x: DeviceArray, q: DeviceArray, scales: DeviceArray) -> None:
+        """Rows of x (float32 or bf16) in e4m3 (uint8 bytes) with a scale each."""
+        rows, cols = _matrix(x, "x")
+        _expect(q, "q", (DTYPE_FP8,), (rows, cols))
+        _expect(scales, "scales", (DTYPE_F32,), (rows,))
+        check(load().dc_hip_quantize_fp8(self.handle, x.ptr, dtype_of(x), cols, q.ptr, cols, scales.ptr, rows, cols),
+              "dc_hip_quantize_fp8")
+
+    def linear(self, args: Linear) -> None:
+        check(load().dc_hip_linear(self.handle, args), "dc_hip_linear")
+
+    def linear_backward(self, args: LinearGrad) -> None:
+        check(load().dc_hip_linear_backward(self.handle, args), "dc_hip_linear_backward")
+
+    def adamw_step(self, args: AdamW, tensors: AdamWTensors) -> None:
+        args.state_dtype = tensors.state_dtype
+        check(load().dc_hip_adamw_step(self.handle, args, tensors.items, len(tensors.items)), "dc_hip_adamw_step")
 
     def spmv_csr_f32(self, rp: DeviceArray, col: DeviceArray, val: DeviceArray, x: DeviceArray, y: DeviceArray,
                      rows: int, cols: int, nnz: int) -> None:

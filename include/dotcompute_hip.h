@@ -541,6 +541,142 @@ DC_HIP_API int32_t dc_hip_spmv_plan_info(const dc_hip_spmv_plan* plan, int32_t* 
 /* Waits for the device, then frees the plan. */
 DC_HIP_API int32_t dc_hip_spmv_plan_destroy(dc_hip_spmv_plan* plan);
 
+/* ---------------------------------------------------------------------------------------------
+ * Operators of a feed-forward block, for training one and for serving tokens through it: RMS norm with the
+ * residual's addition, matrix products with bias, activation and residual in their epilogue, their
+ * gradients, and the AdamW step of many tensors. They have no counterpart in the reference, whose dense
+ * arithmetic stops at MultiplyAsync (src/Extensions/DotCompute.Algorithms/LinearAlgebra/Operations/
+ * MatrixOperations.cs:28-64); an argument block each, since most of their operands may be absent.
+ *
+ * Conventions: matrices are row-major; a *_stride is the distance of two rows in elements, at least the row's
+ * length. All pointers are device pointers at the alignment of one element. bf16 values are uint16 bit patterns.
+ * 8-bit values are e4m3 (1 sign, 4 exponent, 3 fraction bits, bias 7, largest 448, no infinity), and stand for
+ * themselves times their scale, max / 448 over the row or block that shares it; a NaN in one makes its scale NaN.
+ * Sums, statistics and scales are float32. Results are the same bits from call to call.
+ * ------------------------------------------------------------------------------------------- */
+typedef enum dc_dtype {
+  DC_DTYPE_F32 = 0,
+  DC_DTYPE_BF16 = 1,
+  DC_DTYPE_FP8 = 2 /* e4m3, with scales */
+} dc_dtype;
+
+typedef enum dc_activation {
+  DC_ACT_NONE = 0,
+  DC_ACT_RELU = 1,
+  DC_ACT_GELU = 2,      /* z P(z), P the normal distribution's function */
+  DC_ACT_GELU_TANH = 3, /* z / (1 + exp(-2u)), u = sqrt(2/pi) (z + 0.044715 z^3) */
+  DC_ACT_SILU = 4       /* z / (1 + exp(-z)) */
+} dc_activation;
+
+/* h = x + residual; y = h * weight / sqrt(mean(h^2) + eps), row by row.
+ * dtype: x, residual, weight, sum. y has y_dtype: dtype, or FP8 with a scale per row. `residual` may be NULL
+ * (h = x); `sum` receives h, rounded to dtype (y is formed from the unrounded one), or is NULL. `sum` may be x or
+ * residual, and `y` of type dtype x, residual, at the same stride. */
+typedef struct dc_rms_norm {
+  int64_t rows, cols;
+  int32_t dtype, y_dtype; /* F32 or BF16; the same or FP8 */
+  float eps;
+  int32_t reserved; /* 0 */
+  const void* x;
+  const void* residual;
+  const void* weight; /* [cols] */
+  void* sum;
+  void* y;
+  float* scales; /* [rows]; FP8 only, else NULL */
+  int64_t x_stride, residual_stride, sum_stride, y_stride;
+} dc_rms_norm;
+DC_HIP_API int32_t dc_hip_rms_norm(dc_hip_ctx* ctx, const dc_rms_norm* args);
+
+/* Gradients of y = h * weight / sqrt(mean(h^2) + eps): with s = 1 / sqrt(mean(h^2) + eps) and g = dy * weight,
+ * dx = s (g - h s mean(g h s)) + dh, the gradient of x and of residual alike; dweight = the sum over rows of dy h s.
+ * dtype: dy, h, weight, dh, dx; dweight is float32. `dh` (the gradient that reaches h by its other uses) may be
+ * NULL, as may dx or dweight; `dx` may be dh or dy at the same stride. */
+typedef struct dc_rms_norm_grad {
+  int64_t rows, cols;
+  int32_t dtype; /* F32 or BF16 */
+  float eps;
+  const void* dy;
+  const void* h;
+  const void* weight; /* [cols] */
+  const void* dh;
+  void* dx;
+  float* dweight; /* [cols] */
+  int64_t dy_stride, h_stride, dh_stride, dx_stride;
+} dc_rms_norm_grad;
+DC_HIP_API int32_t dc_hip_rms_norm_backward(dc_hip_ctx* ctx, const dc_rms_norm_grad* args);
+
+/* Rows in 8 bits: scales[r] = max|x[r]| / 448, q[r] = e4m3(x[r] * (448 / max|x[r]|)). dtype: F32 or BF16. */
+DC_HIP_API int32_t dc_hip_quantize_fp8(dc_hip_ctx* ctx, const void* x, int32_t dtype, int64_t x_stride,
+                                       uint8_t* q, int64_t q_stride, float* scales, int64_t rows,
+                                       int64_t cols);
+
+/* z = x w^T (x_scales w_scales) + bias; y = act(z) + residual: x is [m][k], w [n][k] (a row per output), y [m][n].
+ * dtype: x and w, BF16 or FP8 (then with x_scales[m] and w_scales[n], else both NULL). bias[n], residual and pre are
+ * BF16; y has y_dtype, BF16 or F32. bias, residual may be NULL; `pre` receives z for the backward pass, or is NULL.
+ * `y` may be residual at the same stride (both BF16). */
+typedef struct dc_linear {
+  int64_t m, n, k;
+  int32_t dtype, y_dtype, activation;
+  int32_t reserved; /* 0 */
+  const void* x;
+  const void* w;
+  const float* x_scales;
+  const float* w_scales;
+  const uint16_t* bias;
+  const uint16_t* residual;
+  uint16_t* pre;
+  void* y;
+  int64_t x_stride, w_stride, residual_stride, pre_stride, y_stride;
+} dc_linear;
+DC_HIP_API int32_t dc_hip_linear(dc_hip_ctx* ctx, const dc_linear* args);
+
+/* Gradients of y = act(x w^T + bias) + residual, all BF16 but dbias: dz = dy act'(pre), rounded to bf16 for the matrix
+ * cores; dx = dz w, dw = dz^T x, dbias = the sum over rows of dz (unrounded). The residual's gradient is dy itself.
+ * `pre` may be NULL when activation is NONE; dx, dw or dbias may be NULL, as may the operands that only they need. */
+typedef struct dc_linear_grad {
+  int64_t m, n, k;
+  int32_t activation;
+  int32_t reserved; /* 0 */
+  const uint16_t* dy;
+  const uint16_t* x;
+  const uint16_t* w;
+  const uint16_t* pre;
+  uint16_t* dx;
+  uint16_t* dw;
+  float* dbias;
+  int64_t dy_stride, x_stride, w_stride, pre_stride, dx_stride, dw_stride;
+} dc_linear_grad;
+DC_HIP_API int32_t dc_hip_linear_backward(dc_hip_ctx* ctx, const dc_linear_grad* args);
+
+/* One AdamW step, over `count` tensors at once (an array in host memory, read during the call): with g = grad *
+ * grad_scale, m = beta1 m + (1 - beta1) g, v = beta2 v + (1 - beta2) g^2 and t = step (from 1),
+ *   param = param (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps).
+ * param is float32; `copy`, where it is not NULL, receives the new param in bf16. state_dtype F32: m and v are
+ * float32, and the scales are NULL. FP8: m holds e4m3 values with a scale for every 256 elements
+ * (ceil(n / 256) scales; the last block may be short), v the same of sqrt(v), whose values above zero are held as at
+ * least the smallest e4m3 value, so that none becomes a zero denominator. Zeroed states and scales are step 1's. */
+#define DC_ADAMW_BLOCK 256
+typedef struct dc_adamw {
+  double lr, beta1, beta2, eps, weight_decay, grad_scale; /* (1 - beta is formed from the double) */
+  int64_t step;
+  int32_t state_dtype; /* F32 or FP8 */
+  int32_t reserved;    /* 0 */
+} dc_adamw;
+typedef struct dc_adamw_tensor {
+  float* param;
+  const void* grad;
+  void* m;
+  void* v;
+  float* m_scales;
+  float* v_scales;
+  uint16_t* copy;
+  int64_t n;
+  int32_t grad_dtype; /* F32 or BF16 */
+  int32_t reserved;   /* 0 */
+} dc_adamw_tensor;
+DC_HIP_API int32_t dc_hip_adamw_step(dc_hip_ctx* ctx, const dc_adamw* args, const dc_adamw_tensor* tensors,
+                                     int32_t count);
+
 #ifdef __cplusplus
 }
 #endif
