@@ -6,8 +6,7 @@
 // Kernels:
 //   - product_kernel: D[i][j] = sum_c A(i, c) B(j, c) in tiles on the matrix cores. A's rows run along c. B's do too
 //     (forward), or are the rows c of a row-major [c][j] matrix (the gradients).
-//   - few_rows_kernel: forward with few rows of x. Bound by reading w, which goes from memory to the matrix
-//     cores' operands without a stop in LDS.
+//   - few_rows_kernel, few_rows_any_kernel: forward with few rows of x.
 //   - slope_kernel: dz and its transpose in bf16 (what the two gradients' products run along), and dbias's parts.
 //   - pack_kernel: rows that the direct-to-LDS loads cannot take (not 16-byte aligned, or no whole number of
 //     16 bytes) copied to ones padded with zeros.
@@ -39,31 +38,80 @@ __device__ inline float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.0f + _
 constexpr float kTanhArg = 2.0f * 0.7978845608f;  // 2 sqrt(2 / pi)
 constexpr float kTanhCube = 0.044715f;
 
-__device__ inline float act_value(int act, float z) {
+// P(z), the normal distribution's function, from *e = exp(-z^2 / 2): 1 - erf(x) = e^(-x^2) times a polynomial of the fifth
+// degree in 1 / (1 + 0.3275911 x) for x >= 0, within 1.5e-7 (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26);
+// the tail on the left is that product itself, so nothing cancels there.
+__device__ inline float normal_part(float z, float* e) {
+  const float x = __builtin_fabsf(z) * 0.70710678f;
+  *e = __expf(-0.5f * z * z);
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.0f));
+  float q = __builtin_fmaf(1.061405429f, t, -1.453152027f);
+  q = __builtin_fmaf(q, t, 1.421413741f);
+  q = __builtin_fmaf(q, t, -0.284496736f);
+  q = __builtin_fmaf(q, t, 0.254829592f);
+  q *= 0.5f * t * *e;
+  return z > 0.0f ? 1.0f - q : q;
+}
+
+// z = act(z), E of them; the choice is made once.
+template <int E>
+__device__ inline void activate(int act, float (&z)[E]) {
   switch (act) {
-    case DC_ACT_RELU: return z < 0.0f ? 0.0f : z;
-    case DC_ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678f));
-    case DC_ACT_GELU_TANH: return z * sigmoid(kTanhArg * (z + kTanhCube * z * z * z));
-    case DC_ACT_SILU: return z * sigmoid(z);
-    default: return z;
+    case DC_ACT_RELU:
+#pragma unroll
+      for (int e = 0; e < E; ++e) z[e] = z[e] < 0.0f ? 0.0f : z[e];
+      break;
+    case DC_ACT_GELU:
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        float t;
+        z[e] *= normal_part(z[e], &t);
+      }
+      break;
+    case DC_ACT_GELU_TANH:
+#pragma unroll
+      for (int e = 0; e < E; ++e) z[e] *= sigmoid(kTanhArg * z[e] * __builtin_fmaf(kTanhCube, z[e] * z[e], 1.0f));
+      break;
+    case DC_ACT_SILU:
+#pragma unroll
+      for (int e = 0; e < E; ++e) z[e] *= sigmoid(z[e]);
+      break;
+    default: break;
   }
 }
 
-__device__ inline float act_slope(int act, float z) {
+// g *= act'(z)
+template <int E>
+__device__ inline void apply_slope(int act, const float (&z)[E], float (&g)[E]) {
   switch (act) {
-    case DC_ACT_RELU: return z > 0.0f ? 1.0f : 0.0f;
+    case DC_ACT_RELU:
+#pragma unroll
+      for (int e = 0; e < E; ++e) g[e] *= z[e] > 0.0f ? 1.0f : 0.0f;
+      break;
     case DC_ACT_GELU:
-      return 0.5f * (1.0f + erff(z * 0.70710678f)) + z * (__expf(-0.5f * z * z) * 0.3989422804f);
-    case DC_ACT_GELU_TANH: {
-      const float zz = fminf(z * z, 1e4f);  // (past |z| = 100 the slope is 0 or 1, and z^2 may not be finite)
-      const float s = sigmoid(kTanhArg * z * (1.0f + kTanhCube * zz));
-      return s + z * s * (1.0f - s) * (kTanhArg * (1.0f + 3.0f * kTanhCube * zz));
-    }
-    case DC_ACT_SILU: {
-      const float s = sigmoid(z);
-      return s * (1.0f + z * (1.0f - s));
-    }
-    default: return 1.0f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        float t;
+        const float part = normal_part(z[e], &t);
+        g[e] *= part + z[e] * t * 0.3989422804f;
+      }
+      break;
+    case DC_ACT_GELU_TANH:
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float zz = fminf(z[e] * z[e], 1e4f);  // (past |z| = 100 the slope is 0 or 1, and z^2 may not be finite)
+        const float s = sigmoid(kTanhArg * z[e] * __builtin_fmaf(kTanhCube, zz, 1.0f));
+        g[e] *= s + z[e] * s * (1.0f - s) * (kTanhArg * __builtin_fmaf(3.0f * kTanhCube, zz, 1.0f));
+      }
+      break;
+    case DC_ACT_SILU:
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const float s = sigmoid(z[e]);
+        g[e] *= s * __builtin_fmaf(z[e], 1.0f - s, 1.0f);
+      }
+      break;
+    default: break;
   }
 }
 
@@ -78,18 +126,32 @@ struct Epilogue {
   int32_t y_f32;
 };
 
-// The E neighbouring results (i, j..) from their sums; `left`: how many columns there are from j on (at least one).
+// What the results of E neighbouring columns j.. share, whatever their row: read once.
 template <int E>
-__device__ inline void finish(const Epilogue& p, int64_t i, int64_t j, int64_t left, float (&z)[E]) {
-  auto load = [&](const bf16* q, float (&v)[E]) __attribute__((always_inline)) {
+struct Columns {
+  float bias[E], scale[E];
+  int64_t j, left;  // columns there are from j on
+
+  __device__ inline void read(const Epilogue& p, int64_t first, int64_t n) {
+    j = first, left = n - first;
+#pragma unroll
+    for (int e = 0; e < E; ++e) bias[e] = scale[e] = 0.0f;
+    if (left <= 0) return;
+    if (p.bias) load(p.bias + j, bias);
+    if (p.b_scales)
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (e < left) scale[e] = p.b_scales[j + e];
+  }
+  __device__ inline void load(const bf16* q, float (&v)[E]) const {
     if constexpr (E == 8) {
       dc::load_some(q, left, v);
     } else {
 #pragma unroll
       for (int e = 0; e < E; ++e) v[e] = e < left ? dc::to_f32(q[e]) : 0.0f;
     }
-  };
-  auto store = [&](bf16* q, const float (&v)[E]) __attribute__((always_inline)) {
+  }
+  __device__ inline void store(bf16* q, const float (&v)[E]) const {
     if constexpr (E == 8) {
       dc::store_some(q, left, v);
     } else {
@@ -97,42 +159,33 @@ __device__ inline void finish(const Epilogue& p, int64_t i, int64_t j, int64_t l
       for (int e = 0; e < E; ++e)
         if (e < left) q[e] = dc::from_f32<bf16>(v[e]);
     }
-  };
-  if (p.a_scales) {
-    const float s = p.a_scales[i];
-    float b[E];
+  }
+  // The results of row i (left > 0) from their sums.
+  __device__ inline void finish(const Epilogue& p, int64_t i, float (&z)[E]) const {
+    float r[E];
+    if (p.residual) load(p.residual + i * p.residual_stride + j, r);
+    if (p.a_scales) {
+      const float s = p.a_scales[i];
 #pragma unroll
-    for (int e = 0; e < E; e += 4) {
-      float (&q)[4] = *reinterpret_cast<float (*)[4]>(b + e);
-      dc::load_some(p.b_scales + j + e, left - e, q);
+      for (int e = 0; e < E; ++e) z[e] = z[e] * s * scale[e];
     }
+    if (p.bias)
 #pragma unroll
-    for (int e = 0; e < E; ++e) z[e] = z[e] * s * b[e];
-  }
-  float u[E];
-  if (p.bias) {
-    load(p.bias + j, u);
+      for (int e = 0; e < E; ++e) z[e] += bias[e];
+    if (p.pre) store(p.pre + i * p.pre_stride + j, z);
+    activate(p.act, z);
+    if (p.residual)
 #pragma unroll
-    for (int e = 0; e < E; ++e) z[e] += u[e];
-  }
-  if (p.pre) store(p.pre + i * p.pre_stride + j, z);
-  if (p.act != DC_ACT_NONE) {
+      for (int e = 0; e < E; ++e) z[e] += r[e];
+    if (p.y_f32) {
+      float* q = static_cast<float*>(p.y) + i * p.y_stride + j;
 #pragma unroll
-    for (int e = 0; e < E; ++e) z[e] = act_value(p.act, z[e]);
+      for (int e = 0; e < E; e += 4) dc::store_some(q + e, left - e, *reinterpret_cast<const float (*)[4]>(z + e));
+    } else {
+      store(static_cast<bf16*>(p.y) + i * p.y_stride + j, z);
+    }
   }
-  if (p.residual) {
-    load(p.residual + i * p.residual_stride + j, u);
-#pragma unroll
-    for (int e = 0; e < E; ++e) z[e] += u[e];
-  }
-  if (p.y_f32) {
-    float* q = static_cast<float*>(p.y) + i * p.y_stride + j;
-#pragma unroll
-    for (int e = 0; e < E; e += 4) dc::store_some(q + e, left - e, *reinterpret_cast<const float (*)[4]>(z + e));
-  } else {
-    store(static_cast<bf16*>(p.y) + i * p.y_stride + j, z);
-  }
-}
+};
 
 // ---- tiles -----------------------------------------------------------------------------------------
 // Macro tile TM×TN, 128 bytes of c at a time (64 bf16 or 128 e4m3), double-buffered LDS, WM×WN waves of
@@ -403,7 +456,8 @@ __global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void pro
   constexpr int kCols = 32 * kNT, kPitch = kCols + 4, kLanes = kCols / 8;
   static_assert(sizeof(Smem) >= kWaves * 32 * kPitch * sizeof(float), "the waves' blocks fit in the buffers");
   float* own = reinterpret_cast<float*>(&sms[0]) + wave * 32 * kPitch;
-  const int64_t j = n0 + wn * kCols + 8 * (lane % kLanes), left = o.n - j;
+  Columns<8> cols;
+  cols.read(ep, n0 + wn * kCols + 8 * (lane % kLanes), o.n);
 #pragma unroll
   for (int mt = 0; mt < kMT; ++mt) {
 #pragma unroll
@@ -421,97 +475,259 @@ __global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void pro
       float z[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) z[e] = own[row * kPitch + 8 * (lane % kLanes) + e];
-      if (i < o.m && left > 0) finish(ep, i, j, left, z);
+      if (i < o.m && cols.left > 0) cols.finish(ep, i, z);
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
 }
 
 // ---- few rows ----------------------------------------------------------------------------------------
-// 16·NB outputs (rows of w) and 16·MT rows of x per workgroup, whose W waves take the 128-byte steps along c in turn:
-// lane l of a wave holds pieces l / 16 and 4 + l / 16 of row l % 16, of w (the instruction's first operand) and of x
-// (its second), straight from memory at any alignment. A wave's sums go to LDS, and each lane adds the waves' in
-// order for four neighbouring outputs of one row of x.
-__device__ inline dc::u32x4 load_piece(const unsigned char* row, int64_t at, int64_t bytes) {
+// Bound by reading w once. A workgroup takes a few outputs (rows of w) and up to 64 rows of x; its W waves take the 128-byte
+// steps along c in turn, each on its own, and their sums are added in the order of the waves at the end. What the loads
+// cost was found by measurement: a CU takes about 14 bytes a cycle in loads to registers, whatever their number in flight and
+// whether they ask for whole 128-byte lines, and 28 in direct-to-LDS loads. So:
+//   - few_rows_kernel: 16-byte aligned operands, through LDS. 16·NB outputs and 8·XB rows of x a workgroup; each wave has
+//     D stages of LDS to itself (1 KiB for 8 rows and a step, in product_kernel's image) and keeps D - 1 steps' loads in
+//     flight, so the loop has no barrier. us for bf16, loads to registers / tiles of 64 / this: 1×4096×4096 8.8 / 16.6 / 7.4 (4.6
+//     TB/s with the launch), 16×4096×4096 10.0 / 16.0 / 8.0, 32×8192×4096 19.1 / 17.5 / 14.0, 32×2048×8192 23.8 / 28.4 / 11.5,
+//     64×2048×8192 38.0 / 30.6 / 16.0.
+//   - few_rows_any_kernel: any alignment, straight from memory to the operands of v_mfma_f32_16x16x32_*. A load asks for 8 rows
+//     of 128 bytes: lane l the piece 4·p + g of row l % 8, with p = l / 8 % 2 and g = l / 16. As the instruction's operands that is
+//     16 rows (8 of w, each with both halves p of the step) times 16 columns (8 of x, likewise); of its results those with
+//     the same half on both sides are wanted, and the two halves' are added.
+// The 16 bytes at `from`, of which `left` exist, in a row of `bytes`: a ragged piece is cut out of the row's last 16 bytes.
+__device__ inline dc::u32x4 load_piece(const unsigned char* from, int64_t left, int64_t bytes) {
   dc::u32x4 w = {0, 0, 0, 0};
-  if (at + 16 <= bytes) {
-    w = *reinterpret_cast<const dc::u32x4_at1*>(row + at);
-  } else if (at < bytes) {
+  if (left >= 16) {
+    w = *reinterpret_cast<const dc::u32x4_at1*>(from);
+  } else if (left > 0 && bytes >= 16) {
+    w = *reinterpret_cast<const dc::u32x4_at1*>(from + left - 16);
+    w = __builtin_bit_cast(dc::u32x4, __builtin_bit_cast(unsigned __int128, w) >> (8 * (16 - (int)left)));
+  } else if (left > 0) {
     unsigned char* p = reinterpret_cast<unsigned char*>(&w);
 #pragma unroll
     for (int i = 0; i < 16; ++i)
-      if (at + i < bytes) p[i] = row[at + i];
+      if (i < left) p[i] = from[i];
   }
   return w;
 }
 
 template <bool kFp8, int MT, int NB, int W, int U>
-__global__ __launch_bounds__(64 * W) void few_rows_kernel(Operands o, Epilogue ep) {
-  __shared__ f32x4 sums[W][NB * MT][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int r = lane & 15, g = lane >> 4;
-  const int64_t n0 = (int64_t)blockIdx.x * 16 * NB;
+__global__ __launch_bounds__(64 * W) void few_rows_any_kernel(Operands o, Epilogue ep) {
+  __shared__ f32x4 sums[W][NB * MT][32];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool wanted = (lane >> 3 & 1) == lane >> 5;  // of the results
+  const int r = lane & 7, piece = 16 * (4 * (lane >> 3 & 1) + (lane >> 4));
+  const int64_t n0 = (int64_t)blockIdx.x * 8 * NB;
   const unsigned char* wrow[NB];
 #pragma unroll
-  for (int i = 0; i < NB; ++i) wrow[i] = o.b + std::min<int64_t>(n0 + 16 * i + r, o.n - 1) * o.b_pitch;
-  const int64_t bytes = o.c_bytes;
-  const int64_t steps = (bytes + kTileBytes - 1) / kTileBytes;
-  for (int64_t m0 = (int64_t)blockIdx.y * 16 * MT; m0 < o.m; m0 += (int64_t)gridDim.y * 16 * MT) {
+  for (int i = 0; i < NB; ++i) wrow[i] = o.b + std::min<int64_t>(n0 + 8 * i + r, o.n - 1) * o.b_pitch + piece;
+  const int bytes = o.c_bytes, whole = bytes / kTileBytes, steps = (bytes + kTileBytes - 1) / kTileBytes;
+  for (int64_t m0 = (int64_t)blockIdx.y * 8 * MT; m0 < o.m; m0 += (int64_t)gridDim.y * 8 * MT) {
     const unsigned char* xrow[MT];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) xrow[i] = o.a + std::min<int64_t>(m0 + 16 * i + r, o.m - 1) * o.a_pitch;
+    for (int i = 0; i < MT; ++i) xrow[i] = o.a + std::min<int64_t>(m0 + 8 * i + r, o.m - 1) * o.a_pitch + piece;
     f32x4 acc[NB][MT];
 #pragma unroll
     for (int i = 0; i < NB; ++i)
 #pragma unroll
       for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (int64_t s0 = wave; s0 < steps; s0 += W * U) {
-      dc::u32x4 wv[U][NB][2], xv[U][MT][2];
+    // U steps of this wave from step s on: the next U steps' loads are in flight while the products of these run. (Steps past
+    // the last whole one are zeros; the conditions are uniform.)
+    auto load = [&](dc::u32x4 (&wv)[U][NB], dc::u32x4 (&xv)[U][MT], int s) __attribute__((always_inline)) {
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int64_t at = (s0 + u * W) * kTileBytes + 16 * g;
+        const int64_t at = (int64_t)(s + u * W) * kTileBytes;
+        if (s + u * W < whole) {
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
+          for (int i = 0; i < NB; ++i) wv[u][i] = *reinterpret_cast<const dc::u32x4_at1*>(wrow[i] + at);
 #pragma unroll
-          for (int i = 0; i < NB; ++i) wv[u][i][p] = load_piece(wrow[i], at + 64 * p, bytes);
+          for (int i = 0; i < MT; ++i) xv[u][i] = *reinterpret_cast<const dc::u32x4_at1*>(xrow[i] + at);
+        } else {
 #pragma unroll
-          for (int i = 0; i < MT; ++i) xv[u][i][p] = load_piece(xrow[i], at + 64 * p, bytes);
+          for (int i = 0; i < NB; ++i) wv[u][i] = dc::u32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int i = 0; i < MT; ++i) xv[u][i] = dc::u32x4{0, 0, 0, 0};
         }
       }
+      __builtin_amdgcn_sched_barrier(0);  // (else the compiler saves registers by waiting for each pair)
+    };
+    auto add = [&](const dc::u32x4 (&wv)[NB], const dc::u32x4 (&xv)[MT]) __attribute__((always_inline)) {
 #pragma unroll
-      for (int u = 0; u < U; ++u)
+      for (int i = 0; i < NB; ++i)
 #pragma unroll
-        for (int i = 0; i < NB; ++i)
+        for (int j = 0; j < MT; ++j) {
+          const dc::u32x4 a = wv[i], b = xv[j];
+          if constexpr (kFp8) {
 #pragma unroll
-          for (int j = 0; j < MT; ++j) {
-            if constexpr (kFp8) {
-              const i32x8 a = __builtin_bit_cast(i32x8, __builtin_shufflevector(wv[u][i][0], wv[u][i][1], 0, 1, 2, 3, 4, 5, 6, 7));
-              const i32x8 b = __builtin_bit_cast(i32x8, __builtin_shufflevector(xv[u][j][0], xv[u][j][1], 0, 1, 2, 3, 4, 5, 6, 7));
-              acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[i][j], 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
-            } else {
-#pragma unroll
-              for (int p = 0; p < 2; ++p)
-                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, wv[u][i][p]),
-                                                                   __builtin_bit_cast(bf16x8, xv[u][j][p]), acc[i][j], 0, 0, 0);
+            for (int q = 0; q < 2; ++q) {
+              const dc::u32x2 ah = {a[2 * q], a[2 * q + 1]}, bh = {b[2 * q], b[2 * q + 1]};
+              acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_fp8_fp8(__builtin_bit_cast(long, ah), __builtin_bit_cast(long, bh),
+                                                                    acc[i][j], 0, 0, 0);
             }
+          } else {
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b),
+                                                               acc[i][j], 0, 0, 0);
           }
+        }
+    };
+    dc::u32x4 wa[U][NB], xa[U][MT], wb[U][NB], xb[U][MT];
+    load(wa, xa, wave);
+    for (int s = wave; s < whole; s += 2 * U * W) {
+      load(wb, xb, s + U * W);
+#pragma unroll
+      for (int u = 0; u < U; ++u) add(wa[u], xa[u]);
+      if (s + U * W >= whole) break;
+      load(wa, xa, s + 2 * U * W);
+#pragma unroll
+      for (int u = 0; u < U; ++u) add(wb[u], xb[u]);
+    }
+    if (steps > whole && whole % W == wave) {  // the last, ragged step
+      const int64_t at = (int64_t)whole * kTileBytes;
+#pragma unroll
+      for (int i = 0; i < NB; ++i) wa[0][i] = load_piece(wrow[i] + at, bytes - at - piece, bytes);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) xa[0][i] = load_piece(xrow[i] + at, bytes - at - piece, bytes);
+      add(wa[0], xa[0]);
     }
 #pragma unroll
     for (int i = 0; i < NB; ++i)
 #pragma unroll
-      for (int j = 0; j < MT; ++j) sums[wave][i * MT + j][lane] = acc[i][j];
+      for (int j = 0; j < MT; ++j)
+        if (wanted) sums[wave][i * MT + j][lane & 31] = acc[i][j];
     __syncthreads();
-    // acc[i][j][v]: output 16·i + 4·g + v of row 16·j + r of x
-    for (int t = threadIdx.x; t < NB * MT * 64; t += 64 * W) {
-      const int b = t >> 6, l = t & 63;
-      f32x4 v = sums[0][b][l];
+    // acc[i][j][v] of lane 16·g + c: row 4·g + v, column c. Output 8·i + 4·q + v of row 8·j + l of x: row 4·q + v, column l
+    // (the first halves: lane 16·q + l) and row 8 + 4·q + v, column 8 + l (lane 32 + 16·q + 8 + l).
+    for (int t = threadIdx.x; t < NB * MT * 16; t += 64 * W) {
+      const int b = t >> 4, l = t & 7, q = t >> 3 & 1;
+      f32x4 v = sums[0][b][16 * q + l] + sums[0][b][16 * q + 8 + l];
 #pragma unroll
-      for (int w = 1; w < W; ++w) v += sums[w][b][l];
-      const int64_t i = m0 + 16 * (b % MT) + (l & 15), j = n0 + 16 * (b / MT) + 4 * (l >> 4);
+      for (int w = 1; w < W; ++w) v += sums[w][b][16 * q + l] + sums[w][b][16 * q + 8 + l];
+      const int64_t i = m0 + 8 * (b % MT) + l, j = n0 + 8 * (b / MT) + 4 * q;
       float z[4] = {v.x, v.y, v.z, v.w};
-      if (i < o.m && j < o.n) finish(ep, i, j, o.n - j, z);
+      if (i < o.m && j < o.n) {
+        Columns<4> cols;
+        cols.read(ep, j, o.n);
+        cols.finish(ep, i, z);
+      }
     }
     __syncthreads();
+  }
+}
+
+template <int N>
+__device__ inline void wait_loads() {  // until at most N of the wave's loads are in flight
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
+template <bool kFp8, int XB, int NB, int W, int D>
+__global__ __launch_bounds__(64 * W) void few_rows_kernel(Operands o, Epilogue ep) {
+  constexpr int MT = (XB + 1) / 2, kStage = (2 * NB + XB) * 1024, kLoads = 2 * NB + XB;
+  static_assert((D - 1) * kLoads < 64 && W * D * kStage <= 160 * 1024 && W * NB * MT * 1024 <= W * D * kStage);
+  __shared__ __align__(16) unsigned char ring[W * D * kStage];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  unsigned char* own = ring + wave * D * kStage;
+  const int64_t n0 = (int64_t)blockIdx.x * 16 * NB, m0 = (int64_t)blockIdx.y * 8 * XB;
+  // load side: lane -> row lane / 8 of a block of 8, slot lane % 8, which holds the piece of the swizzle
+  const int piece = 16 * ((lane & 7) ^ (lane >> 4));  // of even blocks; of odd ones 64 bytes away
+  uint32_t woff[2 * NB], xoff[XB];
+#pragma unroll
+  for (int i = 0; i < 2 * NB; ++i) {
+    const int row = 8 * i + (lane >> 3);
+    woff[i] = n0 + row < o.n ? (uint32_t)row * (uint32_t)o.b_pitch + (uint32_t)(piece ^ (64 * (i & 1))) : kPast;
+  }
+#pragma unroll
+  for (int i = 0; i < XB; ++i) {
+    const int row = 8 * i + (lane >> 3);
+    xoff[i] = m0 + row < o.m ? (uint32_t)row * (uint32_t)o.a_pitch + (uint32_t)(piece ^ (64 * (i & 1))) : kPast;
+  }
+  const unsigned char *wbase = o.b + n0 * o.b_pitch, *xbase = o.a + m0 * o.a_pitch;
+  const int steps = (o.c_bytes + kTileBytes - 1) / kTileBytes;
+  auto load = [&](unsigned char* stage, int s) __attribute__((always_inline)) {
+    const int64_t at = (int64_t)s * kTileBytes;
+    const int left = o.c_bytes - s * kTileBytes;
+#pragma unroll
+    for (int i = 0; i < 2 * NB; ++i)
+      load_block(wbase + at, stage + i * 1024, (piece ^ (64 * (i & 1))) < left ? woff[i] : kPast, 0);
+#pragma unroll
+    for (int i = 0; i < XB; ++i)
+      load_block(xbase + at, stage + (2 * NB + i) * 1024, (piece ^ (64 * (i & 1))) < left ? xoff[i] : kPast, 0);
+  };
+  // read side: pieces g and 4 + g of row lane % 16 (of an x block that is not there: another's, to no effect)
+  const int r = lane & 15, g = lane >> 4, swz = (r >> 1) & 7;
+  const uint32_t lo = 16u * (uint32_t)(g ^ swz), hi = 16u * (uint32_t)((4 + g) ^ swz);
+  f32x4 acc[NB][MT];
+#pragma unroll
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  auto read = [&](const unsigned char* stage, int row, dc::u32x4 (&v)[2]) __attribute__((always_inline)) {
+    v[0] = *reinterpret_cast<const dc::u32x4*>(stage + row * kTileBytes + lo);
+    v[1] = *reinterpret_cast<const dc::u32x4*>(stage + row * kTileBytes + hi);
+  };
+  auto add = [&](const unsigned char* stage) __attribute__((always_inline)) {
+    dc::u32x4 wv[NB][2], xv[MT][2];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) read(stage, 16 * i + r, wv[i]);
+#pragma unroll
+    for (int j = 0; j < MT; ++j) read(stage + 2 * NB * 1024, 16 * j + (16 * j + 8 < 8 * XB ? r : r & 7), xv[j]);
+#pragma unroll
+    for (int i = 0; i < NB; ++i)
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        if constexpr (kFp8) {
+          const i32x8 a = __builtin_bit_cast(i32x8, __builtin_shufflevector(wv[i][0], wv[i][1], 0, 1, 2, 3, 4, 5, 6, 7));
+          const i32x8 b = __builtin_bit_cast(i32x8, __builtin_shufflevector(xv[j][0], xv[j][1], 0, 1, 2, 3, 4, 5, 6, 7));
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, acc[i][j], 0, 0, 0, 0x7f7f7f7f, 0, 0x7f7f7f7f);
+        } else {
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            const dc::u32x4 a = wv[i][p], b = xv[j][p];
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b),
+                                                               acc[i][j], 0, 0, 0);
+          }
+        }
+      }
+  };
+  const int count = steps > wave ? (steps - wave + W - 1) / W : 0;  // this wave's steps: wave, wave + W, ...
+#pragma unroll
+  for (int d = 0; d < D - 1; ++d)
+    if (d < count) load(own + d * kStage, wave + d * W);
+  int slot = 0;
+  for (int t = 0; t < count; ++t) {
+    const int next = t + D - 1;
+    if (next < count) {
+      // (its stage was read in the turn before; those reads have returned, as their products have been issued)
+      load(own + (slot == 0 ? D - 1 : slot - 1) * kStage, wave + next * W);
+      wait_loads<(D - 1) * kLoads>();
+    } else {
+      wait_loads<0>();
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    add(own + slot * kStage);
+    __builtin_amdgcn_sched_barrier(0);
+    slot = slot + 1 == D ? 0 : slot + 1;
+  }
+  __syncthreads();
+  f32x4* sums = reinterpret_cast<f32x4*>(ring);
+#pragma unroll
+  for (int i = 0; i < NB; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) sums[(wave * NB * MT + i * MT + j) * 64 + lane] = acc[i][j];
+  __syncthreads();
+  // acc[i][j][v] of lane 16·g + r: output 16·i + 4·g + v of row 16·j + r of x
+  for (int t = threadIdx.x; t < NB * MT * 64; t += 64 * W) {
+    const int b = t >> 6, l = t & 63;
+    f32x4 v = sums[b * 64 + l];
+#pragma unroll
+    for (int w = 1; w < W; ++w) v += sums[(w * NB * MT + b) * 64 + l];
+    const int64_t i = m0 + 16 * (b % MT) + (l & 15), j = n0 + 16 * (b / MT) + 4 * (l >> 4);
+    float z[4] = {v.x, v.y, v.z, v.w};
+    if (16 * (b % MT) + (l & 15) < 8 * XB && i < o.m && j < o.n) {
+      Columns<4> cols;
+      cols.read(ep, j, o.n);
+      cols.finish(ep, i, z);
+    }
   }
 }
 
@@ -542,9 +758,8 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeArgs a) {
       dc::load_some(a.dy + i * a.dy_stride + j, a.n - j, dz[q]);
       if (a.act != DC_ACT_NONE) {
         float z[8];
-        dc::load_some(a.pre + i * a.pre_stride + j, a.n - j, z);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) dz[q][e] *= j + e < a.n ? act_slope(a.act, z[e]) : 0.0f;
+        dc::load_some(a.pre + i * a.pre_stride + j, a.n - j, z);  // (zeros past the last: their dz stays zero)
+        apply_slope(a.act, z, dz[q]);
       }
     } else {
 #pragma unroll
@@ -590,7 +805,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
   const int64_t pieces = a.to_pitch / 16, total = a.rows * pieces, step = (int64_t)gridDim.x * 256;
   for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += step) {
     const int64_t row = t / pieces, at = 16 * (t - row * pieces);
-    *reinterpret_cast<dc::u32x4*>(a.to + row * a.to_pitch + at) = load_piece(a.from + row * a.from_pitch, at, a.bytes);
+    *reinterpret_cast<dc::u32x4*>(a.to + row * a.to_pitch + at) = load_piece(a.from + row * a.from_pitch + at, a.bytes - at, a.bytes);
   }
 }
 
@@ -618,16 +833,37 @@ int32_t product(dc_hip_ctx* ctx, const Operands& o, const Epilogue& ep) {
   return DC_ERR_INVALID_ARGUMENT;
 }
 
-template <bool kFp8, int MT>
+// NB blocks of 16 outputs and XB blocks of 8 rows of x, W waves, and as many stages as fit in `kLds` KiB of LDS.
+template <bool kFp8, int XB, int NB, int W, int kLds>
 int32_t launch_few_rows(dc_hip_ctx* ctx, const Operands& o, const Epilogue& ep) {
-  const unsigned gy = (unsigned)std::min((o.m + 16 * MT - 1) / (16 * MT), 32768);
-  few_rows_kernel<kFp8, MT, 1, 8, 4><<<dim3((unsigned)((o.n + 15) / 16), gy), 512, 0, ctx->stream>>>(o, ep);
+  constexpr int kFit = kLds / W / (2 * NB + XB), kStages = kFit < 4 ? kFit : 4;
+  const dim3 grid((unsigned)((o.n + 16 * NB - 1) / (16 * NB)), (unsigned)((o.m + 8 * XB - 1) / (8 * XB)));
+  few_rows_kernel<kFp8, XB, NB, W, kStages><<<grid, 64 * W, 0, ctx->stream>>>(o, ep);
   return dc::last_launch_status();
 }
 
 template <bool kFp8>
 int32_t few_rows(dc_hip_ctx* ctx, const Operands& o, const Epilogue& ep) {
-  return o.m <= 16 ? launch_few_rows<kFp8, 1>(ctx, o, ep) : launch_few_rows<kFp8, 2>(ctx, o, ep);
+  const bool wide = dc::linear_wide_few_rows(o.m, o.n, std::max(1, ctx->cu_count));
+  if (o.m <= 8) return wide ? launch_few_rows<kFp8, 1, 4, 4, 80>(ctx, o, ep) : launch_few_rows<kFp8, 1, 1, 8, 80>(ctx, o, ep);
+  if (o.m <= 16) return wide ? launch_few_rows<kFp8, 2, 4, 4, 80>(ctx, o, ep) : launch_few_rows<kFp8, 2, 1, 8, 80>(ctx, o, ep);
+  if (o.m <= 24) return wide ? launch_few_rows<kFp8, 3, 4, 4, 160>(ctx, o, ep) : launch_few_rows<kFp8, 3, 1, 8, 80>(ctx, o, ep);
+  if (o.m <= 32) return wide ? launch_few_rows<kFp8, 4, 4, 4, 160>(ctx, o, ep) : launch_few_rows<kFp8, 4, 1, 4, 80>(ctx, o, ep);
+  return launch_few_rows<kFp8, 8, 1, 4, 80>(ctx, o, ep);
+}
+
+template <bool kFp8, int MT>
+int32_t launch_few_rows_any(dc_hip_ctx* ctx, const Operands& o, const Epilogue& ep) {
+  const dim3 grid((unsigned)((o.n + 15) / 16), (unsigned)std::min((o.m + 8 * MT - 1) / (8 * MT), 32768));
+  few_rows_any_kernel<kFp8, MT, 2, 8, 2><<<grid, 512, 0, ctx->stream>>>(o, ep);
+  return dc::last_launch_status();
+}
+
+template <bool kFp8>
+int32_t few_rows_any(dc_hip_ctx* ctx, const Operands& o, const Epilogue& ep) {
+  if (o.m <= 8) return launch_few_rows_any<kFp8, 1>(ctx, o, ep);
+  if (o.m <= 16) return launch_few_rows_any<kFp8, 2>(ctx, o, ep);
+  return launch_few_rows_any<kFp8, 4>(ctx, o, ep);
 }
 
 bool aligned_to(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
@@ -722,7 +958,12 @@ DC_HIP_API int32_t dc_hip_linear(dc_hip_ctx* ctx, const dc_linear* args) {
              (int32_t)p.n,
              (int32_t)(p.k * size),
              0};
-  if (p.k == 0 || dc::linear_few_rows(p.m, p.n, p.k * size)) return fp8 ? few_rows<true>(ctx, o, ep) : few_rows<false>(ctx, o, ep);
+  const bool whole = aligned_to(o.a, 16) && aligned_to(o.b, 16) && o.a_pitch % 16 == 0 && o.b_pitch % 16 == 0 &&
+                     o.c_bytes % 16 == 0 && std::max(o.a_pitch, o.b_pitch) <= dc::kLinearPitch;
+  if (p.k == 0 || (!whole && p.m <= dc::kLinearFewRows))
+    return fp8 ? few_rows_any<true>(ctx, o, ep) : few_rows_any<false>(ctx, o, ep);
+  if (whole && dc::linear_few_rows(p.m, p.n, std::max(1, ctx->cu_count)))
+    return fp8 ? few_rows<true>(ctx, o, ep) : few_rows<false>(ctx, o, ep);
   Scratch scratch;
   Rows x{o.a, o.a_pitch, p.m, o.c_bytes}, w{o.b, o.b_pitch, p.n, o.c_bytes};
   x.plan(scratch);
@@ -755,7 +996,7 @@ DC_HIP_API int32_t dc_hip_linear_backward(dc_hip_ctx* ctx, const dc_linear_grad*
   DC_CTX_ENTER(ctx);
   if (!dx && !dw && !dbias) return DC_OK;
   // dz runs along n in dx and along m in dw: a copy of each, padded to whole 16-byte pieces, in scratch; dy itself where
-  // it serves as dz. (Without rows, or columns, of dz the sums are empty: few_rows with no steps writes the zeros.)
+  // it serves as dz. (Without rows, or columns, of dz the sums are empty: few_rows_any with no steps writes the zeros.)
   Scratch scratch;
   Rows dz{reinterpret_cast<const unsigned char*>(p.dy), 2 * p.dy_stride, p.m, 2 * p.n};
   Rows w{reinterpret_cast<const unsigned char*>(p.w), 2 * p.w_stride, p.n, 2 * p.k};
@@ -792,7 +1033,7 @@ DC_HIP_API int32_t dc_hip_linear_backward(dc_hip_ctx* ctx, const dc_linear_grad*
   // One gradient: the product of `rows` (m of them, along c) and `b` (c rows of k), or zeros where c is empty.
   auto gradient = [&](const unsigned char* rows, int64_t pitch, int64_t m, int64_t c, Rows& b, void* out, int64_t stride) -> int32_t {
     ep.y = out, ep.y_stride = stride;
-    if (!inputs) return few_rows<false>(ctx, Operands{nullptr, nullptr, 0, 0, (int32_t)m, (int32_t)p.k, 0, 0, 0}, ep);
+    if (!inputs) return few_rows_any<false>(ctx, Operands{nullptr, nullptr, 0, 0, (int32_t)m, (int32_t)p.k, 0, 0, 0}, ep);
     DC_RETURN_IF(b.lay_out(ctx));
     const Operands o{rows, b.p, pitch, b.pitch, (int32_t)m, (int32_t)p.k, (int32_t)(2 * c), (int32_t)c, (int32_t)padded(p.k, 8)};
     return product<false, true>(ctx, o, ep);

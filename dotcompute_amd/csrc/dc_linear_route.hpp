@@ -29,7 +29,15 @@ inline LinearTile linear_tile(int64_t m, int64_t n, int64_t c_bytes, int64_t a_p
   return LinearTile::k64x4;
 }
 
-// Few rows of x.
-inline bool linear_few_rows(int64_t m, int64_t n, int64_t c_bytes) { return m <= 32; }
+// Few rows of x: kernels that read w once for up to 64 of them. Measured in bf16, us (few rows / tiles): 32×16384×2048 13.3 /
+// 13.8, 64×4096×4096 10.5 / 17.9, 64×6144×4096 17.1 / 18.3, 64×8192×4096 19.7 / 18.7; so up to kLinearFewRows always, and
+// beyond where every 64 rows and 16 outputs still find a CU of their own.
+constexpr int64_t kLinearFewRows = 32;
+inline bool linear_few_rows(int64_t m, int64_t n, int64_t cus) {
+  return m <= kLinearFewRows || (m + 63) / 64 * ((n + 15) / 16) <= cus;
+}
+// 64 outputs a workgroup instead of 16, where that leaves two for a CU (8×16384×2048: 11.7 us, 12.6; 8×8192×4096: 11.7, 12.2;
+// 8×4096×4096: 9.6, 7.4).
+inline bool linear_wide_few_rows(int64_t m, int64_t n, int64_t cus) { return m <= kLinearFewRows && (n + 15) / 16 > 2 * cus; }
 
 }  // namespace dc
