@@ -126,6 +126,33 @@ struct Epilogue {
   int32_t y_f32;
 };
 
+// E neighbouring bf16 values of which `left` exist (zeros for the others).
+template <int E>
+__device__ inline void load_bf16(const bf16* q, int64_t left, float (&v)[E]) {
+  if constexpr (E == 8) {
+    dc::load_some(q, left, v);
+  } else if (left >= 4) {
+    const dc::u32x2_at2 w = *reinterpret_cast<const dc::u32x2_at2*>(q);
+    v[0] = dc::bf16_lo(w.x), v[1] = dc::bf16_hi(w.x), v[2] = dc::bf16_lo(w.y), v[3] = dc::bf16_hi(w.y);
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = e < left ? dc::to_f32(q[e]) : 0.0f;
+  }
+}
+template <int E>
+__device__ inline void store_bf16(bf16* q, int64_t left, const float (&v)[E]) {
+  if constexpr (E == 8) {
+    dc::store_some(q, left, v);
+  } else if (left >= 4) {
+    const dc::u32x2 w = {dc::pack_bf16(v[0], v[1]), dc::pack_bf16(v[2], v[3])};
+    *reinterpret_cast<dc::u32x2_at2*>(q) = w;
+  } else {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+      if (e < left) q[e] = dc::from_f32<bf16>(v[e]);
+  }
+}
+
 // What the results of E neighbouring columns j.. share, whatever their row: read once.
 template <int E>
 struct Columns {
@@ -137,52 +164,41 @@ struct Columns {
 #pragma unroll
     for (int e = 0; e < E; ++e) bias[e] = scale[e] = 0.0f;
     if (left <= 0) return;
-    if (p.bias) load(p.bias + j, bias);
+    if (p.bias) load_bf16(p.bias + j, left, bias);
     if (p.b_scales)
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (e < left) scale[e] = p.b_scales[j + e];
+      for (int e = 0; e < E; e += 4)
+        dc::load_some(p.b_scales + j + e, left - e, *reinterpret_cast<float (*)[4]>(scale + e));
   }
-  __device__ inline void load(const bf16* q, float (&v)[E]) const {
-    if constexpr (E == 8) {
-      dc::load_some(q, left, v);
-    } else {
-#pragma unroll
-      for (int e = 0; e < E; ++e) v[e] = e < left ? dc::to_f32(q[e]) : 0.0f;
-    }
+};
+
+// What E neighbouring results of one row take from memory, and the results from that and their sums.
+template <int E>
+struct Results {
+  float residual[E], scale;
+
+  __device__ inline void read(const Epilogue& p, const Columns<E>& c, int64_t i) {
+    if (p.residual) load_bf16(p.residual + i * p.residual_stride + c.j, c.left, residual);
+    if (p.a_scales) scale = p.a_scales[i];
   }
-  __device__ inline void store(bf16* q, const float (&v)[E]) const {
-    if constexpr (E == 8) {
-      dc::store_some(q, left, v);
-    } else {
+  __device__ inline void finish(const Epilogue& p, const Columns<E>& c, int64_t i, float (&z)[E]) const {
+    if (p.a_scales)
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (e < left) q[e] = dc::from_f32<bf16>(v[e]);
-    }
-  }
-  // The results of row i (left > 0) from their sums.
-  __device__ inline void finish(const Epilogue& p, int64_t i, float (&z)[E]) const {
-    float r[E];
-    if (p.residual) load(p.residual + i * p.residual_stride + j, r);
-    if (p.a_scales) {
-      const float s = p.a_scales[i];
-#pragma unroll
-      for (int e = 0; e < E; ++e) z[e] = z[e] * s * scale[e];
-    }
+      for (int e = 0; e < E; ++e) z[e] = z[e] * scale * c.scale[e];
     if (p.bias)
 #pragma unroll
-      for (int e = 0; e < E; ++e) z[e] += bias[e];
-    if (p.pre) store(p.pre + i * p.pre_stride + j, z);
+      for (int e = 0; e < E; ++e) z[e] += c.bias[e];
+    if (p.pre) store_bf16(p.pre + i * p.pre_stride + c.j, c.left, z);
     activate(p.act, z);
     if (p.residual)
 #pragma unroll
-      for (int e = 0; e < E; ++e) z[e] += r[e];
+      for (int e = 0; e < E; ++e) z[e] += residual[e];
     if (p.y_f32) {
-      float* q = static_cast<float*>(p.y) + i * p.y_stride + j;
+      float* q = static_cast<float*>(p.y) + i * p.y_stride + c.j;
 #pragma unroll
-      for (int e = 0; e < E; e += 4) dc::store_some(q + e, left - e, *reinterpret_cast<const float (*)[4]>(z + e));
+      for (int e = 0; e < E; e += 4) dc::store_some(q + e, c.left - e, *reinterpret_cast<const float (*)[4]>(z + e));
     } else {
-      store(static_cast<bf16*>(p.y) + i * p.y_stride + j, z);
+      store_bf16(static_cast<bf16*>(p.y) + i * p.y_stride + c.j, c.left, z);
     }
   }
 };
@@ -475,7 +491,11 @@ __global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void pro
       float z[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) z[e] = own[row * kPitch + 8 * (lane % kLanes) + e];
-      if (i < o.m && cols.left > 0) cols.finish(ep, i, z);
+      if (i < o.m && cols.left > 0) {
+        Results<8> out;
+        out.read(ep, cols, i);
+        out.finish(ep, cols, i, z);
+      }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   }
@@ -607,8 +627,10 @@ __global__ __launch_bounds__(64 * W) void few_rows_any_kernel(Operands o, Epilog
       float z[4] = {v.x, v.y, v.z, v.w};
       if (i < o.m && j < o.n) {
         Columns<4> cols;
+        Results<4> out;
         cols.read(ep, j, o.n);
-        cols.finish(ep, i, z);
+        out.read(ep, cols, i);
+        out.finish(ep, cols, i, z);
       }
     }
     __syncthreads();
@@ -693,6 +715,22 @@ __global__ __launch_bounds__(64 * W) void few_rows_kernel(Operands o, Epilogue e
 #pragma unroll
   for (int d = 0; d < D - 1; ++d)
     if (d < count) load(own + d * kStage, wave + d * W);
+  // The results this thread will finish, and what they take from memory, asked for before the loop: acc[i][j][v] of lane
+  // 16·g + r is output 16·i + 4·g + v of row 16·j + r of x.
+  constexpr int kItems = (NB * MT + W - 1) / W;
+  Columns<4> cols[kItems];
+  Results<4> out[kItems];
+  bool mine[kItems];
+#pragma unroll
+  for (int q = 0; q < kItems; ++q) {
+    const int t = threadIdx.x + q * 64 * W, b = t >> 6, l = t & 63;
+    const int64_t i = m0 + 16 * (b % MT) + (l & 15), j = n0 + 16 * (b / MT) + 4 * (l >> 4);
+    mine[q] = b < NB * MT && 16 * (b % MT) + (l & 15) < 8 * XB && i < o.m && j < o.n;
+    if (mine[q]) {
+      cols[q].read(ep, j, o.n);
+      out[q].read(ep, cols[q], i);
+    }
+  }
   int slot = 0;
   for (int t = 0; t < count; ++t) {
     const int next = t + D - 1;
@@ -715,19 +753,15 @@ __global__ __launch_bounds__(64 * W) void few_rows_kernel(Operands o, Epilogue e
 #pragma unroll
     for (int j = 0; j < MT; ++j) sums[(wave * NB * MT + i * MT + j) * 64 + lane] = acc[i][j];
   __syncthreads();
-  // acc[i][j][v] of lane 16·g + r: output 16·i + 4·g + v of row 16·j + r of x
-  for (int t = threadIdx.x; t < NB * MT * 64; t += 64 * W) {
-    const int b = t >> 6, l = t & 63;
+#pragma unroll
+  for (int q = 0; q < kItems; ++q) {
+    const int t = threadIdx.x + q * 64 * W, b = t >> 6, l = t & 63;
+    if (!mine[q]) continue;
     f32x4 v = sums[b * 64 + l];
 #pragma unroll
     for (int w = 1; w < W; ++w) v += sums[(w * NB * MT + b) * 64 + l];
-    const int64_t i = m0 + 16 * (b % MT) + (l & 15), j = n0 + 16 * (b / MT) + 4 * (l >> 4);
     float z[4] = {v.x, v.y, v.z, v.w};
-    if (16 * (b % MT) + (l & 15) < 8 * XB && i < o.m && j < o.n) {
-      Columns<4> cols;
-      cols.read(ep, j, o.n);
-      cols.finish(ep, i, z);
-    }
+    out[q].finish(ep, cols[q], m0 + 16 * (b % MT) + (l & 15), z);
   }
 }
 

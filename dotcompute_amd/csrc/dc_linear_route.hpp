@@ -16,6 +16,17 @@ static_assert(64 * kLinearPitch < kLinearRange && 2 * kLinearWidth <= kLinearPit
 // Tiles, square, and groups of waves that take the steps along c in turn.
 enum class LinearTile { k256, k128, k128x2, k64, k64x2, k64x4 };
 
+// By rounds of the tiles over the CUs, as dc_gemm_route.hpp's rule, measured again (results m x n, sums over c; us for
+// tiles of 256 / 128 / 128x2 / 64 / 64x2 / 64x4, w by rows of c where it says so):
+//   bf16: 4096x4096x1024 34.5 / 39.7 / 51.7 / 52.4 / 59.4 / 94;  5120x5120x1024 58.8 / 64.4 / 89 / 80 / 92 / 145
+//   2000x3000x1000 30.5 / 21.6 / 29.4 / 27.8 / 28.7 / 41;  2048^3 44 / 25.3 / 22.7 / 25.6 / 27.4 / 38
+//   1537x2049x1024 27.4 / 15.2 / 14.8 / 13.8 / 17.7 / 26;  1024^3 26 / 11.7 / 11.7 / 6.9 / 6.4 / 6.5
+//   rows c: 8192x2048x8192 208 / 244 / 278 / 358 / 377 / 529;  4096x1024x4096 86 / 47 / 39.9 / 49 / 52 / 73
+//   2000x1000x3000 71 / 41 / 36 / 29.1 / 27.9 / 37;  3000x1000x2000 51 / 30.2 / 26.5 / 27.9 / 33.8 / 38
+//   512x512x4096 83 / 34 / 29.8 / 32.6 / 24.1 / 20.2;  64x2048x8192 155 / 80 / 60 / 61 / 43.8 / 34.9
+//   e4m3: 4096^3 58 / 66 / 92 / 96 / 110 / 157;  2048^3 31.6 / 15.2 / 14.6 / 13.8 / 16 / 24;  1537x2049x1024 22 / 11.2 / 11.1 / 9.0 / 11 / 19
+// (Three and four stages of LDS instead of two, and tiles of 128x64, 256x128 and 128x256, were no faster on any of these but
+// e4m3 2048^3, 13.5.)
 inline LinearTile linear_tile(int64_t m, int64_t n, int64_t c_bytes, int64_t a_pitch, int64_t b_pitch, bool rows_c, int64_t cus) {
   auto tiles = [&](int64_t t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
   auto fits = [&](int64_t t) { return t * a_pitch < kLinearRange && (rows_c || t * b_pitch < kLinearRange); };
@@ -23,7 +34,7 @@ inline LinearTile linear_tile(int64_t m, int64_t n, int64_t c_bytes, int64_t a_p
   const bool brief = (k <= 64 && (t256 > cus || 4 * t256 <= 3 * cus)) || (k <= 128 && t256 > 2 * cus);
   if (fits(256) && 2 * t256 > cus && (t256 <= cus || 10 * t256 > 13 * cus) && !brief) return LinearTile::k256;
   if (fits(128) && t128 > cus && !brief) return LinearTile::k128;
-  if (fits(128) && 4 * t128 > 3 * cus && k > 128) return LinearTile::k128x2;
+  if (fits(128) && 4 * t128 > 3 * cus && k >= 1536) return LinearTile::k128x2;
   if (t64 > 2 * cus || k < 512) return LinearTile::k64;
   if (2 * t64 > cus || k < 2048) return LinearTile::k64x2;
   return LinearTile::k64x4;

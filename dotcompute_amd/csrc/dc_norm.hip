@@ -2,8 +2,8 @@
 //
 // Forward, a row at a time: h = x + r, s = 1 / sqrt(mean(h^2) + eps), y = h w s. Memory-bound: 8 bytes an element in
 // bf16 (x, r in; h, y out), 7 with y in 8 bits. A row stays in registers between its one read and its write, so nothing
-// is read twice: W waves hold it in C 16-byte chunks a lane (W = 1: no barrier, the wave sums by DPP; W = 4 or 16:
-// the waves' sums meet in LDS). Rows too long for 16 waves are read again from the caches for each pass (C = 0).
+// is read twice: as many waves as it needs hold it in C 16-byte chunks a lane, and their sums meet in LDS. Rows too long
+// for 16 waves are read again from the caches for each pass.
 //
 // Backward: g = dy w, dx = s (g - h s mean(g h s)) + dh, dw = sum over rows of dy h s. Also one read of each operand; a
 // workgroup walks over rows and keeps its part of dw in registers, the parts are added in a fixed order by a
@@ -27,55 +27,189 @@ struct NormArgs {
   float eps;
 };
 
-// Sum (or unsigned maximum) over the W waves that share a row, in every lane. `scratch`: W words, which nobody writes
-// again before the caller's next barrier.
-template <int W>
-__device__ inline float row_sum(float v, float* scratch, int wave) {
-  v = dc::wave_sum_f32(v);
-  if constexpr (W > 1) {
-    if ((threadIdx.x & 63) == 0) scratch[wave] = v;
-    __syncthreads();
-    v = scratch[0];
-#pragma unroll
-    for (int i = 1; i < W; ++i) v += scratch[i];
+// Waves that share a row, at most: each leaves its sum in a word of LDS, and every wave adds the words in order, those of
+// waves that are not there too (zeros from the start of the kernel): few wide reads and no loop.
+constexpr int kWaves = 16;
+
+__device__ inline float add_words(const float* scratch, int waves) {
+  const dc::f32x4* q = reinterpret_cast<const dc::f32x4*>(scratch);
+  const dc::f32x4 a = q[0], b = q[1];
+  float v = ((a.x + a.y) + (a.z + a.w)) + ((b.x + b.y) + (b.z + b.w));
+  if (waves > 8) {
+    const dc::f32x4 c = q[2], d = q[3];
+    v += ((c.x + c.y) + (c.z + c.w)) + ((d.x + d.y) + (d.z + d.w));
   }
   return v;
 }
-template <int W>
-__device__ inline uint32_t row_max(uint32_t v, float* scratch, int wave) {
+
+// Sum (or unsigned maximum) over the `waves` waves that share a row, in every lane. `scratch`: nobody writes it again
+// before the caller's next barrier.
+__device__ inline float row_sum(float v, float* scratch, int wave, int waves) {
+  v = dc::wave_sum_f32(v);
+  if (waves > 1) {
+    if ((threadIdx.x & 63) == 0) scratch[wave] = v;
+    __syncthreads();
+    v = add_words(scratch, waves);
+  }
+  return v;
+}
+__device__ inline uint32_t row_max(uint32_t v, float* scratch, int wave, int waves) {
   v = dc::wave_max_u32(v);
-  if constexpr (W > 1) {
+  if (waves > 1) {
     uint32_t* s = reinterpret_cast<uint32_t*>(scratch);
     if ((threadIdx.x & 63) == 0) s[wave] = v;
     __syncthreads();
-    v = s[0];
-#pragma unroll
-    for (int i = 1; i < W; ++i) v = max(v, s[i]);
+    const dc::u32x4* q = reinterpret_cast<const dc::u32x4*>(scratch);
+    const dc::u32x4 a = q[0], b = q[1], c = q[2], d = q[3];
+    v = max(max(max(max(a.x, a.y), max(a.z, a.w)), max(max(b.x, b.y), max(b.z, b.w))),
+            max(max(max(c.x, c.y), max(c.z, c.w)), max(max(d.x, d.y), max(d.z, d.w))));
   }
   return v;
 }
+// Zeros in `sets` sets of words, before their first use.
+__device__ inline void clear_words(float (*scratch)[kWaves], int sets, int waves) {
+  if (waves > 1) {
+    if ((int)threadIdx.x < sets * kWaves) scratch[0][threadIdx.x] = 0.0f;
+    __syncthreads();
+  }
+}
 
-// Workgroups of W waves take a row each, or, for W = 1, of four waves with a row each.
-template <int W>
-constexpr int kNormThreads = W == 1 ? 256 : 64 * W;
-template <int W>
-constexpr int kNormRows = W == 1 ? 4 : 1;
+// The chunks c_i = ((i waves + wave) 64 + lane) E, i < C, of a row of `cols` elements, as they lie in memory, zeros past its
+// end. No branch stands between the loads, so that all of them are in flight at once: a chunk that reaches past the end is
+// cut out of the row's last 16 bytes, one beyond it loads those too, to no effect.
+template <typename T, int C>
+struct Row {
+  static constexpr int E = kElems<T>;
+  int64_t cols;
+  int waves, wave, lane;
+  __device__ inline int64_t at(int i) const { return (int64_t)((i * waves + wave) * 64 + lane) * E; }
+  __device__ inline void load(const T* p, dc::u32x4 (&raw)[C]) const {
+    if (cols >= E) {
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        const int64_t c = at(i);
+        raw[i] = dc::load_raw(p + (c < cols - E ? c : cols - E));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        float v[E];
+        dc::load_some(p, i == 0 && wave == 0 && lane == 0 ? cols : 0, v);
+        raw[i] = dc::u32x4{0, 0, 0, 0};
+        if constexpr (E == 4) raw[i] = __builtin_bit_cast(dc::u32x4, dc::f32x4{v[0], v[1], v[2], v[3]});
+        else
+#pragma unroll
+          for (int e = 0; e < 4; ++e) raw[i][e] = dc::pack_bf16(v[2 * e], v[2 * e + 1]);
+      }
+    }
+  }
+  // What load() left of the row's last 16 bytes in the chunks at and past its end.
+  __device__ inline void cut(dc::u32x4 (&raw)[C]) const {
+    if (cols < E) return;
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      if ((int64_t)((i * waves + wave) * 64 + 64) * E > cols) {  // (uniform)
+        const int64_t past = at(i) - (cols - E);
+        if (past > 0) raw[i] = dc::shift_down(raw[i], past * (int64_t)sizeof(T));
+      }
+  }
+};
 
-// y = x itself (a conversion to 8 bits): no norm, no weight.
-template <typename T, typename Y, int W, int C, bool kNorm>
-__global__ __launch_bounds__(kNormThreads<W>) void rms_norm_kernel(NormArgs a) {
+// A row a workgroup; or, where a wave holds a row, one for each of its four waves.
+// kNorm false: y = x itself (a conversion to 8 bits), no norm, no weight.
+template <typename T, typename Y, int C, bool kNorm>
+__global__ __launch_bounds__(C == 4 ? 1024 : 512) void rms_norm_kernel(NormArgs a, int waves) {
   constexpr int E = kElems<T>;
   constexpr bool kFp8 = sizeof(Y) == 1;
-  __shared__ float scratch[3][W == 1 ? 1 : W];
-  const int lane = threadIdx.x & 63, wave = W == 1 ? 0 : threadIdx.x >> 6;
+  __shared__ __align__(16) float scratch[2][kWaves];
+  const int lane = threadIdx.x & 63, group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = waves == 1 ? 0 : group;
   const int64_t cols = a.cols;
+  const Row<T, C> R{cols, waves, wave, lane};
+  clear_words(scratch, 2, waves);
+  const int per = waves == 1 ? 4 : 1;
+  const int64_t step = (int64_t)gridDim.x * per;
+  for (int64_t row = (int64_t)blockIdx.x * per + (waves == 1 ? group : 0); row < a.rows; row += step) {
+    T* sum = a.sum ? static_cast<T*>(a.sum) + row * a.sum_stride : nullptr;
+    Y* y = static_cast<Y*>(a.y) + row * a.y_stride;
+    dc::u32x4 xr[C], rr[C], wr[C];
+    R.load(static_cast<const T*>(a.x) + row * a.x_stride, xr);
+    if (a.residual) R.load(static_cast<const T*>(a.residual) + row * a.residual_stride, rr);
+    if constexpr (kNorm) R.load(static_cast<const T*>(a.weight), wr);
+    R.cut(xr);
+    if (a.residual) R.cut(rr);
+    float h[C][E];
+#pragma unroll
+    for (int i = 0; i < C; ++i) dc::unpack(xr[i], h[i]);
+    if (a.residual)
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        float u[E];
+        dc::unpack(rr[i], u);
+#pragma unroll
+        for (int e = 0; e < E; ++e) h[i][e] += u[e];
+      }
+    if constexpr (kNorm) {
+      float ss = 0.0f;
+#pragma unroll
+      for (int i = 0; i < C; ++i)
+#pragma unroll
+        for (int e = 0; e < E; ++e) ss += h[i][e] * h[i][e];
+      if (sum)
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+          const int64_t c = R.at(i);
+          if (c < cols) dc::store_some(sum + c, cols - c, h[i]);
+        }
+      const float s = 1.0f / sqrtf(row_sum(ss, scratch[0], wave, waves) / (float)a.cols + a.eps);
+      R.cut(wr);
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        float w[E];
+        dc::unpack(wr[i], w);
+#pragma unroll
+        for (int e = 0; e < E; ++e) h[i][e] = h[i][e] * s * w[e];
+      }
+    }
+    if constexpr (kFp8) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < C; ++i)
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (R.at(i) + e < cols) top = max(top, dc::magnitude(h[i][e]));
+      const float t = __builtin_bit_cast(float, row_max(top, scratch[1], wave, waves));
+      const float factor = dc::fp8_factor(t);
+      if (lane == 0 && wave == 0) a.scales[row] = t / dc::kFp8Top;
+#pragma unroll
+      for (int i = 0; i < C; ++i)
+#pragma unroll
+        for (int e = 0; e < E; ++e) h[i][e] *= factor;
+    }
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const int64_t c = R.at(i);
+      if (c < cols) dc::store_some(y + c, cols - c, h[i]);
+    }
+    if (waves > 1) __syncthreads();  // the next row writes the scratch words again
+  }
+}
+
+// The same for rows that 16 waves cannot hold: read again, from the caches where they last, for each pass.
+template <typename T, typename Y, bool kNorm>
+__global__ __launch_bounds__(1024) void rms_norm_long_kernel(NormArgs a) {
+  constexpr int E = kElems<T>;
+  constexpr bool kFp8 = sizeof(Y) == 1;
+  constexpr int64_t kStep = 64 * kWaves * E;
+  __shared__ __align__(16) float scratch[2][kWaves];
+  const int wave = threadIdx.x >> 6;
+  const int64_t cols = a.cols, first = (int64_t)threadIdx.x * E;
   const T* weight = static_cast<const T*>(a.weight);
-  const int64_t step = (int64_t)gridDim.x * kNormRows<W>;
-  for (int64_t row = (int64_t)blockIdx.x * kNormRows<W> + (W == 1 ? threadIdx.x >> 6 : 0); row < a.rows; row += step) {
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* x = static_cast<const T*>(a.x) + row * a.x_stride;
     const T* r = a.residual ? static_cast<const T*>(a.residual) + row * a.residual_stride : nullptr;
     T* sum = a.sum ? static_cast<T*>(a.sum) + row * a.sum_stride : nullptr;
     Y* y = static_cast<Y*>(a.y) + row * a.y_stride;
+    float s = 1.0f;
     auto read = [&](int64_t c, float (&v)[E]) __attribute__((always_inline)) {
       dc::load_some(x + c, cols - c, v);
       if (r) {
@@ -85,106 +219,50 @@ __global__ __launch_bounds__(kNormThreads<W>) void rms_norm_kernel(NormArgs a) {
         for (int e = 0; e < E; ++e) v[e] += u[e];
       }
     };
-    if constexpr (C > 0) {
-      float h[C][E];
+    auto normed = [&](int64_t c, float (&v)[E]) __attribute__((always_inline)) {
+      if constexpr (kNorm) {
+        float w[E];
+        dc::load_some(weight + c, cols - c, w);
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] = v[e] * s * w[e];
+      }
+    };
+    if constexpr (kNorm) {
       float ss = 0.0f;
-#pragma unroll
-      for (int i = 0; i < C; ++i) {
-        const int64_t c = (int64_t)((i * W + wave) * 64 + lane) * E;
-        if (c < cols) {
-          read(c, h[i]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < E; ++e) h[i][e] = 0.0f;
-        }
-      }
-      if constexpr (kNorm) {
-#pragma unroll
-        for (int i = 0; i < C; ++i)
-#pragma unroll
-          for (int e = 0; e < E; ++e) ss += h[i][e] * h[i][e];
-        const float s = 1.0f / sqrtf(row_sum<W>(ss, scratch[0], wave) / (float)a.cols + a.eps);
-#pragma unroll
-        for (int i = 0; i < C; ++i) {
-          const int64_t c = (int64_t)((i * W + wave) * 64 + lane) * E;
-          if (c < cols) {
-            if (sum) dc::store_some(sum + c, cols - c, h[i]);
-            float w[E];
-            dc::load_some(weight + c, cols - c, w);
-#pragma unroll
-            for (int e = 0; e < E; ++e) h[i][e] = h[i][e] * s * w[e];
-          }
-        }
-      }
-      float factor = 1.0f;
-      if constexpr (kFp8) {
-        uint32_t top = 0;
-#pragma unroll
-        for (int i = 0; i < C; ++i)
-#pragma unroll
-          for (int e = 0; e < E; ++e) top = max(top, dc::magnitude(h[i][e]));
-        const float t = __builtin_bit_cast(float, row_max<W>(top, scratch[1], wave));
-        factor = dc::fp8_factor(t);
-        if (lane == 0 && wave == 0) a.scales[row] = t / dc::kFp8Top;
-      }
-#pragma unroll
-      for (int i = 0; i < C; ++i) {
-        const int64_t c = (int64_t)((i * W + wave) * 64 + lane) * E;
-        if (c < cols) {
-          if constexpr (kFp8)
-#pragma unroll
-            for (int e = 0; e < E; ++e) h[i][e] *= factor;
-          dc::store_some(y + c, cols - c, h[i]);
-        }
-      }
-    } else {
-      const int64_t first = (int64_t)threadIdx.x * E;
-      constexpr int64_t kStep = 64 * W * E;
-      float s = 1.0f;
-      if constexpr (kNorm) {
-        float ss = 0.0f;
-        for (int64_t c = first; c < cols; c += kStep) {
-          float v[E];
-          read(c, v);
-#pragma unroll
-          for (int e = 0; e < E; ++e) ss += v[e] * v[e];
-        }
-        s = 1.0f / sqrtf(row_sum<W>(ss, scratch[0], wave) / (float)a.cols + a.eps);
-      }
-      auto normed = [&](int64_t c, float (&v)[E]) __attribute__((always_inline)) {
-        if constexpr (kNorm) {
-          float w[E];
-          dc::load_some(weight + c, cols - c, w);
-#pragma unroll
-          for (int e = 0; e < E; ++e) v[e] = v[e] * s * w[e];
-        }
-      };
-      float factor = 1.0f;
-      if constexpr (kFp8) {
-        uint32_t top = 0;
-        for (int64_t c = first; c < cols; c += kStep) {
-          float v[E];
-          read(c, v);
-          normed(c, v);
-#pragma unroll
-          for (int e = 0; e < E; ++e) top = max(top, dc::magnitude(v[e]));
-        }
-        const float t = __builtin_bit_cast(float, row_max<W>(top, scratch[1], wave));
-        factor = dc::fp8_factor(t);
-        if (lane == 0 && wave == 0) a.scales[row] = t / dc::kFp8Top;
-      }
-      for (int64_t c = first; c < cols; c += kStep) {  // (a lane writes only what it alone has read)
+      for (int64_t c = first; c < cols; c += kStep) {
         float v[E];
         read(c, v);
-        if (sum) dc::store_some(sum + c, cols - c, v);
-        normed(c, v);
-        if constexpr (kFp8)
 #pragma unroll
-          for (int e = 0; e < E; ++e) v[e] *= factor;
-        dc::store_some(y + c, cols - c, v);
+        for (int e = 0; e < E; ++e) ss += v[e] * v[e];
       }
+      s = 1.0f / sqrtf(row_sum(ss, scratch[0], wave, kWaves) / (float)a.cols + a.eps);
     }
-    if constexpr (W > 1) __syncthreads();  // the next row writes the scratch words again
+    float factor = 1.0f;
+    if constexpr (kFp8) {
+      uint32_t top = 0;
+      for (int64_t c = first; c < cols; c += kStep) {
+        float v[E];
+        read(c, v);
+        normed(c, v);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (c + e < cols) top = max(top, dc::magnitude(v[e]));
+      }
+      const float t = __builtin_bit_cast(float, row_max(top, scratch[1], wave, kWaves));
+      factor = dc::fp8_factor(t);
+      if (threadIdx.x == 0) a.scales[row] = t / dc::kFp8Top;
+    }
+    for (int64_t c = first; c < cols; c += kStep) {  // (a lane writes only what it alone has read)
+      float v[E];
+      read(c, v);
+      if (sum) dc::store_some(sum + c, cols - c, v);
+      normed(c, v);
+      if constexpr (kFp8)
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] *= factor;
+      dc::store_some(y + c, cols - c, v);
+    }
+    __syncthreads();
   }
 }
 
@@ -197,89 +275,150 @@ struct NormGradArgs {
   float eps;
 };
 
-template <typename T, int W, int C>
-__global__ __launch_bounds__(64 * W) void rms_norm_grad_kernel(NormGradArgs a) {
+// The sums of h^2 and g h over the waves that share a row; two sets of words in turn, so that one barrier a row does: a
+// wave writes a set again only past the barrier of the row between.
+__device__ inline void row_sums(float& hh, float& gh, float (*scratch)[kWaves], int lane, int wave, int waves) {
+  hh = dc::wave_sum_f32(hh);
+  gh = dc::wave_sum_f32(gh);
+  if (waves > 1) {
+    if (lane == 0) {
+      scratch[0][wave] = hh;
+      scratch[1][wave] = gh;
+    }
+    __syncthreads();
+    hh = add_words(scratch[0], waves);
+    gh = add_words(scratch[1], waves);
+  }
+}
+
+// A workgroup's rows are blockIdx.x, + gridDim.x, ...; the next row's operands are asked for before this one's sums.
+// Workgroups a CU: as many waves as hide a row's latency, and no more, as each workgroup leaves a row of dweight's parts to be
+// added. Measured, us for 1 / 2 / 3 / 4 workgroups of a row's waves a CU: 8192×4096 51.4 / 55.5 (8 waves; 5.2 TB/s), 8191×2050 45 /
+// 34.9 / 32.8 (5 waves; 4.1 TB/s); 16384×512 with 8 of one wave 19.1, with 16 23.2.
+template <typename T, int C>
+__global__ __launch_bounds__(512) void rms_norm_grad_kernel(NormGradArgs a, int waves) {
   constexpr int E = kElems<T>;
-  constexpr int kC = C > 0 ? C : 1;
-  __shared__ float scratch[4][W];
+  __shared__ __align__(16) float scratch[4][kWaves];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t cols = a.cols;
+  const Row<T, C> R{cols, waves, wave, lane};
+  clear_words(scratch, 4, waves);
+  float acc[C][E];
+#pragma unroll
+  for (int i = 0; i < C; ++i)
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[i][e] = 0.0f;
+  dc::u32x4 wr[C], hr[C], dr[C], ur[C];
+  auto load = [&](int64_t row) __attribute__((always_inline)) {
+    R.load(static_cast<const T*>(a.h) + row * a.h_stride, hr);
+    R.load(static_cast<const T*>(a.dy) + row * a.dy_stride, dr);
+    if (a.dh && a.dx) R.load(static_cast<const T*>(a.dh) + row * a.dh_stride, ur);
+  };
+  R.load(static_cast<const T*>(a.weight), wr);
+  load(blockIdx.x);
+  R.cut(wr);
+  int flip = 0;
+  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    R.cut(hr);
+    R.cut(dr);
+    float hv[C][E], dv[C][E];
+    dc::u32x4 uv[C];
+    float hh = 0.0f, gh = 0.0f;
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      float wv[E];
+      dc::unpack(hr[i], hv[i]);
+      dc::unpack(dr[i], dv[i]);
+      dc::unpack(wr[i], wv);
+      uv[i] = ur[i];
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        hh += hv[i][e] * hv[i][e];
+        gh += dv[i][e] * wv[e] * hv[i][e];
+      }
+    }
+    if (row + gridDim.x < a.rows) load(row + gridDim.x);
+    row_sums(hh, gh, scratch + 2 * flip, lane, wave, waves);
+    flip ^= 1;
+    const float s = 1.0f / sqrtf(hh / (float)a.cols + a.eps);
+    const float mean = s * s * (gh / (float)a.cols);  // mean(g h s) s
+    if (a.dx) {
+      T* dx = static_cast<T*>(a.dx) + row * a.dx_stride;
+      if (a.dh) R.cut(uv);
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        float o[E], wv[E];
+        dc::unpack(wr[i], wv);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = s * (dv[i][e] * wv[e] - hv[i][e] * mean);
+        if (a.dh) {
+          float u[E];
+          dc::unpack(uv[i], u);
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[e] += u[e];
+        }
+        const int64_t c = R.at(i);
+        if (c < cols) dc::store_some(dx + c, cols - c, o);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[i][e] += dv[i][e] * (hv[i][e] * s);
+  }
+  if (a.parts) {
+    float* part = a.parts + (int64_t)blockIdx.x * cols;
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+      const int64_t c = R.at(i);
+#pragma unroll
+      for (int e = 0; e < E; e += 4)
+        if (c + e < cols) dc::store_some(part + c + e, cols - c - e, *reinterpret_cast<const float (*)[4]>(acc[i] + e));
+    }
+  }
+}
+
+// The same for rows that 16 waves cannot hold: read twice, and dweight's part kept in memory.
+template <typename T>
+__global__ __launch_bounds__(1024) void rms_norm_grad_long_kernel(NormGradArgs a) {
+  constexpr int E = kElems<T>;
+  __shared__ __align__(16) float scratch[4][kWaves];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int64_t cols = a.cols;
   const T* weight = static_cast<const T*>(a.weight);
   float* part = a.parts ? a.parts + (int64_t)blockIdx.x * cols : nullptr;
-  float acc[kC][E];
-#pragma unroll
-  for (int i = 0; i < kC; ++i)
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[i][e] = 0.0f;
-  if (C == 0 && part)
-    for (int64_t c = threadIdx.x; c < cols; c += 64 * W) part[c] = 0.0f;
-  if constexpr (C == 0) __syncthreads();
   int flip = 0;
+  bool fresh = true;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* dy = static_cast<const T*>(a.dy) + row * a.dy_stride;
     const T* h = static_cast<const T*>(a.h) + row * a.h_stride;
     const T* dh = a.dh ? static_cast<const T*>(a.dh) + row * a.dh_stride : nullptr;
     T* dx = a.dx ? static_cast<T*>(a.dx) + row * a.dx_stride : nullptr;
     float hh = 0.0f, gh = 0.0f;
-    float hv[kC][E], dv[kC][E], wv[kC][E];
-    auto read = [&](int64_t c, float (&hr)[E], float (&dr)[E], float (&wr)[E]) __attribute__((always_inline)) {
-      dc::load_some(h + c, cols - c, hr);
-      dc::load_some(dy + c, cols - c, dr);
-      dc::load_some(weight + c, cols - c, wr);
+    float hv[E], dv[E], wv[E];
+    auto read = [&](int64_t c) __attribute__((always_inline)) {
+      dc::load_some(h + c, cols - c, hv);
+      dc::load_some(dy + c, cols - c, dv);
+      dc::load_some(weight + c, cols - c, wv);
     };
-    auto add = [&](const float (&hr)[E], const float (&dr)[E], const float (&wr)[E]) __attribute__((always_inline)) {
+    for (int64_t c = (int64_t)threadIdx.x * E; c < cols; c += 64 * kWaves * E) {
+      read(c);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        hh += hr[e] * hr[e];
-        gh += dr[e] * wr[e] * hr[e];
-      }
-    };
-    if constexpr (C > 0) {
-#pragma unroll
-      for (int i = 0; i < C; ++i) {
-        const int64_t c = (int64_t)((i * W + wave) * 64 + lane) * E;
-        if (c < cols) {
-          read(c, hv[i], dv[i], wv[i]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < E; ++e) hv[i][e] = dv[i][e] = wv[i][e] = 0.0f;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < C; ++i) add(hv[i], dv[i], wv[i]);
-    } else {
-      for (int64_t c = (int64_t)threadIdx.x * E; c < cols; c += 64 * W * E) {
-        read(c, hv[0], dv[0], wv[0]);
-        add(hv[0], dv[0], wv[0]);
+        hh += hv[e] * hv[e];
+        gh += dv[e] * wv[e] * hv[e];
       }
     }
-    // (two sets of words in turn: a wave writes a set again only past the barrier of the row between)
-    hh = dc::wave_sum_f32(hh);
-    gh = dc::wave_sum_f32(gh);
-    if constexpr (W > 1) {
-      float *s0 = scratch[2 * flip], *s1 = scratch[2 * flip + 1];
-      flip ^= 1;
-      if (lane == 0) {
-        s0[wave] = hh;
-        s1[wave] = gh;
-      }
-      __syncthreads();
-      hh = s0[0];
-      gh = s1[0];
-#pragma unroll
-      for (int i = 1; i < W; ++i) {
-        hh += s0[i];
-        gh += s1[i];
-      }
-    }
+    row_sums(hh, gh, scratch + 2 * flip, lane, wave, kWaves);
+    flip ^= 1;
     const float s = 1.0f / sqrtf(hh / (float)a.cols + a.eps);
-    const float mean = s * s * (gh / (float)a.cols);  // mean(g h s) s
-    auto finish = [&](int64_t c, const float (&hr)[E], const float (&dr)[E], const float (&wr)[E], float (&ac)[E])
-        __attribute__((always_inline)) {
+    const float mean = s * s * (gh / (float)a.cols);
+    for (int64_t c = (int64_t)threadIdx.x * E; c < cols; c += 64 * kWaves * E) {
+      read(c);
       if (dx) {
         float o[E], u[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = s * (dr[e] * wr[e] - hr[e] * mean);
+        for (int e = 0; e < E; ++e) o[e] = s * (dv[e] * wv[e] - hv[e] * mean);
         if (dh) {
           dc::load_some(dh + c, cols - c, u);
 #pragma unroll
@@ -287,99 +426,74 @@ __global__ __launch_bounds__(64 * W) void rms_norm_grad_kernel(NormGradArgs a) {
         }
         dc::store_some(dx + c, cols - c, o);
       }
+      if (part)  // (a thread's own columns)
 #pragma unroll
-      for (int e = 0; e < E; ++e) ac[e] += dr[e] * (hr[e] * s);
-    };
-    if constexpr (C > 0) {
-#pragma unroll
-      for (int i = 0; i < C; ++i) {
-        const int64_t c = (int64_t)((i * W + wave) * 64 + lane) * E;
-        if (c < cols) finish(c, hv[i], dv[i], wv[i], acc[i]);
-      }
-    } else {
-      for (int64_t c = (int64_t)threadIdx.x * E; c < cols; c += 64 * W * E) {
-        read(c, hv[0], dv[0], wv[0]);
-        float ac[E];
-#pragma unroll
-        for (int e = 0; e < E; ++e) ac[e] = part && c + e < cols ? part[c + e] : 0.0f;
-        finish(c, hv[0], dv[0], wv[0], ac);
-        if (part)
-#pragma unroll
-          for (int e = 0; e < E; ++e)
-            if (c + e < cols) part[c + e] = ac[e];
-      }
+        for (int e = 0; e < E; ++e)
+          if (c + e < cols) part[c + e] = (fresh ? 0.0f : part[c + e]) + dv[e] * (hv[e] * s);
     }
+    fresh = false;
   }
-  if (C > 0 && part)
-#pragma unroll
-    for (int i = 0; i < C; ++i) {
-      const int64_t c = (int64_t)((i * W + wave) * 64 + lane) * E;
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (c + e < cols) part[c + e] = acc[i][e];
-    }
 }
 
-// out[c] = parts[0][c] + ... + parts[count - 1][c]: 64 columns a workgroup, 16 threads a column that each add every
-// 16th part, then those 16 sums in order.
-constexpr int kSumGroups = 16;
-__global__ __launch_bounds__(64 * kSumGroups) void column_sums_kernel(const float* __restrict__ parts, float* __restrict__ out,
-                                                                      int64_t count, int64_t cols) {
-  __shared__ float sums[kSumGroups][64];
-  const int lane = threadIdx.x & 63, g = threadIdx.x >> 6;
-  const int64_t c = (int64_t)blockIdx.x * 64 + lane;
+// out[c] = parts[0][c] + ... + parts[count - 1][c]: 16 columns a workgroup, 64 threads a column that each add every 64th
+// part, then those sums in order (16 columns: enough workgroups for rows of a few thousand).
+constexpr int kSumGroups = 64, kSumCols = 16;
+__global__ __launch_bounds__(kSumCols * kSumGroups) void column_sums_kernel(const float* __restrict__ parts, float* __restrict__ out,
+                                                                            int64_t count, int64_t cols) {
+  __shared__ float sums[kSumGroups][kSumCols + 1];
+  const int lane = threadIdx.x % kSumCols, g = threadIdx.x / kSumCols;
+  const int64_t c = (int64_t)blockIdx.x * kSumCols + lane;
   float v = 0.0f;
   if (c < cols)
 #pragma unroll 8
     for (int64_t i = g; i < count; i += kSumGroups) v += parts[i * cols + c];
   sums[g][lane] = v;
   __syncthreads();
-  if (g == 0 && c < cols) {
+  if (g < 4) {  // (a wave: 16 columns, 4 quarters of the sums)
+    v = sums[16 * g][lane];
 #pragma unroll
-    for (int i = 1; i < kSumGroups; ++i) v += sums[i][lane];
-    out[c] = v;
+    for (int i = 1; i < 16; ++i) v += sums[16 * g + i][lane];
+    sums[16 * g][lane] = v;
   }
+  __syncthreads();
+  if (g == 0 && c < cols) out[c] = ((v + sums[16][lane]) + sums[32][lane]) + sums[48][lane];
 }
 
-constexpr int64_t kMaxCols = int64_t(1) << 27;
+constexpr int64_t kMaxCols = int64_t(1) << 25;
 constexpr int64_t kMaxGrid = 1 << 20;  // rows beyond are walked over by the same workgroups
 
-template <typename T, typename Y, int W, int C, bool kNorm>
-int32_t launch_norm(dc_hip_ctx* ctx, const NormArgs& a) {
-  const int64_t groups = (a.rows + kNormRows<W> - 1) / kNormRows<W>;
-  rms_norm_kernel<T, Y, W, C, kNorm>
-      <<<(unsigned)std::min<int64_t>(groups, kMaxGrid), kNormThreads<W>, 0, ctx->stream>>>(a);
+// Waves that hold a row of `chunks` 16-byte chunks, C to a lane.
+int waves_for(int64_t chunks, int c) { return (int)((chunks + 64 * c - 1) / (64 * c)); }
+
+template <typename T, typename Y, int C, bool kNorm>
+int32_t launch_norm(dc_hip_ctx* ctx, const NormArgs& a, int64_t chunks) {
+  const int waves = waves_for(chunks, C);
+  const int64_t groups = waves == 1 ? (a.rows + 3) / 4 : a.rows;
+  rms_norm_kernel<T, Y, C, kNorm>
+      <<<(unsigned)std::min(groups, kMaxGrid), waves == 1 ? 256 : 64 * waves, 0, ctx->stream>>>(a, waves);
   return dc::last_launch_status();
 }
 
+// Measured, us, bf16 with a residual (TB/s): 16384×4096 with C = 2 and 4 waves 89.8 (5.98), C = 1 and 8 waves 88.8, a wave a row
+// (C = 8) 100; to 8 bits 81.8 (5.75), 92.1, 106, as its second sum over the row is another barrier; 8191×2050, whose
+// rows lie at 4-byte boundaries, 27.2 (4.95), C = 1 29.8; 16384×512 11.4 (5.9).
 template <typename T, typename Y, bool kNorm>
 int32_t norm_by_shape(dc_hip_ctx* ctx, const NormArgs& a) {
   const int64_t chunks = (a.cols + kElems<T> - 1) / kElems<T>;
-  if (chunks <= 512 && a.rows >= 8 * (int64_t)ctx->cu_count) {
-    if (chunks <= 64) return launch_norm<T, Y, 1, 1, kNorm>(ctx, a);
-    if (chunks <= 128) return launch_norm<T, Y, 1, 2, kNorm>(ctx, a);
-    if (chunks <= 256) return launch_norm<T, Y, 1, 4, kNorm>(ctx, a);
-    return launch_norm<T, Y, 1, 8, kNorm>(ctx, a);
-  }
-  if (chunks <= 256) return launch_norm<T, Y, 4, 1, kNorm>(ctx, a);
-  if (chunks <= 512) return launch_norm<T, Y, 4, 2, kNorm>(ctx, a);
-  if (chunks <= 1024) return launch_norm<T, Y, 4, 4, kNorm>(ctx, a);
-  if (chunks <= 2048) return launch_norm<T, Y, 4, 8, kNorm>(ctx, a);
-  if (chunks <= 4096) return launch_norm<T, Y, 16, 4, kNorm>(ctx, a);
-  if (chunks <= 8192) return launch_norm<T, Y, 16, 8, kNorm>(ctx, a);
-  return launch_norm<T, Y, 16, 0, kNorm>(ctx, a);
+  if (chunks <= 256) return launch_norm<T, Y, 1, kNorm>(ctx, a, chunks);
+  if (chunks <= 1024) return launch_norm<T, Y, 2, kNorm>(ctx, a, chunks);
+  if (chunks <= 64 * 4 * kWaves) return launch_norm<T, Y, 4, kNorm>(ctx, a, chunks);
+  rms_norm_long_kernel<T, Y, kNorm><<<(unsigned)std::min(a.rows, kMaxGrid), 64 * kWaves, 0, ctx->stream>>>(a);
+  return dc::last_launch_status();
 }
 
 template <typename T>
-int32_t norm_grad_by_shape(dc_hip_ctx* ctx, const NormGradArgs& a, int64_t grid) {
-  const int64_t chunks = (a.cols + kElems<T> - 1) / kElems<T>;
+int32_t norm_grad_by_shape(dc_hip_ctx* ctx, const NormGradArgs& a, int64_t grid, int c, int waves) {
   const unsigned g = (unsigned)grid;
-  if (chunks <= 64) rms_norm_grad_kernel<T, 1, 1><<<g, 64, 0, ctx->stream>>>(a);
-  else if (chunks <= 256) rms_norm_grad_kernel<T, 4, 1><<<g, 256, 0, ctx->stream>>>(a);
-  else if (chunks <= 512) rms_norm_grad_kernel<T, 4, 2><<<g, 256, 0, ctx->stream>>>(a);
-  else if (chunks <= 1024) rms_norm_grad_kernel<T, 4, 4><<<g, 256, 0, ctx->stream>>>(a);
-  else if (chunks <= 4096) rms_norm_grad_kernel<T, 16, 4><<<g, 1024, 0, ctx->stream>>>(a);
-  else rms_norm_grad_kernel<T, 16, 0><<<g, 1024, 0, ctx->stream>>>(a);
+  if (c == 1) rms_norm_grad_kernel<T, 1><<<g, 64 * waves, 0, ctx->stream>>>(a, waves);
+  else if (c == 2) rms_norm_grad_kernel<T, 2><<<g, 64 * waves, 0, ctx->stream>>>(a, waves);
+  else if (c == 4) rms_norm_grad_kernel<T, 4><<<g, 64 * waves, 0, ctx->stream>>>(a, waves);
+  else rms_norm_grad_long_kernel<T><<<g, 64 * kWaves, 0, ctx->stream>>>(a);
   return dc::last_launch_status();
 }
 
@@ -403,8 +517,8 @@ int32_t check_shape(int64_t rows, int64_t cols) {
 namespace dc {
 
 int32_t launch_column_sums(dc_hip_ctx* ctx, const float* parts, float* out, int64_t count, int64_t cols) {
-  // (1024 work items for 64 columns, at most kMaxCols of them: within the 2^32 of a launch)
-  column_sums_kernel<<<(unsigned)((cols + 63) / 64), 64 * kSumGroups, 0, ctx->stream>>>(parts, out, count, cols);
+  // (1024 work items for 16 columns, at most kMaxCols of them: within the 2^32 of a launch)
+  column_sums_kernel<<<(unsigned)((cols + kSumCols - 1) / kSumCols), kSumCols * kSumGroups, 0, ctx->stream>>>(parts, out, count, cols);
   return last_launch_status();
 }
 
@@ -454,7 +568,10 @@ DC_HIP_API int32_t dc_hip_rms_norm_backward(dc_hip_ctx* ctx, const dc_rms_norm_g
   DC_CTX_ENTER(ctx);
   if (p.cols == 0 || (!p.dx && !p.dweight)) return DC_OK;
   if (p.rows == 0) return p.dweight ? dc::zero_async(ctx, p.dweight, (size_t)p.cols * sizeof(float)) : DC_OK;
-  const int64_t grid = std::min<int64_t>(p.rows, 4 * (int64_t)std::max(1, ctx->cu_count));
+  const int64_t elems = 16 / size_of(p.dtype), chunks = (p.cols + elems - 1) / elems;
+  const int c = chunks <= 512 ? 1 : chunks <= 1024 ? 2 : chunks <= 2048 ? 4 : 0, waves = c ? waves_for(chunks, c) : kWaves;
+  const int per_cu = waves <= 2 ? 8 / waves : std::max(1, 15 / waves);
+  const int64_t grid = std::min<int64_t>(p.rows, per_cu * (int64_t)std::max(1, ctx->cu_count));
   float* parts = nullptr;
   if (p.dweight) {
     DC_RETURN_IF(dc::ensure_partials(ctx, (size_t)(grid * p.cols) * sizeof(float)));
@@ -462,7 +579,7 @@ DC_HIP_API int32_t dc_hip_rms_norm_backward(dc_hip_ctx* ctx, const dc_rms_norm_g
   }
   const NormGradArgs a{p.dy,   p.h,         p.weight,   p.dh,        p.dx,        parts,
                        p.rows, p.dy_stride, p.h_stride, p.dh_stride, p.dx_stride, (int32_t)p.cols, p.eps};
-  DC_RETURN_IF(p.dtype == DC_DTYPE_F32 ? norm_grad_by_shape<float>(ctx, a, grid) : norm_grad_by_shape<bf16>(ctx, a, grid));
+  DC_RETURN_IF(p.dtype == DC_DTYPE_F32 ? norm_grad_by_shape<float>(ctx, a, grid, c, waves) : norm_grad_by_shape<bf16>(ctx, a, grid, c, waves));
   return p.dweight ? dc::launch_column_sums(ctx, parts, p.dweight, grid, p.cols) : DC_OK;
 }
 

@@ -92,6 +92,24 @@ __device__ inline void store_chunk(uint8_t* p, const float (&v)[4]) {
 template <>
 __device__ inline uint8_t from_f32<uint8_t>(float v) { return (uint8_t)pack_fp8(v, v, v, v); }
 
+// Chunks as they lie in memory, and their values.
+template <typename T>
+__device__ inline u32x4 load_raw(const T* p) {
+  if constexpr (sizeof(T) == 4) return __builtin_bit_cast(u32x4, *reinterpret_cast<const f32x4_at4*>(p));
+  else return *reinterpret_cast<const u32x4_at2*>(p);
+}
+__device__ inline void unpack(u32x4 w, float (&v)[8]) { unpack_bf16(w, v); }
+__device__ inline void unpack(u32x4 w, float (&v)[4]) {
+  const f32x4 f = __builtin_bit_cast(f32x4, w);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = f[i];
+}
+// w moved down by `bytes`, zeros from above (none left from 16 on).
+__device__ inline u32x4 shift_down(u32x4 w, int64_t bytes) {
+  const unsigned __int128 all = __builtin_bit_cast(unsigned __int128, w);
+  return __builtin_bit_cast(u32x4, bytes < 16 ? all >> (8 * (int)bytes) : (unsigned __int128)0);
+}
+
 // The chunk at p of which `left` elements exist (the rest reads as zero, and is not stored).
 template <typename T, int E>
 __device__ inline void load_some(const T* p, int64_t left, float (&v)[E]) {
