@@ -124,6 +124,7 @@ struct Epilogue {
   int64_t residual_stride, pre_stride, y_stride;
   int32_t act;
   int32_t y_f32;
+  int64_t part_stride;  // elements of y from one part of c to the next, where c is split (0: it is not)
 };
 
 // E neighbouring bf16 values of which `left` exist (zeros for the others).
@@ -194,7 +195,7 @@ struct Results {
 #pragma unroll
       for (int e = 0; e < E; ++e) z[e] += residual[e];
     if (p.y_f32) {
-      float* q = static_cast<float*>(p.y) + i * p.y_stride + c.j;
+      float* q = static_cast<float*>(p.y) + i * p.y_stride + c.j + (int64_t)blockIdx.z * p.part_stride;
 #pragma unroll
       for (int e = 0; e < E; e += 4) dc::store_some(q + e, c.left - e, *reinterpret_cast<const float (*)[4]>(z + e));
     } else {
@@ -254,7 +255,7 @@ __device__ inline void load_block(const unsigned char* base, unsigned char* to, 
 
 template <int TM, int TN, int WM, int WN, int KS, bool kFp8, bool kRowsC>
 __global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void product_kernel(Operands o, Epilogue ep,
-                                                                                           int tiles_m, int tiles_n) {
+                                                                                           int tiles_m, int tiles_n, int turns) {
   static_assert(!(kFp8 && kRowsC), "8-bit operands run along c");
   constexpr int kWaves = WM * WN;
   constexpr int kMT = TM / WM / 32, kNT = TN / WN / 32;
@@ -270,7 +271,9 @@ __global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void pro
   const int wm = wave / WN, wn = wave % WN;
   const int r = lane & 31, h = lane >> 5;
   const int tiles_c = (o.c_bytes + kTileBytes - 1) / kTileBytes;
-  const int kt_count = (tiles_c + KS - 1) / KS;  // of a group
+  // Tiles along c of a group: `turns` of them from kt_first on, fewer in the last of the parts that c is split into
+  const int kt_first = (int)blockIdx.z * turns;
+  const int kt_count = min((tiles_c + KS - 1) / KS - kt_first, turns);
 
   // ---- load side. Rows along c: lane -> row lane / 8 of a block, slot lane % 8, which holds the piece of the swizzle.
   const int lrow = lane >> 3;
@@ -295,7 +298,7 @@ __global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void pro
   const unsigned char* bbase = kRowsC ? o.b + (int64_t)n0 * 2 : o.b + (int64_t)n0 * o.b_pitch;
   auto load_tile = [&](auto BUF, int KT) __attribute__((always_inline)) {
     constexpr int kBuf = decltype(BUF)::value;
-    const int t = KT * KS + group;
+    const int t = (kt_first + KT) * KS + group;
     const int at = t * kTileBytes;  // bytes into A's rows (past the last: every load is past the range)
     const int left = o.c_bytes - at;
 #pragma unroll
@@ -829,42 +832,111 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeArgs a) {
   }
 }
 
+// The results from the sums over `count` parts of c: a lane takes eight neighbouring columns, and adds the parts in order.
+struct JoinArgs {
+  const float* parts;  // [count][m][pitch]
+  int64_t m, n, pitch;
+  int32_t count;
+};
+__global__ __launch_bounds__(256) void join_kernel(JoinArgs a, Epilogue ep) {
+  const int64_t across = (a.n + 7) / 8, total = a.m * across, step = (int64_t)gridDim.x * 256;
+  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += step) {
+    const int64_t i = t / across, j = 8 * (t - i * across);
+    Columns<8> cols;
+    Results<8> out;
+    cols.read(ep, j, a.n);
+    out.read(ep, cols, i);
+    const f32x4* q = reinterpret_cast<const f32x4*>(a.parts + i * a.pitch + j);
+    f32x4 lo = q[0], hi = q[1];
+#pragma unroll 4
+    for (int32_t c = 1; c < a.count; ++c) {
+      const f32x4* r = reinterpret_cast<const f32x4*>(a.parts + (c * a.m + i) * a.pitch + j);
+      lo += r[0];
+      hi += r[1];
+    }
+    float z[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+    out.finish(ep, cols, i, z);
+  }
+}
+
 // Rows of `bytes` bytes at any alignment to rows of `to_pitch` (a multiple of 16), padded with zeros.
-struct PackArgs {
+struct PackJob {
   const unsigned char* from;
   unsigned char* to;
   int64_t rows, bytes, from_pitch, to_pitch;
 };
-__global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
+struct PackArgs {
+  PackJob job[2];
+};
+__global__ __launch_bounds__(256) void pack_kernel(PackArgs args) {
+  const PackJob& a = args.job[blockIdx.y];
   const int64_t pieces = a.to_pitch / 16, total = a.rows * pieces, step = (int64_t)gridDim.x * 256;
   for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += step) {
     const int64_t row = t / pieces, at = 16 * (t - row * pieces);
-    *reinterpret_cast<dc::u32x4*>(a.to + row * a.to_pitch + at) = load_piece(a.from + row * a.from_pitch + at, a.bytes - at, a.bytes);
+    *reinterpret_cast<dc::u32x4*>(a.to + row * a.to_pitch + at) =
+        load_piece(a.from + row * a.from_pitch + at, a.bytes - at, a.bytes);
   }
 }
 
 // ---- host ------------------------------------------------------------------------------------------------
+int64_t padded(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
+
+// Scratch of one call: pieces of ctx->partials, each at a multiple of 256 bytes.
+struct Scratch {
+  size_t bytes = 0;
+  size_t take(int64_t n) {
+    const size_t at = bytes;
+    bytes += (size_t)padded(n, 256);
+    return at;
+  }
+};
+
+// A product's tile and the parts that c is split into, whose sums stand in scratch.
+struct ProductPlan {
+  dc::LinearTile tile;
+  dc::LinearSplit split;
+  size_t at = 0;
+  ProductPlan(dc_hip_ctx* ctx, Scratch& s, int64_t m, int64_t n, int64_t c_bytes, int64_t a_pitch, int64_t b_pitch, bool rows_c) {
+    const int64_t cus = std::max(1, ctx->cu_count);
+    tile = dc::linear_tile(m, n, c_bytes, a_pitch, b_pitch, rows_c, cus);
+    split = dc::linear_split(tile, m, n, c_bytes, cus);
+    if (split.parts > 1) at = s.take(split.parts * m * padded(n, 8) * (int64_t)sizeof(float));
+  }
+};
+
 template <int TM, int TN, int WM, int WN, int KS, bool kFp8, bool kRowsC>
-int32_t launch_product(dc_hip_ctx* ctx, const Operands& o, const Epilogue& ep) {
+int32_t launch_product(dc_hip_ctx* ctx, const Operands& o, const Epilogue& ep, const dc::LinearSplit& split) {
   constexpr int kThr = 64 * WM * WN * KS;
   const int tiles_m = (o.m + TM - 1) / TM, tiles_n = (o.n + TN - 1) / TN;
-  product_kernel<TM, TN, WM, WN, KS, kFp8, kRowsC>
-      <<<dc::tile_grid(tiles_m, tiles_n, kThr), kThr, 0, ctx->stream>>>(o, ep, tiles_m, tiles_n);
+  dim3 grid = dc::tile_grid(tiles_m, tiles_n, kThr);
+  grid.z = (unsigned)split.parts;
+  product_kernel<TM, TN, WM, WN, KS, kFp8, kRowsC><<<grid, kThr, 0, ctx->stream>>>(o, ep, tiles_m, tiles_n, (int)split.turns);
   return dc::last_launch_status();
 }
 
 template <bool kFp8, bool kRowsC>
-int32_t product(dc_hip_ctx* ctx, const Operands& o, const Epilogue& ep) {
+int32_t product(dc_hip_ctx* ctx, const Operands& o, const Epilogue& ep, const ProductPlan& plan) {
   using dc::LinearTile;
-  switch (dc::linear_tile(o.m, o.n, o.c_bytes, o.a_pitch, o.b_pitch, kRowsC, std::max(1, ctx->cu_count))) {
-    case LinearTile::k256: return launch_product<256, 256, 2, 4, 1, kFp8, kRowsC>(ctx, o, ep);
-    case LinearTile::k128: return launch_product<128, 128, 2, 2, 1, kFp8, kRowsC>(ctx, o, ep);
-    case LinearTile::k128x2: return launch_product<128, 128, 2, 2, 2, kFp8, kRowsC>(ctx, o, ep);
-    case LinearTile::k64: return launch_product<64, 64, 2, 2, 1, kFp8, kRowsC>(ctx, o, ep);
-    case LinearTile::k64x2: return launch_product<64, 64, 2, 2, 2, kFp8, kRowsC>(ctx, o, ep);
-    case LinearTile::k64x4: return launch_product<64, 64, 2, 2, 4, kFp8, kRowsC>(ctx, o, ep);
+  const dc::LinearSplit& split = plan.split;
+  float* parts = reinterpret_cast<float*>(static_cast<unsigned char*>(ctx->partials) + plan.at);
+  const int64_t pitch = padded(o.n, 8);
+  Epilogue part{};  // the sums alone
+  part.y = parts, part.y_stride = pitch, part.y_f32 = 1, part.part_stride = o.m * pitch;
+  const Epilogue& e = split.parts > 1 ? part : ep;
+  int32_t status = DC_ERR_INVALID_ARGUMENT;
+  switch (plan.tile) {
+    case LinearTile::k256: status = launch_product<256, 256, 2, 4, 1, kFp8, kRowsC>(ctx, o, e, split); break;
+    case LinearTile::k128: status = launch_product<128, 128, 2, 2, 1, kFp8, kRowsC>(ctx, o, e, split); break;
+    case LinearTile::k128x2: status = launch_product<128, 128, 2, 2, 2, kFp8, kRowsC>(ctx, o, e, split); break;
+    case LinearTile::k64: status = launch_product<64, 64, 2, 2, 1, kFp8, kRowsC>(ctx, o, e, split); break;
+    case LinearTile::k64x2: status = launch_product<64, 64, 2, 2, 2, kFp8, kRowsC>(ctx, o, e, split); break;
+    case LinearTile::k64x4: status = launch_product<64, 64, 2, 2, 4, kFp8, kRowsC>(ctx, o, e, split); break;
   }
-  return DC_ERR_INVALID_ARGUMENT;
+  if (split.parts == 1 || status != DC_OK) return status;
+  const int64_t groups = (o.m * (pitch / 8) + 255) / 256;
+  join_kernel<<<(unsigned)std::min<int64_t>(groups, 1 << 16), 256, 0, ctx->stream>>>(
+      JoinArgs{parts, o.m, o.n, pitch, (int32_t)split.parts}, ep);
+  return dc::last_launch_status();
 }
 
 // NB blocks of 16 outputs and XB blocks of 8 rows of x, W waves, and as many stages as fit in `kLds` KiB of LDS.
@@ -901,18 +973,6 @@ int32_t few_rows_any(dc_hip_ctx* ctx, const Operands& o, const Epilogue& ep) {
 }
 
 bool aligned_to(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
-int64_t padded(int64_t v, int64_t to) { return (v + to - 1) / to * to; }
-
-// Scratch of one call: pieces of ctx->partials, each at a multiple of 256 bytes.
-struct Scratch {
-  size_t bytes = 0;
-  size_t take(int64_t n) {
-    const size_t at = bytes;
-    bytes += (size_t)padded(n, 256);
-    return at;
-  }
-};
-
 // An operand as the direct-to-LDS loads take it: 16-byte aligned rows of whole 16-byte pieces, with a pitch that keeps
 // a tile's rows in range; else a copy that is.
 struct Rows {
@@ -924,17 +984,26 @@ struct Rows {
     copied = !aligned_to(p, 16) || pitch % 16 != 0 || bytes % 16 != 0 || pitch > dc::kLinearPitch;
     if (copied) at = s.take(rows * padded(bytes, 16));
   }
-  int32_t lay_out(dc_hip_ctx* ctx) {
-    if (!copied) return DC_OK;
-    unsigned char* to = static_cast<unsigned char*>(ctx->partials) + at;
-    const PackArgs a{p, to, rows, bytes, pitch, padded(bytes, 16)};
-    const int64_t groups = (rows * (a.to_pitch / 16) + 255) / 256;
-    pack_kernel<<<(unsigned)std::min<int64_t>(groups, 65536), 256, 0, ctx->stream>>>(a);
-    p = to;
-    pitch = a.to_pitch;
-    return dc::last_launch_status();
-  }
+  int64_t width() const { return copied ? padded(bytes, 16) : pitch; }  // the pitch it will have
 };
+
+// Lays out those of the (at most two) operands that have to be, in one launch.
+int32_t lay_out(dc_hip_ctx* ctx, Rows* a, Rows* b) {
+  PackArgs args{};
+  int jobs = 0;
+  int64_t most = 0;
+  for (Rows* r : {a, b}) {
+    if (!r || !r->copied) continue;
+    unsigned char* to = static_cast<unsigned char*>(ctx->partials) + r->at;
+    args.job[jobs++] = PackJob{r->p, to, r->rows, r->bytes, r->pitch, r->width()};
+    most = std::max(most, r->rows * (r->width() / 16));
+    r->p = to;
+    r->pitch = r->width();
+  }
+  if (jobs == 0) return DC_OK;
+  pack_kernel<<<dim3((unsigned)std::min<int64_t>((most + 255) / 256, 65536), (unsigned)jobs), 256, 0, ctx->stream>>>(args);
+  return dc::last_launch_status();
+}
 
 int32_t check_rows(const void* p, int64_t size, int64_t stride, int64_t rows, int64_t cols) {
   if (!p) return DC_ERR_INVALID_ARGUMENT;
@@ -992,21 +1061,26 @@ DC_HIP_API int32_t dc_hip_linear(dc_hip_ctx* ctx, const dc_linear* args) {
              (int32_t)p.n,
              (int32_t)(p.k * size),
              0};
-  const bool whole = aligned_to(o.a, 16) && aligned_to(o.b, 16) && o.a_pitch % 16 == 0 && o.b_pitch % 16 == 0 &&
-                     o.c_bytes % 16 == 0 && std::max(o.a_pitch, o.b_pitch) <= dc::kLinearPitch;
-  if (p.k == 0 || (!whole && p.m <= dc::kLinearFewRows))
-    return fp8 ? few_rows_any<true>(ctx, o, ep) : few_rows_any<false>(ctx, o, ep);
-  if (whole && dc::linear_few_rows(p.m, p.n, std::max(1, ctx->cu_count)))
-    return fp8 ? few_rows<true>(ctx, o, ep) : few_rows<false>(ctx, o, ep);
   Scratch scratch;
   Rows x{o.a, o.a_pitch, p.m, o.c_bytes}, w{o.b, o.b_pitch, p.n, o.c_bytes};
   x.plan(scratch);
   w.plan(scratch);
-  if (scratch.bytes) DC_RETURN_IF(dc::ensure_partials(ctx, scratch.bytes));
-  DC_RETURN_IF(x.lay_out(ctx));
-  DC_RETURN_IF(w.lay_out(ctx));
-  o.a = x.p, o.b = w.p, o.a_pitch = x.pitch, o.b_pitch = w.pitch;
-  return fp8 ? product<true, false>(ctx, o, ep) : product<false, false>(ctx, o, ep);
+  if (p.k == 0 || ((x.copied || w.copied) && dc::linear_few_rows_any(p.m, p.n, o.c_bytes)))
+    return fp8 ? few_rows_any<true>(ctx, o, ep) : few_rows_any<false>(ctx, o, ep);
+  auto lay_out_all = [&]() -> int32_t {
+    if (scratch.bytes) DC_RETURN_IF(dc::ensure_partials(ctx, scratch.bytes));
+    DC_RETURN_IF(lay_out(ctx, &x, &w));
+    o.a = x.p, o.b = w.p, o.a_pitch = x.pitch, o.b_pitch = w.pitch;
+    o.c_bytes = (int32_t)padded(o.c_bytes, 16);  // (ragged rows have been copied, with zeros there)
+    return DC_OK;
+  };
+  if (dc::linear_few_rows(p.m, p.n, std::max(1, ctx->cu_count))) {
+    DC_RETURN_IF(lay_out_all());
+    return fp8 ? few_rows<true>(ctx, o, ep) : few_rows<false>(ctx, o, ep);
+  }
+  const ProductPlan plan(ctx, scratch, p.m, p.n, o.c_bytes, x.width(), w.width(), false);
+  DC_RETURN_IF(lay_out_all());
+  return fp8 ? product<true, false>(ctx, o, ep, plan) : product<false, false>(ctx, o, ep, plan);
 }
 
 DC_HIP_API int32_t dc_hip_linear_backward(dc_hip_ctx* ctx, const dc_linear_grad* args) {
@@ -1030,57 +1104,63 @@ DC_HIP_API int32_t dc_hip_linear_backward(dc_hip_ctx* ctx, const dc_linear_grad*
   DC_CTX_ENTER(ctx);
   if (!dx && !dw && !dbias) return DC_OK;
   // dz runs along n in dx and along m in dw: a copy of each, padded to whole 16-byte pieces, in scratch; dy itself where
-  // it serves as dz. (Without rows, or columns, of dz the sums are empty: few_rows_any with no steps writes the zeros.)
+  // it serves as dz.
   Scratch scratch;
   Rows dz{reinterpret_cast<const unsigned char*>(p.dy), 2 * p.dy_stride, p.m, 2 * p.n};
   Rows w{reinterpret_cast<const unsigned char*>(p.w), 2 * p.w_stride, p.n, 2 * p.k};
   Rows x{reinterpret_cast<const unsigned char*>(p.x), 2 * p.x_stride, p.m, 2 * p.k};
   SlopeArgs s{reinterpret_cast<const bf16*>(p.dy), reinterpret_cast<const bf16*>(p.pre), nullptr, nullptr, nullptr, p.m, p.n,
               p.dy_stride, p.pre_stride, padded(p.n, 8), padded(p.m, 8), p.activation};
-  size_t at_dz = 0, at_dzt = 0, at_parts = 0;
-  bool own_dz = false;
+  size_t at_dzt = 0, at_parts = 0;
   const int64_t pieces = (p.m + 63) / 64;
-  if (inputs) {
-    if (dx) {
-      dz.plan(scratch);
-      own_dz = act || dz.copied;
-      if (own_dz) at_dz = dz.copied ? dz.at : scratch.take(p.m * 2 * s.dz_pitch);
-      w.plan(scratch);
-    }
-    if (dw) {
-      at_dzt = scratch.take(p.n * 2 * s.t_pitch);
-      x.plan(scratch);
-    }
-    if (dbias) at_parts = scratch.take(pieces * p.n * (int64_t)sizeof(float));
-    if (scratch.bytes) DC_RETURN_IF(dc::ensure_partials(ctx, scratch.bytes));
-    unsigned char* base = static_cast<unsigned char*>(ctx->partials);
-    if (own_dz) s.dz = reinterpret_cast<bf16*>(base + at_dz);
-    if (dw) s.dzt = reinterpret_cast<bf16*>(base + at_dzt);
-    if (dbias) s.parts = reinterpret_cast<float*>(base + at_parts);
-    if (s.dz || s.dzt || s.parts) {
-      const int64_t grid = std::min<int64_t>((p.n + 63) / 64 * pieces, 1 << 20);
-      slope_kernel<<<(unsigned)grid, 256, 0, ctx->stream>>>(s);
-      DC_RETURN_IF(dc::last_launch_status());
-    }
+  if (!inputs) {  // (no rows, or columns, of dz: the sums are empty, which few_rows_any writes as such)
+    auto zeros = [&](uint16_t* out, int64_t rows, int64_t stride) -> int32_t {
+      Epilogue ep{};
+      ep.y = out, ep.y_stride = stride;
+      return few_rows_any<false>(ctx, Operands{nullptr, nullptr, 0, 0, (int32_t)rows, (int32_t)p.k, 0, 0, 0}, ep);
+    };
+    if (dx) DC_RETURN_IF(zeros(p.dx, p.m, p.dx_stride));
+    if (dw) DC_RETURN_IF(zeros(p.dw, p.n, p.dw_stride));
+    return dbias ? dc::zero_async(ctx, p.dbias, (size_t)p.n * sizeof(float)) : DC_OK;
   }
-  Epilogue ep{};
-  // One gradient: the product of `rows` (m of them, along c) and `b` (c rows of k), or zeros where c is empty.
-  auto gradient = [&](const unsigned char* rows, int64_t pitch, int64_t m, int64_t c, Rows& b, void* out, int64_t stride) -> int32_t {
-    ep.y = out, ep.y_stride = stride;
-    if (!inputs) return few_rows_any<false>(ctx, Operands{nullptr, nullptr, 0, 0, (int32_t)m, (int32_t)p.k, 0, 0, 0}, ep);
-    DC_RETURN_IF(b.lay_out(ctx));
-    const Operands o{rows, b.p, pitch, b.pitch, (int32_t)m, (int32_t)p.k, (int32_t)(2 * c), (int32_t)c, (int32_t)padded(p.k, 8)};
-    return product<false, true>(ctx, o, ep);
-  };
   if (dx) {
-    const unsigned char* rows = s.dz ? reinterpret_cast<const unsigned char*>(s.dz) : dz.p;
-    DC_RETURN_IF(gradient(rows, s.dz ? 2 * s.dz_pitch : dz.pitch, p.m, p.n, w, p.dx, p.dx_stride));
+    dz.plan(scratch);
+    if (act && !dz.copied) dz.at = scratch.take(p.m * 2 * s.dz_pitch);
+    w.plan(scratch);
   }
-  if (dw)
-    DC_RETURN_IF(gradient(reinterpret_cast<const unsigned char*>(s.dzt), 2 * s.t_pitch, p.n, p.m, x, p.dw, p.dw_stride));
-  if (!dbias) return DC_OK;
-  if (!inputs) return dc::zero_async(ctx, p.dbias, (size_t)p.n * sizeof(float));
-  return dc::launch_column_sums(ctx, s.parts, p.dbias, pieces, p.n);
+  const bool own_dz = dx && (act || dz.copied);
+  if (dw) {
+    at_dzt = scratch.take(p.n * 2 * s.t_pitch);
+    x.plan(scratch);
+  }
+  if (dbias && pieces > 1) at_parts = scratch.take(pieces * p.n * (int64_t)sizeof(float));
+  const int64_t dz_pitch = own_dz ? 2 * s.dz_pitch : dz.pitch;
+  const ProductPlan dx_plan(ctx, scratch, p.m, p.k, 2 * p.n, dz_pitch, w.width(), true);
+  const ProductPlan dw_plan(ctx, scratch, p.n, p.k, 2 * p.m, 2 * s.t_pitch, x.width(), true);
+  if (scratch.bytes) DC_RETURN_IF(dc::ensure_partials(ctx, scratch.bytes));
+  unsigned char* base = static_cast<unsigned char*>(ctx->partials);
+  if (own_dz) s.dz = reinterpret_cast<bf16*>(base + dz.at);
+  if (dw) s.dzt = reinterpret_cast<bf16*>(base + at_dzt);
+  if (dbias) s.parts = pieces > 1 ? reinterpret_cast<float*>(base + at_parts) : p.dbias;
+  if (s.dz || s.dzt || s.parts) {
+    const int64_t grid = std::min<int64_t>((p.n + 63) / 64 * pieces, 1 << 20);
+    slope_kernel<<<(unsigned)grid, 256, 0, ctx->stream>>>(s);
+    DC_RETURN_IF(dc::last_launch_status());
+  }
+  DC_RETURN_IF(lay_out(ctx, dx ? &w : nullptr, dw ? &x : nullptr));
+  // One gradient: the product of `rows` (m of them, along c) and `b` (c rows of k).
+  auto gradient = [&](const void* rows, int64_t pitch, int64_t m, int64_t c, const Rows& b, void* out, int64_t stride,
+                      const ProductPlan& plan) {
+    Epilogue ep{};
+    ep.y = out, ep.y_stride = stride;
+    return product<false, true>(ctx, Operands{static_cast<const unsigned char*>(rows), b.p, pitch, b.pitch, (int32_t)m, (int32_t)p.k,
+                                              (int32_t)(2 * c), (int32_t)c, (int32_t)padded(p.k, 8)},
+                                ep, plan);
+  };
+  if (dx)
+    DC_RETURN_IF(gradient(own_dz ? static_cast<const void*>(s.dz) : p.dy, dz_pitch, p.m, p.n, w, p.dx, p.dx_stride, dx_plan));
+  if (dw) DC_RETURN_IF(gradient(s.dzt, 2 * s.t_pitch, p.n, p.m, x, p.dw, p.dw_stride, dw_plan));
+  return dbias && pieces > 1 ? dc::launch_column_sums(ctx, s.parts, p.dbias, pieces, p.n) : DC_OK;
 }
 
 }  // extern "C"

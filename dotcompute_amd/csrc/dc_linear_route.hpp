@@ -40,6 +40,27 @@ inline LinearTile linear_tile(int64_t m, int64_t n, int64_t c_bytes, int64_t a_p
   return LinearTile::k64x4;
 }
 
+inline int64_t linear_tile_side(LinearTile t) {
+  return t == LinearTile::k256 ? 256 : t == LinearTile::k128 || t == LinearTile::k128x2 ? 128 : 64;
+}
+inline int64_t linear_tile_groups(LinearTile t) {
+  return t == LinearTile::k64x4 ? 4 : t == LinearTile::k128x2 || t == LinearTile::k64x2 ? 2 : 1;
+}
+
+// c in `parts` of `turns` tiles a group, whose sums are added by a kernel of their own: where the tiles leave most CUs idle and
+// their sums are long.
+struct LinearSplit {
+  int64_t parts, turns;
+};
+inline LinearSplit linear_split(LinearTile tile, int64_t m, int64_t n, int64_t c_bytes, int64_t cus) {
+  const int64_t side = linear_tile_side(tile), tiles = ((m + side - 1) / side) * ((n + side - 1) / side);
+  const int64_t step = 128 * linear_tile_groups(tile), all = (c_bytes + step - 1) / step;
+  const int64_t most = tiles > 0 ? cus / tiles : 1;
+  if (all < 8 || most < 2) return {1, all};
+  const int64_t turns = (all + most - 1) / most < 3 ? 3 : (all + most - 1) / most;
+  return {(all + turns - 1) / turns, turns};
+}
+
 // Few rows of x: kernels that read w once for up to 64 of them. Measured in bf16, us (few rows / tiles): 32×16384×2048 13.3 /
 // 13.8, 64×4096×4096 10.5 / 17.9, 64×6144×4096 17.1 / 18.3, 64×8192×4096 19.7 / 18.7; so up to kLinearFewRows always, and
 // beyond where every 64 rows and 16 outputs still find a CU of their own.
@@ -47,6 +68,8 @@ constexpr int64_t kLinearFewRows = 32;
 inline bool linear_few_rows(int64_t m, int64_t n, int64_t cus) {
   return m <= kLinearFewRows || (m + 63) / 64 * ((n + 15) / 16) <= cus;
 }
+// Rows that would have to be copied for those: read as they lie.
+inline bool linear_few_rows_any(int64_t m, int64_t n, int64_t c_bytes) { return m <= kLinearFewRows; }
 // 64 outputs a workgroup instead of 16, where that leaves two for a CU (8×16384×2048: 11.7 us, 12.6; 8×8192×4096: 11.7, 12.2;
 // 8×4096×4096: 9.6, 7.4).
 inline bool linear_wide_few_rows(int64_t m, int64_t n, int64_t cus) { return m <= kLinearFewRows && (n + 15) / 16 > 2 * cus; }
