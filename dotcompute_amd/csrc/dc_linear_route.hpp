@@ -47,15 +47,17 @@ inline int64_t linear_tile_groups(LinearTile t) {
   return t == LinearTile::k64x4 ? 4 : t == LinearTile::k128x2 || t == LinearTile::k64x2 ? 2 : 1;
 }
 
-// c in `parts` of `turns` tiles a group, whose sums are added by a kernel of their own: where the tiles leave most CUs idle and
-// their sums are long.
+// c in `parts` of `turns` tiles a group, whose sums are added by a kernel of their own: where the tiles leave CUs idle and their
+// sums are long; two workgroups a CU where they are longer still. Measured, us in one part / two workgroups a CU / four (results m x n,
+// sums over c): bf16 2515x256x5120 30.2 / 21.0 / 24.9; 1024x1024x4096 22.5 / 20.3 / 26.2; 1024^3 6.4 / 13.5 / 17.4; e4m3 1024x1024x4096
+// 9.7 / 16.2 / 18.4. And with many parts, before / now: 315x256x5168 27 / 11.4, 64x2048x8192 (rows c) 34.9 / 14.4.
 struct LinearSplit {
   int64_t parts, turns;
 };
 inline LinearSplit linear_split(LinearTile tile, int64_t m, int64_t n, int64_t c_bytes, int64_t cus) {
   const int64_t side = linear_tile_side(tile), tiles = ((m + side - 1) / side) * ((n + side - 1) / side);
   const int64_t step = 128 * linear_tile_groups(tile), all = (c_bytes + step - 1) / step;
-  const int64_t most = tiles > 0 ? cus / tiles : 1;
+  const int64_t most = tiles > 0 ? (all >= 32 ? 2 : 1) * cus / tiles : 1;
   if (all < 8 || most < 2) return {1, all};
   const int64_t turns = (all + most - 1) / most < 3 ? 3 : (all + most - 1) / most;
   return {(all + turns - 1) / turns, turns};
@@ -68,8 +70,15 @@ constexpr int64_t kLinearFewRows = 32;
 inline bool linear_few_rows(int64_t m, int64_t n, int64_t cus) {
   return m <= kLinearFewRows || (m + 63) / 64 * ((n + 15) / 16) <= cus;
 }
-// Rows that would have to be copied for those: read as they lie.
-inline bool linear_few_rows_any(int64_t m, int64_t n, int64_t c_bytes) { return m <= kLinearFewRows; }
+// Rows that would have to be copied for those: read as they lie, which takes a time that grows with their length, 1.5 ns a
+// byte for up to 8 rows of x and 4096 outputs, where copying takes 3.5 us and 0.42 ps for each byte of w. Measured (as they
+// lie / copied), us in bf16: 1×1000×333 3.7 / 7.5, 1×1024×4095 15.7 / 10.6, 1×4096×4095 15.9 / 21.0, 16×4096×1023 9.4 / 10.4,
+// 16×4096×4095 27.9 / 21.3, 32×216×7977 60 / 16.8.
+inline bool linear_few_rows_any(int64_t m, int64_t n, int64_t c_bytes) {
+  if (m > kLinearFewRows) return false;
+  const double rows = 0.3 + 0.7 * (double)((m + 7) / 8), rounds = (double)((n + 4095) / 4096);
+  return 1.5 * (double)c_bytes * rows * rounds < 3500.0 + 0.42e-3 * (double)n * (double)c_bytes;
+}
 // 64 outputs a workgroup instead of 16, where that leaves two for a CU (8×16384×2048: 11.7 us, 12.6; 8×8192×4096: 11.7, 12.2;
 // 8×4096×4096: 9.6, 7.4).
 inline bool linear_wide_few_rows(int64_t m, int64_t n, int64_t cus) { return m <= kLinearFewRows && (n + 15) / 16 > 2 * cus; }
