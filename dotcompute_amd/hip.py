@@ -7,6 +7,7 @@ missing, or no gfx950 device is present, the calls raise.
 from __future__ import annotations
 
 import ctypes as C
+import math
 import os
 from dataclasses import dataclass
 
@@ -129,13 +130,15 @@ class LinqChain(C.Structure):
         return ch
 
 
+_DTYPE_CODES = {np.dtype(np.float32): DTYPE_F32, np.dtype(np.uint16): DTYPE_BF16, np.dtype(np.uint8): DTYPE_FP8}
+
+
 def dtype_of(a: "DeviceArray") -> int:
     """dc_dtype of an array: float32, bf16 bit patterns (uint16) or e4m3 bytes (uint8)."""
-    try:
-        return {np.dtype(np.float32): DTYPE_F32, np.dtype(np.uint16): DTYPE_BF16,
-                np.dtype(np.uint8): DTYPE_FP8}[np.dtype(a.dtype)]
-    except KeyError:
-        raise ValueError(f"no operator takes elements of type {a.dtype}") from None
+    code = _DTYPE_CODES.get(a.dtype)
+    if code is None:
+        raise ValueError(f"no operator takes elements of type {a.dtype}")
+    return code
 
 
 def _matrix(a: "DeviceArray", name: str) -> tuple:
@@ -290,15 +293,15 @@ class AdamWTensors:
         for t, part in zip(items, parts):
             n = part["param"].size
             state = dtype_of(part["m"])
-            flat = {name: tuple(a.shape) for name, a in part.items()}
+            types = {}
             for name, a in part.items():
                 if name not in AdamWTensor.__dict__:
                     raise ValueError(f"a step takes no array called {name}")
                 want = -(-n // ADAMW_BLOCK) if name.endswith("scales") else n
                 if a.size != want:
-                    raise ValueError(f"{name}: {want} elements expected (got {flat[name]})")
+                    raise ValueError(f"{name}: {want} elements expected (got {a.shape})")
                 setattr(t, name, a.ptr)
-            types = {name: dtype_of(a) for name, a in part.items()}
+                types[name] = dtype_of(a)
             if types["param"] != DTYPE_F32 or types["grad"] == DTYPE_FP8 or state == DTYPE_BF16 or types["v"] != state \
                     or types.get("copy", DTYPE_BF16) != DTYPE_BF16:
                 raise ValueError(f"no such types: {types}")
@@ -492,7 +495,7 @@ class DeviceArray:
 
     @property
     def size(self) -> int:
-        return int(np.prod(self.shape)) if self.shape else 1
+        return math.prod(self.shape)
 
     def copy_from(self, host: np.ndarray) -> "DeviceArray":
         host = np.ascontiguousarray(host, self.dtype)
