@@ -274,6 +274,10 @@ __global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void pro
   // Tiles along c of a group: `turns` of them from kt_first on, fewer in the last of the parts that c is split into
   const int kt_first = (int)blockIdx.z * turns;
   const int kt_count = min((tiles_c + KS - 1) / KS - kt_first, turns);
+  // Where c ends here. kAlways: tiles past it are asked for too, as zeros, so that no branch stands between a tile's products
+  // (the compiler would move those before it past it, and past the barrier).
+  constexpr bool kAlways = TM == 256 && kFp8;
+  const int c_end = min(o.c_bytes, (kt_first + kt_count) * KS * kTileBytes), c_rows = min(o.c_rows, c_end / 2);
 
   // ---- load side. Rows along c: lane -> row lane / 8 of a block, slot lane % 8, which holds the piece of the swizzle.
   const int lrow = lane >> 3;
@@ -300,7 +304,7 @@ __global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void pro
     constexpr int kBuf = decltype(BUF)::value;
     const int t = (kt_first + KT) * KS + group;
     const int at = t * kTileBytes;  // bytes into A's rows (past the last: every load is past the range)
-    const int left = o.c_bytes - at;
+    const int left = c_end - at;
 #pragma unroll
     for (int i = 0; i < kABlocks; ++i)
       load_block(abase + at, sm.a[kBuf] + (i * kWaves + wave) * 1024, piece < left ? avoff[i] : kPast, 0);
@@ -310,7 +314,7 @@ __global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void pro
       for (int i = 0; i < kBBlocks; ++i) {
         const int row = kRows * (i * kWaves + wave);
         load_block(bbase + (int64_t)c0 * o.b_pitch, sm.b[kBuf] + (i * kWaves + wave) * 1024,
-                   c0 + row + brow < o.c_rows ? bvoff[0] : kPast, row * (int)o.b_pitch);
+                   c0 + row + brow < c_rows ? bvoff[0] : kPast, row * (int)o.b_pitch);
       }
     } else {
 #pragma unroll
@@ -419,7 +423,8 @@ __global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void pro
   if constexpr (kRowsC) read_b_tile(kBuf0, fb[0]);
   else read_b(kBuf0, 0, fb[0][0]);
   read_a(kBuf0, 0, fa[0]);
-  if (kt_count > 1) load_tile(kBuf1, 1);
+  __builtin_amdgcn_sched_barrier(0);
+  if (kAlways || kt_count > 1) load_tile(kBuf1, 1);
   // (a macro, so that the fragment arrays stay plain registers)
 #define DC_TILE(BUF, KT)                                                                            \
   {                                                                                                 \
@@ -434,7 +439,8 @@ __global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void pro
     }                                                                                               \
     dc::dma_barrier();                                                                              \
     if constexpr (kRowsC) read_b_tile(kBuf##BUF##Other, fb[1 - (BUF)]);                             \
-    if ((KT) + 2 < kt_count) load_tile(kBuf##BUF, (KT) + 2);                                        \
+    __builtin_amdgcn_sched_barrier(0);                                                              \
+    if (kAlways || (KT) + 2 < kt_count) load_tile(kBuf##BUF, (KT) + 2);                             \
     __builtin_amdgcn_sched_barrier(0);                                                              \
     read_a(kBuf##BUF##Other, 0, fa[0]);                                                             \
     if constexpr (!kRowsC) read_b(kBuf##BUF##Other, 0, fb[0][0]);                                   \
@@ -453,8 +459,8 @@ __global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void pro
   } while (kt < kt_count);
 #undef DC_TILE
 
-  // (after the last tile: reads of the other buffer that nobody uses; every wave is past them beyond this barrier)
-  __syncthreads();
+  // (after the last tile: loads of zeros, and reads of the other buffer, that nobody uses; all are over beyond this barrier)
+  dc::dma_barrier();
   if constexpr (KS > 1) {  // the groups' sums, added in group order by group 0
     static_assert(sizeof(Smem) >= kWaves * 64 * kMT * kNT * 16 * sizeof(float), "a group's sums fit in its buffers");
     float* part = reinterpret_cast<float*>(&sm) + tid % (64 * kWaves);
@@ -785,7 +791,8 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeArgs a) {
   const int t = threadIdx.x, c8 = t & 7, pair = t >> 3;
   const int64_t across = (a.n + 63) / 64, total = across * ((a.m + 63) / 64);
   for (int64_t at = blockIdx.x; at < total; at += gridDim.x) {
-  const int64_t m0 = at / across * 64, n0 = at % across * 64;
+  const int64_t down = total <= UINT32_MAX ? (int64_t)((uint32_t)at / (uint32_t)across) : at / across;
+  const int64_t m0 = down * 64, n0 = (at - down * across) * 64;
   const int64_t j = n0 + 8 * c8;
   float dz[2][8];
 #pragma unroll
@@ -868,13 +875,22 @@ struct PackJob {
 struct PackArgs {
   PackJob job[2];
 };
+constexpr int64_t kPackBytes = 4096;  // of a row that a wave takes, all asked for at once
 __global__ __launch_bounds__(256) void pack_kernel(PackArgs args) {
   const PackJob& a = args.job[blockIdx.y];
-  const int64_t pieces = a.to_pitch / 16, total = a.rows * pieces, step = (int64_t)gridDim.x * 256;
-  for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += step) {
-    const int64_t row = t / pieces, at = 16 * (t - row * pieces);
-    *reinterpret_cast<dc::u32x4*>(a.to + row * a.to_pitch + at) =
-        load_piece(a.from + row * a.from_pitch + at, a.bytes - at, a.bytes);
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t across = (a.to_pitch + kPackBytes - 1) / kPackBytes, total = a.rows * across;
+  for (int64_t t = (int64_t)blockIdx.x * 4 + wave; t < total; t += (int64_t)gridDim.x * 4) {
+    const int64_t row = total <= UINT32_MAX ? (int64_t)((uint32_t)t / (uint32_t)across) : t / across;
+    const unsigned char* from = a.from + row * a.from_pitch;
+    unsigned char* to = a.to + row * a.to_pitch;
+    const int64_t first = (t - row * across) * kPackBytes + 16 * lane;
+    dc::u32x4 w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = load_piece(from + first + 1024 * i, a.bytes - first - 1024 * i, a.bytes);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (first + 1024 * i < a.to_pitch) *reinterpret_cast<dc::u32x4*>(to + first + 1024 * i) = w[i];
   }
 }
 
@@ -996,12 +1012,12 @@ int32_t lay_out(dc_hip_ctx* ctx, Rows* a, Rows* b) {
     if (!r || !r->copied) continue;
     unsigned char* to = static_cast<unsigned char*>(ctx->partials) + r->at;
     args.job[jobs++] = PackJob{r->p, to, r->rows, r->bytes, r->pitch, r->width()};
-    most = std::max(most, r->rows * (r->width() / 16));
+    most = std::max(most, (r->rows * ((r->width() + kPackBytes - 1) / kPackBytes) + 3) / 4);
     r->p = to;
     r->pitch = r->width();
   }
   if (jobs == 0) return DC_OK;
-  pack_kernel<<<dim3((unsigned)std::min<int64_t>((most + 255) / 256, 65536), (unsigned)jobs), 256, 0, ctx->stream>>>(args);
+  pack_kernel<<<dim3((unsigned)std::min<int64_t>(most, 65536), (unsigned)jobs), 256, 0, ctx->stream>>>(args);
   return dc::last_launch_status();
 }
 

@@ -57,7 +57,7 @@ struct LinearSplit {
 inline LinearSplit linear_split(LinearTile tile, int64_t m, int64_t n, int64_t c_bytes, int64_t cus) {
   const int64_t side = linear_tile_side(tile), tiles = ((m + side - 1) / side) * ((n + side - 1) / side);
   const int64_t step = 128 * linear_tile_groups(tile), all = (c_bytes + step - 1) / step;
-  const int64_t most = tiles > 0 ? (all >= 32 ? 2 : 1) * cus / tiles : 1;
+  const int64_t most = tiles > 0 ? (side == 64 && all >= 32 ? 2 : 1) * cus / tiles : 1;
   if (all < 8 || most < 2) return {1, all};
   const int64_t turns = (all + most - 1) / most < 3 ? 3 : (all + most - 1) / most;
   return {(all + turns - 1) / turns, turns};
