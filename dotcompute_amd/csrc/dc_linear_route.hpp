@@ -1,5 +1,5 @@
 // dc_linear_route.hpp — which kernel of dc_linear.hip takes a shape: pure functions of the sizes and the number of
-// CUs, checked on the CPU by tests/cpp/host_tests.cpp.
+// CUs, checked on the CPU by tests/cpp/feed_forward_tests.cpp.
 #pragma once
 
 #include <cstdint>
@@ -20,6 +20,7 @@ enum class LinearTile { k256, k128, k128x2, k64, k64x2, k64x4 };
 // tiles of 256 / 128 / 128x2 / 64 / 64x2 / 64x4, w by rows of c where it says so):
 //   bf16: 4096x4096x1024 34.5 / 39.7 / 51.7 / 52.4 / 59.4 / 94;  5120x5120x1024 58.8 / 64.4 / 89 / 80 / 92 / 145
 //   2000x3000x1000 30.5 / 21.6 / 29.4 / 27.8 / 28.7 / 41;  2048^3 44 / 25.3 / 22.7 / 25.6 / 27.4 / 38
+//   2048x2048x816 25.4 / 13.3 / 13.8 / 15.2 / 16.1 / 23;  2048x2048x512 18.6 / 9.7 / 10.3 / 9.1 / 11.3 / 18
 //   1537x2049x1024 27.4 / 15.2 / 14.8 / 13.8 / 17.7 / 26;  1024^3 26 / 11.7 / 11.7 / 6.9 / 6.4 / 6.5
 //   rows c: 8192x2048x8192 208 / 244 / 278 / 358 / 377 / 529;  4096x1024x4096 86 / 47 / 39.9 / 49 / 52 / 73
 //   2000x1000x3000 71 / 41 / 36 / 29.1 / 27.9 / 37;  3000x1000x2000 51 / 30.2 / 26.5 / 27.9 / 33.8 / 38
@@ -35,6 +36,7 @@ inline LinearTile linear_tile(int64_t m, int64_t n, int64_t c_bytes, int64_t a_p
   if (fits(256) && 2 * t256 > cus && (t256 <= cus || 10 * t256 > 13 * cus) && !brief) return LinearTile::k256;
   if (fits(128) && t128 > cus && !brief) return LinearTile::k128;
   if (fits(128) && 4 * t128 > 3 * cus && k >= 1536) return LinearTile::k128x2;
+  if (fits(128) && 10 * t128 > 9 * cus && k >= 768) return LinearTile::k128;
   if (t64 > 2 * cus || k < 512) return LinearTile::k64;
   if (2 * t64 > cus || k < 2048) return LinearTile::k64x2;
   return LinearTile::k64x4;
