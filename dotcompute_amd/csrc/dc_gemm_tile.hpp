@@ -19,11 +19,8 @@ struct TileCoord {
 
 constexpr int kTileGroupM = 8;
 
-__device__ inline TileCoord map_tile(int tiles_m, int tiles_n) {
+__device__ inline TileCoord map_tile(int b, int tiles_m, int tiles_n) {
   const int total = tiles_m * tiles_n;
-  // (gemm_grid's rows; workgroups past the last tile form that one too: an early exit here costs
-  // every launch 0.1-0.2 us)
-  const int b = min((int)(blockIdx.x + (blockIdx.y << kGemmGridRowBits)), total - 1);
   const int t = (total % 8 == 0) ? (b % 8) * (total / 8) + b / 8 : b;
   const int group = kTileGroupM * tiles_n;
   const int g = t / group;
@@ -31,6 +28,10 @@ __device__ inline TileCoord map_tile(int tiles_m, int tiles_n) {
   const int gm = min(tiles_m - first_m, kTileGroupM);
   const int in_g = t - g * group;
   return TileCoord{first_m + in_g % gm, in_g / gm};
+}
+// (gemm_grid's rows; workgroups past the last tile form that one too: an early exit here costs every launch 0.1-0.2 us)
+__device__ inline TileCoord map_tile(int tiles_m, int tiles_n) {
+  return map_tile(min((int)(blockIdx.x + (blockIdx.y << kGemmGridRowBits)), tiles_m * tiles_n - 1), tiles_m, tiles_n);
 }
 
 typedef __attribute__((address_space(3))) void* lds_ptr_t;

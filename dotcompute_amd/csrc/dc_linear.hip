@@ -182,7 +182,7 @@ struct Results {
     if (p.residual) load_bf16(p.residual + i * p.residual_stride + c.j, c.left, residual);
     if (p.a_scales) scale = p.a_scales[i];
   }
-  __device__ inline void finish(const Epilogue& p, const Columns<E>& c, int64_t i, float (&z)[E]) const {
+  __device__ inline void finish(const Epilogue& p, const Columns<E>& c, int64_t i, float (&z)[E], int part = 0) const {
     if (p.a_scales)
 #pragma unroll
       for (int e = 0; e < E; ++e) z[e] = z[e] * scale * c.scale[e];
@@ -195,7 +195,7 @@ struct Results {
 #pragma unroll
       for (int e = 0; e < E; ++e) z[e] += residual[e];
     if (p.y_f32) {
-      float* q = static_cast<float*>(p.y) + i * p.y_stride + c.j + (int64_t)blockIdx.z * p.part_stride;
+      float* q = static_cast<float*>(p.y) + i * p.y_stride + c.j + part * p.part_stride;
 #pragma unroll
       for (int e = 0; e < E; e += 4) dc::store_some(q + e, c.left - e, *reinterpret_cast<const float (*)[4]>(z + e));
     } else {
@@ -253,9 +253,25 @@ __device__ inline void load_block(const unsigned char* base, unsigned char* to, 
   __builtin_amdgcn_raw_ptr_buffer_load_lds(dc::range_rsrc(base, kRange), (dc::lds_ptr_t)to, 16, voff, soff, 0, 0);
 }
 
+// The products of one launch. Workgroups take the first's tiles, part of c by part, then the second's: the two
+// gradients of a layer have no more tiles than CUs each where it is of ordinary size, and run side by side.
+struct Job {
+  Operands o;
+  Epilogue ep;
+  int32_t tiles_m, tiles_n;
+  int32_t parts, turns;  // of c, and tiles along c in each
+};
+template <int N>
+struct Jobs {
+  Job job[N];
+  int32_t first;  // workgroups of the first
+  int32_t base;   // workgroups of the launches before this one
+};
+template <bool kRowsC>
+constexpr int kJobs = kRowsC ? 2 : 1;
+
 template <int TM, int TN, int WM, int WN, int KS, bool kFp8, bool kRowsC>
-__global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void product_kernel(Operands o, Epilogue ep,
-                                                                                           int tiles_m, int tiles_n, int turns) {
+__global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void product_kernel(Jobs<kJobs<kRowsC>> jobs) {
   static_assert(!(kFp8 && kRowsC), "8-bit operands run along c");
   constexpr int kWaves = WM * WN;
   constexpr int kMT = TM / WM / 32, kNT = TN / WN / 32;
@@ -263,7 +279,14 @@ __global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void pro
   constexpr int kSteps = kFp8 ? 2 : 4;                                   // instructions along c of a tile
   using Smem = TileSmem<TM, TN>;
   __shared__ __align__(16) Smem sms[KS];
-  const dc::TileCoord tc = dc::map_tile(tiles_m, tiles_n);
+  int block = jobs.base + (int)blockIdx.x;
+  const bool second = kRowsC && block >= jobs.first;
+  if (second) block -= jobs.first;
+  const Job& job = jobs.job[second ? kJobs<kRowsC> - 1 : 0];
+  const Operands& o = job.o;
+  const Epilogue& ep = job.ep;
+  const int tiles = job.tiles_m * job.tiles_n, part = job.parts > 1 ? block / tiles : 0, turns = job.turns;
+  const dc::TileCoord tc = dc::map_tile(block - part * tiles, job.tiles_m, job.tiles_n);
   const int m0 = tc.tm * TM, n0 = tc.tn * TN;
   const int tid = threadIdx.x, lane = tid & 63, gwave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int group = gwave / kWaves, wave = gwave % kWaves;
@@ -272,7 +295,7 @@ __global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void pro
   const int r = lane & 31, h = lane >> 5;
   const int tiles_c = (o.c_bytes + kTileBytes - 1) / kTileBytes;
   // Tiles along c of a group: `turns` of them from kt_first on, fewer in the last of the parts that c is split into
-  const int kt_first = (int)blockIdx.z * turns;
+  const int kt_first = part * turns;
   const int kt_count = min((tiles_c + KS - 1) / KS - kt_first, turns);
   // Where c ends here. kAlways: tiles past it are asked for too, as zeros, so that no branch stands between a tile's products
   // (the compiler would move those before it past it, and past the barrier).
@@ -503,7 +526,7 @@ __global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void pro
       if (i < o.m && cols.left > 0) {
         Results<8> out;
         out.read(ep, cols, i);
-        out.finish(ep, cols, i, z);
+        out.finish(ep, cols, i, z, part);
       }
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -791,51 +814,51 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeArgs a) {
   const int t = threadIdx.x, c8 = t & 7, pair = t >> 3;
   const int64_t across = (a.n + 63) / 64, total = across * ((a.m + 63) / 64);
   for (int64_t at = blockIdx.x; at < total; at += gridDim.x) {
-  const int64_t down = total <= UINT32_MAX ? (int64_t)((uint32_t)at / (uint32_t)across) : at / across;
-  const int64_t m0 = down * 64, n0 = (at - down * across) * 64;
-  const int64_t j = n0 + 8 * c8;
-  float dz[2][8];
+    const int64_t down = total <= UINT32_MAX ? (int64_t)((uint32_t)at / (uint32_t)across) : at / across;
+    const int64_t m0 = down * 64, n0 = (at - down * across) * 64;
+    const int64_t j = n0 + 8 * c8;
+    float dz[2][8];
 #pragma unroll
-  for (int q = 0; q < 2; ++q) {
-    const int64_t i = m0 + 2 * pair + q;
-    if (i < a.m && j < a.n) {
-      dc::load_some(a.dy + i * a.dy_stride + j, a.n - j, dz[q]);
-      if (a.act != DC_ACT_NONE) {
-        float z[8];
-        dc::load_some(a.pre + i * a.pre_stride + j, a.n - j, z);  // (zeros past the last: their dz stays zero)
-        apply_slope(a.act, z, dz[q]);
+    for (int q = 0; q < 2; ++q) {
+      const int64_t i = m0 + 2 * pair + q;
+      if (i < a.m && j < a.n) {
+        dc::load_some(a.dy + i * a.dy_stride + j, a.n - j, dz[q]);
+        if (a.act != DC_ACT_NONE) {
+          float z[8];
+          dc::load_some(a.pre + i * a.pre_stride + j, a.n - j, z);  // (zeros past the last: their dz stays zero)
+          apply_slope(a.act, z, dz[q]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dz[q][e] = 0.0f;
       }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) dz[q][e] = 0.0f;
+      if (a.dz && i < a.m && j < a.dz_pitch) dc::store_chunk(a.dz + i * a.dz_pitch + j, dz[q]);
     }
-    if (a.dz && i < a.m && j < a.dz_pitch) dc::store_chunk(a.dz + i * a.dz_pitch + j, dz[q]);
-  }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    turned[8 * c8 + e][pair] = dc::pack_bf16(dz[0][e], dz[1][e]);
-    sums[pair][8 * c8 + e] = dz[0][e] + dz[1][e];
-  }
-  __syncthreads();
-  if (a.dzt) {
+    for (int e = 0; e < 8; ++e) {
+      turned[8 * c8 + e][pair] = dc::pack_bf16(dz[0][e], dz[1][e]);
+      sums[pair][8 * c8 + e] = dz[0][e] + dz[1][e];
+    }
+    __syncthreads();
+    if (a.dzt) {
 #pragma unroll
-    for (int q = 0; q < 2; ++q) {  // 64 rows of 8 16-byte chunks
-      const int row = (t >> 3) + 32 * q, chunk = t & 7;
-      const int64_t c = m0 + 8 * chunk;
-      if (n0 + row < a.n && c < a.t_pitch) {
-        const dc::u32x4 w = {turned[row][4 * chunk], turned[row][4 * chunk + 1], turned[row][4 * chunk + 2],
-                             turned[row][4 * chunk + 3]};
-        *reinterpret_cast<dc::u32x4*>(a.dzt + (n0 + row) * a.t_pitch + c) = w;
+      for (int q = 0; q < 2; ++q) {  // 64 rows of 8 16-byte chunks
+        const int row = (t >> 3) + 32 * q, chunk = t & 7;
+        const int64_t c = m0 + 8 * chunk;
+        if (n0 + row < a.n && c < a.t_pitch) {
+          const dc::u32x4 w = {turned[row][4 * chunk], turned[row][4 * chunk + 1], turned[row][4 * chunk + 2],
+                               turned[row][4 * chunk + 3]};
+          *reinterpret_cast<dc::u32x4*>(a.dzt + (n0 + row) * a.t_pitch + c) = w;
+        }
       }
     }
-  }
-  if (a.parts && t < 64 && n0 + t < a.n) {
-    float s = 0.0f;
+    if (a.parts && t < 64 && n0 + t < a.n) {
+      float s = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 32; ++i) s += sums[i][t];
-    a.parts[m0 / 64 * a.n + n0 + t] = s;
-  }
-  __syncthreads();
+      for (int i = 0; i < 32; ++i) s += sums[i][t];
+      a.parts[m0 / 64 * a.n + n0 + t] = s;
+    }
+    __syncthreads();
   }
 }
 
@@ -912,47 +935,78 @@ struct ProductPlan {
   dc::LinearTile tile;
   dc::LinearSplit split;
   size_t at = 0;
-  ProductPlan(dc_hip_ctx* ctx, Scratch& s, int64_t m, int64_t n, int64_t c_bytes, int64_t a_pitch, int64_t b_pitch, bool rows_c) {
+  ProductPlan(dc_hip_ctx* ctx, Scratch& s, const dc::LinearSize& size, bool rows_c) {
     const int64_t cus = std::max(1, ctx->cu_count);
-    tile = dc::linear_tile(m, n, c_bytes, a_pitch, b_pitch, rows_c, cus);
-    split = dc::linear_split(tile, m, n, c_bytes, cus);
-    if (split.parts > 1) at = s.take(split.parts * m * padded(n, 8) * (int64_t)sizeof(float));
+    tile = dc::linear_tile(size, rows_c, cus);
+    split = dc::linear_split(tile, size, cus);
+    if (split.parts > 1) at = s.take(split.parts * size.m * padded(size.n, 8) * (int64_t)sizeof(float));
   }
 };
 
+// One product to launch: all of it, its results in scratch where c is split.
+struct Product {
+  Operands o;
+  Epilogue ep;
+  ProductPlan plan;
+  float* parts(dc_hip_ctx* ctx) const { return reinterpret_cast<float*>(static_cast<unsigned char*>(ctx->partials) + plan.at); }
+  int64_t pitch() const { return padded(o.n, 8); }  // of those
+};
+
+constexpr int64_t kLaunchItems = int64_t(1) << 32;  // a launch has fewer work items
+
 template <int TM, int TN, int WM, int WN, int KS, bool kFp8, bool kRowsC>
-int32_t launch_product(dc_hip_ctx* ctx, const Operands& o, const Epilogue& ep, const dc::LinearSplit& split) {
+int32_t launch_products(dc_hip_ctx* ctx, const Product* const (&p)[kJobs<kRowsC>]) {
   constexpr int kThr = 64 * WM * WN * KS;
-  const int tiles_m = (o.m + TM - 1) / TM, tiles_n = (o.n + TN - 1) / TN;
-  dim3 grid = dc::tile_grid(tiles_m, tiles_n, kThr);
-  grid.z = (unsigned)split.parts;
-  product_kernel<TM, TN, WM, WN, KS, kFp8, kRowsC><<<grid, kThr, 0, ctx->stream>>>(o, ep, tiles_m, tiles_n, (int)split.turns);
+  Jobs<kJobs<kRowsC>> jobs{};
+  int64_t total = 0;
+  for (int i = 0; i < kJobs<kRowsC>; ++i) {
+    if (i == 1) jobs.first = (int32_t)total;
+    if (!p[i]) continue;
+    Job& j = jobs.job[i];
+    j.o = p[i]->o, j.ep = p[i]->ep;
+    j.tiles_m = (j.o.m + TM - 1) / TM, j.tiles_n = (j.o.n + TN - 1) / TN;
+    j.parts = (int32_t)p[i]->plan.split.parts, j.turns = (int32_t)p[i]->plan.split.turns;
+    if (j.parts > 1) {  // the sums alone
+      j.ep = Epilogue{};
+      j.ep.y = p[i]->parts(ctx), j.ep.y_stride = p[i]->pitch(), j.ep.y_f32 = 1, j.ep.part_stride = j.o.m * p[i]->pitch();
+    }
+    total += (int64_t)j.tiles_m * j.tiles_n * j.parts;
+    if (total > INT32_MAX) return DC_ERR_UNSUPPORTED;
+  }
+  for (int64_t base = 0; base < total;) {
+    const int64_t count = std::min(total - base, kLaunchItems / kThr - 1);
+    jobs.base = (int32_t)base;
+    product_kernel<TM, TN, WM, WN, KS, kFp8, kRowsC><<<(unsigned)count, kThr, 0, ctx->stream>>>(jobs);
+    DC_RETURN_IF(dc::last_launch_status());
+    base += count;
+  }
+  return DC_OK;
+}
+
+int32_t join(dc_hip_ctx* ctx, const Product& p) {
+  if (p.plan.split.parts == 1) return DC_OK;
+  const int64_t groups = (p.o.m * (p.pitch() / 8) + 255) / 256;
+  join_kernel<<<(unsigned)std::min<int64_t>(groups, 1 << 16), 256, 0, ctx->stream>>>(
+      JoinArgs{p.parts(ctx), p.o.m, p.o.n, p.pitch(), (int32_t)p.plan.split.parts}, p.ep);
   return dc::last_launch_status();
 }
 
+// Products of one tile.
 template <bool kFp8, bool kRowsC>
-int32_t product(dc_hip_ctx* ctx, const Operands& o, const Epilogue& ep, const ProductPlan& plan) {
+int32_t products(dc_hip_ctx* ctx, const Product* const (&p)[kJobs<kRowsC>]) {
   using dc::LinearTile;
-  const dc::LinearSplit& split = plan.split;
-  float* parts = reinterpret_cast<float*>(static_cast<unsigned char*>(ctx->partials) + plan.at);
-  const int64_t pitch = padded(o.n, 8);
-  Epilogue part{};  // the sums alone
-  part.y = parts, part.y_stride = pitch, part.y_f32 = 1, part.part_stride = o.m * pitch;
-  const Epilogue& e = split.parts > 1 ? part : ep;
   int32_t status = DC_ERR_INVALID_ARGUMENT;
-  switch (plan.tile) {
-    case LinearTile::k256: status = launch_product<256, 256, 2, 4, 1, kFp8, kRowsC>(ctx, o, e, split); break;
-    case LinearTile::k128: status = launch_product<128, 128, 2, 2, 1, kFp8, kRowsC>(ctx, o, e, split); break;
-    case LinearTile::k128x2: status = launch_product<128, 128, 2, 2, 2, kFp8, kRowsC>(ctx, o, e, split); break;
-    case LinearTile::k64: status = launch_product<64, 64, 2, 2, 1, kFp8, kRowsC>(ctx, o, e, split); break;
-    case LinearTile::k64x2: status = launch_product<64, 64, 2, 2, 2, kFp8, kRowsC>(ctx, o, e, split); break;
-    case LinearTile::k64x4: status = launch_product<64, 64, 2, 2, 4, kFp8, kRowsC>(ctx, o, e, split); break;
+  switch (p[0]->plan.tile) {
+    case LinearTile::k256: status = launch_products<256, 256, 2, 4, 1, kFp8, kRowsC>(ctx, p); break;
+    case LinearTile::k128: status = launch_products<128, 128, 2, 2, 1, kFp8, kRowsC>(ctx, p); break;
+    case LinearTile::k128x2: status = launch_products<128, 128, 2, 2, 2, kFp8, kRowsC>(ctx, p); break;
+    case LinearTile::k64: status = launch_products<64, 64, 2, 2, 1, kFp8, kRowsC>(ctx, p); break;
+    case LinearTile::k64x2: status = launch_products<64, 64, 2, 2, 2, kFp8, kRowsC>(ctx, p); break;
+    case LinearTile::k64x4: status = launch_products<64, 64, 2, 2, 4, kFp8, kRowsC>(ctx, p); break;
   }
-  if (split.parts == 1 || status != DC_OK) return status;
-  const int64_t groups = (o.m * (pitch / 8) + 255) / 256;
-  join_kernel<<<(unsigned)std::min<int64_t>(groups, 1 << 16), 256, 0, ctx->stream>>>(
-      JoinArgs{parts, o.m, o.n, pitch, (int32_t)split.parts}, ep);
-  return dc::last_launch_status();
+  for (const Product* q : p)
+    if (q && status == DC_OK) status = join(ctx, *q);
+  return status;
 }
 
 // NB blocks of 16 outputs and XB blocks of 8 rows of x, W waves, and as many stages as fit in `kLds` KiB of LDS.
@@ -1027,6 +1081,9 @@ int32_t check_rows(const void* p, int64_t size, int64_t stride, int64_t rows, in
   return rows > 1 && stride < cols ? DC_ERR_DIMENSION : DC_OK;
 }
 
+// Bytes from row to row. (The stride of a single row says nothing, and is not looked at.)
+int64_t pitch_of(int64_t stride, int64_t rows, int64_t cols, int64_t size) { return (rows > 1 ? stride : cols) * size; }
+
 int32_t check_dims(int64_t m, int64_t n, int64_t k, int32_t act) {
   if (m < 0 || n < 0 || k < 0 || act < DC_ACT_NONE || act > DC_ACT_SILU) return DC_ERR_INVALID_ARGUMENT;
   if (m > INT32_MAX / 2) return DC_ERR_INVALID_ARGUMENT;
@@ -1071,8 +1128,8 @@ DC_HIP_API int32_t dc_hip_linear(dc_hip_ctx* ctx, const dc_linear* args) {
                     y_f32};
   Operands o{static_cast<const unsigned char*>(p.x),
              static_cast<const unsigned char*>(p.w),
-             p.x_stride * size,
-             p.w_stride * size,
+             pitch_of(p.x_stride, p.m, p.k, size),
+             pitch_of(p.w_stride, p.n, p.k, size),
              (int32_t)p.m,
              (int32_t)p.n,
              (int32_t)(p.k * size),
@@ -1094,9 +1151,10 @@ DC_HIP_API int32_t dc_hip_linear(dc_hip_ctx* ctx, const dc_linear* args) {
     DC_RETURN_IF(lay_out_all());
     return fp8 ? few_rows<true>(ctx, o, ep) : few_rows<false>(ctx, o, ep);
   }
-  const ProductPlan plan(ctx, scratch, p.m, p.n, o.c_bytes, x.width(), w.width(), false);
+  const ProductPlan plan(ctx, scratch, {p.m, p.n, o.c_bytes, x.width(), w.width()}, false);
   DC_RETURN_IF(lay_out_all());
-  return fp8 ? product<true, false>(ctx, o, ep, plan) : product<false, false>(ctx, o, ep, plan);
+  const Product all{o, ep, plan};
+  return fp8 ? products<true, false>(ctx, {&all}) : products<false, false>(ctx, {&all});
 }
 
 DC_HIP_API int32_t dc_hip_linear_backward(dc_hip_ctx* ctx, const dc_linear_grad* args) {
@@ -1122,9 +1180,9 @@ DC_HIP_API int32_t dc_hip_linear_backward(dc_hip_ctx* ctx, const dc_linear_grad*
   // dz runs along n in dx and along m in dw: a copy of each, padded to whole 16-byte pieces, in scratch; dy itself where
   // it serves as dz.
   Scratch scratch;
-  Rows dz{reinterpret_cast<const unsigned char*>(p.dy), 2 * p.dy_stride, p.m, 2 * p.n};
-  Rows w{reinterpret_cast<const unsigned char*>(p.w), 2 * p.w_stride, p.n, 2 * p.k};
-  Rows x{reinterpret_cast<const unsigned char*>(p.x), 2 * p.x_stride, p.m, 2 * p.k};
+  Rows dz{reinterpret_cast<const unsigned char*>(p.dy), pitch_of(p.dy_stride, p.m, p.n, 2), p.m, 2 * p.n};
+  Rows w{reinterpret_cast<const unsigned char*>(p.w), pitch_of(p.w_stride, p.n, p.k, 2), p.n, 2 * p.k};
+  Rows x{reinterpret_cast<const unsigned char*>(p.x), pitch_of(p.x_stride, p.m, p.k, 2), p.m, 2 * p.k};
   SlopeArgs s{reinterpret_cast<const bf16*>(p.dy), reinterpret_cast<const bf16*>(p.pre), nullptr, nullptr, nullptr, p.m, p.n,
               p.dy_stride, p.pre_stride, padded(p.n, 8), padded(p.m, 8), p.activation};
   size_t at_dzt = 0, at_parts = 0;
@@ -1151,8 +1209,14 @@ DC_HIP_API int32_t dc_hip_linear_backward(dc_hip_ctx* ctx, const dc_linear_grad*
   }
   if (dbias && pieces > 1) at_parts = scratch.take(pieces * p.n * (int64_t)sizeof(float));
   const int64_t dz_pitch = own_dz ? 2 * s.dz_pitch : dz.pitch;
-  const ProductPlan dx_plan(ctx, scratch, p.m, p.k, 2 * p.n, dz_pitch, w.width(), true);
-  const ProductPlan dw_plan(ctx, scratch, p.n, p.k, 2 * p.m, 2 * s.t_pitch, x.width(), true);
+  const dc::LinearSize dx_size{p.m, p.k, 2 * p.n, dz_pitch, w.width()}, dw_size{p.n, p.k, 2 * p.m, 2 * s.t_pitch, x.width()};
+  ProductPlan dx_plan(ctx, scratch, dx_size, true), dw_plan(ctx, scratch, dw_size, true);
+  const bool together = dx && dw && dc::linear_alike(dx_size, dw_size) && dx_plan.split.parts == 1 && dw_plan.split.parts == 1;
+  if (together) {
+    dx_plan.tile = dw_plan.tile = dc::linear_tile_of_two(dx_size, dw_size, true, std::max(1, ctx->cu_count));
+    dx_plan.split = dc::linear_whole(dx_plan.tile, dx_size);
+    dw_plan.split = dc::linear_whole(dw_plan.tile, dw_size);
+  }
   if (scratch.bytes) DC_RETURN_IF(dc::ensure_partials(ctx, scratch.bytes));
   unsigned char* base = static_cast<unsigned char*>(ctx->partials);
   if (own_dz) s.dz = reinterpret_cast<bf16*>(base + dz.at);
@@ -1169,13 +1233,19 @@ DC_HIP_API int32_t dc_hip_linear_backward(dc_hip_ctx* ctx, const dc_linear_grad*
                       const ProductPlan& plan) {
     Epilogue ep{};
     ep.y = out, ep.y_stride = stride;
-    return product<false, true>(ctx, Operands{static_cast<const unsigned char*>(rows), b.p, pitch, b.pitch, (int32_t)m, (int32_t)p.k,
-                                              (int32_t)(2 * c), (int32_t)c, (int32_t)padded(p.k, 8)},
-                                ep, plan);
+    return Product{Operands{static_cast<const unsigned char*>(rows), b.p, pitch, b.pitch, (int32_t)m, (int32_t)p.k, (int32_t)(2 * c),
+                            (int32_t)c, (int32_t)padded(p.k, 8)},
+                   ep, plan};
   };
-  if (dx)
-    DC_RETURN_IF(gradient(own_dz ? static_cast<const void*>(s.dz) : p.dy, dz_pitch, p.m, p.n, w, p.dx, p.dx_stride, dx_plan));
-  if (dw) DC_RETURN_IF(gradient(s.dzt, 2 * s.t_pitch, p.n, p.m, x, p.dw, p.dw_stride, dw_plan));
+  const Product of_x = gradient(own_dz ? static_cast<const void*>(s.dz) : p.dy, dz_pitch, p.m, p.n, w, p.dx, p.dx_stride, dx_plan);
+  const Product of_w = gradient(s.dzt, 2 * s.t_pitch, p.n, p.m, x, p.dw, p.dw_stride, dw_plan);
+  auto run = [&](const Product* first, const Product* second) { return products<false, true>(ctx, {first, second}); };
+  if (together) {
+    DC_RETURN_IF(p.n >= p.m ? run(&of_x, &of_w) : run(&of_w, &of_x));  // (the longer sums first)
+  } else {
+    if (dx) DC_RETURN_IF(run(&of_x, nullptr));
+    if (dw) DC_RETURN_IF(run(&of_w, nullptr));
+  }
   return dbias && pieces > 1 ? dc::launch_column_sums(ctx, s.parts, p.dbias, pieces, p.n) : DC_OK;
 }
 

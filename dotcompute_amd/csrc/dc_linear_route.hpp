@@ -28,18 +28,43 @@ enum class LinearTile { k256, k128, k128x2, k64, k64x2, k64x4 };
 //   e4m3: 4096^3 58 / 66 / 92 / 96 / 110 / 157;  2048^3 31.6 / 15.2 / 14.6 / 13.8 / 16 / 24;  1537x2049x1024 22 / 11.2 / 11.1 / 9.0 / 11 / 19
 // (Three and four stages of LDS instead of two, and tiles of 128x64, 256x128 and 128x256, were no faster on any of these but
 // e4m3 2048^3, 13.5.)
-inline LinearTile linear_tile(int64_t m, int64_t n, int64_t c_bytes, int64_t a_pitch, int64_t b_pitch, bool rows_c, int64_t cus) {
-  auto tiles = [&](int64_t t) { return ((m + t - 1) / t) * ((n + t - 1) / t); };
-  auto fits = [&](int64_t t) { return t * a_pitch < kLinearRange && (rows_c || t * b_pitch < kLinearRange); };
-  const int64_t t256 = tiles(256), t128 = tiles(128), t64 = tiles(64), k = c_bytes / 2;
+struct LinearSize {
+  int64_t m, n, c_bytes;     // results, and bytes of c
+  int64_t a_pitch, b_pitch;  // bytes from row to row of the operands
+};
+inline int64_t linear_tiles(const LinearSize& s, int64_t side) { return ((s.m + side - 1) / side) * ((s.n + side - 1) / side); }
+inline bool linear_fits(const LinearSize& s, bool rows_c, int64_t side) {
+  return side * s.a_pitch < kLinearRange && (rows_c || side * s.b_pitch < kLinearRange);
+}
+// By the numbers of tiles and the elements of c (8-bit ones count half).
+inline LinearTile linear_tile_by(int64_t t256, int64_t t128, int64_t t64, int64_t k, bool fits256, bool fits128, int64_t cus) {
   const bool brief = (k <= 64 && (t256 > cus || 4 * t256 <= 3 * cus)) || (k <= 128 && t256 > 2 * cus);
-  if (fits(256) && 2 * t256 > cus && (t256 <= cus || 10 * t256 > 13 * cus) && !brief) return LinearTile::k256;
-  if (fits(128) && t128 > cus && !brief) return LinearTile::k128;
-  if (fits(128) && 4 * t128 > 3 * cus && k >= 1536) return LinearTile::k128x2;
-  if (fits(128) && 10 * t128 > 9 * cus && k >= 768) return LinearTile::k128;
+  if (fits256 && 2 * t256 > cus && (t256 <= cus || 10 * t256 > 13 * cus) && !brief) return LinearTile::k256;
+  if (fits128 && t128 > cus && !brief) return LinearTile::k128;
+  if (fits128 && 4 * t128 > 3 * cus && k >= 1536) return LinearTile::k128x2;
+  if (fits128 && 10 * t128 > 9 * cus && k >= 768) return LinearTile::k128;
   if (t64 > 2 * cus || k < 512) return LinearTile::k64;
   if (2 * t64 > cus || k < 2048) return LinearTile::k64x2;
   return LinearTile::k64x4;
+}
+inline LinearTile linear_tile(const LinearSize& s, bool rows_c, int64_t cus) {
+  return linear_tile_by(linear_tiles(s, 256), linear_tiles(s, 128), linear_tiles(s, 64), s.c_bytes / 2, linear_fits(s, rows_c, 256),
+                        linear_fits(s, rows_c, 128), cus);
+}
+// Two products in one launch, where their c are alike: the tile that the one with the longer c would take if it had as many
+// tiles as take the time of both; 128x2, of which a CU holds one, only where the shorter ones find room beside the longer.
+// Measured, both gradients of m, n, k with silu and dbias, us in two launches / in one: 2000,3000,1000 70.7 / 61.4 (128x2 71.0);
+// 1024^3 26.2 / 20.7; 2048^3 61.4 / 50.5; 1000,2000,1000 38.9 / 34.4; 2048,4096,1024 68.1 / 64.7 (128 67.9); 4096,4096,1024 105 /
+// 94; 8192,4096,1024 216 / 205; 8192,8192,2048 550 / 550; 200,400,512 16.8 / 13.4. Where one c is three times the other or more:
+// 1000,3000,1000 49.6 / 55.4, 3000,200,2500 48.6 / 87, 64,4096,4096 32.2 / 36.6.
+inline bool linear_alike(const LinearSize& a, const LinearSize& b) { return a.c_bytes <= 2 * b.c_bytes && b.c_bytes <= 2 * a.c_bytes; }
+inline LinearTile linear_tile_of_two(const LinearSize& a, const LinearSize& b, bool rows_c, int64_t cus) {
+  const LinearSize &l = a.c_bytes >= b.c_bytes ? a : b, &s = a.c_bytes >= b.c_bytes ? b : a;
+  auto tiles = [&](int64_t side) { return linear_tiles(l, side) + (linear_tiles(s, side) * s.c_bytes + l.c_bytes - 1) / l.c_bytes; };
+  auto fits = [&](int64_t side) { return linear_fits(a, rows_c, side) && linear_fits(b, rows_c, side); };
+  int64_t t128 = tiles(128);
+  if (t128 <= cus && 4 * t128 > 3 * cus && linear_tiles(s, 128) > (cus - linear_tiles(l, 128)) * (l.c_bytes / s.c_bytes)) t128 = cus + 1;
+  return linear_tile_by(tiles(256), t128, tiles(64), l.c_bytes / 2, fits(256), fits(128), cus);
 }
 
 inline int64_t linear_tile_side(LinearTile t) {
@@ -56,9 +81,12 @@ inline int64_t linear_tile_groups(LinearTile t) {
 struct LinearSplit {
   int64_t parts, turns;
 };
-inline LinearSplit linear_split(LinearTile tile, int64_t m, int64_t n, int64_t c_bytes, int64_t cus) {
-  const int64_t side = linear_tile_side(tile), tiles = ((m + side - 1) / side) * ((n + side - 1) / side);
-  const int64_t step = 128 * linear_tile_groups(tile), all = (c_bytes + step - 1) / step;
+inline LinearSplit linear_whole(LinearTile tile, const LinearSize& s) {
+  const int64_t step = 128 * linear_tile_groups(tile);
+  return {1, (s.c_bytes + step - 1) / step};
+}
+inline LinearSplit linear_split(LinearTile tile, const LinearSize& s, int64_t cus) {
+  const int64_t side = linear_tile_side(tile), tiles = linear_tiles(s, side), all = linear_whole(tile, s).turns;
   const int64_t most = tiles > 0 ? (side == 64 && all >= 32 ? 2 : 1) * cus / tiles : 1;
   if (all < 8 || most < 2) return {1, all};
   const int64_t turns = (all + most - 1) / most < 3 ? 3 : (all + most - 1) / most;

@@ -275,6 +275,27 @@ def test_linear_backward_in_parts(ctx, activation):
     run_backward(ctx, 100, 136, 72, activation, dx=False, dw=False)
 
 
+@pytest.mark.parametrize("stride", [-8, 0, 3, 1 << 40])
+def test_the_stride_of_a_single_row_says_nothing(ctx, stride):
+    rng = np.random.default_rng(5)
+    x, w, dy = bf16(rng, (1, 136)), bf16(rng, (72, 136)), bf16(rng, (1, 72))
+    a = {name: ctx.to_device(v) for name, v in dict(x=x, w=w, dy=dy).items()}
+    y, dx, dw = ctx.empty((1, 72), np.uint16), ctx.empty((1, 136), np.uint16), ctx.empty((72, 136), np.uint16)
+    got = []
+    for one in ({}, {"stride": stride}):
+        s = {name + "_stride": v for name in ("x", "y", "dy", "dx") for v in one.values()}
+        ctx.linear(hip.Linear.of(a["x"], a["w"], y, **{k: v for k, v in s.items() if k in ("x_stride", "y_stride")}))
+        ctx.linear_backward(hip.LinearGrad.of(a["dy"], a["x"], a["w"], dx=dx, dw=dw, **{k: v for k, v in s.items() if k != "y_stride"}))
+        # one output: w is the single row
+        w1 = hip.DeviceArray(ctx, a["w"].ptr, 272, np.dtype(np.uint16), (1, 136))
+        dw1, dy1, dx1 = ctx.empty((1, 136), np.uint16), ctx.to_device(dy.reshape(72, 1)), ctx.empty((72, 136), np.uint16)
+        ctx.linear_backward(hip.LinearGrad.of(dy1, a["w"], w1, dx=dx1, dw=dw1, **{k + "_stride": v for k in ("w", "dw") for v in one.values()}))
+        ctx.synchronize()
+        got.append([t.to_host() for t in (y, dx, dw, dw1, dx1)])
+    assert all(np.array_equal(p, q) for p, q in zip(*got))
+    within(wide(got[0][4]), wide(dy).T @ wide(w[:1]), 2.0 ** -8 * np.abs(wide(dy).T @ wide(w[:1])), "dx of one output")
+
+
 def test_linear_backward_of_nothing(ctx):
     """No rows: dw and dbias are empty sums; no outputs: dx is."""
     e, w, db = ctx.empty(8, np.uint16), ctx.to_device(np.full((9, 5), 7, np.uint16)), ctx.to_device(np.full(9, 7.0, np.float32))
