@@ -154,6 +154,16 @@ __device__ inline void store_bf16(bf16* q, int64_t left, const float (&v)[E]) {
   }
 }
 
+// Eight of them as they lie in memory.
+__device__ inline dc::u32x4 load_raw_some(const bf16* q, int64_t left) {
+  if (left >= 8) return dc::load_raw(q);
+  dc::u32x4 w = {0, 0, 0, 0};
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (e < left) w[e / 2] |= (uint32_t)q[e].bits << (16 * (e & 1));
+  return w;
+}
+
 // What the results of E neighbouring columns j.. share, whatever their row: read once.
 template <int E>
 struct Columns {
@@ -182,6 +192,7 @@ struct Results {
     if (p.residual) load_bf16(p.residual + i * p.residual_stride + c.j, c.left, residual);
     if (p.a_scales) scale = p.a_scales[i];
   }
+  template <bool kResidual = true>
   __device__ inline void finish(const Epilogue& p, const Columns<E>& c, int64_t i, float (&z)[E], int part = 0) const {
     if (p.a_scales)
 #pragma unroll
@@ -191,7 +202,7 @@ struct Results {
       for (int e = 0; e < E; ++e) z[e] += c.bias[e];
     if (p.pre) store_bf16(p.pre + i * p.pre_stride + c.j, c.left, z);
     activate(p.act, z);
-    if (p.residual)
+    if (kResidual && p.residual)
 #pragma unroll
       for (int e = 0; e < E; ++e) z[e] += residual[e];
     if (p.y_f32) {
@@ -500,37 +511,65 @@ __global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void pro
     }
   }
 
-  // acc[mt][nt][v]: i = r, j = 8·(v / 4) + 4·h + v % 4 of the 32×32 block. A wave's 32 rows of 32·kNT sums at a time.
-  constexpr int kCols = 32 * kNT, kPitch = kCols + 4, kLanes = kCols / 8;
+  // acc[mt][nt][v]: i = r, j = 8·(v / 4) + 4·h + v % 4 of the 32×32 block. A wave's 32 rows of 32·kNT sums at a time, with the
+  // rows' scales in the columns past them; a lane's residual is asked for kTurns turns of the loop ahead.
+  constexpr int kCols = 32 * kNT, kPitch = kCols + 4, kLanes = kCols / 8, kRowsTurn = 64 / kLanes, kTurns = 32 / kRowsTurn;
   static_assert(sizeof(Smem) >= kWaves * 32 * kPitch * sizeof(float), "the waves' blocks fit in the buffers");
   float* own = reinterpret_cast<float*>(&sms[0]) + wave * 32 * kPitch;
+  const int i0 = m0 + wm * kMT * 32, own_row = lane / kLanes, own_col = 8 * (lane % kLanes);
   Columns<8> cols;
-  cols.read(ep, n0 + wn * kCols + 8 * (lane % kLanes), o.n);
+  cols.read(ep, n0 + wn * kCols + own_col, o.n);
+  float scales[kMT];
+  if constexpr (kFp8)
 #pragma unroll
-  for (int mt = 0; mt < kMT; ++mt) {
+    for (int mt = 0; mt < kMT; ++mt) scales[mt] = ep.a_scales ? ep.a_scales[min(i0 + 32 * mt + r, o.m - 1)] : 1.0f;
+  auto write = [&](auto RESIDUAL) __attribute__((always_inline)) {
+    constexpr bool kResidual = decltype(RESIDUAL)::value;
+    dc::u32x4 ahead[kTurns];
+    auto ask = [&](int row) __attribute__((always_inline)) {
+      dc::u32x4 w = {0, 0, 0, 0};
+      if (ep.residual && i0 + row < o.m && cols.left > 0) w = load_raw_some(ep.residual + (i0 + row) * ep.residual_stride + cols.j, cols.left);
+      return w;
+    };
+    if constexpr (kResidual)
 #pragma unroll
-    for (int nt = 0; nt < kNT; ++nt)
+      for (int q = 0; q < kTurns; ++q) ahead[q] = ask(own_row + q * kRowsTurn);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const f32x4 v = {acc[mt][nt][4 * q], acc[mt][nt][4 * q + 1], acc[mt][nt][4 * q + 2], acc[mt][nt][4 * q + 3]};
-        *reinterpret_cast<f32x4*>(own + r * kPitch + 32 * nt + 8 * q + 4 * h) = v;
-      }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    for (int mt = 0; mt < kMT; ++mt) {
+#pragma unroll
+      for (int nt = 0; nt < kNT; ++nt)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const f32x4 v = {acc[mt][nt][4 * q], acc[mt][nt][4 * q + 1], acc[mt][nt][4 * q + 2], acc[mt][nt][4 * q + 3]};
+          *reinterpret_cast<f32x4*>(own + r * kPitch + 32 * nt + 8 * q + 4 * h) = v;
+        }
+      if constexpr (kFp8) own[r * kPitch + kCols] = scales[mt];
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll 1
-    for (int r0 = 0; r0 < 32; r0 += 64 / kLanes) {
-      const int row = r0 + lane / kLanes;
-      const int64_t i = m0 + (wm * kMT + mt) * 32 + row;
-      float z[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) z[e] = own[row * kPitch + 8 * (lane % kLanes) + e];
-      if (i < o.m && cols.left > 0) {
+      for (int r0 = 0; r0 < 32; r0 += kRowsTurn) {
+        const int row = r0 + own_row;
+        const int64_t i = i0 + 32 * mt + row;
         Results<8> out;
-        out.read(ep, cols, i);
-        out.finish(ep, cols, i, z, part);
+        if constexpr (kResidual) {
+          dc::unpack(ahead[0], out.residual);
+#pragma unroll
+          for (int q = 0; q + 1 < kTurns; ++q) ahead[q] = ahead[q + 1];
+          if (mt + 1 < kMT) ahead[kTurns - 1] = ask(32 * mt + row + 32);
+        }
+        if constexpr (kFp8) out.scale = own[row * kPitch + kCols];
+        float z[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[e] = own[row * kPitch + own_col + e];
+        if (i < o.m && cols.left > 0) out.template finish<kResidual>(ep, cols, i, z, part);
       }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  }
+  };
+  // (8 bits go one way for both: with two the compiler spills, and 4096×8192×4096 measured 115.9 us, with a residual 123.5, where
+  // this is 113.6 and 121.7. Residual asked for in the turn that needs it: 126.9; bf16 4096^3 120.2, as it is now 117.3.)
+  if constexpr (kFp8) write(std::true_type{});
+  else if (!kRowsC && ep.residual) write(std::true_type{});
+  else write(std::false_type{});
 }
 
 // ---- few rows ----------------------------------------------------------------------------------------
