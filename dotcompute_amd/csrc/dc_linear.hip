@@ -5,11 +5,18 @@
 //
 // Kernels:
 //   - product_kernel: D[i][j] = sum_c A(i, c) B(j, c) in tiles on the matrix cores. A's rows run along c. B's do too
-//     (forward), or are the rows c of a row-major [c][j] matrix (the gradients).
+//     (forward), or are the rows c of a row-major [c][j] matrix (the gradients, both in one launch where their c are alike).
+//   - join_kernel: the results from the sums over parts of c, where few tiles have long sums.
 //   - few_rows_kernel, few_rows_any_kernel: forward with few rows of x.
 //   - slope_kernel: dz and its transpose in bf16 (what the two gradients' products run along), and dbias's parts.
 //   - pack_kernel: rows that the direct-to-LDS loads cannot take (not 16-byte aligned, or no whole number of
 //     16 bytes) copied to ones padded with zeros.
+//
+// What is rounded: results to their type once, from float32 sums; `pre` to bf16 from the z that the activation also takes
+// unrounded; dz to bf16, as the matrix cores take no float32 at a useful rate (dbias adds it unrounded). The 8-bit matrix instructions
+// add 64 or 128 products at a time and cut each at 2^-13 of the largest of a lane's share of them (measured with pairs of powers of
+// two; sums of whole numbers are exact): far less than the 2^-4 by which rounding to e4m3 may have moved each operand, so
+// their full rate is taken. Their sums are float32 from there on.
 #include <algorithm>
 
 #include <cstddef>
@@ -229,6 +236,12 @@ struct Results {
 // The instructions get B's fragment first and A's second, so a lane ends up with four neighbouring j of one i: the
 // sums go through LDS once more, a wave at a time in its own part, and the epilogue reads and writes rows of 8 results
 // a lane, 64 or 128 bytes a row, whatever the activation, in one short loop.
+//
+// Bound by the matrix cores (by the clock they hold) in 256-tiles: bf16 8192^3 842-853 us (1.29-1.31 PFLOP/s), 876 with tanh-gelu
+// and pre; 8192×2048×8192 213; both gradients of 8192,8192,2048 445 for 550 GFLOP; e4m3 4096×8192×4096 113.6 (2.42). What is left is each round's end: the
+// 256 tiles of a round write 33.5 MB at once, and their epilogue has no products beside it (8-14 us a round; a persistent workgroup that
+// loads its next tile over its epilogue gained 2-3 % in bf16 and spilled in 8 bits). Smaller tiles are bound by the 28
+// bytes a cycle that a CU's direct-to-LDS loads bring, and by launch and latency: 2048^3 22.7, 1537×2049×1024 13.7.
 constexpr int kTileBytes = 128;  // of c
 constexpr int kRange = dc::kLinearRange;
 constexpr uint32_t kPast = 0x80000000u;  // a byte offset past every range: loads zeros
@@ -869,7 +882,9 @@ __global__ __launch_bounds__(64 * W) void few_rows_kernel(Operands o, Epilogue e
 // ---- what the gradients' products run along ---------------------------------------------------------------
 // dz = dy act'(pre) over 64×64 pieces: dz itself (pitch dz_pitch, columns from n to there zero), its transpose (pitch
 // t_pitch, columns from m to there zero) through LDS, and the piece's column sums, unrounded. A thread holds two
-// neighbouring rows of 8 columns, so the transpose's LDS words are pairs of rows.
+// neighbouring rows of 8 columns, so the transpose's LDS words are pairs of rows. Bound by memory: 8192×8192 with silu, dz, its
+// transpose and parts 98-103 us (537 MB, 5.2-5.5 TB/s); 2000×3000 with gelu 12.8, half of it the slope's arithmetic. (All four
+// loads in flight at once, by addresses that need no branch: 13.2 for 12.2 without the writes, 2000×3000.)
 struct SlopeArgs {
   const bf16 *dy, *pre;
   bf16 *dz, *dzt;  // either may be NULL
@@ -932,6 +947,7 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeArgs a) {
 }
 
 // The results from the sums over `count` parts of c: a lane takes eight neighbouring columns, and adds the parts in order.
+// (The parts have just been written, and come from the caches.)
 struct JoinArgs {
   const float* parts;  // [count][m][pitch]
   int64_t m, n, pitch;
@@ -958,7 +974,8 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a, Epilogue ep) {
   }
 }
 
-// Rows of `bytes` bytes at any alignment to rows of `to_pitch` (a multiple of 16), padded with zeros.
+// Rows of `bytes` bytes at any alignment to rows of `to_pitch` (a multiple of 16), padded with zeros. Bound by launch and latency
+// at ordinary sizes: 1537 and 2049 rows of 2046 bytes, both operands in one launch, 5.5-8 us, a third of the product's call.
 struct PackJob {
   const unsigned char* from;
   unsigned char* to;
