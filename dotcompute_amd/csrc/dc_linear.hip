@@ -5,7 +5,7 @@
 //
 // Kernels:
 //   - product_kernel: D[i][j] = sum_c A(i, c) B(j, c) in tiles on the matrix cores. A's rows run along c. B's do too
-//     (forward), or are the rows c of a row-major [c][j] matrix (the gradients, both in one launch where their c are alike).
+//     (forward), or are the rows c of a row-major [c][j] matrix (the gradients, both in one launch).
 //   - join_kernel: the results from the sums over parts of c, where few tiles have long sums.
 //   - few_rows_kernel, few_rows_any_kernel: forward with few rows of x.
 //   - slope_kernel: dz and its transpose in bf16 (what the two gradients' products run along), and dbias's parts.
@@ -278,7 +278,7 @@ __device__ inline void load_block(const unsigned char* base, unsigned char* to, 
 }
 
 // The products of one launch. Workgroups take the first's tiles, part of c by part, then the second's: the two
-// gradients of a layer have no more tiles than CUs each where it is of ordinary size, and run side by side.
+// gradients of a layer seldom fill the chip by themselves, and a launch saved is 3-5 us.
 struct Job {
   Operands o;
   Epilogue ep;
@@ -948,19 +948,24 @@ __global__ __launch_bounds__(256) void slope_kernel(SlopeArgs a) {
 
 // The results from the sums over `count` parts of c: a lane takes eight neighbouring columns, and adds the parts in order.
 // (The parts have just been written, and come from the caches.)
-struct JoinArgs {
+struct JoinJob {
   const float* parts;  // [count][m][pitch]
   int64_t m, n, pitch;
   int32_t count;
+  Epilogue ep;
 };
-__global__ __launch_bounds__(256) void join_kernel(JoinArgs a, Epilogue ep) {
+struct JoinArgs {
+  JoinJob job[2];
+};
+__global__ __launch_bounds__(256) void join_kernel(JoinArgs args) {
+  const JoinJob& a = args.job[blockIdx.y];
   const int64_t across = (a.n + 7) / 8, total = a.m * across, step = (int64_t)gridDim.x * 256;
   for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < total; t += step) {
-    const int64_t i = t / across, j = 8 * (t - i * across);
+    const int64_t i = total <= UINT32_MAX ? (int64_t)((uint32_t)t / (uint32_t)across) : t / across, j = 8 * (t - i * across);
     Columns<8> cols;
     Results<8> out;
-    cols.read(ep, j, a.n);
-    out.read(ep, cols, i);
+    cols.read(a.ep, j, a.n);
+    out.read(a.ep, cols, i);
     const f32x4* q = reinterpret_cast<const f32x4*>(a.parts + i * a.pitch + j);
     f32x4 lo = q[0], hi = q[1];
 #pragma unroll 4
@@ -970,7 +975,7 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs a, Epilogue ep) {
       hi += r[1];
     }
     float z[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
-    out.finish(ep, cols, i, z);
+    out.finish(a.ep, cols, i, z);
   }
 }
 
@@ -1021,10 +1026,7 @@ struct ProductPlan {
   dc::LinearTile tile;
   dc::LinearSplit split;
   size_t at = 0;
-  ProductPlan(dc_hip_ctx* ctx, Scratch& s, const dc::LinearSize& size, bool rows_c) {
-    const int64_t cus = std::max(1, ctx->cu_count);
-    tile = dc::linear_tile(size, rows_c, cus);
-    split = dc::linear_split(tile, size, cus);
+  ProductPlan(Scratch& s, const dc::LinearSize& size, dc::LinearTile t, const dc::LinearSplit& c) : tile(t), split(c) {
     if (split.parts > 1) at = s.take(split.parts * size.m * padded(size.n, 8) * (int64_t)sizeof(float));
   }
 };
@@ -1072,11 +1074,19 @@ int32_t launch_products(dc_hip_ctx* ctx, const Product* const (&p)[kJobs<kRowsC>
   return DC_OK;
 }
 
-int32_t join(dc_hip_ctx* ctx, const Product& p) {
-  if (p.plan.split.parts == 1) return DC_OK;
-  const int64_t groups = (p.o.m * (p.pitch() / 8) + 255) / 256;
-  join_kernel<<<(unsigned)std::min<int64_t>(groups, 1 << 16), 256, 0, ctx->stream>>>(
-      JoinArgs{p.parts(ctx), p.o.m, p.o.n, p.pitch(), (int32_t)p.plan.split.parts}, p.ep);
+// Adds the parts of those (at most two) products that have them, in one launch.
+int32_t join(dc_hip_ctx* ctx, const Product* const* products, int count) {
+  JoinArgs args{};
+  int jobs = 0;
+  int64_t most = 0;
+  for (int i = 0; i < count; ++i) {
+    if (!products[i] || products[i]->plan.split.parts == 1) continue;
+    const Product& p = *products[i];
+    args.job[jobs++] = JoinJob{p.parts(ctx), p.o.m, p.o.n, p.pitch(), (int32_t)p.plan.split.parts, p.ep};
+    most = std::max(most, (p.o.m * (p.pitch() / 8) + 255) / 256);
+  }
+  if (jobs == 0) return DC_OK;
+  join_kernel<<<dim3((unsigned)std::min<int64_t>(most, 1 << 16), (unsigned)jobs), 256, 0, ctx->stream>>>(args);
   return dc::last_launch_status();
 }
 
@@ -1093,9 +1103,7 @@ int32_t products(dc_hip_ctx* ctx, const Product* const (&p)[kJobs<kRowsC>], cons
     case LinearTile::k64x2: status = launch_products<64, 64, 2, 2, 2, kFp8, kRowsC>(ctx, p, columns); break;
     case LinearTile::k64x4: status = launch_products<64, 64, 2, 2, 4, kFp8, kRowsC>(ctx, p, columns); break;
   }
-  for (const Product* q : p)
-    if (q && status == DC_OK) status = join(ctx, *q);
-  return status;
+  return status == DC_OK ? join(ctx, p, kJobs<kRowsC>) : status;
 }
 
 // NB blocks of 16 outputs and XB blocks of 8 rows of x, W waves, and as many stages as fit in `kLds` KiB of LDS.
@@ -1240,7 +1248,9 @@ DC_HIP_API int32_t dc_hip_linear(dc_hip_ctx* ctx, const dc_linear* args) {
     DC_RETURN_IF(lay_out_all());
     return fp8 ? few_rows<true>(ctx, o, ep) : few_rows<false>(ctx, o, ep);
   }
-  const ProductPlan plan(ctx, scratch, {p.m, p.n, o.c_bytes, x.width(), w.width()}, false);
+  const dc::LinearSize shape{p.m, p.n, o.c_bytes, x.width(), w.width()};
+  const dc::LinearPlan best = dc::linear_plan(shape, {false, fp8}, std::max(1, ctx->cu_count));
+  const ProductPlan plan(scratch, shape, best.tile, best.split);
   DC_RETURN_IF(lay_out_all());
   const Product all{o, ep, plan};
   return fp8 ? products<true, false>(ctx, {&all}) : products<false, false>(ctx, {&all});
@@ -1299,13 +1309,18 @@ DC_HIP_API int32_t dc_hip_linear_backward(dc_hip_ctx* ctx, const dc_linear_grad*
   if (dbias && pieces > 1) at_parts = scratch.take(pieces * p.n * (int64_t)sizeof(float));
   const int64_t dz_pitch = own_dz ? 2 * s.dz_pitch : dz.pitch;
   const dc::LinearSize dx_size{p.m, p.k, 2 * p.n, dz_pitch, w.width()}, dw_size{p.n, p.k, 2 * p.m, 2 * s.t_pitch, x.width()};
-  ProductPlan dx_plan(ctx, scratch, dx_size, true), dw_plan(ctx, scratch, dw_size, true);
-  const bool together = dx && dw && dc::linear_alike(dx_size, dw_size) && dx_plan.split.parts == 1 && dw_plan.split.parts == 1;
+  const int64_t cus = std::max(1, ctx->cu_count);
+  const bool together = dx && dw;
+  dc::LinearPlan dx_best{dc::LinearTile::k64, {1, 1}, 0.0}, dw_best = dx_best;
   if (together) {
-    dx_plan.tile = dw_plan.tile = dc::linear_tile_of_two(dx_size, dw_size, true, std::max(1, ctx->cu_count));
-    dx_plan.split = dc::linear_whole(dx_plan.tile, dx_size);
-    dw_plan.split = dc::linear_whole(dw_plan.tile, dw_size);
+    const dc::LinearPair pair = dc::linear_plan_of_two(dx_size, dw_size, cus);
+    dx_best = {pair.tile, pair.a, pair.time}, dw_best = {pair.tile, pair.b, pair.time};
+  } else if (dx) {
+    dx_best = dc::linear_plan(dx_size, {true, false}, cus);
+  } else if (dw) {
+    dw_best = dc::linear_plan(dw_size, {true, false}, cus);
   }
+  const ProductPlan dx_plan(scratch, dx_size, dx_best.tile, dx_best.split), dw_plan(scratch, dw_size, dw_best.tile, dw_best.split);
   if (scratch.bytes) DC_RETURN_IF(dc::ensure_partials(ctx, scratch.bytes));
   unsigned char* base = static_cast<unsigned char*>(ctx->partials);
   if (own_dz) s.dz = reinterpret_cast<bf16*>(base + dz.at);
@@ -1330,11 +1345,10 @@ DC_HIP_API int32_t dc_hip_linear_backward(dc_hip_ctx* ctx, const dc_linear_grad*
   const Product of_w = gradient(s.dzt, 2 * s.t_pitch, p.n, p.m, x, p.dw, p.dw_stride, dw_plan);
   ColumnParts columns{};
   if (dbias && pieces > 1) columns = {s.parts, p.dbias, (int32_t)pieces, (int32_t)p.n};
-  auto run = [&](const Product* first, const Product* second, const ColumnParts& c) { return products<false, true>(ctx, {first, second}, c); };
-  if (together) return p.n >= p.m ? run(&of_x, &of_w, columns) : run(&of_w, &of_x, columns);  // (the longer sums first)
-  if (dx) DC_RETURN_IF(run(&of_x, nullptr, dw ? ColumnParts{} : columns));
-  if (dw) return run(&of_w, nullptr, columns);
-  return !dx && columns.n > 0 ? dc::launch_column_sums(ctx, s.parts, p.dbias, pieces, p.n) : DC_OK;
+  auto run = [&](const Product* first, const Product* second) { return products<false, true>(ctx, {first, second}, columns); };
+  if (together) return p.n >= p.m ? run(&of_x, &of_w) : run(&of_w, &of_x);  // (the longer sums first)
+  if (dx || dw) return run(dx ? &of_x : &of_w, nullptr);
+  return columns.n > 0 ? dc::launch_column_sums(ctx, s.parts, p.dbias, pieces, p.n) : DC_OK;
 }
 
 }  // extern "C"

@@ -3,6 +3,7 @@
 #pragma once
 
 #include <cstdint>
+#include <initializer_list>
 
 namespace dc {
 
@@ -15,57 +16,8 @@ static_assert(64 * kLinearPitch < kLinearRange && 2 * kLinearWidth <= kLinearPit
 
 // Tiles, square, and groups of waves that take the steps along c in turn.
 enum class LinearTile { k256, k128, k128x2, k64, k64x2, k64x4 };
-
-// By rounds of the tiles over the CUs, as dc_gemm_route.hpp's rule, measured again (results m x n, sums over c; us for
-// tiles of 256 / 128 / 128x2 / 64 / 64x2 / 64x4, w by rows of c where it says so):
-//   bf16: 4096x4096x1024 34.5 / 39.7 / 51.7 / 52.4 / 59.4 / 94;  5120x5120x1024 58.8 / 64.4 / 89 / 80 / 92 / 145
-//   2000x3000x1000 30.5 / 21.6 / 29.4 / 27.8 / 28.7 / 41;  2048^3 44 / 25.3 / 22.7 / 25.6 / 27.4 / 38
-//   2048x2048x816 25.4 / 13.3 / 13.8 / 15.2 / 16.1 / 23;  2048x2048x512 18.6 / 9.7 / 10.3 / 9.1 / 11.3 / 18
-//   1537x2049x1024 27.4 / 15.2 / 14.8 / 13.8 / 17.7 / 26;  1024^3 26 / 11.7 / 11.7 / 6.9 / 6.4 / 6.5
-//   rows c: 8192x2048x8192 208 / 244 / 278 / 358 / 377 / 529;  4096x1024x4096 86 / 47 / 39.9 / 49 / 52 / 73
-//   2000x1000x3000 71 / 41 / 36 / 29.1 / 27.9 / 37;  3000x1000x2000 51 / 30.2 / 26.5 / 27.9 / 33.8 / 38
-//   512x512x4096 83 / 34 / 29.8 / 32.6 / 24.1 / 20.2;  64x2048x8192 155 / 80 / 60 / 61 / 43.8 / 34.9
-//   e4m3: 4096^3 58 / 66 / 92 / 96 / 110 / 157;  2048^3 31.6 / 15.2 / 14.6 / 13.8 / 16 / 24;  1537x2049x1024 22 / 11.2 / 11.1 / 9.0 / 11 / 19
-// (Three and four stages of LDS instead of two, and tiles of 128x64, 256x128 and 128x256, were no faster on any of these but
-// e4m3 2048^3, 13.5.)
-struct LinearSize {
-  int64_t m, n, c_bytes;     // results, and bytes of c
-  int64_t a_pitch, b_pitch;  // bytes from row to row of the operands
-};
-inline int64_t linear_tiles(const LinearSize& s, int64_t side) { return ((s.m + side - 1) / side) * ((s.n + side - 1) / side); }
-inline bool linear_fits(const LinearSize& s, bool rows_c, int64_t side) {
-  return side * s.a_pitch < kLinearRange && (rows_c || side * s.b_pitch < kLinearRange);
-}
-// By the numbers of tiles and the elements of c (8-bit ones count half).
-inline LinearTile linear_tile_by(int64_t t256, int64_t t128, int64_t t64, int64_t k, bool fits256, bool fits128, int64_t cus) {
-  const bool brief = (k <= 64 && (t256 > cus || 4 * t256 <= 3 * cus)) || (k <= 128 && t256 > 2 * cus);
-  if (fits256 && 2 * t256 > cus && (t256 <= cus || 10 * t256 > 13 * cus) && !brief) return LinearTile::k256;
-  if (fits128 && t128 > cus && !brief) return LinearTile::k128;
-  if (fits128 && 4 * t128 > 3 * cus && k >= 1536) return LinearTile::k128x2;
-  if (fits128 && 10 * t128 > 9 * cus && k >= 768) return LinearTile::k128;
-  if (t64 > 2 * cus || k < 512) return LinearTile::k64;
-  if (2 * t64 > cus || k < 2048) return LinearTile::k64x2;
-  return LinearTile::k64x4;
-}
-inline LinearTile linear_tile(const LinearSize& s, bool rows_c, int64_t cus) {
-  return linear_tile_by(linear_tiles(s, 256), linear_tiles(s, 128), linear_tiles(s, 64), s.c_bytes / 2, linear_fits(s, rows_c, 256),
-                        linear_fits(s, rows_c, 128), cus);
-}
-// Two products in one launch, where their c are alike: the tile that the one with the longer c would take if it had as many
-// tiles as take the time of both; 128x2, of which a CU holds one, only where the shorter ones find room beside the longer.
-// Measured, both gradients of m, n, k with silu and dbias, us in two launches / in one: 2000,3000,1000 70.7 / 61.4 (128x2 71.0);
-// 1024^3 26.2 / 20.7; 2048^3 61.4 / 50.5; 1000,2000,1000 38.9 / 34.4; 2048,4096,1024 68.1 / 64.7 (128 67.9); 4096,4096,1024 105 /
-// 94; 8192,4096,1024 216 / 205; 8192,8192,2048 550 / 550; 200,400,512 16.8 / 13.4. Where one c is three times the other or more:
-// 1000,3000,1000 49.6 / 55.4, 3000,200,2500 48.6 / 87, 64,4096,4096 32.2 / 36.6.
-inline bool linear_alike(const LinearSize& a, const LinearSize& b) { return a.c_bytes <= 2 * b.c_bytes && b.c_bytes <= 2 * a.c_bytes; }
-inline LinearTile linear_tile_of_two(const LinearSize& a, const LinearSize& b, bool rows_c, int64_t cus) {
-  const LinearSize &l = a.c_bytes >= b.c_bytes ? a : b, &s = a.c_bytes >= b.c_bytes ? b : a;
-  auto tiles = [&](int64_t side) { return linear_tiles(l, side) + (linear_tiles(s, side) * s.c_bytes + l.c_bytes - 1) / l.c_bytes; };
-  auto fits = [&](int64_t side) { return linear_fits(a, rows_c, side) && linear_fits(b, rows_c, side); };
-  int64_t t128 = tiles(128);
-  if (t128 <= cus && 4 * t128 > 3 * cus && linear_tiles(s, 128) > (cus - linear_tiles(l, 128)) * (l.c_bytes / s.c_bytes)) t128 = cus + 1;
-  return linear_tile_by(tiles(256), t128, tiles(64), l.c_bytes / 2, fits(256), fits(128), cus);
-}
+constexpr LinearTile kLinearTiles[] = {LinearTile::k256, LinearTile::k128,  LinearTile::k128x2,
+                                       LinearTile::k64,  LinearTile::k64x2, LinearTile::k64x4};
 
 inline int64_t linear_tile_side(LinearTile t) {
   return t == LinearTile::k256 ? 256 : t == LinearTile::k128 || t == LinearTile::k128x2 ? 128 : 64;
@@ -74,23 +26,133 @@ inline int64_t linear_tile_groups(LinearTile t) {
   return t == LinearTile::k64x4 ? 4 : t == LinearTile::k128x2 || t == LinearTile::k64x2 ? 2 : 1;
 }
 
-// c in `parts` of `turns` tiles a group, whose sums are added by a kernel of their own: where the tiles leave CUs idle and their
-// sums are long; two workgroups a CU where they are longer still. Measured, us in one part / two workgroups a CU / four (results m x n,
-// sums over c): bf16 2515x256x5120 30.2 / 21.0 / 24.9; 1024x1024x4096 22.5 / 20.3 / 26.2; 1024^3 6.4 / 13.5 / 17.4; e4m3 1024x1024x4096
-// 9.7 / 16.2 / 18.4. And with many parts, before / now: 315x256x5168 27 / 11.4, 64x2048x8192 (rows c) 34.9 / 14.4.
+struct LinearSize {
+  int64_t m, n, c_bytes;     // results, and bytes of c
+  int64_t a_pitch, b_pitch;  // bytes from row to row of the operands
+};
+inline int64_t linear_tiles(const LinearSize& s, LinearTile t) {
+  const int64_t side = linear_tile_side(t);
+  return ((s.m + side - 1) / side) * ((s.n + side - 1) / side);
+}
+inline bool linear_fits(const LinearSize& s, bool rows_c, LinearTile t) {
+  const int64_t side = linear_tile_side(t);
+  return side * s.a_pitch < kLinearRange && (rows_c || side * s.b_pitch < kLinearRange);
+}
+
+// c in `parts` of `turns` tiles a group of waves; the sums of more than one part are added by a kernel of their own.
 struct LinearSplit {
   int64_t parts, turns;
 };
-inline LinearSplit linear_whole(LinearTile tile, const LinearSize& s) {
-  const int64_t step = 128 * linear_tile_groups(tile);
-  return {1, (s.c_bytes + step - 1) / step};
-}
-inline LinearSplit linear_split(LinearTile tile, const LinearSize& s, int64_t cus) {
-  const int64_t side = linear_tile_side(tile), tiles = linear_tiles(s, side), all = linear_whole(tile, s).turns;
-  const int64_t most = tiles > 0 ? (side == 64 && all >= 32 ? 2 : 1) * cus / tiles : 1;
-  if (all < 8 || most < 2) return {1, all};
-  const int64_t turns = (all + most - 1) / most < 3 ? 3 : (all + most - 1) / most;
+inline LinearSplit linear_split(LinearTile tile, const LinearSize& s, int64_t parts) {
+  const int64_t step = 128 * linear_tile_groups(tile), all = (s.c_bytes + step - 1) / step, turns = (all + parts - 1) / parts;
   return {(all + turns - 1) / turns, turns};
+}
+
+// The tile, and the parts of c, are those with the least time by this estimate, in us: a CU's workgroups take turns of 128 bytes of c, each
+// bound by the loads of the two operands or the matrix cores, or, where few are there to cover it, by a turn's
+// latency; each workgroup has its epilogue, each round of workgroups its start, and parts of c their sums' way through memory and
+// the adding kernel. The numbers were fitted to the times of all tiles with 1 to 16 parts on 124 shapes (bf16, e4m3, B by
+// rows of c; 64 to 16384 results a side, c 64 to 8192): what it picks takes 1.2 % more time than the best in the mean, where
+// rules by the number of tiles took 6.4 %. Measured, us, those rules / this / the best: bf16 1500×1500×6000 67.5 / 48.9 / 48.9
+// (128-tiles, 3 parts), 300×1024×1024 9.2 / 6.1 / 6.1, 2048^3 23.3 / 23.5 / 23.3, 7958×332×5760 51.7 / 61.6 / 51.7; by rows of c 545×3768×5632
+// 66.7 / 52.1 / 52.1 (256-tiles, 4 parts), 8192×2048×8192 220 / 211 / 211; e4m3 128×4096×4096 12.1 / 9.0 / 9.0.
+struct LinearCost {
+  double call, groups;            // of a launch, and more for each further group of waves
+  double start, more_start;       // of a round, and for each further 64-tile's worth of loads in a turn
+  double end[3];                  // of a workgroup of side 64, 128, 256
+  double loads[2], latency, more_latency;  // of a turn, by 64-tile's worths; loads of 64-tiles of small operands, and else
+  double uneven[2];               // how much a CU with more workgroups than others counts, where it holds two, five
+  double join, join_bytes;        // the adding kernel, and bytes of parts a us
+  double side[3], group[3];       // what is left: factors for the sides 64, 128, 256, and 1, 2, 4 groups
+};
+constexpr LinearCost kLinearRowsA = {2.4, 0.52, 0.59, 0.19, {0.575, 2.95, 15.0}, {0.23, 0.26}, 0.61, 0.21, {0.96, 0.44}, 7.0, 5.9e6,
+                                     {1.0, 1.0, 0.863}, {1.0, 1.1, 1.12}};
+constexpr LinearCost kLinearRowsC = {2.03, 0.44, 0.374, 0.0, {0.475, 1.9, 7.6}, {0.223, 0.223}, 0.432, 0.197, {0.75, 0.75}, 3.4, 4.9e6,
+                                     {1.0, 1.04, 0.93}, {1.0, 1.0, 1.0}};
+constexpr int64_t kLinearSmall = int64_t(8) << 20;  // bytes of both operands, most of which an XCD's L2 (4 MiB) holds
+struct LinearKind {
+  bool rows_c, fp8;
+};
+inline const LinearCost& linear_cost(LinearKind kind) { return kind.rows_c ? kLinearRowsC : kLinearRowsA; }
+// `groups` workgroups of at most `turns` turns, `all` in all; `small`: the operands are.
+inline double linear_time(LinearTile t, LinearKind kind, double groups, double turns, double all, double cus, bool small) {
+  const LinearCost& k = linear_cost(kind);
+  const int by = t == LinearTile::k256 ? 2 : t == LinearTile::k128 || t == LinearTile::k128x2 ? 1 : 0;
+  const int waves = t == LinearTile::k64x4 ? 2 : t == LinearTile::k128x2 || t == LinearTile::k64x2 ? 1 : 0;
+  constexpr double kHeld[3][3] = {{5, 2, 1}, {2, 1, 1}, {1, 1, 1}};  // workgroups that a CU holds
+  const double held = kHeld[by][waves], g = 1 << waves, units = g * (1 << by);
+  const double loads = k.loads[!(small && units == 1)] * units, cores = (kind.fp8 ? 0.118 : 0.048) * units * (1 << by);
+  const double turn = loads > cores ? loads : cores, latency = k.latency + k.more_latency * (units - 1);
+  const double equal = all / turns / cus, whole = (double)(int64_t)(equal + 0.999999);
+  double each = whole < 1 ? 1 : whole;
+  const double rounds = (double)(int64_t)((each + held - 1) / held);
+  if (held > 1) {
+    const double u = k.uneven[held > 2];
+    each = u * each + (1 - u) * (equal < 1 ? 1 : equal);
+  }
+  const double busy = each * turns * turn, waits = rounds * turns * latency, ends = groups / cus > each ? groups / cus : each;
+  return (k.call + k.groups * (g - 1) + (k.start + k.more_start * (units - 1)) * rounds + k.end[by] * ends + (busy > waits ? busy : waits)) *
+         k.side[by] * k.group[waves];
+}
+inline double linear_parts_time(const LinearSize& s, LinearKind kind, int64_t parts) {
+  return parts > 1 ? (double)parts * (double)s.m * (double)s.n * 8.0 / linear_cost(kind).join_bytes : 0.0;
+}
+constexpr int64_t kLinearParts[] = {1, 2, 3, 4, 5, 6, 8, 11, 16};
+
+struct LinearPlan {
+  LinearTile tile;
+  LinearSplit split;
+  double time;
+};
+inline LinearPlan linear_plan(const LinearSize& s, LinearKind kind, int64_t cus) {
+  LinearPlan best{LinearTile::k64, linear_split(LinearTile::k64, s, 1), 1e300};
+  const bool small = s.c_bytes >= 1024 && (s.m + s.n) * s.c_bytes <= kLinearSmall;
+  for (LinearTile t : kLinearTiles) {
+    if (!linear_fits(s, kind.rows_c, t)) continue;
+    const int64_t tiles = linear_tiles(s, t);
+    for (int64_t parts : kLinearParts) {
+      // (few steps are over before a second kernel starts, and parts beyond what the chip holds only move more)
+      if (parts > 1 && (s.c_bytes < 1024 || s.c_bytes < 256 * parts * linear_tile_groups(t) || tiles * (parts - 1) > 4 * cus)) break;
+      const LinearSplit split = linear_split(t, s, parts);
+      const double groups = (double)(tiles * split.parts);
+      const double time = linear_time(t, kind, groups, (double)split.turns, groups * (double)split.turns, (double)cus, small) +
+                          linear_parts_time(s, kind, split.parts) + (split.parts > 1 ? linear_cost(kind).join : 0.0);
+      if (time < best.time) best = {t, split, time};
+    }
+  }
+  return best;
+}
+
+// Two products (B by rows of c) in one launch: the shorter c in parts of about the longer one's turns. (Tiles of which a CU holds one
+// workgroup of many waves were the best for none of 60 pairs but one or two, as they leave the second product no room beside them.) On those
+// 60 the pick takes 2.3 % more than the best in the mean. Measured, both gradients of m, n, k with silu and dbias, us apart / together:
+// 2000,3000,1000 70.7 / 58.5; 2048^3 60.3 / 47.0; 8192,4096,1024 214 / 184; 500,1500,700 30.7 / 24.4; 64,4096,4096 36.2 / 29.4;
+// 589,288,192 17.5 / 11.6; 6,200,72 12.6 / 8.6; 8192,8192,2048 545 / 540. Apart was never more than 3 % faster.
+struct LinearPair {
+  LinearTile tile;
+  LinearSplit a, b;
+  double time;
+};
+inline LinearPair linear_plan_of_two(const LinearSize& a, const LinearSize& b, int64_t cus) {
+  const bool longer = a.c_bytes >= b.c_bytes;
+  const LinearSize &l = longer ? a : b, &s = longer ? b : a;
+  const LinearKind kind{true, false};
+  LinearPair best{LinearTile::k64, {1, 1}, {1, 1}, 1e300};
+  for (LinearTile t : {LinearTile::k256, LinearTile::k128, LinearTile::k64, LinearTile::k64x2}) {
+    if (!linear_fits(l, true, t) || !linear_fits(s, true, t)) continue;
+    const int64_t tl = linear_tiles(l, t), ts = linear_tiles(s, t), all = linear_split(t, s, 1).turns;
+    for (int64_t parts : kLinearParts) {
+      if (parts > 1 && (l.c_bytes < 1024 || l.c_bytes < 256 * parts * linear_tile_groups(t) || tl * (parts - 1) > 4 * cus)) break;
+      const LinearSplit sl = linear_split(t, l, parts), ss = linear_split(t, s, (all + sl.turns - 1) / sl.turns);
+      const double gl = (double)(tl * sl.parts), gs = (double)(ts * ss.parts);
+      const double time = linear_time(t, kind, gl + gs, (double)(sl.turns > ss.turns ? sl.turns : ss.turns),
+                                      gl * (double)sl.turns + gs * (double)ss.turns, (double)cus, false) +
+                          linear_parts_time(l, kind, sl.parts) + linear_parts_time(s, kind, ss.parts) +
+                          (sl.parts > 1 || ss.parts > 1 ? kLinearRowsC.join : 0.0);
+      if (time < best.time) best = longer ? LinearPair{t, sl, ss, time} : LinearPair{t, ss, sl, time};
+    }
+  }
+  return best;
 }
 
 // Few rows of x: kernels that read w once for up to 64 of them. Measured in bf16, us (few rows / tiles): 32×16384×2048 13.3 /

@@ -215,40 +215,44 @@ TEST_CPU(linear_routes) {
   using dc::LinearTile;
   struct Row {
     int64_t m, n, c_bytes;
-    bool rows_c;
+    bool rows_c, fp8;
     LinearTile want;
+    int64_t parts;
   };
   const Row rows[] = {
-      {8192, 8192, 16384, false, LinearTile::k256}, {8192, 2048, 16384, true, LinearTile::k256},
-      {4352, 4096, 2048, false, LinearTile::k128},  {2048, 2048, 4096, false, LinearTile::k128x2},
-      {2048, 2048, 1632, false, LinearTile::k128},  {1537, 2049, 2048, false, LinearTile::k64},
-      {1024, 1024, 2048, false, LinearTile::k64x2}, {512, 512, 8192, false, LinearTile::k64x4},
-      {8192, 8192, 64, false, LinearTile::k64},
+      {8192, 8192, 16384, false, false, LinearTile::k256, 1},  {8192, 2048, 16384, true, false, LinearTile::k256, 1},
+      {8192, 8192, 128, false, false, LinearTile::k256, 1},    {4096, 8192, 4096, false, true, LinearTile::k256, 1},
+      {4352, 4096, 2048, false, false, LinearTile::k128, 1},   {2048, 2048, 4096, false, false, LinearTile::k128x2, 1},
+      {300, 4096, 2048, false, false, LinearTile::k64, 1},
+      {1500, 1500, 12000, false, false, LinearTile::k128, 3},
   };
-  for (const Row& r : rows) CHECK(dc::linear_tile({r.m, r.n, r.c_bytes, r.c_bytes, r.c_bytes}, r.rows_c, 256) == r.want);
+  for (const Row& r : rows) {
+    const dc::LinearPlan p = dc::linear_plan({r.m, r.n, r.c_bytes, r.c_bytes, r.c_bytes}, {r.rows_c, r.fp8}, 256);
+    CHECK(p.tile == r.want && p.split.parts == r.parts);
+  }
   // the widest rows stay within the loads' range: small tiles only
-  CHECK(dc::linear_tile({8192, 8192, 16384, dc::kLinearPitch, dc::kLinearPitch}, false, 256) == LinearTile::k64);
-  CHECK(dc::linear_tile({8192, 8192, 16384, 16384, dc::kLinearPitch}, true, 256) == LinearTile::k256);
-  // two products together: both gradients of 2000 rows fill the chip in 128-tiles, as neither does
-  const dc::LinearSize dx{2000, 1000, 6000, 6000, 2000}, dw{3000, 1000, 4000, 4000, 2000};
-  CHECK(dc::linear_tile(dx, true, 256) == LinearTile::k64x2 && dc::linear_tile_of_two(dx, dw, true, 256) == LinearTile::k128);
-  CHECK(dc::linear_tile_of_two(dx, dw, true, 256) == dc::linear_tile_of_two(dw, dx, true, 256));
-  CHECK(dc::linear_tile_of_two({2048, 1024, 8192, 8192, 2048}, {4096, 1024, 4096, 4096, 2048}, true, 256) == LinearTile::k128x2);
-  CHECK(dc::linear_tile_of_two({8192, 2048, 16384, 16384, 4096}, {8192, 2048, 16384, 16384, 4096}, true, 256) == LinearTile::k256);
-  CHECK(dc::linear_alike(dx, dw) && !dc::linear_alike({1000, 1000, 6000, 6000, 2000}, {3000, 1000, 2000, 2000, 2000}));
-  CHECK(dc::linear_whole(LinearTile::k128, dx).turns == 47 && dc::linear_whole(LinearTile::k64x2, dw).turns == 16);
+  const LinearTile narrow = dc::linear_plan({8192, 8192, 16384, dc::kLinearPitch, dc::kLinearPitch}, {false, false}, 256).tile;
+  CHECK(dc::linear_tile_side(narrow) == 64);
+  CHECK(dc::linear_plan({8192, 8192, 16384, 16384, dc::kLinearPitch}, {true, false}, 256).tile == LinearTile::k256);
   // splits: every tile along c belongs to exactly one part, and none is empty
-  for (LinearTile t : {LinearTile::k256, LinearTile::k128, LinearTile::k128x2, LinearTile::k64, LinearTile::k64x2, LinearTile::k64x4})
-    for (int64_t m : {1, 64, 300, 2515, 8192})
-      for (int64_t n : {1, 64, 256, 1000, 8192})
-        for (int64_t c : {2, 128, 1000, 2046, 10336, 1 << 24}) {
-          const dc::LinearSplit s = dc::linear_split(t, {m, n, c, c, c}, 256);
-          const int64_t step = 128 * dc::linear_tile_groups(t), all = (c + step - 1) / step;
-          CHECK(s.parts >= 1 && s.parts <= 512 && s.turns >= 1);
-          CHECK(s.parts * s.turns >= all && (s.parts - 1) * s.turns < all);
-        }
-  CHECK(dc::linear_split(LinearTile::k64x4, {64, 2048, 16384, 16384, 4096}, 256).parts > 1);
-  CHECK(dc::linear_split(LinearTile::k256, {8192, 2048, 16384, 16384, 4096}, 256).parts == 1);
+  auto whole = [](const dc::LinearSplit& s, LinearTile t, int64_t c) {
+    const int64_t step = 128 * dc::linear_tile_groups(t), all = (c + step - 1) / step;
+    return s.parts >= 1 && s.parts <= 64 && s.turns >= 1 && s.parts * s.turns >= all && (s.parts - 1) * s.turns < all;
+  };
+  for (int64_t m : {1, 64, 300, 2515, 8192})
+    for (int64_t n : {1, 64, 256, 1000, 8192})
+      for (int64_t c : {2, 128, 1000, 2046, 10336, 1 << 24}) {
+        const dc::LinearSize a{m, n, c, c, c}, b{n, m, 2 * m, 2 * m, 2 * m};
+        const dc::LinearPlan p = dc::linear_plan(a, {false, false}, 256);
+        CHECK(whole(p.split, p.tile, c) && p.time > 0.0 && p.time < 1e12);
+        const dc::LinearPair q = dc::linear_plan_of_two(a, b, 256);
+        CHECK(whole(q.a, q.tile, a.c_bytes) && whole(q.b, q.tile, b.c_bytes));
+        const dc::LinearPair r = dc::linear_plan_of_two(b, a, 256);  // (in either order)
+        CHECK(a.c_bytes == b.c_bytes || (r.tile == q.tile && r.a.parts == q.b.parts && r.b.parts == q.a.parts));
+      }
+  // both gradients of an ordinary layer: 128-tiles fill the chip together, as neither's do
+  const dc::LinearSize dx{2000, 1000, 6000, 6000, 2000}, dw{3000, 1000, 4000, 4000, 2000};
+  CHECK(dc::linear_plan_of_two(dx, dw, 256).tile == LinearTile::k128 && dc::linear_plan(dx, {true, false}, 256).tile != LinearTile::k128);
   CHECK(dc::linear_few_rows(1, 1, 256) && dc::linear_few_rows(32, 100000, 256) && dc::linear_few_rows(64, 4096, 256));
   CHECK(!dc::linear_few_rows(64, 4112, 256) && !dc::linear_few_rows(33, 8192, 256) && dc::linear_few_rows(4096, 64, 256));
   CHECK(dc::linear_wide_few_rows(8, 16384, 256) && !dc::linear_wide_few_rows(8, 8192, 256));
