@@ -879,6 +879,37 @@ __global__ __launch_bounds__(64 * W) void few_rows_kernel(Operands o, Epilogue e
   }
 }
 
+// ---- copies ------------------------------------------------------------------------------------------------
+// Rows of `bytes` bytes at any alignment to rows of `to_pitch` (a multiple of 16), padded with zeros. Bound by launch and latency
+// at ordinary sizes: 1537 and 2049 rows of 2046 bytes, both operands in one launch, 5.5-8 us, a third of the product's call.
+struct PackJob {
+  const unsigned char* from;
+  unsigned char* to;
+  int64_t rows, bytes, from_pitch, to_pitch;
+};
+struct PackArgs {
+  PackJob job[2];
+};
+constexpr int64_t kPackBytes = 4096;  // of a row that a wave takes, all asked for at once
+// Workgroup `block` of `blocks`, of four waves.
+__device__ inline void pack_rows(const PackJob& a, int64_t block, int64_t blocks) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int64_t across = (a.to_pitch + kPackBytes - 1) / kPackBytes, total = a.rows * across;
+  for (int64_t t = block * 4 + wave; t < total; t += blocks * 4) {
+    const int64_t row = total <= UINT32_MAX ? (int64_t)((uint32_t)t / (uint32_t)across) : t / across;
+    const unsigned char* from = a.from + row * a.from_pitch;
+    unsigned char* to = a.to + row * a.to_pitch;
+    const int64_t first = (t - row * across) * kPackBytes + 16 * lane;
+    dc::u32x4 w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = load_piece(from + first + 1024 * i, a.bytes - first - 1024 * i, a.bytes);
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (first + 1024 * i < a.to_pitch) *reinterpret_cast<dc::u32x4*>(to + first + 1024 * i) = w[i];
+  }
+}
+__global__ __launch_bounds__(256) void pack_kernel(PackArgs args) { pack_rows(args.job[blockIdx.y], blockIdx.x, gridDim.x); }
+
 // ---- what the gradients' products run along ---------------------------------------------------------------
 // dz = dy act'(pre) over 64×64 pieces: dz itself (pitch dz_pitch, columns from n to there zero), its transpose (pitch
 // t_pitch, columns from m to there zero) through LDS, and the piece's column sums, unrounded. A thread holds two
@@ -892,9 +923,11 @@ struct SlopeArgs {
   int64_t m, n, dy_stride, pre_stride, dz_pitch, t_pitch;
   int32_t act;
 };
-__global__ __launch_bounds__(256) void slope_kernel(SlopeArgs a) {
+// (The workgroups with blockIdx.y > 0 copy the operands that have to be, beside it.)
+__global__ __launch_bounds__(256) void slope_kernel(SlopeArgs a, PackArgs copies) {
   __shared__ uint32_t turned[64][33];
   __shared__ float sums[32][65];
+  if (blockIdx.y > 0) return pack_rows(copies.job[blockIdx.y - 1], blockIdx.x, gridDim.x);
   const int t = threadIdx.x, c8 = t & 7, pair = t >> 3;
   const int64_t across = (a.n + 63) / 64, total = across * ((a.m + 63) / 64);
   for (int64_t at = blockIdx.x; at < total; at += gridDim.x) {
@@ -976,35 +1009,6 @@ __global__ __launch_bounds__(256) void join_kernel(JoinArgs args) {
     }
     float z[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
     out.finish(a.ep, cols, i, z);
-  }
-}
-
-// Rows of `bytes` bytes at any alignment to rows of `to_pitch` (a multiple of 16), padded with zeros. Bound by launch and latency
-// at ordinary sizes: 1537 and 2049 rows of 2046 bytes, both operands in one launch, 5.5-8 us, a third of the product's call.
-struct PackJob {
-  const unsigned char* from;
-  unsigned char* to;
-  int64_t rows, bytes, from_pitch, to_pitch;
-};
-struct PackArgs {
-  PackJob job[2];
-};
-constexpr int64_t kPackBytes = 4096;  // of a row that a wave takes, all asked for at once
-__global__ __launch_bounds__(256) void pack_kernel(PackArgs args) {
-  const PackJob& a = args.job[blockIdx.y];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t across = (a.to_pitch + kPackBytes - 1) / kPackBytes, total = a.rows * across;
-  for (int64_t t = (int64_t)blockIdx.x * 4 + wave; t < total; t += (int64_t)gridDim.x * 4) {
-    const int64_t row = total <= UINT32_MAX ? (int64_t)((uint32_t)t / (uint32_t)across) : t / across;
-    const unsigned char* from = a.from + row * a.from_pitch;
-    unsigned char* to = a.to + row * a.to_pitch;
-    const int64_t first = (t - row * across) * kPackBytes + 16 * lane;
-    dc::u32x4 w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = load_piece(from + first + 1024 * i, a.bytes - first - 1024 * i, a.bytes);
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (first + 1024 * i < a.to_pitch) *reinterpret_cast<dc::u32x4*>(to + first + 1024 * i) = w[i];
   }
 }
 
@@ -1154,21 +1158,28 @@ struct Rows {
   int64_t width() const { return copied ? padded(bytes, 16) : pitch; }  // the pitch it will have
 };
 
-// Lays out those of the (at most two) operands that have to be, in one launch.
-int32_t lay_out(dc_hip_ctx* ctx, Rows* a, Rows* b) {
+// The copies of those of the (at most two) operands that have to be laid out, which are taken to be in place from here on.
+struct Copies {
   PackArgs args{};
   int jobs = 0;
-  int64_t most = 0;
+  int64_t groups = 0;  // of workgroups for the larger
+};
+Copies lay_out(dc_hip_ctx* ctx, Rows* a, Rows* b) {
+  Copies c;
   for (Rows* r : {a, b}) {
     if (!r || !r->copied) continue;
     unsigned char* to = static_cast<unsigned char*>(ctx->partials) + r->at;
-    args.job[jobs++] = PackJob{r->p, to, r->rows, r->bytes, r->pitch, r->width()};
-    most = std::max(most, (r->rows * ((r->width() + kPackBytes - 1) / kPackBytes) + 3) / 4);
+    c.args.job[c.jobs++] = PackJob{r->p, to, r->rows, r->bytes, r->pitch, r->width()};
+    c.groups = std::max(c.groups, (r->rows * ((r->width() + kPackBytes - 1) / kPackBytes) + 3) / 4);
     r->p = to;
     r->pitch = r->width();
   }
-  if (jobs == 0) return DC_OK;
-  pack_kernel<<<dim3((unsigned)std::min<int64_t>(most, 65536), (unsigned)jobs), 256, 0, ctx->stream>>>(args);
+  c.groups = std::min<int64_t>(c.groups, 65536);
+  return c;
+}
+int32_t copy_rows(dc_hip_ctx* ctx, const Copies& c) {
+  if (c.jobs == 0) return DC_OK;
+  pack_kernel<<<dim3((unsigned)c.groups, (unsigned)c.jobs), 256, 0, ctx->stream>>>(c.args);
   return dc::last_launch_status();
 }
 
@@ -1239,7 +1250,7 @@ DC_HIP_API int32_t dc_hip_linear(dc_hip_ctx* ctx, const dc_linear* args) {
     return fp8 ? few_rows_any<true>(ctx, o, ep) : few_rows_any<false>(ctx, o, ep);
   auto lay_out_all = [&]() -> int32_t {
     if (scratch.bytes) DC_RETURN_IF(dc::ensure_partials(ctx, scratch.bytes));
-    DC_RETURN_IF(lay_out(ctx, &x, &w));
+    DC_RETURN_IF(copy_rows(ctx, lay_out(ctx, &x, &w)));
     o.a = x.p, o.b = w.p, o.a_pitch = x.pitch, o.b_pitch = w.pitch;
     o.c_bytes = (int32_t)padded(o.c_bytes, 16);  // (ragged rows have been copied, with zeros there)
     return DC_OK;
@@ -1326,12 +1337,14 @@ DC_HIP_API int32_t dc_hip_linear_backward(dc_hip_ctx* ctx, const dc_linear_grad*
   if (own_dz) s.dz = reinterpret_cast<bf16*>(base + dz.at);
   if (dw) s.dzt = reinterpret_cast<bf16*>(base + at_dzt);
   if (dbias) s.parts = pieces > 1 ? reinterpret_cast<float*>(base + at_parts) : p.dbias;
+  const Copies copies = lay_out(ctx, dx ? &w : nullptr, dw ? &x : nullptr);
   if (s.dz || s.dzt || s.parts) {
-    const int64_t grid = std::min<int64_t>((p.n + 63) / 64 * pieces, 1 << 20);
-    slope_kernel<<<(unsigned)grid, 256, 0, ctx->stream>>>(s);
+    const int64_t grid = std::max(copies.groups, std::min<int64_t>((p.n + 63) / 64 * pieces, 1 << 20));
+    slope_kernel<<<dim3((unsigned)grid, (unsigned)(1 + copies.jobs)), 256, 0, ctx->stream>>>(s, copies.args);
     DC_RETURN_IF(dc::last_launch_status());
+  } else {
+    DC_RETURN_IF(copy_rows(ctx, copies));
   }
-  DC_RETURN_IF(lay_out(ctx, dx ? &w : nullptr, dw ? &x : nullptr));
   // One gradient: the product of `rows` (m of them, along c) and `b` (c rows of k).
   auto gradient = [&](const void* rows, int64_t pitch, int64_t m, int64_t c, const Rows& b, void* out, int64_t stride,
                       const ProductPlan& plan) {
