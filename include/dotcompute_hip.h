@@ -549,7 +549,8 @@ DC_HIP_API int32_t dc_hip_spmv_plan_destroy(dc_hip_spmv_plan* plan);
  * MatrixOperations.cs:28-64); an argument block each, since most of their operands may be absent.
  *
  * Conventions: matrices are row-major; a *_stride is the distance of two rows in elements, at least the row's
- * length. All pointers are device pointers at the alignment of one element. bf16 values are uint16 bit patterns.
+ * length (of a single row: anything). All pointers are device pointers at the alignment of one element. bf16 values are
+ * uint16 bit patterns.
  * 8-bit values are e4m3 (1 sign, 4 exponent, 3 fraction bits, bias 7, largest 448, no infinity), and stand for
  * themselves times their scale, max / 448 over the row or block that shares it; a NaN in one makes its scale NaN.
  * Sums, statistics and scales are float32. Results are the same bits from call to call. Outputs overlap neither inputs
