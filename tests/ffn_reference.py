@@ -1,5 +1,5 @@
-"""The feed-forward block's operators in float64 numpy, and the element types around them: the checker of the
-kernels' tests. Written from the formulas alone; shares no code with the library."""
+"""The feed-forward block's operators in float64 numpy, and the element types around them: what the
+kernels are tested against. Written from the formulas alone; shares no code with the library."""
 import math
 
 import numpy as np

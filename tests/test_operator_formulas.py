@@ -1,4 +1,4 @@
-"""CPU: the checker's gradients (tests/ffn_reference.py) against central differences of its forward formulas, its
+"""CPU: the float64 gradients of tests/ffn_reference.py against central differences of its forward formulas, its
 element types against known codes, and the shapes the argument blocks of the binding accept."""
 import ctypes as C
 import subprocess
