@@ -141,6 +141,14 @@ def test_linear_activations(ctx, activation, m):
         run_linear(ctx, m, 96, 128, "fp8", activation, y, residual=True, bias=False)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "fp8"])
+@pytest.mark.parametrize("m,n,k", [(100, 300, 9000), (300, 300, 8000), (520, 512, 20000), (101, 301, 9001), (1100, 300, 6000)])
+def test_linear_of_long_sums(ctx, m, n, k, dtype):
+    """Few tiles with long sums, which workgroups share: the epilogue is the adding kernel's."""
+    run_linear(ctx, m, n, k, dtype, "silu", residual=True, pre=True)
+    run_linear(ctx, m, n, k, dtype, "none", "f32", bias=False, residual=True, odd=1)
+
+
 @pytest.mark.slow
 @pytest.mark.parametrize("dtype", ["bf16", "fp8"])
 @pytest.mark.parametrize("m,n,k", [(2048, 4096, 256), (4352, 4096, 136), (2000, 3000, 1000), (1537, 2049, 1023), (512, 512, 4096),
@@ -263,6 +271,13 @@ def test_linear_backward_activations(ctx, activation):
 @pytest.mark.slow
 @pytest.mark.parametrize("m,n,k", [(2000, 3000, 1000), (2048, 2048, 520), (4100, 260, 136)])
 def test_linear_backward_larger(ctx, m, n, k):
+    run_backward(ctx, m, n, k, "silu")
+
+
+@pytest.mark.parametrize("m,n,k", [(16, 2048, 520), (64, 2000, 136), (2000, 300, 264), (1, 3000, 200), (2500, 1, 90), (3000, 144, 700),
+                                   (45, 5001, 553), (1717, 104, 1368), (491, 3000, 1500), (4500, 200, 72)])
+def test_linear_backward_of_unlike_sums(ctx, m, n, k):
+    """Sums over few rows beside sums over many outputs, and the other way round: one launch, in parts of their own."""
     run_backward(ctx, m, n, k, "silu")
 
 
