@@ -3,12 +3,12 @@
 // Memory-bound: an element with 32-bit states moves 28 bytes (gradient 2; param, m, v in and out 24; the bf16 copy 2),
 // with 8-bit ones 16. The tensors' addresses travel in the kernel's arguments, kTensors a launch, so a step of a whole
 // model is a few launches, nothing is uploaded and nothing is kept between calls. A workgroup takes kChunk elements of one
-// tensor (found by bisection over the tensors' first chunks, in scalar registers); a wave's 64 lanes take 4 neighbouring
+// tensor (found from the tensors' first chunks); a wave's 64 lanes take 4 neighbouring
 // elements each, which is one 8-bit state block: its maximum is a DPP reduction, and a state's codes and scale are read
 // and written once. What the next step alone reads again passes the caches by (non-temporal); the bf16 copy does not.
 //
 // Measured, us (TB/s of the 28 and 16.06 bytes an element): 134M elements, 32-bit states 647 (5.8), 8-bit 368 (5.9); 484 thousand in
-// 30 tensors 5.1 and 5.7, which is the launch's. A block a wave; four blocks a wave, all loaded first: 699, 374, 7.1, 9.2;
+// 30 tensors 4.5 and 4.8, which is the launch's. A block a wave; four blocks a wave, all loaded first: 699, 374, 7.1, 9.2;
 // that through the caches 718, 401.
 #include <algorithm>
 #include <cmath>
@@ -33,8 +33,7 @@ struct Tensor {
   float *m_scales, *v_scales;
   uint16_t* copy;
   int64_t n;
-  uint32_t first;  // of its chunks in the launch
-  int32_t grad_f32;
+  int64_t grad_f32;
 };
 
 struct Step {
@@ -42,6 +41,7 @@ struct Step {
   float rate, root, eps, decay;      // lr / (1 - beta1^t), 1 / sqrt(1 - beta2^t), eps, 1 - lr weight_decay
   float grad_scale;
   int32_t count;
+  uint32_t first[kTensors];  // chunk of each tensor in the launch
   Tensor t[kTensors];
 };
 
@@ -190,17 +190,28 @@ __device__ inline void step_block(const Step& s, const Tensor& t, int64_t start)
   }
 }
 
-template <bool kFp8>
+// The tensor of a chunk is the last whose first chunk is not past it. In a short launch, which is latency, a wave's lanes
+// compare one each, a single load; in a long one bisection, whose scalar loads hit and cost the vector units nothing. Measured, us, lanes /
+// bisection: 484 thousand elements in 30 tensors 4.5 / 5.0, 8-bit states 4.8 / 5.7; 12 million in 10, 8-bit, 31.8 / 32.3; 134 million
+// in 20, 8-bit, 382 / 369.
+constexpr int64_t kLongLaunch = 32768;  // chunks
+template <bool kFp8, bool kLong>
 __global__ __launch_bounds__(kThreads) void adamw_kernel(Step s) {
   const uint32_t chunk = blockIdx.x;
-  int lo = 0, hi = s.count;  // the last tensor whose first chunk is not past this one
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (s.t[mid].first <= chunk) lo = mid;
-    else hi = mid;
+  int lo = 0;
+  if constexpr (kLong) {
+    for (int hi = s.count; hi - lo > 1;) {
+      const int mid = (lo + hi) >> 1;
+      if (s.first[mid] <= chunk) lo = mid;
+      else hi = mid;
+    }
+  } else {
+    const int lane = threadIdx.x & 63;
+    const uint32_t first = s.first[lane < kTensors ? lane : kTensors - 1];
+    lo = __popcll(__ballot(lane < s.count && first <= chunk)) - 1;
   }
   const Tensor& t = s.t[lo];
-  const int64_t start = (int64_t)(chunk - t.first) * kChunk + (threadIdx.x >> 6) * kBlock;
+  const int64_t start = (int64_t)(chunk - s.first[lo]) * kChunk + (threadIdx.x >> 6) * kBlock;
   if (t.grad_f32) step_block<kFp8, float>(s, t, start);
   else step_block<kFp8, bf16>(s, t, start);
 }
@@ -246,8 +257,12 @@ extern "C" DC_HIP_API int32_t dc_hip_adamw_step(dc_hip_ctx* ctx, const dc_adamw*
   int64_t chunks = 0;
   auto launch = [&]() -> int32_t {
     if (s.count == 0) return DC_OK;
-    if (fp8) adamw_kernel<true><<<(unsigned)chunks, kThreads, 0, ctx->stream>>>(s);
-    else adamw_kernel<false><<<(unsigned)chunks, kThreads, 0, ctx->stream>>>(s);
+    const bool longer = chunks > kLongLaunch;
+    const unsigned grid = (unsigned)chunks;
+    if (fp8 && longer) adamw_kernel<true, true><<<grid, kThreads, 0, ctx->stream>>>(s);
+    else if (fp8) adamw_kernel<true, false><<<grid, kThreads, 0, ctx->stream>>>(s);
+    else if (longer) adamw_kernel<false, true><<<grid, kThreads, 0, ctx->stream>>>(s);
+    else adamw_kernel<false, false><<<grid, kThreads, 0, ctx->stream>>>(s);
     s.count = 0;
     chunks = 0;
     return dc::last_launch_status();
@@ -258,6 +273,7 @@ extern "C" DC_HIP_API int32_t dc_hip_adamw_step(dc_hip_ctx* ctx, const dc_adamw*
     for (int64_t off = 0; off < t.n; off += kMaxPiece) {
       const int64_t n = std::min(t.n - off, kMaxPiece), more = (n + kChunk - 1) / kChunk;
       if (s.count == kTensors || chunks + more > kMaxChunks) DC_RETURN_IF(launch());
+      s.first[s.count] = (uint32_t)chunks;
       s.t[s.count++] = Tensor{t.param + off,
                               static_cast<const char*>(t.grad) + off * grad_size,
                               static_cast<char*>(t.m) + off * state_size,
@@ -266,7 +282,6 @@ extern "C" DC_HIP_API int32_t dc_hip_adamw_step(dc_hip_ctx* ctx, const dc_adamw*
                               fp8 ? t.v_scales + off / kBlock : nullptr,
                               t.copy ? t.copy + off : nullptr,
                               n,
-                              (uint32_t)chunks,
                               t.grad_dtype == DC_DTYPE_F32};
       chunks += more;
     }
