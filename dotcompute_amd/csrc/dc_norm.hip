@@ -445,8 +445,16 @@ __global__ __launch_bounds__(kSumCols * kSumGroups) void column_sums_kernel(cons
   const int64_t c = (int64_t)blockIdx.x * kSumCols + lane;
   float v = 0.0f;
   if (c < cols)
-#pragma unroll 8
-    for (int64_t i = g; i < count; i += kSumGroups) v += parts[i * cols + c];
+    for (int64_t i = g; i < count; i += 8 * kSumGroups) {  // (eight in flight, the last ones too)
+      float u[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int64_t at = i + j * kSumGroups;
+        u[j] = parts[(at < count ? at : count - 1) * cols + c];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v += i + j * kSumGroups < count ? u[j] : 0.0f;
+    }
   sums[g][lane] = v;
   __syncthreads();
   if (g < 4) {  // (a wave: 16 columns, 4 quarters of the sums)
@@ -571,7 +579,10 @@ DC_HIP_API int32_t dc_hip_rms_norm_backward(dc_hip_ctx* ctx, const dc_rms_norm_g
   const int64_t elems = 16 / size_of(p.dtype), chunks = (p.cols + elems - 1) / elems;
   const int c = chunks <= 512 ? 1 : chunks <= 1024 ? 2 : chunks <= 2048 ? 4 : 0, waves = c ? waves_for(chunks, c) : kWaves;
   const int per_cu = waves <= 2 ? 8 / waves : std::max(1, 15 / waves);
-  const int64_t grid = std::min<int64_t>(p.rows, per_cu * (int64_t)std::max(1, ctx->cu_count));
+  const int64_t held = per_cu * (int64_t)std::max(1, ctx->cu_count);  // workgroups
+  // (Few rows: no more parts than workgroups of that many rows each leave. us, 300×8192 15.4 / 12.7, 900×3000 14.3 / 13.7; of many rows
+  // it would leave CUs idle: 8191×2050 32.4 / 33.1. A workgroup a row up to two rows each: 17.8, 17.0.)
+  const int64_t each = (p.rows + held - 1) / held, grid = each <= 4 ? (p.rows + each - 1) / each : held;
   float* parts = nullptr;
   if (p.dweight) {
     DC_RETURN_IF(dc::ensure_partials(ctx, (size_t)(grid * p.cols) * sizeof(float)));
