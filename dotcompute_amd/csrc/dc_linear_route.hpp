@@ -74,18 +74,22 @@ struct LinearKind {
   bool rows_c, fp8;
 };
 inline const LinearCost& linear_cost(LinearKind kind) { return kind.rows_c ? kLinearRowsC : kLinearRowsA; }
-// `groups` workgroups of at most `turns` turns, `all` in all; `small`: the operands are.
-inline double linear_time(LinearTile t, LinearKind kind, double groups, double turns, double all, double cus, bool small) {
+constexpr double kLinearHeld[3][3] = {{5, 2, 1}, {2, 1, 1}, {1, 1, 1}};  // workgroups that a CU holds: by side, and groups
+inline int linear_side_index(LinearTile t) { return t == LinearTile::k256 ? 2 : t == LinearTile::k128 || t == LinearTile::k128x2 ? 1 : 0; }
+inline int linear_group_index(LinearTile t) {
+  return t == LinearTile::k64x4 ? 2 : t == LinearTile::k128x2 || t == LinearTile::k64x2 ? 1 : 0;
+}
+inline double linear_up(double v) { return (double)(int64_t)(v + 0.999999); }
+// `groups` workgroups of at most `turns` turns; the busiest CU has as many turns as `most` of those, the mean CU as `equal`.
+// `small`: the operands are.
+inline double linear_time(LinearTile t, LinearKind kind, double groups, double turns, double most, double equal, double cus, bool small) {
   const LinearCost& k = linear_cost(kind);
-  const int by = t == LinearTile::k256 ? 2 : t == LinearTile::k128 || t == LinearTile::k128x2 ? 1 : 0;
-  const int waves = t == LinearTile::k64x4 ? 2 : t == LinearTile::k128x2 || t == LinearTile::k64x2 ? 1 : 0;
-  constexpr double kHeld[3][3] = {{5, 2, 1}, {2, 1, 1}, {1, 1, 1}};  // workgroups that a CU holds
-  const double held = kHeld[by][waves], g = 1 << waves, units = g * (1 << by);
+  const int by = linear_side_index(t), waves = linear_group_index(t);
+  const double held = kLinearHeld[by][waves], g = 1 << waves, units = g * (1 << by);
   const double loads = k.loads[!(small && units == 1)] * units, cores = (kind.fp8 ? 0.118 : 0.048) * units * (1 << by);
   const double turn = loads > cores ? loads : cores, latency = k.latency + k.more_latency * (units - 1);
-  const double equal = all / turns / cus, whole = (double)(int64_t)(equal + 0.999999);
-  double each = whole < 1 ? 1 : whole;
-  const double rounds = (double)(int64_t)((each + held - 1) / held);
+  double each = most < 1 ? 1 : most;
+  const double rounds = held > 1 ? linear_up(each / held) : each;
   if (held > 1) {
     const double u = k.uneven[held > 2];
     each = u * each + (1 - u) * (equal < 1 ? 1 : equal);
@@ -93,6 +97,16 @@ inline double linear_time(LinearTile t, LinearKind kind, double groups, double t
   const double busy = each * turns * turn, waits = rounds * turns * latency, ends = groups / cus > each ? groups / cus : each;
   return (k.call + k.groups * (g - 1) + (k.start + k.more_start * (units - 1)) * rounds + k.end[by] * ends + (busy > waits ? busy : waits)) *
          k.side[by] * k.group[waves];
+}
+// (Counting the mean CU's turns alone picked 276 workgroups of 256-tiles for 256 CUs: both gradients of 5368,6400,592 217 us, now 158.)
+// Turns of the busiest CU, where each holds one workgroup at a time: `gl` of `tl` turns are handed out, then `gs` of `ts`.
+inline double linear_last(int64_t gl, double tl, int64_t gs, double ts, int64_t cus) {
+  const int64_t over = gl % cus, room = cus - over;  // CUs with one long one more than others, and those others
+  const double base = (double)(gl / cus) * tl, top = over ? base + tl : base;
+  const int64_t beside = over ? (int64_t)(tl / ts) : 0, left = gs - room * beside;  // short ones beside a long one, and after all those
+  if (left <= 0) return top;
+  if (over && left <= room && base + (double)(beside + 1) * ts > top) return base + (double)(beside + 1) * ts;
+  return top + linear_up((double)left / (double)cus) * ts;
 }
 inline double linear_parts_time(const LinearSize& s, LinearKind kind, int64_t parts) {
   return parts > 1 ? (double)parts * (double)s.m * (double)s.n * 8.0 / linear_cost(kind).join_bytes : 0.0;
@@ -115,7 +129,8 @@ inline LinearPlan linear_plan(const LinearSize& s, LinearKind kind, int64_t cus)
       if (parts > 1 && (s.c_bytes < 1024 || s.c_bytes < 256 * parts * linear_tile_groups(t) || tiles * (parts - 1) > 4 * cus)) break;
       const LinearSplit split = linear_split(t, s, parts);
       const double groups = (double)(tiles * split.parts);
-      const double time = linear_time(t, kind, groups, (double)split.turns, groups * (double)split.turns, (double)cus, small) +
+      const double equal = groups / (double)cus;
+      const double time = linear_time(t, kind, groups, (double)split.turns, linear_up(equal), equal, (double)cus, small) +
                           linear_parts_time(s, kind, split.parts) + (split.parts > 1 ? linear_cost(kind).join : 0.0);
       if (time < best.time) best = {t, split, time};
     }
@@ -144,9 +159,12 @@ inline LinearPair linear_plan_of_two(const LinearSize& a, const LinearSize& b, i
     for (int64_t parts : kLinearParts) {
       if (parts > 1 && (l.c_bytes < 1024 || l.c_bytes < 256 * parts * linear_tile_groups(t) || tl * (parts - 1) > 4 * cus)) break;
       const LinearSplit sl = linear_split(t, l, parts), ss = linear_split(t, s, (all + sl.turns - 1) / sl.turns);
-      const double gl = (double)(tl * sl.parts), gs = (double)(ts * ss.parts);
-      const double time = linear_time(t, kind, gl + gs, (double)(sl.turns > ss.turns ? sl.turns : ss.turns),
-                                      gl * (double)sl.turns + gs * (double)ss.turns, (double)cus, false) +
+      const int64_t gl = tl * sl.parts, gs = ts * ss.parts;
+      const double el = (double)sl.turns, es = (double)ss.turns, turns = el > es ? el : es;
+      const double equal = ((double)gl * el + (double)gs * es) / turns / (double)cus;
+      const bool one = kLinearHeld[linear_side_index(t)][linear_group_index(t)] == 1;
+      const double most = !one ? linear_up(equal) : (el >= es ? linear_last(gl, el, gs, es, cus) : linear_last(gs, es, gl, el, cus)) / turns;
+      const double time = linear_time(t, kind, (double)(gl + gs), turns, most, equal, (double)cus, false) +
                           linear_parts_time(l, kind, sl.parts) + linear_parts_time(s, kind, ss.parts) +
                           (sl.parts > 1 || ss.parts > 1 ? kLinearRowsC.join : 0.0);
       if (time < best.time) best = longer ? LinearPair{t, sl, ss, time} : LinearPair{t, ss, sl, time};
