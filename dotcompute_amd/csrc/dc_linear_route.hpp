@@ -51,24 +51,25 @@ inline LinearSplit linear_split(LinearTile tile, const LinearSize& s, int64_t pa
 // The tile, and the parts of c, are those with the least time by this estimate, in us: a CU's workgroups take turns of 128 bytes of c, each
 // bound by the loads of the two operands or the matrix cores, or, where few are there to cover it, by a turn's
 // latency; each workgroup has its epilogue, each round of workgroups its start, and parts of c their sums' way through memory and
-// the adding kernel. The numbers were fitted to the times of all tiles with 1 to 16 parts on 124 shapes (bf16, e4m3, B by
-// rows of c; 64 to 16384 results a side, c 64 to 8192): what it picks takes 1.2 % more time than the best in the mean, where
-// rules by the number of tiles took 6.4 %. Measured, us, those rules / this / the best: bf16 1500×1500×6000 67.5 / 48.9 / 48.9
-// (128-tiles, 3 parts), 300×1024×1024 9.2 / 6.1 / 6.1, 2048^3 23.3 / 23.5 / 23.3, 7958×332×5760 51.7 / 61.6 / 51.7; by rows of c 545×3768×5632
+// the adding kernel. The numbers were fitted to the times of all tiles with 1 to 16 parts on 200 shapes (bf16, e4m3, B by
+// rows of c; 64 to 16384 results a side, c 64 to 8192): what it picks takes 1.3 % more time than the best in the mean, 18 % at most,
+// where rules by the number of tiles took 6 %, and 49 % at most. Measured, us, those rules / this / the best: bf16 1500×1500×6000 67.5 / 48.9 / 48.9
+// (128-tiles, 3 parts), 300×1024×1024 9.2 / 6.1 / 6.1, 2048^3 23.3 / 23.5 / 23.3, 1347×3672×5288 94 / 95 / 84; by rows of c 545×3768×5632
 // 66.7 / 52.1 / 52.1 (256-tiles, 4 parts), 8192×2048×8192 220 / 211 / 211; e4m3 128×4096×4096 12.1 / 9.0 / 9.0.
 struct LinearCost {
   double call, groups;            // of a launch, and more for each further group of waves
   double start, more_start;       // of a round, and for each further 64-tile's worth of loads in a turn
   double end[3];                  // of a workgroup of side 64, 128, 256
-  double loads[2], latency, more_latency;  // of a turn, by 64-tile's worths; loads of 64-tiles of small operands, and else
+  double loads[2], cores[2];      // of a turn, by 64-tile's worths: loads of 64-tiles of small operands, and else; products of bf16, e4m3
+  double latency, more_latency;   // of a turn, and for each further 64-tile's worth
   double uneven[2];               // how much a CU with more workgroups than others counts, where it holds two, five
   double join, join_bytes;        // the adding kernel, and bytes of parts a us
   double side[3], group[3];       // what is left: factors for the sides 64, 128, 256, and 1, 2, 4 groups
 };
-constexpr LinearCost kLinearRowsA = {2.4, 0.52, 0.59, 0.19, {0.575, 2.95, 15.0}, {0.23, 0.26}, 0.61, 0.21, {0.96, 0.44}, 7.0, 5.9e6,
-                                     {1.0, 1.0, 0.863}, {1.0, 1.1, 1.12}};
-constexpr LinearCost kLinearRowsC = {2.03, 0.44, 0.374, 0.0, {0.475, 1.9, 7.6}, {0.223, 0.223}, 0.432, 0.197, {0.75, 0.75}, 3.4, 4.9e6,
-                                     {1.0, 1.04, 0.93}, {1.0, 1.0, 1.0}};
+constexpr LinearCost kLinearRowsA = {2.215, 0.462, 0.497, 0.254, {0.359, 3.318, 8.063}, {0.19, 0.206}, {0.045, 0.083}, 0.625, 0.183, {1.0, 0.428},
+                                     6.58, 4.56e6, {1.0, 0.812, 0.963}, {1.0, 1.118, 1.167}};
+constexpr LinearCost kLinearRowsC = {2.03, 0.44, 0.374, 0.0, {0.475, 1.9, 7.6}, {0.223, 0.223}, {0.048, 0.0}, 0.432, 0.197, {0.75, 0.75},
+                                     3.4, 4.9e6, {1.0, 1.04, 0.93}, {1.0, 1.0, 1.0}};
 constexpr int64_t kLinearSmall = int64_t(8) << 20;  // bytes of both operands, most of which an XCD's L2 (4 MiB) holds
 struct LinearKind {
   bool rows_c, fp8;
@@ -86,7 +87,7 @@ inline double linear_time(LinearTile t, LinearKind kind, double groups, double t
   const LinearCost& k = linear_cost(kind);
   const int by = linear_side_index(t), waves = linear_group_index(t);
   const double held = kLinearHeld[by][waves], g = 1 << waves, units = g * (1 << by);
-  const double loads = k.loads[!(small && units == 1)] * units, cores = (kind.fp8 ? 0.118 : 0.048) * units * (1 << by);
+  const double loads = k.loads[!(small && units == 1)] * units, cores = k.cores[kind.fp8] * units * (1 << by);
   const double turn = loads > cores ? loads : cores, latency = k.latency + k.more_latency * (units - 1);
   double each = most < 1 ? 1 : most;
   const double rounds = held > 1 ? linear_up(each / held) : each;

@@ -223,7 +223,7 @@ TEST_CPU(linear_routes) {
       {8192, 8192, 16384, false, false, LinearTile::k256, 1},  {8192, 2048, 16384, true, false, LinearTile::k256, 1},
       {8192, 8192, 128, false, false, LinearTile::k256, 1},    {4096, 8192, 4096, false, true, LinearTile::k256, 1},
       {4352, 4096, 2048, false, false, LinearTile::k128, 1},   {2048, 2048, 4096, false, false, LinearTile::k128x2, 1},
-      {300, 4096, 2048, false, false, LinearTile::k64, 1},
+      {1537, 2049, 2048, false, false, LinearTile::k64, 1},
       {1500, 1500, 12000, false, false, LinearTile::k128, 3},
   };
   for (const Row& r : rows) {
