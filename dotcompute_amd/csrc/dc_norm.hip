@@ -291,12 +291,13 @@ __device__ inline void row_sums(float& hh, float& gh, float (*scratch)[kWaves], 
   }
 }
 
-// A workgroup's rows are blockIdx.x, + gridDim.x, ...; the next row's operands are asked for before this one's sums.
+// A workgroup's rows are blockIdx.x, + gridDim.x, ...; with kAhead the next row's operands are asked for before this one's sums
+// (without, sixteen floats of each operand a lane leave registers for 16 waves).
 // Workgroups a CU: as many waves as hide a row's latency, and no more, as each workgroup leaves a row of dweight's parts to be
 // added. Measured, us for 1 / 2 / 3 / 4 workgroups of a row's waves a CU: 8192×4096 51.4 / 55.5 (8 waves; 5.2 TB/s), 8191×2050 45 /
 // 34.9 / 32.8 (5 waves; 4.1 TB/s); 16384×512 with 8 of one wave 19.1, with 16 23.2.
-template <typename T, int C>
-__global__ __launch_bounds__(512) void rms_norm_grad_kernel(NormGradArgs a, int waves) {
+template <typename T, int C, bool kAhead>
+__global__ __launch_bounds__(C == 4 && kAhead ? 512 : 1024) void rms_norm_grad_kernel(NormGradArgs a, int waves) {
   constexpr int E = kElems<T>;
   __shared__ __align__(16) float scratch[4][kWaves];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -315,10 +316,11 @@ __global__ __launch_bounds__(512) void rms_norm_grad_kernel(NormGradArgs a, int 
     if (a.dh && a.dx) R.load(static_cast<const T*>(a.dh) + row * a.dh_stride, ur);
   };
   R.load(static_cast<const T*>(a.weight), wr);
-  load(blockIdx.x);
+  if constexpr (kAhead) load(blockIdx.x);
   R.cut(wr);
   int flip = 0;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    if constexpr (!kAhead) load(row);
     R.cut(hr);
     R.cut(dr);
     float hv[C][E], dv[C][E];
@@ -337,7 +339,8 @@ __global__ __launch_bounds__(512) void rms_norm_grad_kernel(NormGradArgs a, int 
         gh += dv[i][e] * wv[e] * hv[i][e];
       }
     }
-    if (row + gridDim.x < a.rows) load(row + gridDim.x);
+    if constexpr (kAhead)
+      if (row + gridDim.x < a.rows) load(row + gridDim.x);
     row_sums(hh, gh, scratch + 2 * flip, lane, wave, waves);
     flip ^= 1;
     const float s = 1.0f / sqrtf(hh / (float)a.cols + a.eps);
@@ -378,7 +381,7 @@ __global__ __launch_bounds__(512) void rms_norm_grad_kernel(NormGradArgs a, int 
   }
 }
 
-// The same for rows that 16 waves cannot hold: read twice, and dweight's part kept in memory.
+// The same for rows that a workgroup cannot hold: read twice, and dweight's part kept in memory.
 template <typename T>
 __global__ __launch_bounds__(1024) void rms_norm_grad_long_kernel(NormGradArgs a) {
   constexpr int E = kElems<T>;
@@ -498,11 +501,22 @@ int32_t norm_by_shape(dc_hip_ctx* ctx, const NormArgs& a) {
 template <typename T>
 int32_t norm_grad_by_shape(dc_hip_ctx* ctx, const NormGradArgs& a, int64_t grid, int c, int waves) {
   const unsigned g = (unsigned)grid;
-  if (c == 1) rms_norm_grad_kernel<T, 1><<<g, 64 * waves, 0, ctx->stream>>>(a, waves);
-  else if (c == 2) rms_norm_grad_kernel<T, 2><<<g, 64 * waves, 0, ctx->stream>>>(a, waves);
-  else if (c == 4) rms_norm_grad_kernel<T, 4><<<g, 64 * waves, 0, ctx->stream>>>(a, waves);
+  constexpr bool kF32 = sizeof(T) == 4;
+  if (c == 1) rms_norm_grad_kernel<T, 1, true><<<g, 64 * waves, 0, ctx->stream>>>(a, waves);
+  else if (kF32 && c == 2) rms_norm_grad_kernel<float, 2, true><<<g, 64 * waves, 0, ctx->stream>>>(a, waves);
+  else if (c == 4) rms_norm_grad_kernel<T, 4, !kF32><<<g, 64 * waves, 0, ctx->stream>>>(a, waves);
   else rms_norm_grad_long_kernel<T><<<g, 64 * kWaves, 0, ctx->stream>>>(a);
   return dc::last_launch_status();
+}
+
+// 16-byte chunks of a row that a lane of the gradient's kernel holds (0: the long kernel). Few, and many waves: four of bf16
+// take all 256 registers; of float32, two do better than one with 16 waves. One workgroup a CU for more than one chunk, so that
+// fewer parts of dweight are left. Measured, us, with the call, for 1 / 2 / 4 chunks: bf16 8000×8192 103 / 138 / 110, 300×8192 13.3 / 14.9 /
+// 18.1, 3000×12000 - / 79 / 69, 4000×16384 - / 127 / 112; float32 8000×4096 111 / 97 / 103, 1443×5056 - / 29.0 / 29.4 (two
+// workgroups of 4 chunks a CU 36.5), 3000×6000 - / 59 / 59; 2000×12000 101 with 4, 140 by the long kernel, 300×16384 34, 46.
+int norm_grad_chunks(bool f32, int64_t chunks) {
+  if (f32) return chunks <= 512 ? 1 : chunks <= 2048 ? 2 : chunks <= 4096 ? 4 : 0;
+  return chunks <= 1024 ? 1 : chunks <= 2048 ? 4 : 0;
 }
 
 bool float_dtype(int32_t t) { return t == DC_DTYPE_F32 || t == DC_DTYPE_BF16; }
@@ -577,10 +591,10 @@ DC_HIP_API int32_t dc_hip_rms_norm_backward(dc_hip_ctx* ctx, const dc_rms_norm_g
   if (p.cols == 0 || (!p.dx && !p.dweight)) return DC_OK;
   if (p.rows == 0) return p.dweight ? dc::zero_async(ctx, p.dweight, (size_t)p.cols * sizeof(float)) : DC_OK;
   const int64_t elems = 16 / size_of(p.dtype), chunks = (p.cols + elems - 1) / elems;
-  const int c = chunks <= 512 ? 1 : chunks <= 1024 ? 2 : chunks <= 2048 ? 4 : 0, waves = c ? waves_for(chunks, c) : kWaves;
-  const int per_cu = waves <= 2 ? 8 / waves : std::max(1, 15 / waves);
+  const int c = norm_grad_chunks(p.dtype == DC_DTYPE_F32, chunks), waves = c ? waves_for(chunks, c) : kWaves;
+  const int per_cu = waves <= 2 ? 8 / waves : c > 1 ? 1 : std::max(1, 15 / waves);
   const int64_t held = per_cu * (int64_t)std::max(1, ctx->cu_count);  // workgroups
-  // (Few rows: no more parts than workgroups of that many rows each leave. us, 300×8192 15.4 / 12.7, 900×3000 14.3 / 13.7; of many rows
+  // (Few rows: no more parts than workgroups of that many rows each leave. us, 900×3000 14.3 / 13.7; of many rows
   // it would leave CUs idle: 8191×2050 32.4 / 33.1. A workgroup a row up to two rows each: 17.8, 17.0.)
   const int64_t each = (p.rows + held - 1) / held, grid = each <= 4 ? (p.rows + each - 1) / each : held;
   float* parts = nullptr;

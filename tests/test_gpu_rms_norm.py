@@ -191,6 +191,14 @@ def test_rms_norm_backward(ctx, rows, cols, dtype):
         ctx.free(a)
 
 
+# Widths on both sides of those where a row's gradient takes another form (float32 2048, 8192, 16384; bf16 8192, 16384), with
+# rows enough for workgroups that walk over several.
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,cols", [(600, 2052), (300, 4097), (530, 8192), (300, 8197), (520, 16381), (270, 16384), (260, 16385)])
+def test_rms_norm_backward_of_wide_rows(ctx, rows, cols, dtype):
+    test_rms_norm_backward(ctx, rows, cols, dtype)
+
+
 def test_nothing_to_do(ctx):
     """No rows: nothing is written but the empty sum; no columns: nothing at all."""
     f = ctx.to_device(np.full(4, 7.0, np.float32))
