@@ -487,11 +487,14 @@ int32_t launch_norm(dc_hip_ctx* ctx, const NormArgs& a, int64_t chunks) {
 
 // Measured, us, bf16 with a residual (TB/s): 16384×4096 with C = 2 and 4 waves 89.8 (5.98), C = 1 and 8 waves 88.8, a wave a row
 // (C = 8) 100; to 8 bits 81.8 (5.75), 92.1, 106, as its second sum over the row is another barrier; 8191×2050, whose
-// rows lie at 4-byte boundaries, 27.2 (4.95), C = 1 29.8; 16384×512 11.4 (5.9).
+// rows lie at 4-byte boundaries, 27.2 (4.95), C = 1 29.8; 16384×512 11.4 (5.9). Rows of 65 to 128 chunks: a wave each with C = 2, so no
+// barrier, but where rows are read and written in float32; C = 1 / 2, with the call: 16384×1001 30.0 / 26.4, to 8 bits 28.8 / 24.6,
+// 16384×576 to 8 bits 23.4 / 18.6, 4000×640 6.7 / 5.9, 2000×1001 5.4 / 5.6; float32 to 8 bits 4000×512 8.1 / 6.9, 16384×384 21.5 / 22.4.
 template <typename T, typename Y, bool kNorm>
 int32_t norm_by_shape(dc_hip_ctx* ctx, const NormArgs& a) {
   const int64_t chunks = (a.cols + kElems<T> - 1) / kElems<T>;
-  if (chunks <= 256) return launch_norm<T, Y, 1, kNorm>(ctx, a, chunks);
+  const bool wave = chunks > 64 && chunks <= 128 && (sizeof(T) == 2 || sizeof(Y) == 1);
+  if (chunks <= 256 && !wave) return launch_norm<T, Y, 1, kNorm>(ctx, a, chunks);
   if (chunks <= 1024) return launch_norm<T, Y, 2, kNorm>(ctx, a, chunks);
   if (chunks <= 64 * 4 * kWaves) return launch_norm<T, Y, 4, kNorm>(ctx, a, chunks);
   rms_norm_long_kernel<T, Y, kNorm><<<(unsigned)std::min(a.rows, kMaxGrid), 64 * kWaves, 0, ctx->stream>>>(a);

@@ -99,6 +99,13 @@ def check_fp8(q, scales, y64):
     assert np.all(off <= bound), np.max(off / bound)
 
 
+# Rows that one wave holds, with one chunk a lane and with two, and the first that it does not; rows that leave waves without one.
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("rows,cols", [(5, 256), (6, 257), (7, 511), (9, 512), (3, 513), (1030, 1001), (2, 1024), (5, 1025)])
+def test_rms_norm_of_a_wave_a_row(ctx, rows, cols, dtype):
+    test_rms_norm(ctx, rows, cols, dtype)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("rows,cols", [(1, 1), (3, 1000), (4, 70001), (2100, 129)])
 def test_quantize(ctx, rows, cols, dtype):
