@@ -37,7 +37,7 @@ class FeedForwardBlock {
   std::vector<float> Gradient(Parameter parameter) const;
 
   // One row of x a token (x.Columns == Width, else ArgumentException). Products of bf16 values, sums in float32; what
-  // Backward needs is kept.
+  // Backward needs is kept; a Forward that throws past its check of x leaves nothing for a Backward.
   Matrix Forward(const Matrix& x);
   // The gradients of a loss by x (returned) and by the parameters (kept), from its gradient by Forward's result.
   // ArgumentException unless dy has the shape of the last Forward's result.

@@ -98,13 +98,12 @@ FeedForwardBlock::Buffer<uint16_t> FeedForwardBlock::ToBf16(const Matrix& x) con
 Matrix FeedForwardBlock::Forward(const Matrix& x) {
   RequireInput(x);
   const int64_t rows = x.Rows(), d = width_, h = hidden_;
+  has_forward_ = false;  // (until all of what Backward reads belongs to these rows)
   x_ = ToBf16(x);
   normed_ = New<uint16_t>(rows * d);
   pre_ = New<uint16_t>(rows * h);
   active_ = New<uint16_t>(rows * h);
   auto y = New<float>(rows * d);
-  rows_ = x.Rows();
-  has_forward_ = true;
 
   dc_rms_norm norm{};
   norm.rows = rows, norm.cols = d, norm.dtype = norm.y_dtype = DC_DTYPE_BF16, norm.eps = epsilon_;
@@ -129,6 +128,8 @@ Matrix FeedForwardBlock::Forward(const Matrix& x) {
   Matrix out(x.Rows(), width_);
   hip_->Synchronize();
   if (out.Size() > 0) y->CopyToHost(out.Data().data(), (size_t)out.Size() * sizeof(float));
+  rows_ = x.Rows();
+  has_forward_ = true;
   return out;
 }
 

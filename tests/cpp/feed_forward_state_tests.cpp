@@ -1,0 +1,29 @@
+// What a FeedForwardBlock keeps between its calls, and which calls it refuses for the lack of it.
+#include <cmath>
+
+#include "DotCompute/FeedForward.hpp"
+#include "test_framework.hpp"
+
+using namespace DotCompute;
+using DotCompute::Algorithms::Activation;
+using DotCompute::Algorithms::AdamWOptions;
+using DotCompute::Algorithms::FeedForwardBlock;
+using DotCompute::Algorithms::Matrix;
+
+namespace {
+
+std::shared_ptr<Backends::Hip::HipAccelerator> Device() {
+  auto acc = Backends::Hip::TryCreateAccelerator();
+  CHECK(acc != nullptr);
+  return acc;
+}
+
+}  // namespace
+
+// More than 2^23 outputs are refused by the first product, after the norm has been enqueued.
+TEST_GPU(feed_forward_block_keeps_nothing_of_a_forward_that_throws) {
+  auto acc = Device();
+  FeedForwardBlock block(1, (1 << 23) + 1, Activation::Relu, *acc);
+  CHECK_THROWS(NotSupportedException, block.Forward(Matrix(2, 1)));
+  CHECK_THROWS(InvalidOperationException, block.Backward(Matrix(2, 1)));
+}
