@@ -40,7 +40,8 @@ class FeedForwardBlock {
   // Backward needs is kept; a Forward that throws past its check of x leaves nothing for a Backward.
   Matrix Forward(const Matrix& x);
   // The gradients of a loss by x (returned) and by the parameters (kept), from its gradient by Forward's result.
-  // ArgumentException unless dy has the shape of the last Forward's result.
+  // InvalidOperationException without a Forward since the last Set or Step, whose values were other ones; ArgumentException
+  // unless dy has the shape of that Forward's result.
   Matrix Backward(const Matrix& dy);
   // One AdamW step of all parameters from those gradients. InvalidOperationException without a Backward since the last.
   void Step(const AdamWOptions& options);

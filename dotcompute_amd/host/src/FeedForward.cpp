@@ -56,9 +56,9 @@ void FeedForwardBlock::Set(Parameter parameter, const std::vector<float>& values
   if ((int64_t)values.size() != t.Size())
     throw ArgumentException("FeedForwardBlock: a parameter of " + std::to_string(t.Size()) + " values was given " +
                             std::to_string(values.size()));
+  has_forward_ = quantized_ = false;  // (both belong to the values before)
   t.value->CopyFromHost(values.data(), values.size() * sizeof(float));
   Check(dc_hip_convert_f32_to_bf16(hip_->Context(), t.value->Data(), t.copy->Data(), t.Size()), "FeedForwardBlock: convert");
-  quantized_ = false;
 }
 
 std::vector<float> FeedForwardBlock::Get(Parameter parameter) const {
@@ -134,7 +134,7 @@ Matrix FeedForwardBlock::Forward(const Matrix& x) {
 }
 
 Matrix FeedForwardBlock::Backward(const Matrix& dy) {
-  if (!has_forward_) throw InvalidOperationException("FeedForwardBlock: Backward follows Forward");
+  if (!has_forward_) throw InvalidOperationException("FeedForwardBlock: Backward follows a Forward with the current parameters");
   if (dy.Rows() != rows_ || dy.Columns() != width_) throw ArgumentException(kShape + Shape(rows_, width_));
   const int64_t rows = rows_, d = width_, h = hidden_;
   auto g = ToBf16(dy);
@@ -186,7 +186,7 @@ void FeedForwardBlock::Step(const AdamWOptions& options) {
   }
   Check(dc_hip_adamw_step(hip_->Context(), &args, tensors, kParameters), "dc_hip_adamw_step");
   ++steps_;
-  has_gradient_ = quantized_ = false;
+  has_forward_ = has_gradient_ = quantized_ = false;
 }
 
 Matrix FeedForwardBlock::ForwardFp8(const Matrix& x) {

@@ -27,3 +27,20 @@ TEST_GPU(feed_forward_block_keeps_nothing_of_a_forward_that_throws) {
   CHECK_THROWS(NotSupportedException, block.Forward(Matrix(2, 1)));
   CHECK_THROWS(InvalidOperationException, block.Backward(Matrix(2, 1)));
 }
+
+// Gradients are those of the network that Forward ran: new values of the parameters ask for a new Forward.
+TEST_GPU(feed_forward_block_refuses_a_backward_of_other_parameters) {
+  auto acc = Device();
+  const Matrix x(2, 3, {1, -2, 3, 0.5f, 2, -1});
+  for (bool set : {false, true}) {
+    FeedForwardBlock block(3, 4, Activation::Silu, *acc);
+    block.Forward(x);
+    block.Backward(x);
+    block.Backward(x);  // (the same network: as often as one likes)
+    if (set) block.Set(FeedForwardBlock::W1, std::vector<float>(12, 0.5f));
+    else block.Step(AdamWOptions());
+    CHECK_THROWS(InvalidOperationException, block.Backward(x));
+    block.Forward(x);
+    CHECK(block.Backward(x).Rows() == 2);
+  }
+}
