@@ -33,7 +33,7 @@ class FeedForwardBlock {
   // ArgumentException when the length is not the parameter's.
   void Set(Parameter parameter, const std::vector<float>& values);
   std::vector<float> Get(Parameter parameter) const;
-  // The gradient that the last Backward left.
+  // The gradient that the last Backward left, before and after a Step. InvalidOperationException before the first.
   std::vector<float> Gradient(Parameter parameter) const;
 
   // One row of x a token (x.Columns == Width, else ArgumentException). Products of bf16 values, sums in float32; what
@@ -71,7 +71,7 @@ class FeedForwardBlock {
   std::array<Tensor, kParameters> p_;
   int64_t steps_ = 0;
   int32_t rows_ = 0;  // of the last Forward
-  bool has_forward_ = false, has_gradient_ = false, quantized_ = false;
+  bool has_forward_ = false, has_gradient_ = false, stepped_ = false, quantized_ = false;
   Buffer<uint16_t> x_, normed_, pre_, active_;  // kept for Backward
   Buffer<uint8_t> q1_, q2_;                     // W1 and W2 in 8 bits, made from the current values when first asked for
   Buffer<float> s1_, s2_;

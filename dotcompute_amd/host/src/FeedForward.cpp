@@ -164,6 +164,7 @@ Matrix FeedForwardBlock::Backward(const Matrix& dy) {
   norm.dy_stride = norm.h_stride = norm.dh_stride = norm.dx_stride = d;
   Check(dc_hip_rms_norm_backward(hip_->Context(), &norm), "dc_hip_rms_norm_backward");
   has_gradient_ = true;
+  stepped_ = false;
 
   std::vector<uint16_t> bits((size_t)(rows * d));
   hip_->Synchronize();
@@ -172,7 +173,7 @@ Matrix FeedForwardBlock::Backward(const Matrix& dy) {
 }
 
 void FeedForwardBlock::Step(const AdamWOptions& options) {
-  if (!has_gradient_) throw InvalidOperationException("FeedForwardBlock: Step follows Backward");
+  if (!has_gradient_ || stepped_) throw InvalidOperationException("FeedForwardBlock: Step follows Backward");
   dc_adamw args{};
   args.lr = options.LearningRate, args.beta1 = options.Beta1, args.beta2 = options.Beta2, args.eps = options.Epsilon;
   args.weight_decay = options.WeightDecay, args.grad_scale = 1.0, args.step = steps_ + 1, args.state_dtype = DC_DTYPE_F32;
@@ -186,7 +187,8 @@ void FeedForwardBlock::Step(const AdamWOptions& options) {
   }
   Check(dc_hip_adamw_step(hip_->Context(), &args, tensors, kParameters), "dc_hip_adamw_step");
   ++steps_;
-  has_forward_ = has_gradient_ = quantized_ = false;
+  has_forward_ = quantized_ = false;
+  stepped_ = true;
 }
 
 Matrix FeedForwardBlock::ForwardFp8(const Matrix& x) {

@@ -44,3 +44,17 @@ TEST_GPU(feed_forward_block_refuses_a_backward_of_other_parameters) {
     CHECK(block.Backward(x).Rows() == 2);
   }
 }
+
+// The gradients stay readable after the step that took them, which is taken once.
+TEST_GPU(feed_forward_block_keeps_gradients_past_a_step) {
+  auto acc = Device();
+  const Matrix x(2, 3, {1, -2, 3, 0.5f, 2, -1});
+  FeedForwardBlock block(3, 4, Activation::Silu, *acc);
+  block.Forward(x);
+  block.Backward(x);
+  const auto before = block.Gradient(FeedForwardBlock::B2);
+  CHECK(before == (std::vector<float>{1.5f, 0.0f, 2.0f}));  // (the sums of dy's columns)
+  block.Step(AdamWOptions());
+  CHECK(block.Gradient(FeedForwardBlock::B2) == before);
+  CHECK_THROWS(InvalidOperationException, block.Step(AdamWOptions()));
+}
