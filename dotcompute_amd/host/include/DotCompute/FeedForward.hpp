@@ -41,7 +41,7 @@ class FeedForwardBlock {
   Matrix Forward(const Matrix& x);
   // The gradients of a loss by x (returned) and by the parameters (kept), from its gradient by Forward's result.
   // InvalidOperationException without a Forward since the last Set or Step, whose values were other ones; ArgumentException
-  // unless dy has the shape of that Forward's result.
+  // unless dy has the shape of that Forward's result. A Backward that throws past these checks leaves no gradients.
   Matrix Backward(const Matrix& dy);
   // One AdamW step of all parameters from those gradients. InvalidOperationException without a Backward since the last.
   void Step(const AdamWOptions& options);

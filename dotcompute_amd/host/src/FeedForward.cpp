@@ -137,6 +137,7 @@ Matrix FeedForwardBlock::Backward(const Matrix& dy) {
   if (!has_forward_) throw InvalidOperationException("FeedForwardBlock: Backward follows a Forward with the current parameters");
   if (dy.Rows() != rows_ || dy.Columns() != width_) throw ArgumentException(kShape + Shape(rows_, width_));
   const int64_t rows = rows_, d = width_, h = hidden_;
+  has_gradient_ = false;  // (until all of them are of this dy)
   auto g = ToBf16(dy);
   auto dactive = New<uint16_t>(rows * h);
   auto dnormed = New<uint16_t>(rows * d);

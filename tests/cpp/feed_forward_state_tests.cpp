@@ -58,3 +58,16 @@ TEST_GPU(feed_forward_block_keeps_gradients_past_a_step) {
   CHECK(block.Gradient(FeedForwardBlock::B2) == before);
   CHECK_THROWS(InvalidOperationException, block.Step(AdamWOptions()));
 }
+
+// Sums over more than 2^23 rows are refused.
+TEST_GPU(feed_forward_block_keeps_no_gradients_of_a_backward_that_throws) {
+  auto acc = Device();
+  FeedForwardBlock block(1, 1, Activation::None, *acc);
+  block.Forward(Matrix(2, 1));
+  block.Backward(Matrix(2, 1));
+  const Matrix tall((1 << 23) + 1, 1);
+  block.Forward(tall);
+  CHECK_THROWS(NotSupportedException, block.Backward(tall));
+  CHECK_THROWS(InvalidOperationException, block.Gradient(FeedForwardBlock::W2));
+  CHECK_THROWS(InvalidOperationException, block.Step(AdamWOptions()));
+}
