@@ -155,6 +155,18 @@ def _expect(a: "DeviceArray | None", name: str, dtypes: tuple, shape: tuple) -> 
         raise ValueError(f"{name}: shape {tuple(shape)} expected, of type {dtypes} (got {tuple(a.shape)}, {a.dtype})")
 
 
+def _check_reach(a: "DeviceArray", name: str, stride: int) -> None:
+    """Rows `stride` elements apart end within the allocation of a's context that they start in. (Of memory that the context has not
+    allocated nothing is known here.)"""
+    rows, cols = a.shape
+    if a.ctx is None or rows < 2:
+        return
+    end = a.ptr + ((rows - 1) * stride + cols) * a.dtype.itemsize
+    for base in a.ctx._arrays:
+        if base.ptr and base.ptr <= a.ptr < base.ptr + base.nbytes and end > base.ptr + base.nbytes:
+            raise ValueError(f"{name}_stride: {rows} rows of {cols}, {stride} apart, reach past their allocation")
+
+
 class _Arguments(C.Structure):
     """An argument block of arrays by name; it keeps them alive as long as it lives."""
 
@@ -165,7 +177,10 @@ class _Arguments(C.Structure):
                 continue
             setattr(self, name, a.ptr)
             if len(a.shape) == 2:
-                setattr(self, name + "_stride", strides.pop(name + "_stride", a.shape[1]))
+                stride = strides.pop(name + "_stride", None)
+                if stride is not None:
+                    _check_reach(a, name, stride)
+                setattr(self, name + "_stride", a.shape[1] if stride is None else stride)
         if strides:
             raise ValueError(f"no such strides: {sorted(strides)}")
 

@@ -1,0 +1,45 @@
+"""CPU: what the binding looks at before an operator's call, since a kernel is handed addresses alone."""
+import types
+
+import numpy as np
+import pytest
+
+from dotcompute_amd import hip
+
+P = 4096  # an address that nobody reads
+BF16, F32, CODE = np.dtype(np.uint16), np.dtype(np.float32), np.dtype(np.uint8)
+
+
+def context(*sizes):
+    """A context with allocations of those many bytes, far from each other."""
+    ctx = types.SimpleNamespace(handle=None)
+    ctx._arrays = [hip.DeviceArray(ctx, P + (i << 20), size, CODE, (size,)) for i, size in enumerate(sizes)]
+    return ctx
+
+
+def rows(ctx, which, at, shape, dtype=BF16):
+    """A matrix whose rows start `at` elements into an allocation."""
+    return hip.DeviceArray(ctx, ctx._arrays[which].ptr + at * dtype.itemsize, int(np.prod(shape)) * dtype.itemsize, dtype, shape)
+
+
+def test_rows_end_within_their_allocation():
+    """Three rows of 8, 10 apart, 2 elements in, take 30 elements."""
+    for size, fits in ((60, True), (59, False), (1 << 16, True), (48, False)):
+        ctx = context(size, 48, 1 << 16)
+        x, w, y = rows(ctx, 0, 2, (3, 8)), rows(ctx, 2, 0, (3, 8)), rows(ctx, 2, 0, (3, 3))
+        if fits:
+            assert hip.Linear.of(x, w, y, x_stride=10).x_stride == 10
+        else:
+            with pytest.raises(ValueError, match="x_stride"):
+                hip.Linear.of(x, w, y, x_stride=10)
+    ctx = context(60, 48, 1 << 16)
+    x, w = rows(ctx, 0, 2, (3, 8)), rows(ctx, 2, 0, (8,))
+    assert hip.RmsNorm.of(x, w, x, x_stride=10, y_stride=10).y_stride == 10
+    for bad in (dict(y_stride=11), dict(x_stride=11)):
+        with pytest.raises(ValueError, match="stride"):
+            hip.RmsNorm.of(x, w, x, **bad)
+    # a single row's stride says nothing; memory of others is taken at its word
+    one = rows(ctx, 0, 2, (1, 8))
+    assert hip.RmsNorm.of(one, w, one, x_stride=1 << 40).x_stride == 1 << 40
+    other = hip.DeviceArray(ctx, P + (9 << 20), 48, BF16, (3, 8))
+    assert hip.RmsNorm.of(other, w, other, x_stride=100, y_stride=100).x_stride == 100
