@@ -318,7 +318,8 @@ class AdamWTensors:
                 setattr(t, name, a.ptr)
                 types[name] = dtype_of(a)
             if types["param"] != DTYPE_F32 or types["grad"] == DTYPE_FP8 or state == DTYPE_BF16 or types["v"] != state \
-                    or types.get("copy", DTYPE_BF16) != DTYPE_BF16:
+                    or types.get("copy", DTYPE_BF16) != DTYPE_BF16 \
+                    or {types.get("m_scales", DTYPE_F32), types.get("v_scales", DTYPE_F32)} != {DTYPE_F32}:
                 raise ValueError(f"no such types: {types}")
             t.n, t.grad_dtype = n, types["grad"]
             states.add(state)

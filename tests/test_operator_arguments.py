@@ -43,3 +43,18 @@ def test_rows_end_within_their_allocation():
     assert hip.RmsNorm.of(one, w, one, x_stride=1 << 40).x_stride == 1 << 40
     other = hip.DeviceArray(ctx, P + (9 << 20), 48, BF16, (3, 8))
     assert hip.RmsNorm.of(other, w, other, x_stride=100, y_stride=100).x_stride == 100
+
+
+def array(shape, dtype):
+    return hip.DeviceArray(None, P, int(np.prod(shape)) * dtype.itemsize, dtype, shape)
+
+
+@pytest.mark.parametrize("name", ["m_scales", "v_scales"])
+@pytest.mark.parametrize("dtype", [BF16, CODE], ids=["u16", "u8"])
+def test_scales_of_adamw_states_are_float32(name, dtype):
+    """The kernel reads and writes four bytes of each: fewer would be another array's."""
+    part = dict(param=array((300,), F32), grad=array((300,), BF16), m=array((300,), CODE), v=array((300,), CODE),
+                m_scales=array((2,), F32), v_scales=array((2,), F32))
+    assert hip.AdamWTensors.of([part]).state_dtype == hip.DTYPE_FP8
+    with pytest.raises(ValueError, match="types"):
+        hip.AdamWTensors.of([{**part, name: array((2,), dtype)}])
