@@ -511,7 +511,7 @@ class DeviceArray:
 
     @property
     def size(self) -> int:
-        return math.prod(self.shape)
+        return math.prod(map(int, self.shape))
 
     def copy_from(self, host: np.ndarray) -> "DeviceArray":
         host = np.ascontiguousarray(host, self.dtype)

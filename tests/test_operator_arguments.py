@@ -58,3 +58,10 @@ def test_scales_of_adamw_states_are_float32(name, dtype):
     assert hip.AdamWTensors.of([part]).state_dtype == hip.DTYPE_FP8
     with pytest.raises(ValueError, match="types"):
         hip.AdamWTensors.of([{**part, name: array((2,), dtype)}])
+
+
+@pytest.mark.parametrize("kind", [int, np.int64, np.int32])
+def test_sizes_of_large_arrays(kind):
+    """Elements are counted in whole numbers, whatever the shape's are."""
+    a = hip.DeviceArray(None, P, 1 << 33, CODE, (kind(1 << 17), kind(1 << 16)))
+    assert a.size == 1 << 33 and type(a.size) is int
