@@ -730,6 +730,7 @@ class Context:
         check(load().dc_hip_linear_backward(self.handle, args), "dc_hip_linear_backward")
 
     def adamw_step(self, args: AdamW, tensors: AdamWTensors) -> None:
+        args = AdamW.from_buffer_copy(args)  # (the caller's may be another step's at the same time)
         args.state_dtype = tensors.state_dtype
         check(load().dc_hip_adamw_step(self.handle, args, tensors.items, len(tensors.items)), "dc_hip_adamw_step")
 

@@ -65,3 +65,13 @@ def test_sizes_of_large_arrays(kind):
     """Elements are counted in whole numbers, whatever the shape's are."""
     a = hip.DeviceArray(None, P, 1 << 33, CODE, (kind(1 << 17), kind(1 << 16)))
     assert a.size == 1 << 33 and type(a.size) is int
+
+
+def test_a_step_leaves_its_argument_block_alone():
+    """One block of numbers serves tensors of either states, in any order and from any thread."""
+    ctx = types.SimpleNamespace(handle=None)
+    args = hip.AdamW.of(lr=1e-3)
+    before = bytes(args)
+    with pytest.raises(hip.HipError):  # (no context)
+        hip.Context.adamw_step(ctx, args, hip.AdamWTensors((hip.AdamWTensor * 0)(), hip.DTYPE_FP8, []))
+    assert bytes(args) == before
