@@ -715,12 +715,17 @@ class Context:
     def rms_norm_backward(self, args: RmsNormGrad) -> None:
         check(load().dc_hip_rms_norm_backward(self.handle, args), "dc_hip_rms_norm_backward")
 
-    def quantize_fp8(self, x: DeviceArray, q: DeviceArray, scales: DeviceArray) -> None:
-        """Rows of x (float32 or bf16) in e4m3 (uint8 bytes) with a scale each."""
+    def quantize_fp8(self, x: DeviceArray, q: DeviceArray, scales: DeviceArray, x_stride: int | None = None,
+                     q_stride: int | None = None) -> None:
+        """Rows of x (float32 or bf16) in e4m3 (uint8 bytes) with a scale each. Row strides in elements, else dense."""
         rows, cols = _matrix(x, "x")
         _expect(q, "q", (DTYPE_FP8,), (rows, cols))
         _expect(scales, "scales", (DTYPE_F32,), (rows,))
-        check(load().dc_hip_quantize_fp8(self.handle, x.ptr, dtype_of(x), cols, q.ptr, cols, scales.ptr, rows, cols),
+        for name, a, stride in (("x", x, x_stride), ("q", q, q_stride)):
+            if stride is not None:
+                _check_reach(a, name, stride)
+        x_stride, q_stride = (cols if s is None else s for s in (x_stride, q_stride))
+        check(load().dc_hip_quantize_fp8(self.handle, x.ptr, dtype_of(x), x_stride, q.ptr, q_stride, scales.ptr, rows, cols),
               "dc_hip_quantize_fp8")
 
     def linear(self, args: Linear) -> None:

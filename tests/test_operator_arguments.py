@@ -75,3 +75,16 @@ def test_a_step_leaves_its_argument_block_alone():
     with pytest.raises(hip.HipError):  # (no context)
         hip.Context.adamw_step(ctx, args, hip.AdamWTensors((hip.AdamWTensor * 0)(), hip.DTYPE_FP8, []))
     assert bytes(args) == before
+
+
+def test_rows_to_8_bits_take_strides():
+    ctx = context(60, 48, 1 << 16)
+    x, q, s = rows(ctx, 0, 2, (3, 8)), rows(ctx, 1, 0, (3, 8), CODE), rows(ctx, 2, 0, (3,), F32)
+    for bad in (dict(x_stride=11), dict(q_stride=21)):
+        with pytest.raises(ValueError, match="stride"):
+            hip.Context.quantize_fp8(ctx, x, q, s, **bad)
+    for status, strides in ((hip.DC_ERR_DIMENSION, dict(x_stride=7)), (hip.DC_ERR_DIMENSION, dict(q_stride=7)),
+                            (hip.DC_ERR_INVALID_ARGUMENT, dict(x_stride=10, q_stride=20)), (hip.DC_ERR_INVALID_ARGUMENT, {})):
+        with pytest.raises(hip.HipError) as e:  # (the last two: no context)
+            hip.Context.quantize_fp8(ctx, x, q, s, **strides)
+        assert e.value.status == status
