@@ -45,18 +45,25 @@ __device__ inline float sigmoid(float v) { return __builtin_amdgcn_rcpf(1.0f + _
 constexpr float kTanhArg = 2.0f * 0.7978845608f;  // 2 sqrt(2 / pi)
 constexpr float kTanhCube = 0.044715f;
 
-// P(z), the normal distribution's function, from *e = exp(-z^2 / 2): 1 - erf(x) = e^(-x^2) times a polynomial of the fifth
-// degree in 1 / (1 + 0.3275911 x) for x >= 0, within 1.5e-7 (Abramowitz and Stegun, Handbook of Mathematical Functions, 7.1.26);
-// the tail on the left is that product itself, so nothing cancels there.
+// P(z), the normal distribution's function, from *e = exp(-z^2 / 2). Left of zero it is e^(-x^2) erfc(x) e^(x^2) / 2 with x = |z| / sqrt(2), a
+// product in which nothing cancels; the scaled erfc is t times a polynomial in t = 1 / (1 + 0.33 x), whose eight coefficients here
+// were fitted to it for the least relative error over x < 9.4 (8.2e-8, by reweighted least squares). So P is within 8e-7 of
+// itself down to z = -5, and 5e-6 down to -13, where e's exponent is what is rounded: results in float32 keep their digits in
+// the tail too. (A polynomial of the fifth degree with an absolute bound, which is three products cheaper, was off by 0.16 %
+// of P at -5 and 1 % at -8, more than the rounding to bf16. Measured, us, that / this:
+// 1537×2049×1023 25.9 / 25.8, 8192×8192×1024 169 / 172, both gradients of 8192,8192,2048 550 / 549.)
 __device__ inline float normal_part(float z, float* e) {
   const float x = __builtin_fabsf(z) * 0.70710678f;
   *e = __expf(-0.5f * z * z);
-  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3275911f, x, 1.0f));
-  float q = __builtin_fmaf(1.061405429f, t, -1.453152027f);
-  q = __builtin_fmaf(q, t, 1.421413741f);
-  q = __builtin_fmaf(q, t, -0.284496736f);
-  q = __builtin_fmaf(q, t, 0.254829592f);
-  q *= 0.5f * t * *e;
+  const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.33f, x, 1.0f));
+  float q = __builtin_fmaf(-0.0679644048f, t, 0.231344149f);
+  q = __builtin_fmaf(q, t, -0.177719533f);
+  q = __builtin_fmaf(q, t, 0.206270859f);
+  q = __builtin_fmaf(q, t, 0.0225052908f);
+  q = __builtin_fmaf(q, t, 0.100961924f);
+  q = __builtin_fmaf(q, t, 0.0914186165f);
+  q = __builtin_fmaf(q, t, 0.0931830555f);
+  q *= t * *e;
   return z > 0.0f ? 1.0f - q : q;
 }
 

@@ -566,7 +566,7 @@ typedef enum dc_dtype {
 typedef enum dc_activation {
   DC_ACT_NONE = 0,
   DC_ACT_RELU = 1,
-  DC_ACT_GELU = 2,      /* z P(z), P the normal distribution's function */
+  DC_ACT_GELU = 2,      /* z P(z), P the normal distribution's function (within 1e-6 of itself to z = -5, 5e-6 to -13) */
   DC_ACT_GELU_TANH = 3, /* z / (1 + exp(-2u)), u = sqrt(2/pi) (z + 0.044715 z^3) */
   DC_ACT_SILU = 4       /* z / (1 + exp(-z)) */
 } dc_activation;
