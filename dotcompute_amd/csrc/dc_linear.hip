@@ -1279,9 +1279,9 @@ DC_HIP_API int32_t dc_hip_linear_backward(dc_hip_ctx* ctx, const dc_linear_grad*
   const dc_linear_grad& p = *args;
   DC_RETURN_IF(check_dims(p.m, p.n, p.k, p.activation));
   if (p.reserved != 0) return DC_ERR_INVALID_ARGUMENT;
-  if (p.m > dc::kLinearWidth) return DC_ERR_UNSUPPORTED;  // dw's sums run along m
   const bool act = p.activation != DC_ACT_NONE;
   const bool dx = p.dx && p.m > 0 && p.k > 0, dw = p.dw && p.n > 0 && p.k > 0, dbias = p.dbias && p.n > 0;
+  if (dw && p.m > dc::kLinearWidth) return DC_ERR_UNSUPPORTED;  // (dw's sums run along m)
   const bool inputs = p.m > 0 && p.n > 0 && (dx || dw || dbias);
   if (inputs) {
     DC_RETURN_IF(check_rows(p.dy, 2, p.dy_stride, p.m, p.n));

@@ -555,7 +555,8 @@ DC_HIP_API int32_t dc_hip_spmv_plan_destroy(dc_hip_spmv_plan* plan);
  * themselves times their scale, max / 448 over the row or block that shares it; a NaN in one makes its scale NaN.
  * Sums, statistics and scales are float32. Results are the same bits from call to call. Outputs overlap neither inputs
  * nor each other but where it is said below. Infinities and NaN do what float32 arithmetic makes of them, within their row.
- * Widths up to 2^25 (norms) and 2^23 (n, k, and m of dw; DC_ERR_UNSUPPORTED beyond); sizes of zero are fine everywhere.
+ * Widths up to 2^25 (norms) and 2^23 (n, k, and m where dw is asked for; DC_ERR_UNSUPPORTED beyond), m below 2^30
+ * (DC_ERR_INVALID_ARGUMENT beyond); sizes of zero are fine everywhere.
  * ------------------------------------------------------------------------------------------- */
 typedef enum dc_dtype {
   DC_DTYPE_F32 = 0,

@@ -88,3 +88,12 @@ def test_rows_to_8_bits_take_strides():
         with pytest.raises(hip.HipError) as e:  # (the last two: no context)
             hip.Context.quantize_fp8(ctx, x, q, s, **strides)
         assert e.value.status == status
+
+
+def test_sums_along_many_rows_are_refused_where_they_are_asked_for():
+    """m beyond 2^23 is too long for dw's sums, and nothing to the other gradients (which get as far as the missing context)."""
+    n = (1 << 23) + 1
+    args = dict(m=n, n=8, k=8, dy=P, x=P, w=P, dy_stride=8, x_stride=8, w_stride=8, dx_stride=8, dw_stride=8)
+    for outputs, status in ((dict(dw=P), hip.DC_ERR_UNSUPPORTED), (dict(dx=P, dw=P), hip.DC_ERR_UNSUPPORTED),
+                            (dict(dx=P), hip.DC_ERR_INVALID_ARGUMENT), (dict(dbias=P), hip.DC_ERR_INVALID_ARGUMENT)):
+        assert hip.load().dc_hip_linear_backward(None, hip.LinearGrad(**args, **outputs)) == status
