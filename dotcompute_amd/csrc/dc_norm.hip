@@ -179,7 +179,7 @@ __global__ __launch_bounds__(C == 4 ? 1024 : 512) void rms_norm_kernel(NormArgs 
           if (R.at(i) + e < cols) top = max(top, dc::magnitude(h[i][e]));
       const float t = __builtin_bit_cast(float, row_max(top, scratch[1], wave, waves));
       const float factor = dc::fp8_factor(t);
-      if (lane == 0 && wave == 0) a.scales[row] = t / dc::kFp8Top;
+      if (lane == 0 && wave == 0) a.scales[row] = dc::fp8_scale(t);
 #pragma unroll
       for (int i = 0; i < C; ++i)
 #pragma unroll
@@ -250,7 +250,7 @@ __global__ __launch_bounds__(1024) void rms_norm_long_kernel(NormArgs a) {
       }
       const float t = __builtin_bit_cast(float, row_max(top, scratch[1], wave, kWaves));
       factor = dc::fp8_factor(t);
-      if (threadIdx.x == 0) a.scales[row] = t / dc::kFp8Top;
+      if (threadIdx.x == 0) a.scales[row] = dc::fp8_scale(t);
     }
     for (int64_t c = first; c < cols; c += kStep) {  // (a lane writes only what it alone has read)
       float v[E];

@@ -47,7 +47,12 @@ __device__ inline uint32_t pack_fp8(float a, float b, float c, float d) {
   const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(clamp_fp8(a), clamp_fp8(b), 0, false);
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(clamp_fp8(c), clamp_fp8(d), lo, true);
 }
-// What a scale `top / 448` multiplies with: 448 / top, at most the largest float (so that zeros stay zeros).
+// The scale of values of at most `top`, and what they are multiplied with to become codes. 448 / top is no float where top is below
+// 448 2^-128: such values are held as their products with 2^128 (the largest float, within its rounding), zeros as zeros.
+__device__ inline float fp8_scale(float top) {
+  const float s = top / kFp8Top;
+  return top > 0.0f && s < 0x1p-128f ? 0x1p-128f : s;
+}
 __device__ inline float fp8_factor(float top) {
   const float f = kFp8Top / top;
   return f > __FLT_MAX__ ? __FLT_MAX__ : f;

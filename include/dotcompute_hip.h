@@ -609,7 +609,8 @@ typedef struct dc_rms_norm_grad {
 } dc_rms_norm_grad;
 DC_HIP_API int32_t dc_hip_rms_norm_backward(dc_hip_ctx* ctx, const dc_rms_norm_grad* args);
 
-/* Rows in 8 bits: scales[r] = max|x[r]| / 448, q[r] = e4m3(x[r] * (448 / max|x[r]|)). dtype: F32 or BF16. */
+/* Rows in 8 bits: scales[r] = max|x[r]| / 448, q[r] = e4m3(x[r] * (448 / max|x[r]|)); where that maximum is above zero and below
+ * 448 2^-128, 2^-128 and e4m3(x[r] 2^128), since 448 / max is no float there. dtype: F32 or BF16. */
 DC_HIP_API int32_t dc_hip_quantize_fp8(dc_hip_ctx* ctx, const void* x, int32_t dtype, int64_t x_stride,
                                        uint8_t* q, int64_t q_stride, float* scales, int64_t rows,
                                        int64_t cols);

@@ -24,3 +24,48 @@ def test_rows_that_lie_apart(ctx, rows, cols, dtype):
     a.read()
     for m in (a.base, q.base, s):
         ctx.free(m)
+
+
+# Maxima on both sides of 448 2^-128 = 1.3e-36, below which their reciprocals are no floats, and the smallest floats.
+TINY = [1e-30, 2e-36, 1.3e-36, 1e-36, 1e-37, 2e-38, 1e-40, 1e-44, 0.0]
+
+
+def check_codes(q, s, want):
+    """Codes stand for the values to half a step of 4 bits or of the smallest code; a scale of at least 2^-128 has 21 bits (where it is one
+    of the smaller floats), and a product that is one itself is off by half the smallest float."""
+    scale = s[:, None].astype(np.float64)
+    off = np.abs(ref.from_fp8(q) * scale - want)
+    assert np.all(off <= np.maximum(np.abs(want) * ref.FP8, ref.LEAST / 2 * scale) * (1 + 2.0 ** -18) + 2.0 ** -149), off.max(axis=1)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("cols", [40, 1000, 5000])
+def test_rows_of_next_to_nothing(ctx, cols, dtype):
+    unit = np.random.default_rng(cols).uniform(-1, 1, size=(len(TINY), cols)).astype(np.float32)
+    unit[:, 3] = 1.0
+    x = unit * np.float32(TINY)[:, None]
+    x = ref.to_bf16(x) if dtype == "bf16" else x
+    dx, q, s = ctx.to_device(x), ctx.empty(x.shape, np.uint8), ctx.empty(len(TINY), np.float32)
+    ctx.quantize_fp8(dx, q, s)
+    ctx.synchronize()
+    check_codes(q.to_host(), s.to_host(), wide(x))
+    assert s.to_host()[-1] == 0 and np.all(ref.from_fp8(q.to_host()[-1]) == 0)  # (zeros of either sign)
+    for a in (dx, q, s):
+        ctx.free(a)
+
+
+@pytest.mark.parametrize("cols", [200, 70001])
+def test_norms_of_next_to_nothing(ctx, cols):
+    """A weight that takes a norm's results there: what float32 makes of h w / rms(h), in 8 bits."""
+    rng = np.random.default_rng(cols)
+    h, w = rng.normal(size=(2, cols)).astype(np.float32), (1e-37 * rng.uniform(0.5, 1, size=cols)).astype(np.float32)
+    dh, dw, q, s = ctx.to_device(h), ctx.to_device(w), ctx.empty(h.shape, np.uint8), ctx.empty(2, np.float32)
+    ctx.rms_norm(hip.RmsNorm.of(dh, dw, q, scales=s))
+    ctx.synchronize()
+    want = ref.rms_norm(wide(h), wide(w), 1e-6)[1]
+    # (the norm's own error, 4e-6 of a value, may move a code's rounding by that)
+    scale = s.to_host()[:, None].astype(np.float64)
+    off = np.abs(ref.from_fp8(q.to_host()) * scale - want)
+    assert np.all(off <= np.maximum(np.abs(want) * ref.FP8, ref.LEAST / 2 * scale) * (1 + 2.0 ** -16) + 2.0 ** -149)
+    for a in (dh, dw, q, s):
+        ctx.free(a)
