@@ -52,9 +52,12 @@ __device__ inline void unpack_fp8(uint32_t w, float (&v)[4]) {
 }
 
 // A block's scale is its largest magnitude times 1 / 448, and its values are held as their products with 448 times the reciprocal
-// of that magnitude (at most the largest float, so that zeros stay zeros): products, where the definition divides, are within an
-// ulp of it, far below a code's step.
-constexpr float kPerTop = 1.0f / dc::kFp8Top;
+// of that magnitude (at most the largest float, where the scale is 2^-128, and zeros stay zeros): products, where the definition
+// divides, are within an ulp of it, far below a code's step.
+__device__ inline float state_scale(float top) {
+  const float s = top * (1.0f / dc::kFp8Top);
+  return top > 0.0f && s < 0x1p-128f ? 0x1p-128f : s;
+}
 __device__ inline float state_factor(float top) {
   const float f = (1.0f / top) * dc::kFp8Top;
   return f > __FLT_MAX__ ? __FLT_MAX__ : f;
@@ -176,8 +179,8 @@ __device__ inline void step_block(const Step& s, const Tensor& t, int64_t start)
       store_codes(static_cast<uint8_t*>(t.m) + at, left, dc::pack_fp8(m[0], m[1], m[2], m[3]));
       store_codes(static_cast<uint8_t*>(t.v) + at, left, dc::pack_fp8(root[0], root[1], root[2], root[3]));
       if (lane == 0) {
-        t.m_scales[start / kBlock] = mt * kPerTop;
-        t.v_scales[start / kBlock] = vt * kPerTop;
+        t.m_scales[start / kBlock] = state_scale(mt);
+        t.v_scales[start / kBlock] = state_scale(vt);
       }
     }
   } else if (left > 0) {

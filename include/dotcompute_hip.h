@@ -661,7 +661,8 @@ DC_HIP_API int32_t dc_hip_linear_backward(dc_hip_ctx* ctx, const dc_linear_grad*
  * float32, and the scales are NULL. FP8: m holds e4m3 values with a scale for every 256 elements
  * (ceil(n / 256) scales; the last block may be short), v the same of sqrt(v), whose values above zero are held as at
  * least the smallest e4m3 value, so that none becomes a zero denominator. Zeroed states and scales are step 1's. (The
- * scales are the maxima times 1 / 448 in float32, the codes those of the values times 448 / maximum, each within an ulp.)
+ * scales are the maxima times 1 / 448 in float32, 2^-128 at least where anything is above zero, the codes those of the values times
+ * 448 / maximum, at most 2^128, each within an ulp.)
  * A NaN or infinite gradient makes its element's states and param such; in 8 bits the other states of its block too. */
 #define DC_ADAMW_BLOCK 256
 typedef struct dc_adamw {
