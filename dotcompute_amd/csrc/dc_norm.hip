@@ -344,7 +344,7 @@ __global__ __launch_bounds__(C == 4 && kAhead ? 512 : 1024) void rms_norm_grad_k
     row_sums(hh, gh, scratch + 2 * flip, lane, wave, waves);
     flip ^= 1;
     const float s = 1.0f / sqrtf(hh / (float)a.cols + a.eps);
-    const float mean = s * s * (gh / (float)a.cols);  // mean(g h s) s
+    const float mean = s * (s * (gh / (float)a.cols));  // mean(g h s) s (s^2 alone may be no float where eps is 0)
     if (a.dx) {
       T* dx = static_cast<T*>(a.dx) + row * a.dx_stride;
       if (a.dh) R.cut(uv);
@@ -415,7 +415,7 @@ __global__ __launch_bounds__(1024) void rms_norm_grad_long_kernel(NormGradArgs a
     row_sums(hh, gh, scratch + 2 * flip, lane, wave, kWaves);
     flip ^= 1;
     const float s = 1.0f / sqrtf(hh / (float)a.cols + a.eps);
-    const float mean = s * s * (gh / (float)a.cols);
+    const float mean = s * (s * (gh / (float)a.cols));
     for (int64_t c = (int64_t)threadIdx.x * E; c < cols; c += 64 * kWaves * E) {
       read(c);
       if (dx) {
