@@ -526,6 +526,11 @@ bool float_dtype(int32_t t) { return t == DC_DTYPE_F32 || t == DC_DTYPE_BF16; }
 int64_t size_of(int32_t t) { return t == DC_DTYPE_F32 ? 4 : t == DC_DTYPE_BF16 ? 2 : 1; }
 bool aligned_to(const void* p, int64_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(bytes - 1)) == 0; }
 
+// Rows of nothing: their maxima, and so their scales, are zeros.
+int32_t empty_scales(dc_hip_ctx* ctx, float* scales, int64_t rows) {
+  return scales && rows > 0 ? dc::zero_async(ctx, scales, (size_t)rows * sizeof(float)) : DC_OK;
+}
+
 // One row, or several with a stride of at least a row's length.
 int32_t check_rows(const void* p, int32_t dtype, int64_t stride, int64_t rows, int64_t cols) {
   if (!aligned_to(p, size_of(dtype))) return DC_ERR_MISALIGNED;
@@ -565,10 +570,10 @@ DC_HIP_API int32_t dc_hip_rms_norm(dc_hip_ctx* ctx, const dc_rms_norm* args) {
     DC_RETURN_IF(check_rows(p.weight, p.dtype, p.cols, 1, p.cols));
     if (p.residual) DC_RETURN_IF(check_rows(p.residual, p.dtype, p.residual_stride, p.rows, p.cols));
     if (p.sum) DC_RETURN_IF(check_rows(p.sum, p.dtype, p.sum_stride, p.rows, p.cols));
-    if (!aligned_to(p.scales, 4)) return DC_ERR_MISALIGNED;
   }
+  if (!aligned_to(p.scales, 4)) return DC_ERR_MISALIGNED;
   DC_CTX_ENTER(ctx);
-  if (p.rows == 0 || p.cols == 0) return DC_OK;
+  if (p.rows == 0 || p.cols == 0) return empty_scales(ctx, p.scales, p.rows);
   const NormArgs a{p.x,    p.residual,        p.weight,     p.sum,      p.y,              p.scales, p.rows,
                    p.x_stride, p.residual_stride, p.sum_stride, p.y_stride, (int32_t)p.cols, p.eps};
   if (p.dtype == DC_DTYPE_F32)
@@ -619,10 +624,10 @@ DC_HIP_API int32_t dc_hip_quantize_fp8(dc_hip_ctx* ctx, const void* x, int32_t d
     if (!x || !q || !scales) return DC_ERR_INVALID_ARGUMENT;
     DC_RETURN_IF(check_rows(x, dtype, x_stride, rows, cols));
     DC_RETURN_IF(check_rows(q, DC_DTYPE_FP8, q_stride, rows, cols));
-    if (!aligned_to(scales, 4)) return DC_ERR_MISALIGNED;
   }
+  if (!aligned_to(scales, 4)) return DC_ERR_MISALIGNED;
   DC_CTX_ENTER(ctx);
-  if (rows == 0 || cols == 0) return DC_OK;
+  if (rows == 0 || cols == 0) return empty_scales(ctx, scales, rows);
   const NormArgs a{x, nullptr, nullptr, nullptr, q, scales, rows, x_stride, 0, 0, q_stride, (int32_t)cols, 0.0f};
   return dtype == DC_DTYPE_F32 ? norm_by_shape<float, uint8_t, false>(ctx, a) : norm_by_shape<bf16, uint8_t, false>(ctx, a);
 }

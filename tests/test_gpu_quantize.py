@@ -69,3 +69,22 @@ def test_norms_of_next_to_nothing(ctx, cols):
     assert np.all(off <= np.maximum(np.abs(want) * ref.FP8, ref.LEAST / 2 * scale) * (1 + 2.0 ** -16) + 2.0 ** -149)
     for a in (dh, dw, q, s):
         ctx.free(a)
+
+
+def test_rows_of_nothing(ctx):
+    """Their scales are those of zeros, so that a product over them is its bias."""
+    m, n = 5, 12
+    e, bias = ctx.empty(8, np.uint16), ctx.to_device(ref.to_bf16(np.arange(n)))
+    s, y = [ctx.to_device(np.full(r, np.nan, np.float32)) for r in (m, n)], ctx.empty((m, n), np.float32)
+
+    def part(dtype, *shape):
+        return hip.DeviceArray(ctx, e.ptr, 0, np.dtype(dtype), shape)
+
+    ctx.rms_norm(hip.RmsNorm.of(part(np.uint16, m, 0), part(np.uint16, 0), part(np.uint8, m, 0), scales=s[0]))
+    ctx.quantize_fp8(part(np.uint16, n, 0), part(np.uint8, n, 0), s[1])
+    ctx.linear(hip.Linear.of(part(np.uint8, m, 0), part(np.uint8, n, 0), y, bias=bias, x_scales=s[0], w_scales=s[1]))
+    ctx.synchronize()
+    assert np.all(s[0].to_host() == 0) and np.all(s[1].to_host() == 0)
+    assert np.array_equal(y.to_host(), np.tile(np.arange(n, dtype=np.float32), (m, 1)))
+    for a in (e, bias, y, *s):
+        ctx.free(a)
