@@ -7,7 +7,8 @@
 //   - product_kernel: D[i][j] = sum_c A(i, c) B(j, c) in tiles on the matrix cores. A's rows run along c. B's do too
 //     (forward), or are the rows c of a row-major [c][j] matrix (the gradients, both in one launch).
 //   - join_kernel: the results from the sums over parts of c, where few tiles have long sums.
-//   - few_rows_kernel, few_rows_any_kernel: forward with few rows of x.
+//   - few_rows_kernel, few_rows_any_kernel: forward with few rows of x, or so few results that 64 rows and 16 outputs of them to a
+//     workgroup leave no CU two.
 //   - slope_kernel: dz and its transpose in bf16 (what the two gradients' products run along), and dbias's parts.
 //   - pack_kernel: rows that the direct-to-LDS loads cannot take (not 16-byte aligned, or no whole number of
 //     16 bytes) copied to ones padded with zeros.
@@ -623,7 +624,7 @@ __global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void pro
 }
 
 // ---- few rows ----------------------------------------------------------------------------------------
-// Bound by reading w once. A workgroup takes a few outputs (rows of w) and up to 64 rows of x; its W waves take the 128-byte
+// Bound by reading w once (for every 64 rows of x). A workgroup takes a few outputs (rows of w) and up to 64 rows of x; its W waves take the 128-byte
 // steps along c in turn, each on its own, and their sums are added in the order of the waves at the end. What the loads
 // cost was found by measurement: a CU takes about 14 bytes a cycle in loads to registers, whatever their number in flight and
 // whether they ask for whole 128-byte lines, and 28 in direct-to-LDS loads. So:

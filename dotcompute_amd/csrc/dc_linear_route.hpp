@@ -174,9 +174,13 @@ inline LinearPair linear_plan_of_two(const LinearSize& a, const LinearSize& b, i
   return best;
 }
 
-// Few rows of x: kernels that read w once for up to 64 of them. Measured in bf16, us (few rows / tiles): 32×16384×2048 13.3 /
-// 13.8, 64×4096×4096 10.5 / 17.9, 64×6144×4096 17.1 / 18.3, 64×8192×4096 19.7 / 18.7; so up to kLinearFewRows always, and
-// beyond where every 64 rows and 16 outputs still find a CU of their own.
+// Few rows of x: kernels whose workgroups take 64 of them and 16 outputs, and read w once for every 64 rows. Measured in bf16, us (few rows /
+// tiles): 32×16384×2048 13.3 / 13.8, 64×4096×4096 10.5 / 17.9, 64×6144×4096 17.1 / 18.3, 64×8192×4096 19.7 / 18.7; so up to
+// kLinearFewRows always, and beyond where every 64 rows and 16 outputs still find a CU of their own, however many rows those are.
+// More of those, bf16 and e4m3 (few rows / tiles): 100×2048×2048 6.4 / 12.6, 4.5 / 6.6; 300×300×2048 6.6 / 11.8, 4.5 / 6.9; 512×512×1024
+// 4.5 / 6.4, 3.9 / 5.3; 512×512×8192 16.5 / 19.6, 10.5 / 14.8; 1024×256×4096 13.0 / 14.6, 8.1 / 14.0. It loses where outputs are fewer than a
+// tile's and sums long, as c is not split over workgroups here: 64×64×8192 11.9 / 9.7, 7.7 / 9.1; 300×64×8000 15.5 / 11.0, 11.0 /
+// 9.5; 4096×64×1024 7.7 / 6.2, 5.7 / 5.3; 4096×64×4096 21.0 / 14.6, 18.8 / 14.1.
 constexpr int64_t kLinearFewRows = 32;
 inline bool linear_few_rows(int64_t m, int64_t n, int64_t cus) {
   return m <= kLinearFewRows || (m + 63) / 64 * ((n + 15) / 16) <= cus;

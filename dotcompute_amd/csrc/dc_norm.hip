@@ -116,7 +116,9 @@ struct Row {
 };
 
 // A row a workgroup; or, where a wave holds a row, one for each of its four waves.
-// kNorm false: y = x itself (a conversion to 8 bits), no norm, no weight.
+// kNorm false: y = x itself (a conversion to 8 bits), no norm, no weight. Memory-bound too, 3 bytes an element of bf16 and 5 of float32; the row's
+// maximum is a barrier between its read and its write. us with the call (TB/s), bf16 and float32: 16384×4096 42.4 (4.75), 67.0 (5.0);
+// 2048×4096 7.8 (3.2), 9.4 (4.5); 8191×2050 16.5 (3.05), 23.1 (3.6); 8×4096 4.3, 4.4, of which the call is 3.7.
 template <typename T, typename Y, int C, bool kNorm>
 __global__ __launch_bounds__(C == 4 ? 1024 : 512) void rms_norm_kernel(NormArgs a, int waves) {
   constexpr int E = kElems<T>;

@@ -557,6 +557,11 @@ DC_HIP_API int32_t dc_hip_spmv_plan_destroy(dc_hip_spmv_plan* plan);
  * nor each other but where it is said below. Infinities and NaN do what float32 arithmetic makes of them, within their row.
  * Widths up to 2^25 (norms) and 2^23 (n, k, and m where dw is asked for; DC_ERR_UNSUPPORTED beyond), m below 2^30
  * (DC_ERR_INVALID_ARGUMENT beyond); sizes of zero are fine everywhere.
+ * Scratch of a call is the context's, kept for the next one and grown where that needs more, which waits for the stream and allocates.
+ * RMS norm's gradient: dweight's parts, cols floats for each of at most 8 workgroups a CU, 1 where rows are wide (32 GiB at 2^25
+ * columns and 256 rows or more). Linear layers: copies of operands whose rows do not lie at multiples of 16 bytes, and float32 parts of the
+ * results where sums are split; their gradients also dz, where it is not dy, and its transpose, 2 m n bytes each, and
+ * n floats for every 64 rows for dbias.
  * ------------------------------------------------------------------------------------------- */
 typedef enum dc_dtype {
   DC_DTYPE_F32 = 0,
