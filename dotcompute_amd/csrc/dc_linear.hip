@@ -922,7 +922,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs args) { pack_rows(ar
 // dz = dy act'(pre) over 64×64 pieces: dz itself (pitch dz_pitch, columns from n to there zero), its transpose (pitch
 // t_pitch, columns from m to there zero) through LDS, and the piece's column sums, unrounded. A thread holds two
 // neighbouring rows of 8 columns, so the transpose's LDS words are pairs of rows. Bound by memory: 8192×8192 with silu, dz, its
-// transpose and parts 98-103 us (537 MB, 5.2-5.5 TB/s); 2000×3000 with gelu 12.8, half of it the slope's arithmetic. (All four
+// transpose and parts 98-103 us (537 MB, 5.2-5.5 TB/s); 2000×3000 with gelu 13.6, half of it the slope's arithmetic. (All four
 // loads in flight at once, by addresses that need no branch: 13.2 for 12.2 without the writes, 2000×3000.)
 struct SlopeArgs {
   const bf16 *dy, *pre;
