@@ -161,6 +161,9 @@ int32_t launch_reduce_sum_f32(dc_hip_ctx* ctx, const float* input, int64_t n, do
 int32_t launch_reduce_partials_f64(dc_hip_ctx* ctx, const double* partials, int count, double* sum_out);
 // out[c] = parts[0][c] + ... + parts[count - 1][c] for float32 rows of `cols`, in a fixed order.
 int32_t launch_column_sums(dc_hip_ctx* ctx, const float* parts, float* out, int64_t count, int64_t cols);
+// The same of rows `pitch` floats apart; out2[c], where it is not NULL, is the sum of what lies `second` floats past out[c]'s.
+int32_t launch_column_sums_of(dc_hip_ctx* ctx, const float* parts, int64_t pitch, int64_t second, float* out, float* out2, int64_t count,
+                              int64_t cols);
 // Fills device memory with zero bytes using a kernel (capture-safe).
 int32_t zero_async(dc_hip_ctx* ctx, void* dst, size_t bytes);
 inline int32_t last_launch_status() { return (int32_t)hipGetLastError(); }

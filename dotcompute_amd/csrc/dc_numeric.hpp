@@ -155,7 +155,40 @@ __device__ inline uint32_t wave_max_u32(uint32_t v) {
   v = max(v, dpp_u32<0x143, 0xC>(v));
   return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
+// The sum over each 16 lanes, in all of them.
+__device__ inline float row16_sum_f32(float v) {
+  v += __builtin_bit_cast(float, dpp_u32<0xB1, 0xF>(__builtin_bit_cast(uint32_t, v)));
+  v += __builtin_bit_cast(float, dpp_u32<0x4E, 0xF>(__builtin_bit_cast(uint32_t, v)));
+  v += __builtin_bit_cast(float, dpp_u32<0x141, 0xF>(__builtin_bit_cast(uint32_t, v)));
+  v += __builtin_bit_cast(float, dpp_u32<0x140, 0xF>(__builtin_bit_cast(uint32_t, v)));
+  return v;
+}
 // |v| as an ordered integer: larger magnitudes compare larger, infinities above all finite ones, NaN above those.
 __device__ inline uint32_t magnitude(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
+
+
+// Blocks of 128 elements of a row in 8 bits share a scale that is a power of two, held as its exponent plus 127 in a byte (255: NaN): what
+// the matrix cores take beside the codes. Of values of at most `top` (a magnitude) it is the least that takes them to 448 = 1.75 2^8
+// or below, 2^-127 at the least; NaN where top is infinite or NaN.
+constexpr int kScaleBlock = 128;
+__device__ inline uint32_t block_scale(uint32_t top) {
+  const int e = (int)(top >> 23) - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return top >= 0x7f800000u ? 255u : (uint32_t)(e > 0 ? e : 0);
+}
+// What values are multiplied with to become codes: 2^(127 - scale), exact.
+__device__ inline float block_factor(uint32_t scale) {
+  return __builtin_bit_cast(float, scale == 255u ? 0x7fc00000u : (254u - scale) << 23);
+}
+// The largest of a block's magnitudes, in its lanes, of which each holds E neighbouring elements: 16 lanes, or 32.
+template <int E>
+__device__ inline uint32_t block_max_u32(uint32_t v) {
+  static_assert(E == 8 || E == 4, "16 or 32 lanes to a block");
+  v = max(v, dpp_u32<0xB1, 0xF>(v));
+  v = max(v, dpp_u32<0x4E, 0xF>(v));
+  v = max(v, dpp_u32<0x141, 0xF>(v));
+  v = max(v, dpp_u32<0x140, 0xF>(v));
+  if constexpr (E == 4) v = max(v, (uint32_t)__shfl_xor((int)v, 16));
+  return v;
+}
 
 }  // namespace dc

@@ -52,6 +52,7 @@ DC_LINQ_MAX_INSTR = 48
 DTYPE_F32, DTYPE_BF16, DTYPE_FP8 = range(3)
 ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 ADAMW_BLOCK = 256  # elements of an 8-bit state that share a scale
+SCALE_BLOCK = 128  # elements of a row in 8 bits that share one, where scales go by blocks
 
 # dc_linq_op
 NOP, LOAD, ADD, SUB, RSUB, MUL, DIV, RDIV, MIN, MAX, NEG, ABS, SQRT, STORE_S0, STORE_S1 = range(15)
@@ -277,6 +278,64 @@ class LinearGrad(_Arguments):
         return a
 
 
+def scale_blocks(cols: int) -> int:
+    """Rows of a matrix of block scales, [scale_blocks(cols), rows] bytes (uint8, e8m0), for rows of `cols` elements."""
+    return -(-int(cols) // SCALE_BLOCK)
+
+
+class LayerNorm(_Arguments):
+    """dc_layer_norm: h = x + residual, y = (h - mean(h)) * weight / sqrt(var(h) + eps) + bias."""
+    _fields_ = ([("rows", C.c_int64), ("cols", C.c_int64), ("dtype", C.c_int32), ("y_dtype", C.c_int32), ("eps", C.c_float),
+                 ("scale_block", C.c_int32)] + [(n, C.c_void_p) for n in ("x", "residual", "weight", "bias", "sum", "y", "scales")] +
+                [(n, C.c_int64) for n in ("x_stride", "residual_stride", "sum_stride", "y_stride", "scales_stride")])
+
+    @classmethod
+    def of(cls, x: "DeviceArray", weight: "DeviceArray", bias: "DeviceArray | None", y: "DeviceArray",
+           residual: "DeviceArray | None" = None, sum: "DeviceArray | None" = None, scales: "DeviceArray | None" = None,
+           eps: float = 1e-5, **strides) -> "LayerNorm":
+        """y in x's type, or uint8 (e4m3) with `scales`: float32 [rows], or uint8 [scale_blocks(cols), rows]. Row strides in elements by
+        name (x_stride=...), else dense."""
+        rows, cols = _matrix(x, "x")
+        same = (dtype_of(x),)
+        _expect(weight, "weight", same, (cols,))
+        _expect(bias, "bias", same, (cols,))
+        _expect(y, "y", same + (DTYPE_FP8,), (rows, cols))
+        _expect(residual, "residual", same, (rows, cols))
+        _expect(sum, "sum", same, (rows, cols))
+        blocks = scales is not None and len(scales.shape) == 2
+        if blocks:
+            _expect(scales, "scales", (DTYPE_FP8,), (scale_blocks(cols), rows))
+        else:
+            _expect(scales, "scales", (DTYPE_F32,), (rows,))
+        a = cls(rows=rows, cols=cols, dtype=dtype_of(x), y_dtype=dtype_of(y), eps=eps, scale_block=SCALE_BLOCK if blocks else 0)
+        a._put(strides, x=x, residual=residual, weight=weight, bias=bias, sum=sum, y=y, scales=scales)
+        return a
+
+
+class LayerNormGrad(_Arguments):
+    """dc_layer_norm_grad: the gradients of LayerNorm's y by h, the weight and the bias."""
+    _fields_ = ([("rows", C.c_int64), ("cols", C.c_int64), ("dtype", C.c_int32), ("eps", C.c_float)] +
+                [(n, C.c_void_p) for n in ("dy", "h", "weight", "dh", "dx", "dweight", "dbias")] +
+                [(n, C.c_int64) for n in ("dy_stride", "h_stride", "dh_stride", "dx_stride")])
+
+    @classmethod
+    def of(cls, dy: "DeviceArray", h: "DeviceArray", weight: "DeviceArray", dx: "DeviceArray | None" = None,
+           dweight: "DeviceArray | None" = None, dbias: "DeviceArray | None" = None, dh: "DeviceArray | None" = None, eps: float = 1e-5,
+           **strides) -> "LayerNormGrad":
+        """dx in h's type (plus dh, where given), dweight and dbias in float32."""
+        rows, cols = _matrix(h, "h")
+        same = (dtype_of(h),)
+        _expect(weight, "weight", same, (cols,))
+        _expect(dy, "dy", same, (rows, cols))
+        _expect(dh, "dh", same, (rows, cols))
+        _expect(dx, "dx", same, (rows, cols))
+        _expect(dweight, "dweight", (DTYPE_F32,), (cols,))
+        _expect(dbias, "dbias", (DTYPE_F32,), (cols,))
+        a = cls(rows=rows, cols=cols, dtype=dtype_of(h), eps=eps)
+        a._put(strides, dy=dy, h=h, weight=weight, dh=dh, dx=dx, dweight=dweight, dbias=dbias)
+        return a
+
+
 class AdamW(C.Structure):
     """dc_adamw: the numbers of one step (`step` counts from 1). The states' type comes with the tensors."""
     _fields_ = ([(n, C.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay", "grad_scale")] +
@@ -430,6 +489,9 @@ SIGNATURES: dict[str, list] = {
     "dc_hip_quantize_fp8": [_P, _P, _i32, _i64, _P, _i64, _P, _i64, _i64],
     "dc_hip_linear": [_P, C.POINTER(Linear)],
     "dc_hip_linear_backward": [_P, C.POINTER(LinearGrad)],
+    "dc_hip_layer_norm": [_P, C.POINTER(LayerNorm)],
+    "dc_hip_layer_norm_backward": [_P, C.POINTER(LayerNormGrad)],
+    "dc_hip_quantize_fp8_blocks": [_P, _P, _i32, _i64, _P, _i64, _P, _i64, _i64, _i64],
     "dc_hip_adamw_step": [_P, C.POINTER(AdamW), C.POINTER(AdamWTensor), _i32],
 }
 _RESTYPES = {"dc_hip_error_string": C.c_char_p, "dc_hip_default_module_path": C.c_char_p}
@@ -733,6 +795,28 @@ class Context:
 
     def linear_backward(self, args: LinearGrad) -> None:
         check(load().dc_hip_linear_backward(self.handle, args), "dc_hip_linear_backward")
+
+    # ---- and of a gated one ----
+    def layer_norm(self, args: LayerNorm) -> None:
+        check(load().dc_hip_layer_norm(self.handle, args), "dc_hip_layer_norm")
+
+    def layer_norm_backward(self, args: LayerNormGrad) -> None:
+        check(load().dc_hip_layer_norm_backward(self.handle, args), "dc_hip_layer_norm_backward")
+
+    def quantize_fp8_blocks(self, x: DeviceArray, q: DeviceArray, scales: DeviceArray, x_stride: int | None = None,
+                            q_stride: int | None = None, scales_stride: int | None = None) -> None:
+        """Rows of x (float32 or bf16) in e4m3 (uint8 bytes) with block scales, uint8 [scale_blocks(cols), rows]. Row strides in
+        elements, else dense."""
+        rows, cols = _matrix(x, "x")
+        _expect(q, "q", (DTYPE_FP8,), (rows, cols))
+        _expect(scales, "scales", (DTYPE_FP8,), (scale_blocks(cols), rows))
+        for name, a, stride in (("x", x, x_stride), ("q", q, q_stride), ("scales", scales, scales_stride)):
+            if stride is not None:
+                _check_reach(a, name, stride)
+        x_stride, q_stride = (cols if s is None else s for s in (x_stride, q_stride))
+        check(load().dc_hip_quantize_fp8_blocks(self.handle, x.ptr, dtype_of(x), x_stride, q.ptr, q_stride, scales.ptr,
+                                                rows if scales_stride is None else scales_stride, rows, cols),
+              "dc_hip_quantize_fp8_blocks")
 
     def adamw_step(self, args: AdamW, tensors: AdamWTensors) -> None:
         args = AdamW.from_buffer_copy(args)  # (the caller's may be another step's at the same time)

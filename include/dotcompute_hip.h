@@ -691,6 +691,61 @@ typedef struct dc_adamw_tensor {
 DC_HIP_API int32_t dc_hip_adamw_step(dc_hip_ctx* ctx, const dc_adamw* args, const dc_adamw_tensor* tensors,
                                      int32_t count);
 
+/* ---------------------------------------------------------------------------------------------
+ * Operators of a gated feed-forward block, beside those above and under their conventions: layer norm, both projections with their gate,
+ * and 8-bit values with a scale for each DC_SCALE_BLOCK elements of a row. They have no counterpart in the reference either.
+ *
+ * Block scales: [ceil(cols / DC_SCALE_BLOCK)][rows] bytes, a row of them for each block of columns, scales_stride bytes apart (at least
+ * `rows`; of a single row of them: anything). A byte s stands for 2^(s - 127), 255 for NaN (e8m0, what the matrix cores take beside
+ * e4m3 values): the least such power of two that takes the block's largest value to 448 or below, and at least 2^-127. The last block of a row may be
+ * short. An infinity or a NaN makes its block NaN.
+ * Scratch: layer norm's gradient takes that of an RMS norm's for each of dweight and dbias; gated layers that of linear layers with 2 n outputs.
+ * ------------------------------------------------------------------------------------------- */
+#define DC_SCALE_BLOCK 128
+
+/* h = x + residual; y = (h - mean(h)) * weight / sqrt(var(h) + eps) + bias, row by row, var the mean of (h - mean(h))^2.
+ * dtype: x, residual, weight, bias, sum. y has y_dtype: dtype, or FP8, with a scale per row (scale_block 0: `scales` is float[rows]) or
+ * block scales (scale_block DC_SCALE_BLOCK). `residual` may be NULL (h = x), as may `bias`; `sum` receives h, rounded to dtype (y is formed from the
+ * unrounded one), or is NULL. `sum` may be x or residual, and `y` of type dtype x, residual, at the same stride. */
+typedef struct dc_layer_norm {
+  int64_t rows, cols;
+  int32_t dtype, y_dtype; /* F32 or BF16; the same or FP8 */
+  float eps;
+  int32_t scale_block; /* 0 or DC_SCALE_BLOCK; 0 where y_dtype is not FP8 */
+  const void* x;
+  const void* residual;
+  const void* weight; /* [cols] */
+  const void* bias;   /* [cols] */
+  void* sum;
+  void* y;
+  void* scales; /* FP8 only, else NULL */
+  int64_t x_stride, residual_stride, sum_stride, y_stride, scales_stride;
+} dc_layer_norm;
+DC_HIP_API int32_t dc_hip_layer_norm(dc_hip_ctx* ctx, const dc_layer_norm* args);
+
+/* Gradients of that y by h, weight and bias: with s = 1 / sqrt(var(h) + eps), u = (h - mean(h)) s and g = dy * weight,
+ * dx = s (g - mean(g) - u mean(g u)) + dh, the gradient of x and of residual alike; dweight = the sum over rows of dy u, dbias of dy.
+ * dtype: dy, h, weight, dh, dx; dweight and dbias are float32. `dh` (the gradient that reaches h by its other uses) may be NULL, as may dx,
+ * dweight or dbias; `dx` may be dh or dy at the same stride. */
+typedef struct dc_layer_norm_grad {
+  int64_t rows, cols;
+  int32_t dtype; /* F32 or BF16 */
+  float eps;
+  const void* dy;
+  const void* h;
+  const void* weight; /* [cols] */
+  const void* dh;
+  void* dx;
+  float* dweight; /* [cols] */
+  float* dbias;   /* [cols] */
+  int64_t dy_stride, h_stride, dh_stride, dx_stride;
+} dc_layer_norm_grad;
+DC_HIP_API int32_t dc_hip_layer_norm_backward(dc_hip_ctx* ctx, const dc_layer_norm_grad* args);
+
+/* Rows in 8 bits with block scales: q = e4m3(x / scale), the division exact. dtype: F32 or BF16. */
+DC_HIP_API int32_t dc_hip_quantize_fp8_blocks(dc_hip_ctx* ctx, const void* x, int32_t dtype, int64_t x_stride, uint8_t* q,
+                                              int64_t q_stride, uint8_t* scales, int64_t scales_stride, int64_t rows, int64_t cols);
+
 #ifdef __cplusplus
 }
 #endif
