@@ -38,7 +38,8 @@ HIP_FLAGS = [
     "-Wall", "-Wno-unused-function",
 ]
 HIP_SOURCES = ["dc_runtime.hip", "dc_streaming.hip", "dc_linq.hip", "dc_linq_jit.hip", "dc_gemm.hip", "dc_spmv.hip",
-               "dc_norm.hip", "dc_layer_norm.hip", "dc_linear.hip", "dc_adamw.hip"]
+               "dc_norm.hip", "dc_layer_norm.hip", "dc_linear.hip", "dc_linear_blocks.hip", "dc_gated.hip", "dc_gated_grad.hip",
+               "dc_adamw.hip"]
 # Headers the run-time LINQ compiler (dc_linq_jit.hip) hands to hipRTC, by the names the sources
 # include them under there.
 JIT_HEADERS = [("dotcompute_hip.h", os.path.join(ROOT, "include", "dotcompute_hip.h")),

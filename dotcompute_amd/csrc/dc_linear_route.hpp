@@ -12,6 +12,7 @@ namespace dc {
 constexpr int32_t kLinearRange = INT32_MAX;
 constexpr int64_t kLinearPitch = (int64_t(1) << 25) - 16;
 constexpr int64_t kLinearWidth = int64_t(1) << 23;
+constexpr int64_t kGatedWidth = kLinearWidth / 2;  // outputs of a gated layer, whose gradients run along those of both projections
 static_assert(64 * kLinearPitch < kLinearRange && 2 * kLinearWidth <= kLinearPitch);
 
 // Tiles, square, and groups of waves that take the steps along c in turn.

@@ -336,6 +336,87 @@ class LayerNormGrad(_Arguments):
         return a
 
 
+class LinearBlocks(_Arguments):
+    """dc_linear_blocks: z = x w^T + bias, y = act(z) + residual, of e4m3 values with block scales."""
+    _fields_ = ([("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64), ("y_dtype", C.c_int32), ("activation", C.c_int32)] +
+                [(n, C.c_void_p) for n in ("x", "w", "x_scales", "w_scales", "bias", "residual", "y")] +
+                [(n, C.c_int64) for n in ("x_stride", "w_stride", "x_scales_stride", "w_scales_stride", "residual_stride", "y_stride")])
+
+    @classmethod
+    def of(cls, x: "DeviceArray", w: "DeviceArray", x_scales: "DeviceArray", w_scales: "DeviceArray", y: "DeviceArray",
+           bias: "DeviceArray | None" = None, residual: "DeviceArray | None" = None, activation: str = "none", **strides) -> "LinearBlocks":
+        """x [m, k] and w [n, k] in e4m3 (uint8) with x_scales [scale_blocks(k), m] and w_scales [scale_blocks(k), n] (uint8); bias [n] and
+        residual [m, n] in bf16; y [m, n] in bf16 or float32."""
+        (m, k), (n, _) = _matrix(x, "x"), _matrix(w, "w")
+        _expect(x, "x", (DTYPE_FP8,), (m, k))
+        _expect(w, "w", (DTYPE_FP8,), (n, k))
+        _expect(x_scales, "x_scales", (DTYPE_FP8,), (scale_blocks(k), m))
+        _expect(w_scales, "w_scales", (DTYPE_FP8,), (scale_blocks(k), n))
+        _expect(bias, "bias", (DTYPE_BF16,), (n,))
+        _expect(residual, "residual", (DTYPE_BF16,), (m, n))
+        _expect(y, "y", (DTYPE_BF16, DTYPE_F32), (m, n))
+        a = cls(m=m, n=n, k=k, y_dtype=dtype_of(y), activation=ACTIVATIONS[activation])
+        a._put(strides, x=x, w=w, x_scales=x_scales, w_scales=w_scales, bias=bias, residual=residual, y=y)
+        return a
+
+
+class GatedLinear(_Arguments):
+    """dc_gated_linear: g = x w_gate^T + bias_gate, u = x w_up^T + bias_up, y = act(g) u."""
+    _fields_ = ([("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64), ("dtype", C.c_int32), ("y_dtype", C.c_int32),
+                 ("activation", C.c_int32), ("scale_block", C.c_int32)] +
+                [(n, C.c_void_p) for n in ("x", "w_gate", "w_up", "x_scales", "gate_scales", "up_scales", "bias_gate", "bias_up", "pre_gate",
+                                           "pre_up", "y")] +
+                [(n + "_stride", C.c_int64) for n in ("x", "w_gate", "w_up", "x_scales", "gate_scales", "up_scales", "pre_gate", "pre_up", "y")])
+
+    @classmethod
+    def of(cls, x: "DeviceArray", w_gate: "DeviceArray", w_up: "DeviceArray", y: "DeviceArray", bias_gate: "DeviceArray | None" = None,
+           bias_up: "DeviceArray | None" = None, pre_gate: "DeviceArray | None" = None, pre_up: "DeviceArray | None" = None,
+           x_scales: "DeviceArray | None" = None, gate_scales: "DeviceArray | None" = None, up_scales: "DeviceArray | None" = None,
+           activation: str = "silu", **strides) -> "GatedLinear":
+        """x [m, k], w_gate and w_up [n, k] in bf16, or in e4m3 with float32 scales [m], [n], [n] or block scales (uint8, [scale_blocks(k), m] and
+        so on); biases [n], pre_gate and pre_up (receive g and u) [m, n] in bf16; y [m, n] in bf16 or float32."""
+        (m, k), (n, _) = _matrix(x, "x"), _matrix(w_gate, "w_gate")
+        _expect(x, "x", (DTYPE_BF16, DTYPE_FP8), (m, k))
+        scales = dict(x_scales=x_scales, gate_scales=gate_scales, up_scales=up_scales)
+        blocks = any(s is not None and len(s.shape) == 2 for s in scales.values())
+        for (name, s), rows in zip(scales.items(), (m, n, n)):
+            _expect(s, name, (DTYPE_FP8,) if blocks else (DTYPE_F32,), (scale_blocks(k), rows) if blocks else (rows,))
+        for name, a, types, shape in (("w_gate", w_gate, (dtype_of(x),), (n, k)), ("w_up", w_up, (dtype_of(x),), (n, k)),
+                                      ("bias_gate", bias_gate, (DTYPE_BF16,), (n,)), ("bias_up", bias_up, (DTYPE_BF16,), (n,)),
+                                      ("pre_gate", pre_gate, (DTYPE_BF16,), (m, n)), ("pre_up", pre_up, (DTYPE_BF16,), (m, n)),
+                                      ("y", y, (DTYPE_BF16, DTYPE_F32), (m, n))):
+            _expect(a, name, types, shape)
+        a = cls(m=m, n=n, k=k, dtype=dtype_of(x), y_dtype=dtype_of(y), activation=ACTIVATIONS[activation],
+                scale_block=SCALE_BLOCK if blocks else 0)
+        a._put(strides, x=x, w_gate=w_gate, w_up=w_up, bias_gate=bias_gate, bias_up=bias_up, pre_gate=pre_gate, pre_up=pre_up, y=y, **scales)
+        return a
+
+
+class GatedLinearGrad(_Arguments):
+    """dc_gated_linear_grad: the gradients of GatedLinear's y by x, the weights and the biases."""
+    _fields_ = ([("m", C.c_int64), ("n", C.c_int64), ("k", C.c_int64), ("activation", C.c_int32), ("reserved", C.c_int32)] +
+                [(n, C.c_void_p) for n in ("dy", "x", "w_gate", "w_up", "pre_gate", "pre_up", "dx", "dw_gate", "dw_up", "dbias_gate", "dbias_up")] +
+                [(n + "_stride", C.c_int64) for n in ("dy", "x", "w_gate", "w_up", "pre_gate", "pre_up", "dx", "dw_gate", "dw_up")])
+
+    @classmethod
+    def of(cls, dy: "DeviceArray", x: "DeviceArray", w_gate: "DeviceArray", w_up: "DeviceArray", pre_gate: "DeviceArray",
+           pre_up: "DeviceArray", dx: "DeviceArray | None" = None, dw_gate: "DeviceArray | None" = None, dw_up: "DeviceArray | None" = None,
+           dbias_gate: "DeviceArray | None" = None, dbias_up: "DeviceArray | None" = None, activation: str = "silu",
+           **strides) -> "GatedLinearGrad":
+        """All bf16 but the biases' gradients (float32); pre_gate and pre_up: what GatedLinear wrote there."""
+        (m, k), (n, _) = _matrix(x, "x"), _matrix(w_gate, "w_gate")
+        for name, a, shape in (("dy", dy, (m, n)), ("x", x, (m, k)), ("w_gate", w_gate, (n, k)), ("w_up", w_up, (n, k)),
+                               ("pre_gate", pre_gate, (m, n)), ("pre_up", pre_up, (m, n)), ("dx", dx, (m, k)), ("dw_gate", dw_gate, (n, k)),
+                               ("dw_up", dw_up, (n, k))):
+            _expect(a, name, (DTYPE_BF16,), shape)
+        for name, a in (("dbias_gate", dbias_gate), ("dbias_up", dbias_up)):
+            _expect(a, name, (DTYPE_F32,), (n,))
+        a = cls(m=m, n=n, k=k, activation=ACTIVATIONS[activation])
+        a._put(strides, dy=dy, x=x, w_gate=w_gate, w_up=w_up, pre_gate=pre_gate, pre_up=pre_up, dx=dx, dw_gate=dw_gate, dw_up=dw_up,
+               dbias_gate=dbias_gate, dbias_up=dbias_up)
+        return a
+
+
 class AdamW(C.Structure):
     """dc_adamw: the numbers of one step (`step` counts from 1). The states' type comes with the tensors."""
     _fields_ = ([(n, C.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay", "grad_scale")] +
@@ -491,6 +572,9 @@ SIGNATURES: dict[str, list] = {
     "dc_hip_linear_backward": [_P, C.POINTER(LinearGrad)],
     "dc_hip_layer_norm": [_P, C.POINTER(LayerNorm)],
     "dc_hip_layer_norm_backward": [_P, C.POINTER(LayerNormGrad)],
+    "dc_hip_linear_blocks": [_P, C.POINTER(LinearBlocks)],
+    "dc_hip_gated_linear": [_P, C.POINTER(GatedLinear)],
+    "dc_hip_gated_linear_backward": [_P, C.POINTER(GatedLinearGrad)],
     "dc_hip_quantize_fp8_blocks": [_P, _P, _i32, _i64, _P, _i64, _P, _i64, _i64, _i64],
     "dc_hip_adamw_step": [_P, C.POINTER(AdamW), C.POINTER(AdamWTensor), _i32],
 }
@@ -802,6 +886,15 @@ class Context:
 
     def layer_norm_backward(self, args: LayerNormGrad) -> None:
         check(load().dc_hip_layer_norm_backward(self.handle, args), "dc_hip_layer_norm_backward")
+
+    def gated_linear(self, args: GatedLinear) -> None:
+        check(load().dc_hip_gated_linear(self.handle, args), "dc_hip_gated_linear")
+
+    def gated_linear_backward(self, args: GatedLinearGrad) -> None:
+        check(load().dc_hip_gated_linear_backward(self.handle, args), "dc_hip_gated_linear_backward")
+
+    def linear_blocks(self, args: LinearBlocks) -> None:
+        check(load().dc_hip_linear_blocks(self.handle, args), "dc_hip_linear_blocks")
 
     def quantize_fp8_blocks(self, x: DeviceArray, q: DeviceArray, scales: DeviceArray, x_stride: int | None = None,
                             q_stride: int | None = None, scales_stride: int | None = None) -> None:

@@ -746,6 +746,69 @@ DC_HIP_API int32_t dc_hip_layer_norm_backward(dc_hip_ctx* ctx, const dc_layer_no
 DC_HIP_API int32_t dc_hip_quantize_fp8_blocks(dc_hip_ctx* ctx, const void* x, int32_t dtype, int64_t x_stride, uint8_t* q,
                                               int64_t q_stride, uint8_t* scales, int64_t scales_stride, int64_t rows, int64_t cols);
 
+/* y = act(z) + residual with z = x w^T + bias, as dc_hip_linear's, of e4m3 values with block scales for both operands: x is [m][k] with x_scales
+ * [ceil(k / 128)][m], w [n][k] (a row per output) with w_scales [ceil(k / 128)][n]. Products as dc_hip_linear's in 8 bits. */
+typedef struct dc_linear_blocks {
+  int64_t m, n, k;
+  int32_t y_dtype, activation;
+  const uint8_t* x;
+  const uint8_t* w;
+  const uint8_t* x_scales;
+  const uint8_t* w_scales;
+  const uint16_t* bias;
+  const uint16_t* residual;
+  void* y;
+  int64_t x_stride, w_stride, x_scales_stride, w_scales_stride, residual_stride, y_stride;
+} dc_linear_blocks;
+DC_HIP_API int32_t dc_hip_linear_blocks(dc_hip_ctx* ctx, const dc_linear_blocks* args);
+
+/* g = x w_gate^T + bias_gate, u = x w_up^T + bias_up; y = act(g) u: x is [m][k], the weights [n][k] (a row per output), y [m][n].
+ * dtype: x and the weights, BF16 (the scales are NULL), or FP8 with a scale per row (scale_block 0: float x_scales[m], gate_scales[n], up_scales[n])
+ * or block scales (scale_block DC_SCALE_BLOCK; they may be NULL where k is 0). The biases are BF16 and may be NULL; `pre_gate` and `pre_up` receive g
+ * and u in BF16 for the backward pass, or are NULL; y has y_dtype, BF16 or F32, and is formed from the unrounded g and u. Sums and products as dc_hip_linear's.
+ * n up to 2^22 (DC_ERR_UNSUPPORTED beyond). */
+typedef struct dc_gated_linear {
+  int64_t m, n, k;
+  int32_t dtype, y_dtype, activation;
+  int32_t scale_block; /* 0 or DC_SCALE_BLOCK; 0 where dtype is not FP8 */
+  const void* x;
+  const void* w_gate;
+  const void* w_up;
+  const void* x_scales;
+  const void* gate_scales;
+  const void* up_scales;
+  const uint16_t* bias_gate;
+  const uint16_t* bias_up;
+  uint16_t* pre_gate;
+  uint16_t* pre_up;
+  void* y;
+  int64_t x_stride, w_gate_stride, w_up_stride, x_scales_stride, gate_scales_stride, up_scales_stride, pre_gate_stride, pre_up_stride,
+      y_stride;
+} dc_gated_linear;
+DC_HIP_API int32_t dc_hip_gated_linear(dc_hip_ctx* ctx, const dc_gated_linear* args);
+
+/* Gradients of that y, all BF16 but the biases': dg = dy u act'(g) and du = dy act(g), rounded to bf16 for the matrix cores; dx = dg w_gate + du w_up,
+ * dw_gate = dg^T x, dw_up = du^T x, dbias_gate and dbias_up = the sums over rows of dg and du (unrounded). Any result may be NULL, as may
+ * operands that only it needs. */
+typedef struct dc_gated_linear_grad {
+  int64_t m, n, k;
+  int32_t activation;
+  int32_t reserved; /* 0 */
+  const uint16_t* dy;
+  const uint16_t* x;
+  const uint16_t* w_gate;
+  const uint16_t* w_up;
+  const uint16_t* pre_gate;
+  const uint16_t* pre_up;
+  uint16_t* dx;
+  uint16_t* dw_gate;
+  uint16_t* dw_up;
+  float* dbias_gate;
+  float* dbias_up;
+  int64_t dy_stride, x_stride, w_gate_stride, w_up_stride, pre_gate_stride, pre_up_stride, dx_stride, dw_gate_stride, dw_up_stride;
+} dc_gated_linear_grad;
+DC_HIP_API int32_t dc_hip_gated_linear_backward(dc_hip_ctx* ctx, const dc_gated_linear_grad* args);
+
 #ifdef __cplusplus
 }
 #endif
