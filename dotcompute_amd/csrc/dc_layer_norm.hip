@@ -8,10 +8,11 @@
 // and db in registers; a second kernel adds the parts in a fixed order (no atomics: the same bits from call to call).
 //
 // Statistics. The difference of mean(h^2) and mean(h)^2 loses the variance's digits where the mean is large, and a second sum over a row that
-// several waves share would be a second barrier. So each wave takes the mean of its own part, m, and over that the sums of d = h - m and
-// d^2, in registers; the waves' triples meet in LDS once, and every wave joins them: the row's mean is M + e, with M the rounded mean of the m
-// and e what is left (of the d too, which carry the rounding of m), and sum((h - M - e)^2) = the sum over waves of
-// sum(d^2) + 2 c sum(d) + n c^2, c = m - M - e. Elements are taken as (h - M) - e: exact next to the mean.
+// several waves share would be a second barrier. So each wave takes a value k near its own part's mean, the mean of the first 32 elements (of 256 or
+// 512, or up to four times as many), and the sums of d = h - k and d^2, in registers; the waves' triples meet in LDS once, and every wave joins them: M is
+// the rounded mean, e what is left, and sum((h - M)^2) = the sum over waves of sum(d^2) + 2 c sum(d) + n c^2, c = k - M. Elements
+// are taken as (h - M) - e, exact next to the mean. (However a wave's values lie, (k - mean)^2 is at most n / 32 times their variance, so
+// that at worst 4 to 6 bits of its 24 are lost there, where one value stands out by itself among the first 32; none for others.)
 #include <algorithm>
 
 #include "dc_internal.hpp"
@@ -47,32 +48,42 @@ __device__ inline bool whole_chunk(const Row<T, C>& R, int i) {
   return (int64_t)((i * R.waves + R.wave) * 64 + 64) * kElems<T> <= R.cols;
 }
 
-// A wave's mean of n elements, and the sums of what is left over it and of that squared (elements past the row's end are zeros in h).
+// A value near the mean of a wave's elements, and the sums of what is left over it and of that squared (elements past the row's end are zeros in h).
 struct Moments {
-  float mean, left, squares;
+  float near, left, squares;
 };
+// 1 / the number of elements that `near` is the mean of.
+template <int E>
+__device__ inline float near_weight(int64_t cols, int wave) {
+  const int64_t left = cols - (int64_t)wave * 64 * E;
+  return 1.0f / (float)(left < 4 * E ? left : 4 * E);
+}
 template <typename T, int C>
-__device__ inline Moments wave_moments(const Row<T, C>& R, const float (&h)[C][kElems<T>], float n) {
+__device__ inline float value_near(const float (&h)[C][kElems<T>], float weight) {
   constexpr int E = kElems<T>;
-  float sum = 0.0f;
+  float v = 0.0f;
 #pragma unroll
-  for (int i = 0; i < C; ++i)
-#pragma unroll
-    for (int e = 0; e < E; ++e) sum += h[i][e];
-  Moments m{wave_sum_f32(sum) / n, 0.0f, 0.0f};
+  for (int e = 0; e < E; e += 4) v += (h[0][e] + h[0][e + 1]) + (h[0][e + 2] + h[0][e + 3]);
+  v += __builtin_bit_cast(float, dpp_u32<0xB1, 0xF>(__builtin_bit_cast(uint32_t, v)));
+  v += __builtin_bit_cast(float, dpp_u32<0x4E, 0xF>(__builtin_bit_cast(uint32_t, v)));
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v))) * weight;
+}
+// The lane's part of the sums.
+template <typename T, int C>
+__device__ inline Moments lane_moments(const Row<T, C>& R, const float (&h)[C][kElems<T>], float near) {
+  constexpr int E = kElems<T>;
+  Moments m{near, 0.0f, 0.0f};
 #pragma unroll
   for (int i = 0; i < C; ++i) {
     const bool whole = whole_chunk(R, i);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      float d = h[i][e] - m.mean;
+      float d = h[i][e] - near;
       if (!whole) d = R.at(i) + e < R.cols ? d : 0.0f;
       m.left += d;
       m.squares += d * d;
     }
   }
-  m.left = wave_sum_f32(m.left);
-  m.squares = wave_sum_f32(m.squares);
   return m;
 }
 
@@ -80,29 +91,28 @@ __device__ inline Moments wave_moments(const Row<T, C>& R, const float (&h)[C][k
 struct RowStats {
   float mean, rest, s;
 };
-// The waves' moments, one in each of 16 lanes (`n`: of how many elements, 0 where there is no wave), joined; `c`: what the lane's
-// wave's mean is away from the row's.
-__device__ inline RowStats join_moments(const Moments& m, float n, float cols, float eps, float* c) {
+// The waves' moments, one in each of 16 lanes (`n`: of how many elements, 0 where there is no wave), joined; `off`: what the lane's wave's value
+// is away from the row's mean. `per`: 1 / cols.
+__device__ inline RowStats join_moments(const Moments& m, float n, float per, float eps, float* off) {
   RowStats r;
-  r.mean = row16_sum_f32(n * m.mean) / cols;
-  const float off = m.mean - r.mean;
-  r.rest = row16_sum_f32(__builtin_fmaf(n, off, m.left)) / cols;
-  *c = off - r.rest;
-  const float v = row16_sum_f32(m.squares + *c * __builtin_fmaf(n, *c, 2.0f * m.left));
-  r.s = 1.0f / sqrtf(v / cols + eps);
+  r.mean = row16_sum_f32(__builtin_fmaf(n, m.near, m.left)) * per;
+  *off = m.near - r.mean;
+  const float rest = row16_sum_f32(__builtin_fmaf(n, *off, m.left));
+  const float squares = row16_sum_f32(m.squares + *off * __builtin_fmaf(n, *off, 2.0f * m.left));
+  r.rest = rest * per;
+  r.s = 1.0f / sqrtf((squares - rest * r.rest) * per + eps);
+  return r;
+}
+// Of a row that one wave holds.
+__device__ inline RowStats own_stats(const Moments& m, float per, float eps) {
+  RowStats r;
+  r.mean = m.near;
+  r.rest = m.left * per;
+  r.s = 1.0f / sqrtf((m.squares - m.left * r.rest) * per + eps);
   return r;
 }
 
 typedef float f32x4_lds __attribute__((ext_vector_type(4)));
-
-// Of a row that one wave holds.
-__device__ inline RowStats own_stats(const Moments& m, float cols, float eps) {
-  RowStats r;
-  r.mean = m.mean;
-  r.rest = m.left / cols;
-  r.s = 1.0f / sqrtf((m.squares - m.left * r.rest) / cols + eps);
-  return r;
-}
 
 // A row a workgroup; or, where a wave holds a row, one for each of its four waves. 8 bits: a scale a row, or (kBlocks) one for each 128.
 template <typename T, typename Y, int C, bool kBlocks>
@@ -115,7 +125,8 @@ __global__ __launch_bounds__(C == 4 ? 1024 : 512) void layer_norm_kernel(LayerNo
   const int64_t cols = a.cols;
   const Row<T, C> R{cols, waves, wave, lane};
   const int other = lane & (kWaves - 1);  // whose moments this lane joins
-  const float n = wave_count<E, C>(cols, waves, wave), n_other = other < waves ? wave_count<E, C>(cols, waves, other) : 0.0f;
+  const float weight = near_weight<E>(cols, wave), n_other = other < waves ? wave_count<E, C>(cols, waves, other) : 0.0f;
+  const float per_col = 1.0f / (float)a.cols;
   clear_words(scratch, 1, waves);
   const int per = waves == 1 ? 4 : 1;
   const int64_t step = (int64_t)gridDim.x * per;
@@ -146,20 +157,22 @@ __global__ __launch_bounds__(C == 4 ? 1024 : 512) void layer_norm_kernel(LayerNo
         const int64_t c = R.at(i);
         if (c < cols) store_some(sum + c, cols - c, h[i]);
       }
-    const Moments m = wave_moments(R, h, n);
+    Moments m = lane_moments(R, h, value_near<T, C>(h, weight));
+    m.left = wave_sum_f32(m.left);
+    m.squares = wave_sum_f32(m.squares);
     RowStats r;
     if (waves == 1) {
-      r = own_stats(m, (float)a.cols, a.eps);
+      r = own_stats(m, per_col, a.eps);
     } else {
-      if (lane == 0) words[wave] = f32x4_lds{m.mean, m.left, m.squares, 0.0f};
+      if (lane == 0) words[wave] = f32x4_lds{m.near, m.left, m.squares, 0.0f};
       __syncthreads();
       Moments q{0.0f, 0.0f, 0.0f};
       if (other < waves) {
         const f32x4_lds v = words[other];
         q = Moments{v.x, v.y, v.z};
       }
-      float c;
-      r = join_moments(q, n_other, (float)a.cols, a.eps, &c);
+      float off;
+      r = join_moments(q, n_other, per_col, a.eps, &off);
     }
     R.cut(wr);
     if (a.bias) R.cut(br);
@@ -329,7 +342,8 @@ __global__ __launch_bounds__(1024) void layer_norm_grad_kernel(LayerNormGradArgs
   const int64_t cols = a.cols;
   const Row<T, C> R{cols, waves, wave, lane};
   const int other = lane & (kWaves - 1);
-  const float n = wave_count<E, C>(cols, waves, wave), n_other = other < waves ? wave_count<E, C>(cols, waves, other) : 0.0f;
+  const float weight = near_weight<E>(cols, wave), n_other = other < waves ? wave_count<E, C>(cols, waves, other) : 0.0f;
+  const float per_col = 1.0f / (float)a.cols;
   float dw[C][E], db[C][E];
 #pragma unroll
   for (int i = 0; i < C; ++i)
@@ -359,7 +373,7 @@ __global__ __launch_bounds__(1024) void layer_norm_grad_kernel(LayerNormGradArgs
     }
     if constexpr (kAhead)
       if (row + gridDim.x < a.rows) load(row + gridDim.x);
-    const Moments m = wave_moments(R, h, n);
+    Moments m = lane_moments(R, h, value_near<T, C>(h, weight));
     float g_sum = 0.0f, gd_sum = 0.0f;  // of g and of g d (dy is zero past the end)
 #pragma unroll
     for (int i = 0; i < C; ++i) {
@@ -369,34 +383,36 @@ __global__ __launch_bounds__(1024) void layer_norm_grad_kernel(LayerNormGradArgs
       for (int e = 0; e < E; ++e) {
         const float g = dy[i][e] * w[e];
         g_sum += g;
-        gd_sum += g * (h[i][e] - m.mean);
+        gd_sum += g * (h[i][e] - m.near);
       }
     }
+    m.left = wave_sum_f32(m.left);
+    m.squares = wave_sum_f32(m.squares);
     g_sum = wave_sum_f32(g_sum);
     gd_sum = wave_sum_f32(gd_sum);
     RowStats r;
     if (waves == 1) {
-      r = own_stats(m, (float)a.cols, a.eps);
+      r = own_stats(m, per_col, a.eps);
       gd_sum -= r.rest * g_sum;
     } else {
       if (lane == 0) {
-        words[flip][wave] = f32x4_lds{m.mean, m.left, m.squares, g_sum};
+        words[flip][wave] = f32x4_lds{m.near, m.left, m.squares, g_sum};
         more[flip][wave] = gd_sum;
       }
       __syncthreads();  // (two sets in turn: a wave writes a set again only past the barrier of the row between)
       f32x4_lds v = {0.0f, 0.0f, 0.0f, 0.0f};
-      float gd = 0.0f, c;
+      float gd = 0.0f, off;
       if (other < waves) {
         v = words[flip][other];
         gd = more[flip][other];
       }
       flip ^= 1;
-      r = join_moments(Moments{v.x, v.y, v.z}, n_other, (float)a.cols, a.eps, &c);
+      r = join_moments(Moments{v.x, v.y, v.z}, n_other, per_col, a.eps, &off);
       g_sum = row16_sum_f32(v.w);
-      gd_sum = row16_sum_f32(__builtin_fmaf(c, v.w, gd));
+      gd_sum = row16_sum_f32(__builtin_fmaf(off, v.w, gd)) - r.rest * g_sum;
     }
-    const float g_mean = g_sum / (float)a.cols;
-    const float along = r.s * (r.s * (gd_sum / (float)a.cols));  // mean(g u) s (s^2 alone may be no float where eps is 0)
+    const float g_mean = g_sum * per_col;
+    const float along = r.s * (r.s * (gd_sum * per_col));  // mean(g u) s (s^2 alone may be no float where eps is 0)
     T* dx = a.dx ? static_cast<T*>(a.dx) + row * a.dx_stride : nullptr;
     if (dx && a.dh) R.cut(uv);
 #pragma unroll

@@ -614,20 +614,22 @@ __global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void pro
         }
     }
   };
+  auto mfmas_of = [&](int mt, const F* a, const F* b, auto BUF) __attribute__((always_inline)) {
+#pragma unroll
+    for (int nt = 0; nt < kNT; ++nt) {
+      if constexpr (kBlocks)
+        acc[mt][nt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[nt].v, a[mt].v, acc[mt][nt], 0, 0, 0, bscale[decltype(BUF)::value][nt], 0,
+                                                                     ascale[decltype(BUF)::value][mt]);
+      else if constexpr (kFp8)
+        acc[mt][nt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[nt].v, a[mt].v, acc[mt][nt], 0, 0, 0, 0x7f7f7f7f, 0,
+                                                                     0x7f7f7f7f);
+      else
+        acc[mt][nt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[nt].v, a[mt].v, acc[mt][nt], 0, 0, 0);
+    }
+  };
   auto mfmas = [&](const F* a, const F* b, auto BUF) __attribute__((always_inline)) {
 #pragma unroll
-    for (int mt = 0; mt < kMT; ++mt)
-#pragma unroll
-      for (int nt = 0; nt < kNT; ++nt) {
-        if constexpr (kBlocks)
-          acc[mt][nt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[nt].v, a[mt].v, acc[mt][nt], 0, 0, 0, bscale[decltype(BUF)::value][nt], 0,
-                                                                       ascale[decltype(BUF)::value][mt]);
-        else if constexpr (kFp8)
-          acc[mt][nt] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[nt].v, a[mt].v, acc[mt][nt], 0, 0, 0, 0x7f7f7f7f, 0,
-                                                                       0x7f7f7f7f);
-        else
-          acc[mt][nt] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(b[nt].v, a[mt].v, acc[mt][nt], 0, 0, 0);
-      }
+    for (int mt = 0; mt < kMT; ++mt) mfmas_of(mt, a, b, BUF);
   };
   // LDS reads between the products: as many as there are of each.
   constexpr int kReads = (kMT + (kRowsC ? 0 : kNT)) * (kFp8 ? 2 : 1), kProducts = kMT * kNT;
@@ -637,6 +639,20 @@ __global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void pro
       constexpr int kPer = (kReads + kProducts - 1) / kProducts;
       __builtin_amdgcn_sched_group_barrier(0x100, kPer, 0);
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    }
+  };
+
+  // Where registers are short (scales beside the largest tiles' sums and fragments): the next step's fragments of A are read one by one, each into the
+  // place of one whose products have gone out, so that a wave holds five of A's and not eight.
+  constexpr bool kRolled = kFp8 && (kBlocks || kPairs) && TM == 256;
+  auto rolled = [&](auto FROM, int from_step, F* a, F* b, F* a_next, F* b_next, auto BUF) __attribute__((always_inline)) {
+#pragma unroll
+    for (int mt = 0; mt < kMT; ++mt) {
+      mfmas_of(mt, a, b, BUF);
+      __builtin_amdgcn_sched_barrier(0);
+      if (mt == 0) read_b(FROM, from_step, b_next);
+      a_next[mt] = read_row(arow + (uint32_t)decltype(FROM)::value * TM * kTileBytes + mt * 32 * kTileBytes, from_step);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
 
@@ -661,6 +677,10 @@ __global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void pro
     _Pragma("unroll") for (int step = 0; step + 1 < kSteps; ++step) {                               \
       const int cur = step & 1;                                                                     \
       __builtin_amdgcn_sched_barrier(0);                                                            \
+      if constexpr (kRolled) {                                                                      \
+        rolled(kBuf##BUF, step + 1, fa[cur], fb[cur][0], fa[cur ^ 1], fb[cur ^ 1][0], kBuf##BUF);   \
+        continue;                                                                                   \
+      }                                                                                             \
       read_a(kBuf##BUF, step + 1, fa[cur ^ 1]);                                                     \
       if constexpr (!kRowsC) read_b(kBuf##BUF, step + 1, fb[cur ^ 1][0]);                           \
       mfmas(fa[cur], kRowsC ? fb[BUF][kRowsC ? step : 0] : fb[cur][0], kBuf##BUF);                  \
@@ -672,10 +692,14 @@ __global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void pro
     __builtin_amdgcn_sched_barrier(0);                                                              \
     if (kAlways || (KT) + 2 < kt_count) load_tile(kBuf##BUF, (KT) + 2);                             \
     __builtin_amdgcn_sched_barrier(0);                                                              \
-    read_a(kBuf##BUF##Other, 0, fa[0]);                                                             \
-    if constexpr (!kRowsC) read_b(kBuf##BUF##Other, 0, fb[0][0]);                                   \
-    mfmas(fa[1], kRowsC ? fb[BUF][kRowsC ? kSteps - 1 : 0] : fb[1][0], kBuf##BUF);                  \
-    interleave();                                                                                   \
+    if constexpr (kRolled) {                                                                        \
+      rolled(kBuf##BUF##Other, 0, fa[1], fb[1][0], fa[0], fb[0][0], kBuf##BUF);                     \
+    } else {                                                                                        \
+      read_a(kBuf##BUF##Other, 0, fa[0]);                                                           \
+      if constexpr (!kRowsC) read_b(kBuf##BUF##Other, 0, fb[0][0]);                                 \
+      mfmas(fa[1], kRowsC ? fb[BUF][kRowsC ? kSteps - 1 : 0] : fb[1][0], kBuf##BUF);                \
+      interleave();                                                                                 \
+    }                                                                                               \
     __builtin_amdgcn_sched_barrier(0);                                                              \
     load_scales(kBuf##BUF, (KT) + 2);                                                               \
   }
