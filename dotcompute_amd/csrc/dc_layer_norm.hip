@@ -10,10 +10,11 @@
 // Statistics. The difference of mean(h^2) and mean(h)^2 loses the variance's digits where the mean is large, and a second sum over a row that
 // several waves share would be a second barrier. So each wave takes a value k near its own part's mean, the mean of the first 32 elements (of 256 or
 // 512, or up to four times as many), and the sums of d = h - k and d^2, in registers; the waves' triples meet in LDS once, and every wave joins them: M is
-// the rounded mean, e what is left, and sum((h - M)^2) = the sum over waves of sum(d^2) + 2 c sum(d) + n c^2, c = k - M. Elements
-// are taken as (h - M) - e, exact next to the mean. (However a wave's values lie, (k - mean)^2 is at most n / 32 times their variance, so
+// the rounded mean, e what is left, and sum((h - M)^2) = the sum over waves of sum(d^2) + 2 c sum(d) + n c^2, c = k - M. An
+// element's u is d s + ((k - M) - e) s, whose terms are of u's size. (However a wave's values lie, (k - mean)^2 is at most n / 32 times their variance, so
 // that at worst 4 to 6 bits of its 24 are lost there, where one value stands out by itself among the first 32; none for others.)
 #include <algorithm>
+#include <type_traits>
 
 #include "dc_internal.hpp"
 #include "dc_norm_row.hpp"
@@ -31,7 +32,61 @@ struct LayerNormArgs {
   float eps;
 };
 
-// Elements of a row that a wave holds (Row's chunks).
+// The chunks c_i = ((i waves + wave) 64 + lane) E, i < C, of a row, as dc::Row has them; offsets in 32 bits (a row has at most 2^27 bytes), beside a
+// pointer that all lanes share, which saves registers and additions for each of a row's operands.
+template <typename T, int C>
+struct Span {
+  static constexpr int E = kElems<T>;
+  uint32_t cols, first, step, end;  // first: of the lane; step: from chunk to chunk; end: of the wave's first chunks (uniform)
+  __device__ inline Span(int64_t cols_, int waves, int wave, int lane)
+      : cols((uint32_t)cols_), first((uint32_t)((wave * 64 + lane) * E)), step((uint32_t)(waves * 64 * E)),
+        end((uint32_t)((wave + 1) * 64 * E)) {}
+  __device__ inline uint32_t at(int i) const { return first + i * step; }
+  template <typename P>
+  static __device__ inline P* past(P* p, uint32_t elements) {
+    typedef std::conditional_t<std::is_const_v<P>, const char, char> Byte;
+    return reinterpret_cast<P*>(reinterpret_cast<Byte*>(p) + elements * (uint32_t)sizeof(P));
+  }
+  __device__ inline void load(const T* p, u32x4 (&raw)[C]) const {
+    if (cols >= E) {
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        const uint32_t c = at(i);
+        raw[i] = load_raw(past(p, c < cols - E ? c : cols - E));
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        float v[E];
+        load_some(p, i == 0 && first == 0 ? (int64_t)cols : 0, v);
+        raw[i] = u32x4{0, 0, 0, 0};
+        if constexpr (E == 4) raw[i] = __builtin_bit_cast(u32x4, f32x4{v[0], v[1], v[2], v[3]});
+        else
+#pragma unroll
+          for (int e = 0; e < 4; ++e) raw[i][e] = pack_bf16(v[2 * e], v[2 * e + 1]);
+      }
+    }
+  }
+  // Whether all elements of the wave's chunk i are in the row (uniform).
+  __device__ inline bool whole(int i) const { return end + i * step <= cols; }
+  // What load() left of the row's last 16 bytes in the chunks at and past its end.
+  __device__ inline void cut(u32x4 (&raw)[C]) const {
+    if (cols < E) return;
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      if (!whole(i)) {
+        const int over = (int)(at(i) - (cols - E));
+        if (over > 0) raw[i] = shift_down(raw[i], (int64_t)over * (int)sizeof(T));
+      }
+  }
+  template <typename Y>
+  __device__ inline void store(Y* p, int i, const float (&v)[E]) const {
+    const uint32_t c = at(i);
+    if (c < cols) store_some(past(p, c), (int64_t)cols - c, v);
+  }
+};
+
+// Elements of a row that a wave holds.
 template <int E, int C>
 __device__ inline float wave_count(int64_t cols, int waves, int wave) {
   int64_t n = 0;
@@ -41,11 +96,6 @@ __device__ inline float wave_count(int64_t cols, int waves, int wave) {
     n += left < 0 ? 0 : left > 64 * E ? 64 * E : left;
   }
   return (float)n;
-}
-// Whether all elements of a wave's chunk i are in the row (uniform).
-template <typename T, int C>
-__device__ inline bool whole_chunk(const Row<T, C>& R, int i) {
-  return (int64_t)((i * R.waves + R.wave) * 64 + 64) * kElems<T> <= R.cols;
 }
 
 // A value near the mean of a wave's elements, and the sums of what is left over it and of that squared (elements past the row's end are zeros in h).
@@ -68,62 +118,71 @@ __device__ inline float value_near(const float (&h)[C][kElems<T>], float weight)
   v += __builtin_bit_cast(float, dpp_u32<0x4E, 0xF>(__builtin_bit_cast(uint32_t, v)));
   return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v))) * weight;
 }
-// The lane's part of the sums.
+// h becomes d = h - near (zeros past the row's end); the lane's part of the sums.
 template <typename T, int C>
-__device__ inline Moments lane_moments(const Row<T, C>& R, const float (&h)[C][kElems<T>], float near) {
+__device__ inline Moments lane_moments(const Span<T, C>& R, float (&h)[C][kElems<T>], float near) {
   constexpr int E = kElems<T>;
   Moments m{near, 0.0f, 0.0f};
 #pragma unroll
   for (int i = 0; i < C; ++i) {
-    const bool whole = whole_chunk(R, i);
+    const bool whole = R.whole(i);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      float d = h[i][e] - near;
-      if (!whole) d = R.at(i) + e < R.cols ? d : 0.0f;
-      m.left += d;
-      m.squares += d * d;
+      h[i][e] -= near;
+      if (!whole) h[i][e] = R.at(i) + e < R.cols ? h[i][e] : 0.0f;
+      m.left += h[i][e];
+      m.squares = __builtin_fmaf(h[i][e], h[i][e], m.squares);
     }
   }
   return m;
 }
 
-// A row's mean in two parts, and 1 / sqrt(var + eps).
+// 1 / sqrt(v), an ulp off; v among the smallest floats keeps its digits.
+__device__ inline float inverse_root(float v) {
+  const bool small = v < 0x1p-96f;
+  const float r = __builtin_amdgcn_rsqf(small ? v * 0x1p96f : v);
+  return small ? r * 0x1p48f : r;
+}
+
+// Of a row: s = 1 / sqrt(var + eps), and what u is past d s in this lane's wave.
 struct RowStats {
-  float mean, rest, s;
+  float shift, s;
 };
-// The waves' moments, one in each of 16 lanes (`n`: of how many elements, 0 where there is no wave), joined; `off`: what the lane's wave's value
-// is away from the row's mean. `per`: 1 / cols.
-__device__ inline RowStats join_moments(const Moments& m, float n, float per, float eps, float* off) {
-  RowStats r;
-  r.mean = row16_sum_f32(__builtin_fmaf(n, m.near, m.left)) * per;
-  *off = m.near - r.mean;
-  const float rest = row16_sum_f32(__builtin_fmaf(n, *off, m.left));
-  const float squares = row16_sum_f32(m.squares + *off * __builtin_fmaf(n, *off, 2.0f * m.left));
-  r.rest = rest * per;
-  r.s = 1.0f / sqrtf((squares - rest * r.rest) * per + eps);
-  return r;
+// What the waves left, a wave's in each of 16 lanes (`n`: of how many elements, 0 where there is no wave), joined: what `near` (this lane's wave's) is
+// away from the row's mean by, in two parts.
+struct Joined {
+  float off, rest;
+  RowStats row;
+};
+__device__ inline Joined join_moments(const Moments& m, float n, float near, float per, float eps) {
+  Joined j;
+  const float mean = row16_sum_f32(__builtin_fmaf(n, m.near, m.left)) * per;
+  j.off = m.near - mean;
+  const float rest = row16_sum_f32(__builtin_fmaf(n, j.off, m.left));
+  const float squares = row16_sum_f32(__builtin_fmaf(j.off, __builtin_fmaf(n, j.off, 2.0f * m.left), m.squares));
+  j.rest = rest * per;
+  j.row.s = inverse_root((squares - rest * j.rest) * per + eps);
+  j.row.shift = ((near - mean) - j.rest) * j.row.s;
+  return j;
 }
 // Of a row that one wave holds.
 __device__ inline RowStats own_stats(const Moments& m, float per, float eps) {
-  RowStats r;
-  r.mean = m.near;
-  r.rest = m.left * per;
-  r.s = 1.0f / sqrtf((m.squares - m.left * r.rest) * per + eps);
-  return r;
+  const float rest = m.left * per, s = inverse_root((m.squares - m.left * rest) * per + eps);
+  return RowStats{-rest * s, s};
 }
 
 typedef float f32x4_lds __attribute__((ext_vector_type(4)));
 
 // A row a workgroup; or, where a wave holds a row, one for each of its four waves. 8 bits: a scale a row, or (kBlocks) one for each 128.
 template <typename T, typename Y, int C, bool kBlocks>
-__global__ __launch_bounds__(C == 4 ? 1024 : 512) void layer_norm_kernel(LayerNormArgs a, int waves) {
+__global__ __launch_bounds__(1024) void layer_norm_kernel(LayerNormArgs a, int waves) {
   constexpr int E = kElems<T>;
   constexpr bool kFp8 = sizeof(Y) == 1;
   __shared__ __align__(16) f32x4_lds words[kWaves];
   __shared__ __align__(16) float scratch[1][kWaves];
   const int lane = threadIdx.x & 63, group = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = waves == 1 ? 0 : group;
   const int64_t cols = a.cols;
-  const Row<T, C> R{cols, waves, wave, lane};
+  const Span<T, C> R(cols, waves, wave, lane);
   const int other = lane & (kWaves - 1);  // whose moments this lane joins
   const float weight = near_weight<E>(cols, wave), n_other = other < waves ? wave_count<E, C>(cols, waves, other) : 0.0f;
   const float per_col = 1.0f / (float)a.cols;
@@ -153,10 +212,7 @@ __global__ __launch_bounds__(C == 4 ? 1024 : 512) void layer_norm_kernel(LayerNo
       }
     if (sum)
 #pragma unroll
-      for (int i = 0; i < C; ++i) {
-        const int64_t c = R.at(i);
-        if (c < cols) store_some(sum + c, cols - c, h[i]);
-      }
+      for (int i = 0; i < C; ++i) R.store(sum, i, h[i]);
     Moments m = lane_moments(R, h, value_near<T, C>(h, weight));
     m.left = wave_sum_f32(m.left);
     m.squares = wave_sum_f32(m.squares);
@@ -171,8 +227,7 @@ __global__ __launch_bounds__(C == 4 ? 1024 : 512) void layer_norm_kernel(LayerNo
         const f32x4_lds v = words[other];
         q = Moments{v.x, v.y, v.z};
       }
-      float off;
-      r = join_moments(q, n_other, per_col, a.eps, &off);
+      r = join_moments(q, n_other, m.near, per_col, a.eps).row;
     }
     R.cut(wr);
     if (a.bias) R.cut(br);
@@ -183,7 +238,7 @@ __global__ __launch_bounds__(C == 4 ? 1024 : 512) void layer_norm_kernel(LayerNo
       if (a.bias) unpack(br[i], b);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        h[i][e] = ((h[i][e] - r.mean) - r.rest) * r.s;
+        h[i][e] = __builtin_fmaf(h[i][e], r.s, r.shift);
         h[i][e] = a.bias ? __builtin_fmaf(h[i][e], w[e], b[e]) : h[i][e] * w[e];
       }
     }
@@ -194,15 +249,15 @@ __global__ __launch_bounds__(C == 4 ? 1024 : 512) void layer_norm_kernel(LayerNo
         top[i] = 0;
 #pragma unroll
         for (int e = 0; e < E; ++e)
-          if (R.at(i) + e < cols) top[i] = max(top[i], magnitude(h[i][e]));
+          if (R.at(i) + e < R.cols) top[i] = max(top[i], magnitude(h[i][e]));
       }
       if constexpr (kBlocks) {
 #pragma unroll
         for (int i = 0; i < C; ++i) {
           const uint32_t scale = block_scale(block_max_u32<E>(top[i]));
           const float factor = block_factor(scale);
-          const int64_t c = R.at(i);
-          if (c % kScaleBlock == 0 && c < cols) static_cast<uint8_t*>(a.scales)[c / kScaleBlock * a.scales_stride + row] = (uint8_t)scale;
+          const uint32_t c = R.at(i);
+          if (c % kScaleBlock == 0 && c < R.cols) static_cast<uint8_t*>(a.scales)[c / kScaleBlock * a.scales_stride + row] = (uint8_t)scale;
 #pragma unroll
           for (int e = 0; e < E; ++e) h[i][e] *= factor;
         }
@@ -219,10 +274,7 @@ __global__ __launch_bounds__(C == 4 ? 1024 : 512) void layer_norm_kernel(LayerNo
       }
     }
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-      const int64_t c = R.at(i);
-      if (c < cols) store_some(y + c, cols - c, h[i]);
-    }
+    for (int i = 0; i < C; ++i) R.store(y, i, h[i]);
     if (waves > 1) __syncthreads();  // the next row writes the words again
   }
 }
@@ -332,15 +384,19 @@ struct LayerNormGradArgs {
   float eps;
 };
 
-// A workgroup's rows are blockIdx.x, + gridDim.x, ...; with kAhead the next row's operands are asked for before this one's sums.
+// `groups` rows at a time to a workgroup, `waves` waves to each, at most 16 in all; their parts of dweight and dbias meet in LDS at the end, so that a
+// workgroup leaves one of each. With kAhead the next rows' operands are asked for before these ones' sums.
 template <typename T, int C, bool kAhead>
-__global__ __launch_bounds__(1024) void layer_norm_grad_kernel(LayerNormGradArgs a, int waves) {
+__global__ __launch_bounds__(C == 4 && sizeof(T) == 2 ? 512 : 1024) void layer_norm_grad_kernel(LayerNormGradArgs a, int waves, int groups) {
   constexpr int E = kElems<T>;
+  constexpr bool kKeep = C == 1;  // g over the barrier (of two chunks a lane it does not fit beside the rest, and is formed again)
   __shared__ __align__(16) f32x4_lds words[2][kWaves];
   __shared__ float more[2][kWaves];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  extern __shared__ __align__(16) float left_by[];  // (groups - 1) waves 64 2 C E floats
+  const int lane = threadIdx.x & 63, place = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = place / waves, wave = place - group * waves, first = group * waves;
   const int64_t cols = a.cols;
-  const Row<T, C> R{cols, waves, wave, lane};
+  const Span<T, C> R(cols, waves, wave, lane);
   const int other = lane & (kWaves - 1);
   const float weight = near_weight<E>(cols, wave), n_other = other < waves ? wave_count<E, C>(cols, waves, other) : 0.0f;
   const float per_col = 1.0f / (float)a.cols;
@@ -356,34 +412,40 @@ __global__ __launch_bounds__(1024) void layer_norm_grad_kernel(LayerNormGradArgs
     if (a.dh && a.dx) R.load(static_cast<const T*>(a.dh) + row * a.dh_stride, ur);
   };
   R.load(static_cast<const T*>(a.weight), wr);
-  if constexpr (kAhead) load(blockIdx.x);
+  const int64_t step = (int64_t)gridDim.x * groups;
+  // (a group without a row goes along to the barrier with what it last read, and adds nothing)
+  auto last = [&](int64_t row) __attribute__((always_inline)) { return row < a.rows ? row : a.rows - 1; };
+  if constexpr (kAhead) load(last((int64_t)blockIdx.x * groups + group));
   R.cut(wr);
   int flip = 0;
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    if constexpr (!kAhead) load(row);
+  for (int64_t base = (int64_t)blockIdx.x * groups; base < a.rows; base += step) {
+    const int64_t row = base + group;
+    if constexpr (!kAhead) load(last(row));
     R.cut(hr);
     R.cut(dr);
-    float h[C][E], dy[C][E];
-    u32x4 uv[C];
+    float d[C][E], g[kKeep ? C : 1][E];
+    u32x4 yv[C], uv[C];
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-      unpack(hr[i], h[i]);
-      unpack(dr[i], dy[i]);
+      unpack(hr[i], d[i]);
+      yv[i] = dr[i];
       uv[i] = ur[i];
     }
     if constexpr (kAhead)
-      if (row + gridDim.x < a.rows) load(row + gridDim.x);
-    Moments m = lane_moments(R, h, value_near<T, C>(h, weight));
-    float g_sum = 0.0f, gd_sum = 0.0f;  // of g and of g d (dy is zero past the end)
+      if (row + step < a.rows) load(row + step);
+    Moments m = lane_moments(R, d, value_near<T, C>(d, weight));
+    float g_sum = 0.0f, gd_sum = 0.0f;  // of g and of g d
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-      float w[E];
+      float w[E], dy[E];
+      float(&gi)[E] = g[kKeep ? i : 0];
       unpack(wr[i], w);
+      unpack(yv[i], dy);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const float g = dy[i][e] * w[e];
-        g_sum += g;
-        gd_sum += g * (h[i][e] - m.near);
+        gi[e] = dy[e] * w[e];
+        g_sum += gi[e];
+        gd_sum = __builtin_fmaf(gi[e], d[i][e], gd_sum);
       }
     }
     m.left = wave_sum_f32(m.left);
@@ -393,59 +455,78 @@ __global__ __launch_bounds__(1024) void layer_norm_grad_kernel(LayerNormGradArgs
     RowStats r;
     if (waves == 1) {
       r = own_stats(m, per_col, a.eps);
-      gd_sum -= r.rest * g_sum;
+      gd_sum -= m.left * per_col * g_sum;
     } else {
       if (lane == 0) {
-        words[flip][wave] = f32x4_lds{m.near, m.left, m.squares, g_sum};
-        more[flip][wave] = gd_sum;
+        words[flip][place] = f32x4_lds{m.near, m.left, m.squares, g_sum};
+        more[flip][place] = gd_sum;
       }
       __syncthreads();  // (two sets in turn: a wave writes a set again only past the barrier of the row between)
       f32x4_lds v = {0.0f, 0.0f, 0.0f, 0.0f};
-      float gd = 0.0f, off;
+      float gd = 0.0f;
       if (other < waves) {
-        v = words[flip][other];
-        gd = more[flip][other];
+        v = words[flip][first + other];
+        gd = more[flip][first + other];
       }
       flip ^= 1;
-      r = join_moments(Moments{v.x, v.y, v.z}, n_other, per_col, a.eps, &off);
+      const Joined j = join_moments(Moments{v.x, v.y, v.z}, n_other, m.near, per_col, a.eps);
+      r = j.row;
       g_sum = row16_sum_f32(v.w);
-      gd_sum = row16_sum_f32(__builtin_fmaf(off, v.w, gd)) - r.rest * g_sum;
+      gd_sum = row16_sum_f32(__builtin_fmaf(j.off, v.w, gd)) - j.rest * g_sum;
     }
-    const float g_mean = g_sum * per_col;
-    const float along = r.s * (r.s * (gd_sum * per_col));  // mean(g u) s (s^2 alone may be no float where eps is 0)
+    if (row >= a.rows) continue;
+    // dx = s g - u s mean(g u) - s mean(g) + dh (s^2 alone may be no float where eps is 0)
+    const float along = -r.s * (r.s * (gd_sum * per_col)), flat = -r.s * (g_sum * per_col);
     T* dx = a.dx ? static_cast<T*>(a.dx) + row * a.dx_stride : nullptr;
     if (dx && a.dh) R.cut(uv);
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-      float o[E], w[E];
-      unpack(wr[i], w);
+      float o[E], dy[E], w[E];
+      unpack(yv[i], dy);
+      if constexpr (!kKeep) unpack(wr[i], w);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const float d = (h[i][e] - r.mean) - r.rest;
-        dw[i][e] += dy[i][e] * (d * r.s);
-        db[i][e] += dy[i][e];
-        o[e] = r.s * (dy[i][e] * w[e] - g_mean - d * along);
+        const float u = __builtin_fmaf(d[i][e], r.s, r.shift);
+        dw[i][e] = __builtin_fmaf(dy[e], u, dw[i][e]);
+        db[i][e] += dy[e];
+        o[e] = __builtin_fmaf(kKeep ? g[kKeep ? i : 0][e] : dy[e] * w[e], r.s, __builtin_fmaf(u, along, flat));
       }
       if (dx) {
         if (a.dh) {
-          float u[E];
-          unpack(uv[i], u);
+          float q[E];
+          unpack(uv[i], q);
 #pragma unroll
-          for (int e = 0; e < E; ++e) o[e] += u[e];
+          for (int e = 0; e < E; ++e) o[e] += q[e];
         }
-        const int64_t c = R.at(i);
-        if (c < cols) store_some(dx + c, cols - c, o);
+        R.store(dx, i, o);
       }
     }
+  }
+  if (groups > 1) {
+    const int lanes = waves * 64, at = wave * 64 + lane;
+    f32x4_lds* own = reinterpret_cast<f32x4_lds*>(left_by);
+    auto slot = [&](int g, int q) { return ((g - 1) * 2 * C * (E / 4) + q) * lanes + at; };
+    auto quad = [&](int q) -> f32x4_lds* {
+      const int half = C * (E / 4), i = q % half;
+      return reinterpret_cast<f32x4_lds*>(q < half ? &dw[i / (E / 4)][4 * (i % (E / 4))] : &db[i / (E / 4)][4 * (i % (E / 4))]);
+    };
+    if (group > 0)
+#pragma unroll
+      for (int q = 0; q < 2 * C * (E / 4); ++q) own[slot(group, q)] = *quad(q);
+    __syncthreads();
+    if (group > 0) return;
+    for (int g = 1; g < groups; ++g)
+#pragma unroll
+      for (int q = 0; q < 2 * C * (E / 4); ++q) *quad(q) += own[slot(g, q)];
   }
   auto leave = [&](float* parts, const float (&v)[C][E]) __attribute__((always_inline)) {
     float* part = parts + (int64_t)blockIdx.x * a.part_pitch;
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-      const int64_t c = R.at(i);
+      const uint32_t c = R.at(i);
 #pragma unroll
       for (int e = 0; e < E; e += 4)
-        if (c + e < cols) store_some(part + c + e, cols - c - e, *reinterpret_cast<const float (*)[4]>(v[i] + e));
+        if (c + e < R.cols) store_some(R.past(part, c + e), (int64_t)R.cols - c - e, *reinterpret_cast<const float (*)[4]>(v[i] + e));
     }
   };
   if (a.weight_parts) leave(a.weight_parts, dw);
@@ -588,13 +669,16 @@ int32_t launch_norm(dc_hip_ctx* ctx, const LayerNormArgs& a, int64_t chunks) {
   return last_launch_status();
 }
 
+// Chunks that a lane holds: two where rows are long, or where they let a wave hold a row by itself (but not where they are read and written in
+// float32); one, over up to 16 waves, where every row has a CU of its own, as only its latency counts then. us, with the call, for one / two: bf16
+// 16384×4096 95.8 / 95.8, to 8 bits 103.6 / 98.8, 8191×2050 38.4 / 34.9; 8×4096 to 8 bits 4.31 / 4.78. Four, for rows of 16 waves, spill: 2048×24576
+// 222, read again by the long kernel 124.
 template <typename T, typename Y, bool kBlocks>
 int32_t norm_by_shape(dc_hip_ctx* ctx, const LayerNormArgs& a) {
   const int64_t chunks = (a.cols + kElems<T> - 1) / kElems<T>;
-  const bool wave = chunks > 64 && chunks <= 128 && (sizeof(T) == 2 || sizeof(Y) == 1);
-  if (chunks <= 256 && !wave) return launch_norm<T, Y, 1, kBlocks>(ctx, a, chunks);
-  if (chunks <= 1024) return launch_norm<T, Y, 2, kBlocks>(ctx, a, chunks);
-  if (chunks <= 64 * 4 * kWaves) return launch_norm<T, Y, 4, kBlocks>(ctx, a, chunks);
+  const bool wave = chunks > 64 && chunks <= 128 && (sizeof(T) == 2 || sizeof(Y) == 1), few = a.rows <= ctx->cu_count;
+  if (!wave && chunks <= (few ? 64 * kWaves : 256)) return launch_norm<T, Y, 1, kBlocks>(ctx, a, chunks);
+  if (chunks <= 64 * 2 * kWaves) return launch_norm<T, Y, 2, kBlocks>(ctx, a, chunks);
   layer_norm_long_kernel<T, Y, kBlocks><<<(unsigned)std::min(a.rows, kMaxGrid), 64 * kWaves, 0, ctx->stream>>>(a);
   return last_launch_status();
 }
@@ -605,17 +689,41 @@ int32_t norm_by_output(dc_hip_ctx* ctx, const LayerNormArgs& a, bool fp8, bool b
   return blocks ? norm_by_shape<T, uint8_t, true>(ctx, a) : norm_by_shape<T, uint8_t, false>(ctx, a);
 }
 
+// The gradient's workgroups, and the rows that each takes at a time.
+struct GradGrid {
+  int64_t workgroups;
+  int groups;
+};
+// A workgroup a CU, of 16 waves where rows are short, as each leaves parts of dweight and dbias to be added; but no more rows at a time than leave every CU
+// some. us, with the call, bf16, for workgroups of one row (as many as a CU holds) / of 8 waves / of 16: 16384×512 21.1 / 17.7 / 16.7, 8192×1024
+// 22.0 / 18.5 / 18.5, 8191×2050 38.7 / 61 / 37.5; 1000×1000, in workgroups of one row, 4 and 8 rows 14.9 / 9.2 / 10.3. Float32 rows of 6 to 8 waves:
+// two workgroups of one row, 8192×2048 55.2, one of two rows 59.5, one of one 74; bf16 8192×4096 59.5, 55.4, 53.8, 8192×3500 one of two rows 53.3, of one 77.
+GradGrid norm_grad_grid(bool f32, int64_t rows, int c, int waves, int64_t cus) {
+  const int64_t share = (rows + cus - 1) / cus;
+  const int groups = c == 1 && !(f32 && waves >= 6) ? (int)std::min<int64_t>(std::max(1, kWaves / waves), share) : 1;
+  const int64_t held = cus * (f32 && c == 1 && waves >= 6 && waves <= 8 ? 2 : 1);
+  // (Few rows: no more workgroups than take as many of them each)
+  const int64_t each = (rows + held * groups - 1) / (held * groups);
+  return {each <= 4 ? (rows + each * groups - 1) / (each * groups) : held, groups};
+}
+
 template <typename T>
-int32_t norm_grad_by_shape(dc_hip_ctx* ctx, const LayerNormGradArgs& a, int64_t grid, int c, int waves) {
-  const unsigned g = (unsigned)grid;
-  if (c == 1) layer_norm_grad_kernel<T, 1, true><<<g, 64 * waves, 0, ctx->stream>>>(a, waves);
-  else if (c == 2) layer_norm_grad_kernel<T, 2, false><<<g, 64 * waves, 0, ctx->stream>>>(a, waves);
+int32_t norm_grad_by_shape(dc_hip_ctx* ctx, const LayerNormGradArgs& a, const GradGrid& grid, int c, int waves) {
+  const int groups = grid.groups;
+  const unsigned g = (unsigned)grid.workgroups, threads = 64 * waves * groups;
+  const size_t lds = (size_t)(groups - 1) * waves * 64 * 2 * c * kElems<T> * sizeof(float);
+  if (c == 1) layer_norm_grad_kernel<T, 1, true><<<g, threads, lds, ctx->stream>>>(a, waves, groups);
+  else if (sizeof(T) == 4 && c == 2) layer_norm_grad_kernel<float, 2, false><<<g, threads, lds, ctx->stream>>>(a, waves, groups);
+  else if (c == 4) layer_norm_grad_kernel<T, 4, false><<<g, threads, lds, ctx->stream>>>(a, waves, groups);
   else layer_norm_grad_long_kernel<T><<<g, 64 * kWaves, 0, ctx->stream>>>(a);
   return last_launch_status();
 }
 
-// 16-byte chunks of a row that a lane of the gradient's kernel holds (0: the long kernel).
-int norm_grad_chunks(int64_t chunks) { return chunks <= 64 * kWaves ? 1 : chunks <= 128 * kWaves ? 2 : 0; }
+// 16-byte chunks of a row that a lane of the gradient's kernel holds (0: the long kernel). bf16's four leave 8 waves of 256 registers.
+int norm_grad_chunks(bool f32, int64_t chunks) {
+  if (f32) return chunks <= 64 * kWaves ? 1 : chunks <= 128 * kWaves ? 2 : chunks <= 256 * kWaves ? 4 : 0;
+  return chunks <= 64 * kWaves ? 1 : chunks <= 128 * kWaves ? 4 : 0;
+}
 
 }  // namespace
 
@@ -670,15 +778,13 @@ DC_HIP_API int32_t dc_hip_layer_norm_backward(dc_hip_ctx* ctx, const dc_layer_no
     return DC_OK;
   }
   const int64_t elems = 16 / size_of(p.dtype), chunks = (p.cols + elems - 1) / elems;
-  const int c = norm_grad_chunks(chunks), waves = c ? waves_for(chunks, c) : kWaves;
-  const int per_cu = waves <= 2 ? 8 / waves : c > 1 ? 1 : std::max(1, 15 / waves);
-  const int64_t held = per_cu * (int64_t)std::max(1, ctx->cu_count);  // workgroups
-  const int64_t each = (p.rows + held - 1) / held, grid = each <= 4 ? (p.rows + each - 1) / each : held;
+  const int c = norm_grad_chunks(p.dtype == DC_DTYPE_F32, chunks), waves = c ? waves_for(chunks, c) : kWaves;
+  const GradGrid grid = norm_grad_grid(p.dtype == DC_DTYPE_F32, p.rows, c, waves, std::max(1, ctx->cu_count));
   const int outs = (p.dweight ? 1 : 0) + (p.dbias ? 1 : 0);
   const int64_t pitch = (p.cols + 3) / 4 * 4;
   float *weight_parts = nullptr, *bias_parts = nullptr;
   if (outs > 0) {
-    DC_RETURN_IF(ensure_partials(ctx, (size_t)(grid * outs * pitch) * sizeof(float)));
+    DC_RETURN_IF(ensure_partials(ctx, (size_t)(grid.workgroups * outs * pitch) * sizeof(float)));
     float* parts = static_cast<float*>(ctx->partials);
     if (p.dweight) weight_parts = parts;
     if (p.dbias) bias_parts = parts + (outs - 1) * pitch;
@@ -688,7 +794,7 @@ DC_HIP_API int32_t dc_hip_layer_norm_backward(dc_hip_ctx* ctx, const dc_layer_no
   DC_RETURN_IF(p.dtype == DC_DTYPE_F32 ? norm_grad_by_shape<float>(ctx, a, grid, c, waves) : norm_grad_by_shape<bf16>(ctx, a, grid, c, waves));
   if (outs == 0) return DC_OK;
   return launch_column_sums_of(ctx, static_cast<const float*>(ctx->partials), outs * pitch, pitch, p.dweight ? p.dweight : p.dbias,
-                               outs > 1 ? p.dbias : nullptr, grid, p.cols);
+                               outs > 1 ? p.dbias : nullptr, grid.workgroups, p.cols);
 }
 
 DC_HIP_API int32_t dc_hip_quantize_fp8_blocks(dc_hip_ctx* ctx, const void* x, int32_t dtype, int64_t x_stride, uint8_t* q,
