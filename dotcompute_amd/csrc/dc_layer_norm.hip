@@ -613,49 +613,67 @@ __global__ __launch_bounds__(1024) void layer_norm_grad_long_kernel(LayerNormGra
 }
 
 // ---- rows in 8 bits with a scale for each 128 elements -----------------------------------------------------
-// Memory-bound: 3 bytes an element of bf16, 5 of float32. A wave takes 64 chunks of 16 bytes of a row (512 elements of bf16, 256 of float32), whose blocks'
-// maxima are found among 16 or 32 lanes, without LDS; its workgroup's 16 such pieces lie below each other, so that the scales, which run
-// along the rows, are written 16 neighbouring bytes at a time.
+// Memory-bound: 3 bytes an element of bf16, 5 of float32. A wave takes 64 chunks of 16 bytes (512 elements of bf16, 256 of float32) of kRows rows below each
+// other, all asked for at once; a block's maximum is found among 16 or 32 lanes, without LDS, and its first lane writes the rows' scales, which
+// lie beside each other, in one piece.
 struct QuantizeArgs {
   const void* x;
   uint8_t *q, *scales;
-  int64_t rows, cols, x_stride, q_stride, scales_stride, across;  // across: pieces to a row
+  int64_t rows, cols, x_stride, q_stride, scales_stride, across, total;  // across: pieces to a row; total: pieces
 };
-constexpr int kPieceRows = 16;
-template <typename T>
+template <typename T, int kRows>
 __global__ __launch_bounds__(256) void quantize_blocks_kernel(QuantizeArgs a) {
-  constexpr int E = kElems<T>, kBlocks = 64 * E / kScaleBlock, kEach = kPieceRows / 4;
-  __shared__ uint8_t codes[kBlocks][kPieceRows];
+  constexpr int E = kElems<T>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int64_t total = a.across * ((a.rows + kPieceRows - 1) / kPieceRows);
-  for (int64_t t = blockIdx.x; t < total; t += gridDim.x) {
-    const int64_t down = total <= UINT32_MAX ? (int64_t)((uint32_t)t / (uint32_t)a.across) : t / a.across;
-    const int64_t row0 = down * kPieceRows, c0 = (t - down * a.across) * 64 * E, c = c0 + (int64_t)lane * E;
-    float v[kEach][E];
+  for (int64_t t = (int64_t)blockIdx.x * 4 + wave; t < a.total; t += (int64_t)gridDim.x * 4) {
+    const int64_t down = a.total <= UINT32_MAX ? (int64_t)((uint32_t)t / (uint32_t)a.across) : t / a.across;
+    const int64_t row0 = down * kRows, c0 = (t - down * a.across) * 64 * E, left = a.cols - c0;  // left: elements from here on
+    const int at = lane * E, rows = (int)(a.rows - row0 < kRows ? a.rows - row0 : kRows);
+    const T* x = static_cast<const T*>(a.x) + row0 * a.x_stride + c0;
+    u32x4 raw[kRows];
+    if (a.cols >= E) {  // (a chunk at the row's end is cut out of its last 16 bytes, one past it is zeros; no branch between the loads)
+      const int64_t from = at < left - E ? at : left - E;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int64_t row = row0 + wave * kEach + i;
-      load_some(static_cast<const T*>(a.x) + row * a.x_stride + c, row < a.rows ? a.cols - c : 0, v[i]);
+      for (int i = 0; i < kRows; ++i) raw[i] = load_raw(x + (i < rows ? i : rows - 1) * a.x_stride + from);
+      if (left < 64 * E)
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) raw[i] = shift_down(raw[i], (at - from) * (int64_t)sizeof(T));
+    } else {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        float v[E];
+        load_some(x + (i < rows ? i : rows - 1) * a.x_stride, at == 0 ? left : 0, v);
+        if constexpr (E == 4) raw[i] = __builtin_bit_cast(u32x4, f32x4{v[0], v[1], v[2], v[3]});
+        else
+#pragma unroll
+          for (int e = 0; e < 4; ++e) raw[i][e] = pack_bf16(v[2 * e], v[2 * e + 1]);
+      }
     }
+    uint32_t scales[(kRows + 3) / 4] = {};
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int64_t row = row0 + wave * kEach + i;
+    for (int i = 0; i < kRows; ++i) {
+      float v[E];
+      unpack(raw[i], v);
       uint32_t top = 0;
 #pragma unroll
-      for (int e = 0; e < E; ++e) top = max(top, magnitude(v[i][e]));  // (zeros past the end)
+      for (int e = 0; e < E; ++e) top = max(top, magnitude(v[e]));
       const uint32_t scale = block_scale(block_max_u32<E>(top));
       const float factor = block_factor(scale);
 #pragma unroll
-      for (int e = 0; e < E; ++e) v[i][e] *= factor;
-      if (row < a.rows && c < a.cols) store_some(a.q + row * a.q_stride + c, a.cols - c, v[i]);
-      if (lane % (kScaleBlock / E) == 0) codes[lane / (kScaleBlock / E)][wave * kEach + i] = (uint8_t)scale;
+      for (int e = 0; e < E; ++e) v[e] *= factor;
+      scales[i / 4] |= scale << (8 * (i % 4));
+      if (i < rows && at < left) store_some(a.q + (row0 + i) * a.q_stride + c0 + at, left - at, v);
     }
-    __syncthreads();
-    if (threadIdx.x < kBlocks * kPieceRows) {
-      const int b = threadIdx.x / kPieceRows, i = threadIdx.x % kPieceRows;
-      if (row0 + i < a.rows && c0 + b * kScaleBlock < a.cols) a.scales[(c0 / kScaleBlock + b) * a.scales_stride + row0 + i] = codes[b][i];
+    if (at % kScaleBlock == 0 && at < left) {
+      uint8_t* to = a.scales + (c0 + at) / kScaleBlock * a.scales_stride + row0;
+      if (kRows == 8 && rows == 8) {
+        *reinterpret_cast<u32x2_at1*>(to) = u32x2{scales[0], scales[(kRows + 3) / 4 - 1]};
+      } else {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i)
+          if (i < rows) to[i] = (uint8_t)(scales[i / 4] >> (8 * (i % 4)));
+      }
     }
-    __syncthreads();
   }
 }
 
@@ -810,10 +828,15 @@ DC_HIP_API int32_t dc_hip_quantize_fp8_blocks(dc_hip_ctx* ctx, const void* x, in
   DC_CTX_ENTER(ctx);
   if (rows == 0 || cols == 0) return DC_OK;
   const int64_t piece = 64 * 16 / size_of(dtype), across = (cols + piece - 1) / piece;
-  const QuantizeArgs a{x, q, scales, rows, cols, x_stride, q_stride, scales_stride, across};
-  const unsigned grid = (unsigned)std::min(across * ((rows + kPieceRows - 1) / kPieceRows), kMaxGrid);
-  if (dtype == DC_DTYPE_F32) quantize_blocks_kernel<float><<<grid, 256, 0, ctx->stream>>>(a);
-  else quantize_blocks_kernel<bf16><<<grid, 256, 0, ctx->stream>>>(a);
+  auto launch = [&](auto kernel, int64_t each) {
+    const int64_t total = across * ((rows + each - 1) / each);
+    const QuantizeArgs a{x, q, scales, rows, cols, x_stride, q_stride, scales_stride, across, total};
+    kernel<<<(unsigned)std::min((total + 3) / 4, kMaxGrid), 256, 0, ctx->stream>>>(a);
+  };
+  // (eight rows to a wave where that leaves every CU some waves, else a row to a wave)
+  const bool few = across * ((rows + 7) / 8) < 4 * (int64_t)ctx->cu_count;
+  if (dtype == DC_DTYPE_F32) few ? launch(quantize_blocks_kernel<float, 1>, 1) : launch(quantize_blocks_kernel<float, 8>, 8);
+  else few ? launch(quantize_blocks_kernel<bf16, 1>, 1) : launch(quantize_blocks_kernel<bf16, 8>, 8);
   return last_launch_status();
 }
 
