@@ -53,13 +53,26 @@ int32_t launch_few_rows(dc_hip_ctx* ctx, const MoreOperands& o, const Epilogue& 
   return dc::last_launch_status();
 }
 
+// 32 outputs to a workgroup where that leaves a workgroup for every other CU at least, so that x comes half as often with w through a CU's loads to LDS;
+// with nine rows or more, eight waves of them in a CU's whole LDS, or, where there is more than one workgroup for a CU, four in half of it. us for 16 outputs / 32
+// with eight waves / 32 with four: 1×4096×4096 6.33 / 5.93 / 6.44, 1×8192×4096 10.1 / 8.5 / 8.9; 17×4096×4096 6.85 / 6.37 / 7.15, 17×8192×4096 10.6 / 9.1 / 9.9,
+// 17×16384×2048 9.9 / 10.1 / 8.5, 17×2048×8192 6.9 / 8.6 / 10.1; 32×8192×4096 11.2 / 9.7 / 10.1, 32×16384×2048 10.7 / 10.2 / 8.5. Past 32 rows eight waves of 16
+// outputs: 64×4096×4096 8.4, four 9.1, 256×512×2048 4.8, 5.5.
+template <int XB>
+int32_t few_rows_of(dc_hip_ctx* ctx, const MoreOperands& o, const Epilogue& ep) {
+  const int64_t cus = std::max(1, ctx->cu_count);
+  if ((o.n + 15) / 16 < cus) return launch_few_rows<XB, 1, XB < 4 ? 8 : 4, 80>(ctx, o, ep);
+  if constexpr (XB > 1)
+    return (o.n + 31) / 32 > cus ? launch_few_rows<XB, 2, 4, 80>(ctx, o, ep) : launch_few_rows<XB, 2, 8, 160>(ctx, o, ep);
+  else
+    return launch_few_rows<XB, 2, 8, 80>(ctx, o, ep);
+}
 int32_t few_rows(dc_hip_ctx* ctx, const MoreOperands& o, const Epilogue& ep) {
-  const bool wide = dc::linear_wide_few_rows(o.m, o.n, std::max(1, ctx->cu_count));
-  if (o.m <= 8) return wide ? launch_few_rows<1, 4, 4, 80>(ctx, o, ep) : launch_few_rows<1, 1, 8, 80>(ctx, o, ep);
-  if (o.m <= 16) return wide ? launch_few_rows<2, 4, 4, 80>(ctx, o, ep) : launch_few_rows<2, 1, 8, 80>(ctx, o, ep);
-  if (o.m <= 24) return wide ? launch_few_rows<3, 4, 4, 160>(ctx, o, ep) : launch_few_rows<3, 1, 8, 80>(ctx, o, ep);
-  if (o.m <= 32) return wide ? launch_few_rows<4, 4, 4, 160>(ctx, o, ep) : launch_few_rows<4, 1, 4, 80>(ctx, o, ep);
-  return launch_few_rows<8, 1, 4, 80>(ctx, o, ep);
+  if (o.m <= 8) return few_rows_of<1>(ctx, o, ep);
+  if (o.m <= 16) return few_rows_of<2>(ctx, o, ep);
+  if (o.m <= 24) return few_rows_of<3>(ctx, o, ep);
+  if (o.m <= 32) return few_rows_of<4>(ctx, o, ep);
+  return launch_few_rows<8, 1, 8, 160>(ctx, o, ep);
 }
 
 }  // namespace

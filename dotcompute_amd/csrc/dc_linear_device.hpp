@@ -967,8 +967,8 @@ __device__ inline void wait_loads() {  // until at most N of the wave's loads ar
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-// kGated: the second half of the NB blocks of 16 rows of w are the other weight's, so that a workgroup has 8 NB outputs. kBlocks: a step's scales are
-// asked for the step before.
+// kGated: the second half of the NB blocks of 16 rows of w are the other weight's, so that a workgroup has 8 NB outputs. kBlocks: the lanes of group g
+// hold the scales of every fourth of the wave's steps from its g-th on, a load for four steps; a step's are handed over within the wave.
 template <bool kFp8, int XB, int NB, int W, int D, bool kGated, bool kBlocks>
 __global__ __launch_bounds__(64 * W) void few_rows_kernel(typename ProductTypes<false, kGated, kBlocks>::O o,
                                                           typename ProductTypes<false, kGated, kBlocks>::E ep) {
@@ -1020,24 +1020,35 @@ __global__ __launch_bounds__(64 * W) void few_rows_kernel(typename ProductTypes<
     v[0] = *reinterpret_cast<const dc::u32x4*>(stage + row * kTileBytes + lo);
     v[1] = *reinterpret_cast<const dc::u32x4*>(stage + row * kTileBytes + hi);
   };
-  // Block scales of a step: of the rows of w and x that this lane's operands hold.
+  // Block scales of four of the wave's steps, from step t on, of the rows of w and x that this lane's operands hold.
   struct Codes {
     int w[kBlocks ? NB : 1], x[kBlocks ? MT : 1];
   };
-  auto load_codes = [&](Codes& c, int s) __attribute__((always_inline)) {
+  auto load_codes = [&](Codes& c, int t) __attribute__((always_inline)) {
     if constexpr (kBlocks) {
-      const int64_t kb = min(s, steps - 1);
+      const int kb = min(wave + (t + g) * W, steps - 1);
       const int left_n = (int)min((int64_t)o.n - n0, (int64_t)16 * kOut), left_m = (int)min((int64_t)o.m - m0, (int64_t)8 * XB);
 #pragma unroll
       for (int i = 0; i < NB; ++i) {
-        if constexpr (kGated)
-          c.w[i] = load_code((i < kOut ? o.b_codes + kb * o.b_codes_pitch : o.b2_codes + kb * o.b2_codes_pitch) + n0, left_n, 16 * (i % kOut) + r);
-        else
-          c.w[i] = load_code(o.b_codes + kb * o.b_codes_pitch + n0, left_n, 16 * i + r);
+        const uint8_t* from = o.b_codes + kb * o.b_codes_pitch + n0;
+        if constexpr (kGated) from = i < kOut ? from : o.b2_codes + kb * o.b2_codes_pitch + n0;
+        c.w[i] = from[min(16 * (i % kOut) + r, left_n - 1)];
       }
 #pragma unroll
-      for (int j = 0; j < MT; ++j) c.x[j] = load_code(o.a_codes + kb * o.a_codes_pitch + m0, left_m, 16 * j + (16 * j + 8 < 8 * XB ? r : r & 7));
+      for (int j = 0; j < MT; ++j) c.x[j] = (o.a_codes + kb * o.a_codes_pitch + m0)[min(16 * j + r, left_m - 1)];
     }
+  };
+  // Those of step t, in every lane.
+  auto hand_over = [&](const Codes& c, int t) __attribute__((always_inline)) {
+    Codes now;
+    if constexpr (kBlocks) {
+      const int from = 4 * (16 * (t & 3) + r);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) now.w[i] = __builtin_amdgcn_ds_bpermute(from, c.w[i]);
+#pragma unroll
+      for (int j = 0; j < MT; ++j) now.x[j] = __builtin_amdgcn_ds_bpermute(from, c.x[j]);
+    }
+    return now;
   };
   auto add = [&](const unsigned char* stage, const Codes& c) __attribute__((always_inline)) {
     dc::u32x4 wv[NB][2], xv[MT][2];
@@ -1067,6 +1078,8 @@ __global__ __launch_bounds__(64 * W) void few_rows_kernel(typename ProductTypes<
       }
   };
   const int count = steps > wave ? (steps - wave + W - 1) / W : 0;  // this wave's steps: wave, wave + W, ...
+  Codes four, ahead;
+  load_codes(four, 0);
 #pragma unroll
   for (int d = 0; d < D - 1; ++d)
     if (d < count) load(own + d * kStage, wave + d * W);
@@ -1089,31 +1102,40 @@ __global__ __launch_bounds__(64 * W) void few_rows_kernel(typename ProductTypes<
     }
   }
   int slot = 0;
-  auto turn = [&](int t, const Codes& c, Codes& ahead) __attribute__((always_inline)) {
+  auto turn = [&](int t) __attribute__((always_inline)) {
     const int next = t + D - 1;
-    load_codes(ahead, wave + (t + 1) * W);
+    Codes now;
     if (next < count) {
       // (its stage was read in the turn before; those reads have returned, as their products have been issued. The wait leaves scales out of
       // its count: wherever they stand among the loads, no fewer have landed.)
       load(own + (slot == 0 ? D - 1 : slot - 1) * kStage, wave + next * W);
+      now = hand_over(four, t);
       wait_loads<(D - 1) * kLoads>();
     } else {
+      now = hand_over(four, t);
       wait_loads<0>();
     }
     __builtin_amdgcn_sched_barrier(0);
-    add(own + slot * kStage, c);
+    add(own + slot * kStage, now);
     __builtin_amdgcn_sched_barrier(0);
     slot = slot + 1 == D ? 0 : slot + 1;
   };
-  Codes even, odd;
   if constexpr (kBlocks) {
-    load_codes(even, wave);
-    for (int t = 0; t < count; t += 2) {
-      turn(t, even, odd);
-      if (t + 1 < count) turn(t + 1, odd, even);
+    // (four turns at a time, with no way round any of them into the next four: else the compiler cannot tell how many loads have gone out since the
+    // scales', and waits for all before it takes those)
+    for (int t = 0; t < count; t += 4) {
+      load_codes(ahead, t + 4);
+      turn(t);
+      if (t + 1 >= count) break;
+      turn(t + 1);
+      if (t + 2 >= count) break;
+      turn(t + 2);
+      if (t + 3 >= count) break;
+      turn(t + 3);
+      four = ahead;
     }
   } else {
-    for (int t = 0; t < count; ++t) turn(t, even, odd);
+    for (int t = 0; t < count; ++t) turn(t);
   }
   __syncthreads();
   f32x4* sums = reinterpret_cast<f32x4*>(ring);
