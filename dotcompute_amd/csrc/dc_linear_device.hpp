@@ -559,19 +559,21 @@ __global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void pro
 
   // Block scales of the tiles in turn, of the rows that this lane's fragments hold.
   int ascale[2][kBlocks ? kMT : 1], bscale[2][kBlocks ? kNT : 1];
-  auto load_scales = [&](auto BUF, int KT) __attribute__((always_inline)) {
+  // (`mark`: set in bits that the instructions do not look at, in the first tiles' alone. Without it the compiler sees bytes come into the loop from
+  // both ends, carries bytes round it, and widens them at its head, where it waits for the loads that have just gone out.)
+  auto load_scales = [&](auto BUF, int KT, int mark = 0) __attribute__((always_inline)) {
     if constexpr (kBlocks) {
       constexpr int kBuf = decltype(BUF)::value;
       const int64_t kb = min((kt_first + KT) * KS + group, tiles_c - 1);
       const int i0 = m0 + wm * 32 * kMT, j0 = n0 + wn * (kPairs ? 16 : 32) * kNT;
 #pragma unroll
-      for (int mt = 0; mt < kMT; ++mt) ascale[kBuf][mt] = load_code(o.a_codes + kb * o.a_codes_pitch + i0, o.m - i0, 32 * mt + r);
+      for (int mt = 0; mt < kMT; ++mt) ascale[kBuf][mt] = load_code(o.a_codes + kb * o.a_codes_pitch + i0, o.m - i0, 32 * mt + r) | mark;
 #pragma unroll
       for (int nt = 0; nt < kNT; ++nt) {
         if constexpr (kPairs)
-          bscale[kBuf][nt] = load_code((nt & 1 ? o.b2_codes + kb * o.b2_codes_pitch : o.b_codes + kb * o.b_codes_pitch) + j0, o.n - j0, 32 * (nt >> 1) + r);
+          bscale[kBuf][nt] = load_code((nt & 1 ? o.b2_codes + kb * o.b2_codes_pitch : o.b_codes + kb * o.b_codes_pitch) + j0, o.n - j0, 32 * (nt >> 1) + r) | mark;
         else
-          bscale[kBuf][nt] = load_code(o.b_codes + kb * o.b_codes_pitch + j0, o.n - j0, 32 * nt + r);
+          bscale[kBuf][nt] = load_code(o.b_codes + kb * o.b_codes_pitch + j0, o.n - j0, 32 * nt + r) | mark;
       }
     }
   };
@@ -663,14 +665,14 @@ __global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void pro
   constexpr std::integral_constant<int, 0> kBuf0{};
   constexpr std::integral_constant<int, 1> kBuf1{};
   load_tile(kBuf0, 0);
+  load_scales(kBuf0, 0, kRolled ? 0x100 : 0);
   dc::dma_barrier();
   if constexpr (kRowsC) read_b_tile(kBuf0, fb[0]);
   else read_b(kBuf0, 0, fb[0][0]);
   read_a(kBuf0, 0, fa[0]);
   __builtin_amdgcn_sched_barrier(0);
   if (kAlways || kt_count > 1) load_tile(kBuf1, 1);
-  load_scales(kBuf0, 0);
-  load_scales(kBuf1, 1);
+  load_scales(kBuf1, 1, kRolled ? 0x100 : 0);
   // (a macro, so that the fragment arrays stay plain registers)
 #define DC_TILE(BUF, KT)                                                                            \
   {                                                                                                 \
@@ -701,17 +703,34 @@ __global__ __launch_bounds__(64 * WM * WN * KS, (WM * WN == 8 ? 1 : 2)) void pro
       interleave();                                                                                 \
     }                                                                                               \
     __builtin_amdgcn_sched_barrier(0);                                                              \
-    load_scales(kBuf##BUF, (KT) + 2);                                                               \
   }
   constexpr auto kBuf0Other = kBuf1;
   constexpr auto kBuf1Other = kBuf0;
   __builtin_assume(kt_count > 0);
   int kt = 0;
-  do {
-    DC_TILE(0, kt);
-    if (kt + 1 < kt_count) DC_TILE(1, kt + 1);
-    kt += 2;
-  } while (kt < kt_count);
+  if constexpr (kRolled && kBlocks) {
+    // (no branch within two tiles: where one ends, scales loaded on one side of it would be copied, and waited for: 4096×4096×8192 130 us, 124 without;
+    // smaller tiles lose a workgroup of a CU's five to the registers that it takes, 2048^3 17.2 us, 18.5)
+    for (; kt + 1 < kt_count; kt += 2) {
+      DC_TILE(0, kt);
+      load_scales(kBuf0, kt + 2);
+      __builtin_amdgcn_sched_barrier(0);
+      DC_TILE(1, kt + 1);
+      load_scales(kBuf1, kt + 3);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    if (kt < kt_count) DC_TILE(0, kt);
+  } else {
+    do {
+      DC_TILE(0, kt);
+      load_scales(kBuf0, kt + 2);
+      if (kt + 1 < kt_count) {
+        DC_TILE(1, kt + 1);
+        load_scales(kBuf1, kt + 3);
+      }
+      kt += 2;
+    } while (kt < kt_count);
+  }
 #undef DC_TILE
 
   // (after the last tile: loads of zeros, and reads of the other buffer, that nobody uses; all are over beyond this barrier)
