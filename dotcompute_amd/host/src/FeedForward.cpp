@@ -1,4 +1,4 @@
-// FeedForward.cpp — FeedForwardBlock on the HIP accelerator.
+// FeedForward.cpp — what a block keeps, and FeedForwardBlock, on the HIP accelerator.
 #include "DotCompute/FeedForward.hpp"
 
 #include <cstring>
@@ -20,48 +20,50 @@ std::vector<float> Widen(const std::vector<uint16_t>& bits) {
   for (size_t i = 0; i < bits.size(); ++i) v[i] = Widen(bits[i]);
   return v;
 }
-const char* const kShape = "FeedForwardBlock: expected a matrix of ";
 std::string Shape(int64_t rows, int64_t cols) { return std::to_string(rows) + "x" + std::to_string(cols); }
 }  // namespace
 
 template <typename T>
-FeedForwardBlock::Buffer<T> FeedForwardBlock::New(int64_t count) const {
+BlockParameters::Buffer<T> BlockParameters::New(int64_t count) const {
   return hip_->Memory().AllocateAsync<T>((size_t)std::max<int64_t>(count, 1));
 }
+template BlockParameters::Buffer<float> BlockParameters::New(int64_t) const;
+template BlockParameters::Buffer<uint16_t> BlockParameters::New(int64_t) const;
+template BlockParameters::Buffer<uint8_t> BlockParameters::New(int64_t) const;
 
-FeedForwardBlock::FeedForwardBlock(int32_t width, int32_t hidden, Activation activation, IAccelerator& accelerator, float epsilon)
-    : width_(width), hidden_(hidden), activation_(activation), epsilon_(epsilon) {
-  if (width <= 0 || hidden <= 0) throw ArgumentException("FeedForwardBlock: width and hidden must be positive");
-  if (!(epsilon >= 0.0f)) throw ArgumentException("FeedForwardBlock: epsilon must not be negative");
+BlockParameters::BlockParameters(std::string name, int32_t width, int32_t hidden, IAccelerator& accelerator, float epsilon)
+    : name_(std::move(name)), width_(width), hidden_(hidden), epsilon_(epsilon) {
+  if (width <= 0 || hidden <= 0) throw ArgumentException(name_ + ": width and hidden must be positive");
+  if (!(epsilon >= 0.0f)) throw ArgumentException(name_ + ": epsilon must not be negative");
   hip_ = dynamic_cast<HipAccelerator*>(&accelerator);
-  if (!hip_)
-    throw NotSupportedException("FeedForwardBlock runs on HIP accelerators only (got '" + accelerator.Info().DeviceType + "')");
-  const int64_t shapes[kParameters][2] = {{1, width}, {hidden, width}, {1, hidden}, {width, hidden}, {1, width}};
-  for (int i = 0; i < kParameters; ++i) {
-    Tensor& t = p_[(size_t)i];
-    t.rows = shapes[i][0], t.cols = shapes[i][1];
+  if (!hip_) throw NotSupportedException(name_ + " runs on HIP accelerators only (got '" + accelerator.Info().DeviceType + "')");
+}
+
+void BlockParameters::Allocate(const std::vector<BlockParameters::Shape>& shapes) {
+  p_.resize(shapes.size());
+  for (size_t i = 0; i < shapes.size(); ++i) {
+    Tensor& t = p_[i];
+    t.rows = shapes[i].rows, t.cols = shapes[i].cols;
     const int64_t n = t.Size();
     t.value = New<float>(n), t.m = New<float>(n), t.v = New<float>(n), t.copy = New<uint16_t>(n);
-    const bool matrix = i == W1 || i == W2;
-    if (matrix) t.grad_b16 = New<uint16_t>(n);
+    if (shapes[i].matrix) t.grad_b16 = New<uint16_t>(n);
     else t.grad_f32 = New<float>(n);
     for (auto* b : {&t.m, &t.v})
-      Check(dc_hip_memset_async(hip_->Context(), (*b)->Data(), 0, (size_t)n * sizeof(float)), "FeedForwardBlock: states");
-    Set((Parameter)i, std::vector<float>((size_t)n, i == NormWeight ? 1.0f : 0.0f));
+      Check(dc_hip_memset_async(hip_->Context(), (*b)->Data(), 0, (size_t)n * sizeof(float)), (name_ + ": states").c_str());
+    SetValues((int)i, std::vector<float>((size_t)n, shapes[i].start));
   }
 }
 
-void FeedForwardBlock::Set(Parameter parameter, const std::vector<float>& values) {
+void BlockParameters::SetValues(int parameter, const std::vector<float>& values) {
   Tensor& t = p_.at((size_t)parameter);
   if ((int64_t)values.size() != t.Size())
-    throw ArgumentException("FeedForwardBlock: a parameter of " + std::to_string(t.Size()) + " values was given " +
-                            std::to_string(values.size()));
+    throw ArgumentException(name_ + ": a parameter of " + std::to_string(t.Size()) + " values was given " + std::to_string(values.size()));
   has_forward_ = quantized_ = false;  // (both belong to the values before)
   t.value->CopyFromHost(values.data(), values.size() * sizeof(float));
-  Check(dc_hip_convert_f32_to_bf16(hip_->Context(), t.value->Data(), t.copy->Data(), t.Size()), "FeedForwardBlock: convert");
+  Check(dc_hip_convert_f32_to_bf16(hip_->Context(), t.value->Data(), t.copy->Data(), t.Size()), (name_ + ": convert").c_str());
 }
 
-std::vector<float> FeedForwardBlock::Get(Parameter parameter) const {
+std::vector<float> BlockParameters::Values(int parameter) const {
   const Tensor& t = p_.at((size_t)parameter);
   std::vector<float> v((size_t)t.Size());
   hip_->Synchronize();
@@ -69,8 +71,8 @@ std::vector<float> FeedForwardBlock::Get(Parameter parameter) const {
   return v;
 }
 
-std::vector<float> FeedForwardBlock::Gradient(Parameter parameter) const {
-  if (!has_gradient_) throw InvalidOperationException("FeedForwardBlock: no gradients yet");
+std::vector<float> BlockParameters::GradientOf(int parameter) const {
+  if (!has_gradient_) throw InvalidOperationException(name_ + ": no gradients yet");
   const Tensor& t = p_.at((size_t)parameter);
   hip_->Synchronize();
   if (t.grad_f32) {
@@ -83,16 +85,59 @@ std::vector<float> FeedForwardBlock::Gradient(Parameter parameter) const {
   return Widen(bits);
 }
 
-void FeedForwardBlock::RequireInput(const Matrix& x) const {
-  if (x.Columns() != width_) throw ArgumentException(kShape + ("rows of " + std::to_string(width_)));
+void BlockParameters::RequireInput(const Matrix& x) const {
+  if (x.Columns() != width_) throw ArgumentException(name_ + ": expected a matrix of rows of " + std::to_string(width_));
 }
 
-FeedForwardBlock::Buffer<uint16_t> FeedForwardBlock::ToBf16(const Matrix& x) const {
+void BlockParameters::RequireBackward(const Matrix& dy) const {
+  if (!has_forward_) throw InvalidOperationException(name_ + ": Backward follows a Forward with the current parameters");
+  if (dy.Rows() != rows_ || dy.Columns() != width_) throw ArgumentException(name_ + ": expected a matrix of " + Algorithms::Shape(rows_, width_));
+}
+
+BlockParameters::Buffer<uint16_t> BlockParameters::ToBf16(const Matrix& x) const {
   auto wide = New<float>(x.Size());
   auto bits = New<uint16_t>(x.Size());
   if (x.Size() > 0) wide->CopyFromHost(x.Data().data(), (size_t)x.Size() * sizeof(float));
-  Check(dc_hip_convert_f32_to_bf16(hip_->Context(), wide->Data(), bits->Data(), x.Size()), "FeedForwardBlock: convert");
+  Check(dc_hip_convert_f32_to_bf16(hip_->Context(), wide->Data(), bits->Data(), x.Size()), (name_ + ": convert").c_str());
   return bits;
+}
+
+Matrix BlockParameters::Result(const Buffer<float>& y, int32_t rows) const {
+  Matrix out(rows, width_);
+  hip_->Synchronize();
+  if (out.Size() > 0) y->CopyToHost(out.Data().data(), (size_t)out.Size() * sizeof(float));
+  return out;
+}
+
+Matrix BlockParameters::Result(const Buffer<uint16_t>& y, int32_t rows) const {
+  std::vector<uint16_t> bits((size_t)rows * (size_t)width_);
+  hip_->Synchronize();
+  if (!bits.empty()) y->CopyToHost(bits.data(), bits.size() * sizeof(uint16_t));
+  return Matrix(rows, width_, Widen(bits));
+}
+
+void BlockParameters::Step(const AdamWOptions& options) {
+  if (!has_gradient_ || stepped_) throw InvalidOperationException(name_ + ": Step follows Backward");
+  dc_adamw args{};
+  args.lr = options.LearningRate, args.beta1 = options.Beta1, args.beta2 = options.Beta2, args.eps = options.Epsilon;
+  args.weight_decay = options.WeightDecay, args.grad_scale = 1.0, args.step = steps_ + 1, args.state_dtype = DC_DTYPE_F32;
+  std::vector<dc_adamw_tensor> tensors(p_.size());
+  for (size_t i = 0; i < p_.size(); ++i) {
+    Tensor& t = p_[i];
+    dc_adamw_tensor& a = tensors[i];
+    a.param = t.value->Data(), a.m = t.m->Data(), a.v = t.v->Data(), a.copy = t.copy->Data(), a.n = t.Size();
+    a.grad = t.grad_f32 ? static_cast<const void*>(t.grad_f32->Data()) : t.grad_b16->Data();
+    a.grad_dtype = t.grad_f32 ? DC_DTYPE_F32 : DC_DTYPE_BF16;
+  }
+  Check(dc_hip_adamw_step(hip_->Context(), &args, tensors.data(), (int32_t)tensors.size()), "dc_hip_adamw_step");
+  ++steps_;
+  has_forward_ = quantized_ = false;
+  stepped_ = true;
+}
+
+FeedForwardBlock::FeedForwardBlock(int32_t width, int32_t hidden, Activation activation, IAccelerator& accelerator, float epsilon)
+    : BlockParameters("FeedForwardBlock", width, hidden, accelerator, epsilon), activation_(activation) {
+  Allocate({{false, 1, width, 1.0f}, {true, hidden, width, 0.0f}, {false, 1, hidden, 0.0f}, {true, width, hidden, 0.0f}, {false, 1, width, 0.0f}});
 }
 
 Matrix FeedForwardBlock::Forward(const Matrix& x) {
@@ -125,17 +170,14 @@ Matrix FeedForwardBlock::Forward(const Matrix& x) {
   down.x_stride = down.w_stride = h, down.residual_stride = down.y_stride = d;
   Check(dc_hip_linear(hip_->Context(), &down), "dc_hip_linear");
 
-  Matrix out(x.Rows(), width_);
-  hip_->Synchronize();
-  if (out.Size() > 0) y->CopyToHost(out.Data().data(), (size_t)out.Size() * sizeof(float));
+  Matrix out = Result(y, x.Rows());
   rows_ = x.Rows();
   has_forward_ = true;
   return out;
 }
 
 Matrix FeedForwardBlock::Backward(const Matrix& dy) {
-  if (!has_forward_) throw InvalidOperationException("FeedForwardBlock: Backward follows a Forward with the current parameters");
-  if (dy.Rows() != rows_ || dy.Columns() != width_) throw ArgumentException(kShape + Shape(rows_, width_));
+  RequireBackward(dy);
   const int64_t rows = rows_, d = width_, h = hidden_;
   has_gradient_ = false;  // (until all of them are of this dy)
   auto g = ToBf16(dy);
@@ -167,29 +209,7 @@ Matrix FeedForwardBlock::Backward(const Matrix& dy) {
   has_gradient_ = true;
   stepped_ = false;
 
-  std::vector<uint16_t> bits((size_t)(rows * d));
-  hip_->Synchronize();
-  if (!bits.empty()) dx->CopyToHost(bits.data(), bits.size() * sizeof(uint16_t));
-  return Matrix(rows_, width_, Widen(bits));
-}
-
-void FeedForwardBlock::Step(const AdamWOptions& options) {
-  if (!has_gradient_ || stepped_) throw InvalidOperationException("FeedForwardBlock: Step follows Backward");
-  dc_adamw args{};
-  args.lr = options.LearningRate, args.beta1 = options.Beta1, args.beta2 = options.Beta2, args.eps = options.Epsilon;
-  args.weight_decay = options.WeightDecay, args.grad_scale = 1.0, args.step = steps_ + 1, args.state_dtype = DC_DTYPE_F32;
-  dc_adamw_tensor tensors[kParameters] = {};
-  for (int i = 0; i < kParameters; ++i) {
-    Tensor& t = p_[(size_t)i];
-    dc_adamw_tensor& a = tensors[i];
-    a.param = t.value->Data(), a.m = t.m->Data(), a.v = t.v->Data(), a.copy = t.copy->Data(), a.n = t.Size();
-    a.grad = t.grad_f32 ? static_cast<const void*>(t.grad_f32->Data()) : t.grad_b16->Data();
-    a.grad_dtype = t.grad_f32 ? DC_DTYPE_F32 : DC_DTYPE_BF16;
-  }
-  Check(dc_hip_adamw_step(hip_->Context(), &args, tensors, kParameters), "dc_hip_adamw_step");
-  ++steps_;
-  has_forward_ = quantized_ = false;
-  stepped_ = true;
+  return Result(dx, rows_);
 }
 
 Matrix FeedForwardBlock::ForwardFp8(const Matrix& x) {
@@ -233,10 +253,7 @@ Matrix FeedForwardBlock::ForwardFp8(const Matrix& x) {
   down.x_stride = down.w_stride = h, down.residual_stride = down.y_stride = d;
   Check(dc_hip_linear(hip_->Context(), &down), "dc_hip_linear");
 
-  Matrix out(x.Rows(), width_);
-  hip_->Synchronize();
-  if (out.Size() > 0) y->CopyToHost(out.Data().data(), (size_t)out.Size() * sizeof(float));
-  return out;
+  return Result(y, x.Rows());
 }
 
 }  // namespace DotCompute::Algorithms
