@@ -2,10 +2,12 @@
 
     n1 = norm(x)   z = n1 W1^T + b1   a = silu(z)   s = x + a W2^T + b2   n2 = norm(s)   y = n2 H^T
 
+or, with --gated, layer norms in place of RMS norms and a gate: g = n1 Wg^T + bg   u = n1 Wu^T + bu   a = silu(g) u.
+
 Training runs the products in bf16 and steps float32 parameters with AdamW on 8-bit states. The head's epilogue subtracts the
 target (it is the head's residual with the sign turned), so that its result is the error e, which is also the gradient of
 the loss |e|^2 / 2 by y: no other kernel is needed. Serving runs the same block on a few rows with the weights, and what the
-norms write, in 8 bits.
+norms write, in 8 bits: with a scale a row, or, of a gated block, for each 128 of a row.
 
     python -m dotcompute_amd.examples.feed_forward --rows 4096 --width 1024 --hidden 4096 --steps 100
 """
@@ -33,11 +35,12 @@ def from_bf16(b: np.ndarray) -> np.ndarray:
 class Model:
     """The parameters in float32, their bf16 copies, gradients and AdamW states."""
 
-    def __init__(self, ctx: hip.Context, width: int, hidden: int, outputs: int, seed: int = 0):
-        self.ctx, self.width, self.hidden, self.outputs = ctx, width, hidden, outputs
+    def __init__(self, ctx: hip.Context, width: int, hidden: int, outputs: int, seed: int = 0, gated: bool = False):
+        self.ctx, self.width, self.hidden, self.outputs, self.gated = ctx, width, hidden, outputs, gated
         rng = np.random.default_rng(seed)
-        shapes = {"norm1": (width,), "w1": (hidden, width), "b1": (hidden,), "w2": (width, hidden), "b2": (width,), "norm2": (width,),
-                  "head": (outputs, width)}
+        up = {"wg": (hidden, width), "bg": (hidden,), "wu": (hidden, width), "bu": (hidden,)} if gated else {"w1": (hidden, width), "b1": (hidden,)}
+        shifts = {"shift1": (width,), "shift2": (width,)} if gated else {}
+        shapes = {"norm1": (width,), **up, "w2": (width, hidden), "b2": (width,), "norm2": (width,), "head": (outputs, width), **shifts}
         self.copy, self.grad, parts = {}, {}, []
         for name, shape in shapes.items():
             if len(shape) == 2:
@@ -71,6 +74,25 @@ class Trainer:
         self.x, target = ctx.to_device(x), ctx.to_device(target ^ np.uint16(0x8000))
         n1, z, a, branch, s, n2 = bf16(d), bf16(h), bf16(h), bf16(d), bf16(d), bf16(d)
         self.error, dn2, ds, da, dn1 = bf16(o), bf16(d), bf16(d), bf16(h), bf16(d)
+        if model.gated:
+            u = bf16(h)
+            self.forward = [
+                (ctx.layer_norm, hip.LayerNorm.of(self.x, p["norm1"], p["shift1"], n1)),
+                (ctx.gated_linear, hip.GatedLinear.of(n1, p["wg"], p["wu"], a, bias_gate=p["bg"], bias_up=p["bu"], pre_gate=z, pre_up=u,
+                                                      activation=ACTIVATION)),
+                (ctx.linear, hip.Linear.of(a, p["w2"], branch, bias=p["b2"])),
+                (ctx.layer_norm, hip.LayerNorm.of(branch, p["norm2"], p["shift2"], n2, residual=self.x, sum=s)),
+                (ctx.linear, hip.Linear.of(n2, p["head"], self.error, residual=target)),
+            ]
+            self.backward = [
+                (ctx.linear_backward, hip.LinearGrad.of(self.error, n2, p["head"], dx=dn2, dw=g["head"])),
+                (ctx.layer_norm_backward, hip.LayerNormGrad.of(dn2, s, p["norm2"], dx=ds, dweight=g["norm2"], dbias=g["shift2"])),
+                (ctx.linear_backward, hip.LinearGrad.of(ds, a, p["w2"], dx=da, dw=g["w2"], dbias=g["b2"])),
+                (ctx.gated_linear_backward, hip.GatedLinearGrad.of(da, n1, p["wg"], p["wu"], z, u, dx=dn1, dw_gate=g["wg"], dw_up=g["wu"],
+                                                                   dbias_gate=g["bg"], dbias_up=g["bu"], activation=ACTIVATION)),
+                (ctx.layer_norm_backward, hip.LayerNormGrad.of(dn1, self.x, p["norm1"], dweight=g["norm1"], dbias=g["shift1"])),
+            ]
+            return
         self.forward = [
             (ctx.rms_norm, hip.RmsNorm.of(self.x, p["norm1"], n1)),
             (ctx.linear, hip.Linear.of(n1, p["w1"], a, bias=p["b1"], pre=z, activation=ACTIVATION)),
@@ -106,6 +128,9 @@ class Server:
         bf16 = lambda cols: ctx.empty((rows, cols), np.uint16)  # noqa: E731
         self.ctx, self.x, self.y = ctx, bf16(d), ctx.empty((rows, o), np.float32)
         a, branch, s = bf16(h), bf16(d), bf16(d)
+        if model.gated:
+            self.calls = self._gated_fp8(model, rows, a, branch, s) if fp8 else self._gated(model, a, branch, s, bf16(d), bf16(d))
+            return
         if not fp8:
             n1, n2 = bf16(d), bf16(d)
             self.calls = [
@@ -128,6 +153,33 @@ class Server:
             (ctx.linear, (hip.Linear.of(aq, w["w2"][0], branch, bias=p["b2"], x_scales=sa, w_scales=w["w2"][1]),)),
             (ctx.rms_norm, (hip.RmsNorm.of(branch, p["norm2"], n2, residual=self.x, sum=s, scales=s2),)),
             (ctx.linear, (hip.Linear.of(n2, w["head"][0], self.y, x_scales=s2, w_scales=w["head"][1]),)),
+        ]
+
+    def _gated(self, model: Model, a, branch, s, n1, n2) -> list:
+        ctx, p = model.ctx, model.copy
+        return [
+            (ctx.layer_norm, (hip.LayerNorm.of(self.x, p["norm1"], p["shift1"], n1),)),
+            (ctx.gated_linear, (hip.GatedLinear.of(n1, p["wg"], p["wu"], a, bias_gate=p["bg"], bias_up=p["bu"], activation=ACTIVATION),)),
+            (ctx.linear, (hip.Linear.of(a, p["w2"], branch, bias=p["b2"]),)),
+            (ctx.layer_norm, (hip.LayerNorm.of(branch, p["norm2"], p["shift2"], n2, residual=self.x, sum=s),)),
+            (ctx.linear, (hip.Linear.of(n2, p["head"], self.y),)),
+        ]
+
+    def _gated_fp8(self, model: Model, rows: int, a, branch, s) -> list:
+        ctx, p, d, h = model.ctx, model.copy, model.width, model.hidden
+        codes = lambda r, c: (ctx.empty((r, c), np.uint8), ctx.empty((hip.scale_blocks(c), r), np.uint8))  # noqa: E731
+        w = {name: codes(*p[name].shape) for name in ("wg", "wu", "w2", "head")}
+        for name, (q, scales) in w.items():
+            ctx.quantize_fp8_blocks(p[name], q, scales)
+        (n1, s1), (aq, sa), (n2, s2) = codes(rows, d), codes(rows, h), codes(rows, d)
+        return [
+            (ctx.layer_norm, (hip.LayerNorm.of(self.x, p["norm1"], p["shift1"], n1, scales=s1),)),
+            (ctx.gated_linear, (hip.GatedLinear.of(n1, w["wg"][0], w["wu"][0], a, bias_gate=p["bg"], bias_up=p["bu"], x_scales=s1,
+                                                   gate_scales=w["wg"][1], up_scales=w["wu"][1], activation=ACTIVATION),)),
+            (ctx.quantize_fp8_blocks, (a, aq, sa)),
+            (ctx.linear_blocks, (hip.LinearBlocks.of(aq, w["w2"][0], sa, w["w2"][1], branch, bias=p["b2"]),)),
+            (ctx.layer_norm, (hip.LayerNorm.of(branch, p["norm2"], p["shift2"], n2, residual=self.x, sum=s, scales=s2),)),
+            (ctx.linear_blocks, (hip.LinearBlocks.of(n2, w["head"][0], s2, w["head"][1], self.y),)),
         ]
 
     def run(self) -> None:
@@ -153,9 +205,10 @@ def main() -> None:
     for name, value in (("rows", 4096), ("width", 1024), ("hidden", 4096), ("outputs", 256), ("steps", 100), ("serve", 8)):
         args.add_argument("--" + name, type=int, default=value)
     args.add_argument("--lr", type=float, default=1e-3)
+    args.add_argument("--gated", action="store_true")
     o = args.parse_args()
     with hip.Context() as ctx:
-        model = Model(ctx, o.width, o.hidden, o.outputs)
+        model = Model(ctx, o.width, o.hidden, o.outputs, gated=o.gated)
         x, target = data(o.rows, o.width, o.outputs)
         trainer = Trainer(model, x, target)
         for t in range(o.steps + 1):
