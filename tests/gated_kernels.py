@@ -14,6 +14,8 @@ FORWARD = [
     ("256", 1767, 2989, 406, "fp8"),
 ]
 FORWARD += [(name, m, n, k, "blocks") for name, m, n, k, dtype in FORWARD if dtype == "fp8"]
+# Products with block scales of few rows: 32 outputs to a workgroup, of eight waves and of four (m, n, k)
+BLOCKS = [(5, 4109, 400), (12, 4133, 432), (21, 4201, 400), (30, 4150, 432), (7, 8301, 400), (12, 8437, 208), (21, 8644, 1300), (30, 8247, 2211)]
 # m, n, k
 GRADIENTS = [
     ("64", 33, 62, 200), ("64/a", 1, 410, 8), ("64/b", 812, 4, 8), ("64/a/b", 772, 66, 10), ("64x2", 1, 65, 8), ("64x2/a", 1, 2044, 8),

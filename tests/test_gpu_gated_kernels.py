@@ -2,7 +2,7 @@
 tests/linear_kernels.py), against float64. Tolerances are those of tests/test_gpu_gated.py."""
 import pytest
 
-from gated_kernels import FORWARD, GRADIENTS
+from gated_kernels import BLOCKS, FORWARD, GRADIENTS
 from linear_kernels import FORWARD as LINEAR
 from test_gpu_gated import run_blocks, run_gated, run_gated_backward
 
@@ -28,3 +28,9 @@ def test_gradients(ctx, kernel, m, n, k):
 def test_blocks(ctx, kernel, m, n, k):
     run_blocks(ctx, m, n, k, "silu", residual=True)
     run_blocks(ctx, m, n, k, "relu", bias=False, residual=True, in_place=True)
+
+
+@pytest.mark.parametrize("m,n,k", BLOCKS)
+def test_blocks_of_few_rows(ctx, m, n, k):
+    run_blocks(ctx, m, n, k, "silu", residual=True, odd=1)
+    run_blocks(ctx, m, n, k, "none", "f32")

@@ -51,7 +51,8 @@ def check_blocks(q, scales, y, bound):
 
 # Rows by shape of the kernel: a wave a row (many short rows), 4 and 16 waves a row, rows read again; odd lengths among them.
 SHAPES = [(1, 1), (1, 64), (3, 7), (5, 2050), (2, 4096), (7, 3333), (2, 8191), (3, 16384), (2, 30001), (1, 65536), (2, 66001),
-          (2049, 100), (2048, 513), (2050, 2047), (2051, 4096), (5, 256), (6, 257), (9, 512), (1030, 1001), (2, 1024), (5, 1025)]
+          (2049, 100), (2048, 513), (2050, 2047), (2051, 4096), (5, 256), (6, 257), (9, 512), (1030, 1001), (2, 1024), (5, 1025),
+          (300, 6001), (270, 12001), (260, 16384), (256, 4100), (257, 4100)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
@@ -152,7 +153,8 @@ def test_layer_norm_of_flat_rows_infinities_and_nan(ctx):
 
 
 GRAD_SHAPES = [(1, 1), (1, 300), (4, 7), (1500, 512), (1031, 2050), (9, 4096), (5, 8192), (3, 20001), (2, 32768), (3, 40001), (600, 2052),
-               (300, 4097), (530, 8192), (300, 8197), (520, 16381), (270, 16384), (260, 16385)]
+               (300, 4097), (530, 8192), (300, 8197), (520, 16381), (270, 16384), (260, 16385), (1027, 1030), (4099, 130), (257, 513), (700, 1601),
+               (515, 2816), (1300, 3000), (9000, 8)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
