@@ -215,7 +215,7 @@ DC_HIP_API int32_t dc_hip_gated_linear_backward(dc_hip_ctx* ctx, const dc_gated_
   const dc::LinearSize dw_size{p.n, p.k, 2 * p.m, 2 * s.t_pitch, x.width()}, dws_size{dws * p.n, p.k, 2 * p.m, 2 * s.t_pitch, x.width()};
   dc::LinearPlan dx_best{dc::LinearTile::k64, {1, 1}, 0.0}, dw_best = dx_best;
   if (dx && dw) {
-    const dc::LinearPair pair = dc::linear_plan_of_two(dx_size, dws_size, cus);
+    const dc::LinearPair pair = dc::linear_plan_of_two(dx_size, dws_size, cus, true);
     dx_best = {pair.tile, pair.a, pair.time}, dw_best = {pair.tile, pair.b, pair.time};
   } else if (dx) {
     dx_best = dc::linear_plan(dx_size, {true, false}, cus);

@@ -150,7 +150,9 @@ struct LinearPair {
   LinearSplit a, b;
   double time;
 };
-inline LinearPair linear_plan_of_two(const LinearSize& a, const LinearSize& b, int64_t cus) {
+// `fewer` (the gradients of a gated layer, where b is both weights'): the shorter c in one part less is tried too, which leaves its workgroups longer than the longer
+// one's. Both gradients of 2000,2504,1000 92 us, with it 81 (256-tiles, 3 and 1 parts).
+inline LinearPair linear_plan_of_two(const LinearSize& a, const LinearSize& b, int64_t cus, bool fewer = false) {
   const bool longer = a.c_bytes >= b.c_bytes;
   const LinearSize &l = longer ? a : b, &s = longer ? b : a;
   const LinearKind kind{true, false};
@@ -160,16 +162,20 @@ inline LinearPair linear_plan_of_two(const LinearSize& a, const LinearSize& b, i
     const int64_t tl = linear_tiles(l, t), ts = linear_tiles(s, t), all = linear_split(t, s, 1).turns;
     for (int64_t parts : kLinearParts) {
       if (parts > 1 && (l.c_bytes < 1024 || l.c_bytes < 256 * parts * linear_tile_groups(t) || tl * (parts - 1) > 4 * cus)) break;
-      const LinearSplit sl = linear_split(t, l, parts), ss = linear_split(t, s, (all + sl.turns - 1) / sl.turns);
-      const int64_t gl = tl * sl.parts, gs = ts * ss.parts;
-      const double el = (double)sl.turns, es = (double)ss.turns, turns = el > es ? el : es;
-      const double equal = ((double)gl * el + (double)gs * es) / turns / (double)cus;
-      const bool one = kLinearHeld[linear_side_index(t)][linear_group_index(t)] == 1;
-      const double most = !one ? linear_up(equal) : (el >= es ? linear_last(gl, el, gs, es, cus) : linear_last(gs, es, gl, el, cus)) / turns;
-      const double time = linear_time(t, kind, (double)(gl + gs), turns, most, equal, (double)cus, false) +
-                          linear_parts_time(l, kind, sl.parts) + linear_parts_time(s, kind, ss.parts) +
-                          (sl.parts > 1 || ss.parts > 1 ? kLinearRowsC.join : 0.0);
-      if (time < best.time) best = longer ? LinearPair{t, sl, ss, time} : LinearPair{t, ss, sl, time};
+      const LinearSplit sl = linear_split(t, l, parts);
+      const int64_t most_parts = (all + sl.turns - 1) / sl.turns;
+      for (int64_t short_parts = most_parts; short_parts >= 1 && short_parts >= most_parts - (fewer ? 1 : 0); --short_parts) {
+        const LinearSplit ss = linear_split(t, s, short_parts);
+        const int64_t gl = tl * sl.parts, gs = ts * ss.parts;
+        const double el = (double)sl.turns, es = (double)ss.turns, turns = el > es ? el : es;
+        const double equal = ((double)gl * el + (double)gs * es) / turns / (double)cus;
+        const bool one = kLinearHeld[linear_side_index(t)][linear_group_index(t)] == 1;
+        const double most = !one ? linear_up(equal) : (el >= es ? linear_last(gl, el, gs, es, cus) : linear_last(gs, es, gl, el, cus)) / turns;
+        const double time = linear_time(t, kind, (double)(gl + gs), turns, most, equal, (double)cus, false) +
+                            linear_parts_time(l, kind, sl.parts) + linear_parts_time(s, kind, ss.parts) +
+                            (sl.parts > 1 || ss.parts > 1 ? kLinearRowsC.join : 0.0);
+        if (time < best.time) best = longer ? LinearPair{t, sl, ss, time} : LinearPair{t, ss, sl, time};
+      }
     }
   }
   return best;

@@ -21,5 +21,5 @@ GRADIENTS = [
     ("64", 33, 62, 200), ("64/a", 1, 410, 8), ("64/b", 812, 4, 8), ("64/a/b", 772, 66, 10), ("64x2", 1, 65, 8), ("64x2/a", 1, 2044, 8),
     ("64x2/b", 5378, 3, 8), ("64x2/a/b", 398, 636, 125), ("128", 199, 74, 7187), ("128/a", 66, 876, 2073), ("128/b", 2195, 139, 1022),
     ("128/a/b", 2739, 1557, 69), ("256", 399, 221, 8727), ("256/a", 129, 2761, 1597), ("256/b", 2564, 69, 2988),
-    ("256/a/b", 2154, 3899, 130),
+    ("256/a/b", 2137, 4299, 131),
 ]

@@ -29,7 +29,7 @@ static std::string forward(int64_t m, int64_t n, int64_t k, bool fp8) {
 }
 static std::string gradients(int64_t m, int64_t n, int64_t k) {
   const int64_t pitch = 2 * padded(k, 8), dz = 4 * padded(n, 64);
-  const LinearPair q = linear_plan_of_two({m, k, dz, dz, pitch}, {2 * n, k, 2 * m, 2 * padded(m, 8), pitch}, 256);
+  const LinearPair q = linear_plan_of_two({m, k, dz, dz, pitch}, {2 * n, k, 2 * m, 2 * padded(m, 8), pitch}, 256, true);
   return tile(q.tile) + (q.a.parts > 1 ? "/a" : "") + (q.b.parts > 1 ? "/b" : "");
 }
 int main() {
