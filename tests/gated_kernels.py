@@ -3,13 +3,13 @@ backward call pick, tests/test_gpu_gated_kernels.py runs them. Names as in tests
 gradients /a where workgroups share dx's sums, /b where they share the weights'."""
 FORWARD = [
     ("few1", 1, 62, 198, "bf16"), ("few2", 10, 64, 195, "bf16"), ("few3", 18, 60, 202, "bf16"), ("few4", 26, 60, 214, "bf16"),
-    ("few8", 35, 60, 196, "bf16"), ("64", 276, 415, 199, "bf16"), ("64/split", 267, 437, 1633, "bf16"), ("64x2", 333, 353, 478, "bf16"),
-    ("64x2/split", 347, 448, 2427, "bf16"), ("64x4", 276, 416, 1210, "bf16"), ("128", 1499, 1341, 387, "bf16"),
+    ("few8", 35, 60, 196, "bf16"), ("few8", 276, 415, 199, "bf16"), ("64", 445, 578, 197, "bf16"), ("64/split", 326, 677, 2372, "bf16"), ("64x2", 612, 405, 450, "bf16"),
+    ("64x2/split", 451, 612, 2594, "bf16"), ("64x4", 455, 522, 1188, "bf16"), ("128", 1499, 1341, 387, "bf16"),
     ("128/split", 321, 805, 4671, "bf16"), ("128x2", 851, 1809, 982, "bf16"), ("128x2/split", 398, 896, 3924, "bf16"),
     ("256", 1348, 3742, 193, "bf16"), ("256/split", 138, 5807, 7230, "bf16"),
     ("few1", 3, 60, 397, "fp8"), ("few2", 11, 60, 387, "fp8"), ("few3", 19, 62, 419, "fp8"), ("few4", 29, 63, 392, "fp8"),
-    ("few8", 39, 60, 392, "fp8"), ("64", 212, 541, 398, "fp8"), ("64/split", 202, 530, 3100, "fp8"), ("64x2", 321, 368, 915, "fp8"),
-    ("64x2/split", 570, 280, 4658, "fp8"), ("64x4", 277, 446, 2317, "fp8"), ("128", 1660, 1937, 395, "fp8"),
+    ("few8", 39, 60, 392, "fp8"), ("few8", 212, 541, 398, "fp8"), ("64", 390, 595, 391, "fp8"), ("64/split", 327, 713, 4630, "fp8"), ("64x2", 386, 605, 898, "fp8"),
+    ("64x2/split", 326, 747, 5356, "fp8"), ("64x4", 675, 375, 2348, "fp8"), ("128", 1660, 1937, 395, "fp8"),
     ("128/split", 214, 1593, 6659, "fp8"), ("128x2", 783, 2069, 1755, "fp8"), ("128x2/split", 758, 687, 6558, "fp8"),
     ("256", 1767, 2989, 406, "fp8"),
 ]

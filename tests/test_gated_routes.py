@@ -23,7 +23,7 @@ static std::string tile(LinearTile t) {
 }
 static std::string forward(int64_t m, int64_t n, int64_t k, bool fp8) {
   const int64_t c = k * (fp8 ? 1 : 2), pitch = padded(c, 16);
-  if (linear_few_rows(m, 2 * n, 256)) return "few" + std::to_string(m > 32 ? 8 : (m + 7) / 8);
+  if (linear_few_rows(m, n, 256)) return "few" + std::to_string(m > 32 ? 8 : (m + 7) / 8);
   const LinearPlan p = linear_plan({m, 2 * n, c, pitch, pitch}, {false, fp8}, 256);
   return tile(p.tile) + (p.split.parts > 1 ? "/split" : "");
 }
