@@ -173,7 +173,8 @@ __device__ inline RowStats own_stats(const Moments& m, float per, float eps) {
 
 typedef float f32x4_lds __attribute__((ext_vector_type(4)));
 
-// A row a workgroup; or, where a wave holds a row, one for each of its four waves. 8 bits: a scale a row, or (kBlocks) one for each 128.
+// A workgroup walks over rows, one at a time, or, where a wave holds a row, four; the weights stay in registers, and the next row's operands are asked for before
+// this one's sums. (`sum` and y may lie over x or the residual: a workgroup writes a row after it has read it, and reads no other's.) 8 bits: a scale a row, or (kBlocks) one for each 128.
 template <typename T, typename Y, int C, bool kBlocks>
 __global__ __launch_bounds__(1024) void layer_norm_kernel(LayerNormArgs a, int waves) {
   constexpr int E = kElems<T>;
@@ -189,14 +190,20 @@ __global__ __launch_bounds__(1024) void layer_norm_kernel(LayerNormArgs a, int w
   clear_words(scratch, 1, waves);
   const int per = waves == 1 ? 4 : 1;
   const int64_t step = (int64_t)gridDim.x * per;
-  for (int64_t row = (int64_t)blockIdx.x * per + (waves == 1 ? group : 0); row < a.rows; row += step) {
-    T* sum = a.sum ? static_cast<T*>(a.sum) + row * a.sum_stride : nullptr;
-    Y* y = static_cast<Y*>(a.y) + row * a.y_stride;
-    u32x4 xr[C], rr[C], wr[C], br[C];
+  u32x4 xr[C], rr[C], wr[C], br[C];
+  auto load = [&](int64_t row) __attribute__((always_inline)) {
     R.load(static_cast<const T*>(a.x) + row * a.x_stride, xr);
     if (a.residual) R.load(static_cast<const T*>(a.residual) + row * a.residual_stride, rr);
-    R.load(static_cast<const T*>(a.weight), wr);
-    if (a.bias) R.load(static_cast<const T*>(a.bias), br);
+  };
+  const int64_t first = (int64_t)blockIdx.x * per + (waves == 1 ? group : 0);
+  if (first < a.rows) load(first);
+  R.load(static_cast<const T*>(a.weight), wr);
+  if (a.bias) R.load(static_cast<const T*>(a.bias), br);
+  R.cut(wr);
+  if (a.bias) R.cut(br);
+  for (int64_t row = first; row < a.rows; row += step) {
+    T* sum = a.sum ? static_cast<T*>(a.sum) + row * a.sum_stride : nullptr;
+    Y* y = static_cast<Y*>(a.y) + row * a.y_stride;
     R.cut(xr);
     if (a.residual) R.cut(rr);
     float h[C][E];
@@ -210,6 +217,7 @@ __global__ __launch_bounds__(1024) void layer_norm_kernel(LayerNormArgs a, int w
 #pragma unroll
         for (int e = 0; e < E; ++e) h[i][e] += u[e];
       }
+    if (row + step < a.rows) load(row + step);
     if (sum)
 #pragma unroll
       for (int i = 0; i < C; ++i) R.store(sum, i, h[i]);
@@ -229,8 +237,6 @@ __global__ __launch_bounds__(1024) void layer_norm_kernel(LayerNormArgs a, int w
       }
       r = join_moments(q, n_other, m.near, per_col, a.eps).row;
     }
-    R.cut(wr);
-    if (a.bias) R.cut(br);
 #pragma unroll
     for (int i = 0; i < C; ++i) {
       float w[E], b[E];
@@ -680,22 +686,22 @@ __global__ __launch_bounds__(256) void quantize_blocks_kernel(QuantizeArgs a) {
 // ---- host --------------------------------------------------------------------------------------------------
 template <typename T, typename Y, int C, bool kBlocks>
 int32_t launch_norm(dc_hip_ctx* ctx, const LayerNormArgs& a, int64_t chunks) {
-  const int waves = waves_for(chunks, C);
-  const int64_t groups = waves == 1 ? (a.rows + 3) / 4 : a.rows;
-  layer_norm_kernel<T, Y, C, kBlocks>
-      <<<(unsigned)std::min(groups, kMaxGrid), waves == 1 ? 256 : 64 * waves, 0, ctx->stream>>>(a, waves);
+  const int waves = waves_for(chunks, C), group = waves == 1 ? 4 : waves;  // (16 waves to a CU)
+  const int64_t groups = waves == 1 ? (a.rows + 3) / 4 : a.rows, held = (int64_t)std::max(1, ctx->cu_count) * std::max(1, kWaves / group);
+  layer_norm_kernel<T, Y, C, kBlocks><<<(unsigned)std::min(groups, held), 64 * group, 0, ctx->stream>>>(a, waves);
   return last_launch_status();
 }
 
-// Chunks that a lane holds: two where rows are long, or where they let a wave hold a row by itself (but not where they are read and written in
-// float32); one, over up to 16 waves, where every row has a CU of its own, as only its latency counts then. us, with the call, for one / two: bf16
-// 16384×4096 95.8 / 95.8, to 8 bits 103.6 / 98.8, 8191×2050 38.4 / 34.9; 8×4096 to 8 bits 4.31 / 4.78. Four, for rows of 16 waves, spill: 2048×24576
+// Chunks that a lane holds: one of bf16, over up to 16 waves; two where they let a wave hold a row by itself (but not where it is read and written in float32),
+// and in longer rows. us, with the call, for a workgroup to each row with one to two chunks / workgroups that walk with two / with one, bf16: 16384×4096 95.6 /
+// 103 / 96.0, to 8 bits 98.7 / 93.1 / 94.0; 8191×2050 34.8 / 29.8 / 28.0; 4096×8192 55.7 / 48.5 / 48.6; 2000×12000 53 / 38; 1000×4096 8.6 / 8.5 / 7.6; float32
+// 8192×2048 48.3 / 48.5 / 50.3. With 24 waves a CU 16384×4096 takes 101, with 32 108. Four chunks, for rows of more than 16 waves of two, spill: 2048×24576
 // 222, read again by the long kernel 124.
 template <typename T, typename Y, bool kBlocks>
 int32_t norm_by_shape(dc_hip_ctx* ctx, const LayerNormArgs& a) {
   const int64_t chunks = (a.cols + kElems<T> - 1) / kElems<T>;
-  const bool wave = chunks > 64 && chunks <= 128 && (sizeof(T) == 2 || sizeof(Y) == 1), few = a.rows <= ctx->cu_count;
-  if (!wave && chunks <= (few ? 64 * kWaves : 256)) return launch_norm<T, Y, 1, kBlocks>(ctx, a, chunks);
+  const bool wave = chunks > 64 && chunks <= 128 && (sizeof(T) == 2 || sizeof(Y) == 1), one = sizeof(T) == 2 || a.rows <= ctx->cu_count;
+  if (!wave && chunks <= (one ? 64 * kWaves : 256)) return launch_norm<T, Y, 1, kBlocks>(ctx, a, chunks);
   if (chunks <= 64 * 2 * kWaves) return launch_norm<T, Y, 2, kBlocks>(ctx, a, chunks);
   layer_norm_long_kernel<T, Y, kBlocks><<<(unsigned)std::min(a.rows, kMaxGrid), 64 * kWaves, 0, ctx->stream>>>(a);
   return last_launch_status();
