@@ -33,8 +33,9 @@ struct LayerNormArgs {
 };
 
 // The chunks c_i = ((i waves + wave) 64 + lane) E, i < C, of a row, as dc::Row has them; offsets in 32 bits (a row has at most 2^27 bytes), beside a
-// pointer that all lanes share, which saves registers and additions for each of a row's operands.
-template <typename T, int C>
+// pointer that all lanes share, which saves registers and additions for each of a row's operands. The first kInside chunks are in the row for every wave: where
+// half of them would hold a row there are fewer waves. (The gradients use that: f32 2000×12000 94 us, else 110. Forward it moves the loads' order: 8192×2048 51.7, else 48.5.)
+template <typename T, int C, int kInside = 0>
 struct Span {
   static constexpr int E = kElems<T>;
   uint32_t cols, first, step, end;  // first: of the lane; step: from chunk to chunk; end: of the wave's first chunks (uniform)
@@ -48,11 +49,11 @@ struct Span {
     return reinterpret_cast<P*>(reinterpret_cast<Byte*>(p) + elements * (uint32_t)sizeof(P));
   }
   __device__ inline void load(const T* p, u32x4 (&raw)[C]) const {
-    if (cols >= E) {
+    if (kInside > 0 || cols >= E) {
 #pragma unroll
       for (int i = 0; i < C; ++i) {
         const uint32_t c = at(i);
-        raw[i] = load_raw(past(p, c < cols - E ? c : cols - E));
+        raw[i] = load_raw(past(p, inside(i) || c < cols - E ? c : cols - E));
       }
     } else {
 #pragma unroll
@@ -68,10 +69,11 @@ struct Span {
     }
   }
   // Whether all elements of the wave's chunk i are in the row (uniform).
-  __device__ inline bool whole(int i) const { return end + i * step <= cols; }
+  static __device__ constexpr bool inside(int i) { return i < kInside; }
+  __device__ inline bool whole(int i) const { return inside(i) || end + i * step <= cols; }
   // What load() left of the row's last 16 bytes in the chunks at and past its end.
   __device__ inline void cut(u32x4 (&raw)[C]) const {
-    if (cols < E) return;
+    if (kInside == 0 && cols < E) return;
 #pragma unroll
     for (int i = 0; i < C; ++i)
       if (!whole(i)) {
@@ -82,7 +84,8 @@ struct Span {
   template <typename Y>
   __device__ inline void store(Y* p, int i, const float (&v)[E]) const {
     const uint32_t c = at(i);
-    if (c < cols) store_some(past(p, c), (int64_t)cols - c, v);
+    if (inside(i)) store_chunk(past(p, c), v);
+    else if (c < cols) store_some(past(p, c), (int64_t)cols - c, v);
   }
 };
 
@@ -119,8 +122,8 @@ __device__ inline float value_near(const float (&h)[C][kElems<T>], float weight)
   return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v))) * weight;
 }
 // h becomes d = h - near (zeros past the row's end); the lane's part of the sums.
-template <typename T, int C>
-__device__ inline Moments lane_moments(const Span<T, C>& R, float (&h)[C][kElems<T>], float near) {
+template <typename T, int C, int kInside>
+__device__ inline Moments lane_moments(const Span<T, C, kInside>& R, float (&h)[C][kElems<T>], float near) {
   constexpr int E = kElems<T>;
   Moments m{near, 0.0f, 0.0f};
 #pragma unroll
@@ -135,6 +138,12 @@ __device__ inline Moments lane_moments(const Span<T, C>& R, float (&h)[C][kElems
     }
   }
   return m;
+}
+
+// The variance, from sums of what is left over a value near the mean (no less than zero where rounding would have it so: a row of equal values).
+__device__ inline float variance(float squares, float left, float rest, float per) {
+  const float v = (squares - left * rest) * per;
+  return v < 0.0f ? 0.0f : v;
 }
 
 // 1 / sqrt(v), an ulp off; v among the smallest floats keeps its digits.
@@ -161,13 +170,13 @@ __device__ inline Joined join_moments(const Moments& m, float n, float near, flo
   const float rest = row16_sum_f32(__builtin_fmaf(n, j.off, m.left));
   const float squares = row16_sum_f32(__builtin_fmaf(j.off, __builtin_fmaf(n, j.off, 2.0f * m.left), m.squares));
   j.rest = rest * per;
-  j.row.s = inverse_root((squares - rest * j.rest) * per + eps);
+  j.row.s = inverse_root(variance(squares, rest, j.rest, per) + eps);
   j.row.shift = ((near - mean) - j.rest) * j.row.s;
   return j;
 }
 // Of a row that one wave holds.
 __device__ inline RowStats own_stats(const Moments& m, float per, float eps) {
-  const float rest = m.left * per, s = inverse_root((m.squares - m.left * rest) * per + eps);
+  const float rest = m.left * per, s = inverse_root(variance(m.squares, m.left, rest, per) + eps);
   return RowStats{-rest * s, s};
 }
 
@@ -330,7 +339,7 @@ __global__ __launch_bounds__(1024) void layer_norm_long_kernel(LayerNormArgs a) 
     }
     left = row_sum(left, scratch[1], wave, kWaves);
     squares = row_sum(squares, scratch[2], wave, kWaves);
-    const float rest = left / (float)a.cols, s = 1.0f / sqrtf((squares - left * rest) / (float)a.cols + a.eps);
+    const float rest = left / (float)a.cols, s = 1.0f / sqrtf(variance(squares, left, rest, 1.0f / (float)a.cols) + a.eps);
     auto normed = [&](int64_t c, float (&v)[E]) __attribute__((always_inline)) {
       float w[E], b[E];
       load_some(weight + c, cols - c, w);
@@ -391,18 +400,20 @@ struct LayerNormGradArgs {
 };
 
 // `groups` rows at a time to a workgroup, `waves` waves to each, at most 16 in all; their parts of dweight and dbias meet in LDS at the end, so that a
-// workgroup leaves one of each. With kAhead the next rows' operands are asked for before these ones' sums.
-template <typename T, int C, bool kAhead>
-__global__ __launch_bounds__(C == 4 && sizeof(T) == 2 ? 512 : 1024) void layer_norm_grad_kernel(LayerNormGradArgs a, int waves, int groups) {
-  constexpr int E = kElems<T>;
+// workgroup leaves one of each. With kAhead the next rows' operands are asked for before these ones' sums. With kShared (one row at a time) the parts
+// lie in LDS all along, up to 128 KiB, each lane's where it alone reads them: beside the rest of rows that long registers do not hold them.
+template <typename T, int C, bool kAhead, bool kShared>
+__global__ __launch_bounds__(1024) void layer_norm_grad_kernel(LayerNormGradArgs a, int waves, int groups) {
+  constexpr int E = kElems<T>, kQuads = C * (E / 4);  // of dweight's parts to a lane
   constexpr bool kKeep = C == 1;  // g over the barrier (of two chunks a lane it does not fit beside the rest, and is formed again)
   __shared__ __align__(16) f32x4_lds words[2][kWaves];
   __shared__ float more[2][kWaves];
+  __shared__ __align__(16) f32x4_lds kept[kShared ? 2 * kQuads * 64 * kWaves : 1];
   extern __shared__ __align__(16) float left_by[];  // (groups - 1) waves 64 2 C E floats
   const int lane = threadIdx.x & 63, place = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int group = place / waves, wave = place - group * waves, first = group * waves;
   const int64_t cols = a.cols;
-  const Span<T, C> R(cols, waves, wave, lane);
+  const Span<T, C, C / 2> R(cols, waves, wave, lane);
   const int other = lane & (kWaves - 1);
   const float weight = near_weight<E>(cols, wave), n_other = other < waves ? wave_count<E, C>(cols, waves, other) : 0.0f;
   const float per_col = 1.0f / (float)a.cols;
@@ -411,6 +422,9 @@ __global__ __launch_bounds__(C == 4 && sizeof(T) == 2 ? 512 : 1024) void layer_n
   for (int i = 0; i < C; ++i)
 #pragma unroll
     for (int e = 0; e < E; ++e) dw[i][e] = db[i][e] = 0.0f;
+  if constexpr (kShared)
+#pragma unroll
+    for (int q = 0; q < 2 * kQuads; ++q) kept[q * 64 * kWaves + threadIdx.x] = f32x4_lds{0.0f, 0.0f, 0.0f, 0.0f};
   u32x4 wr[C], hr[C], dr[C], ur[C];
   auto load = [&](int64_t row) __attribute__((always_inline)) {
     R.load(static_cast<const T*>(a.h) + row * a.h_stride, hr);
@@ -490,11 +504,20 @@ __global__ __launch_bounds__(C == 4 && sizeof(T) == 2 ? 512 : 1024) void layer_n
       float o[E], dy[E], w[E];
       unpack(yv[i], dy);
       if constexpr (!kKeep) unpack(wr[i], w);
+      f32x4_lds sums[2];
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const float u = __builtin_fmaf(d[i][e], r.s, r.shift);
-        dw[i][e] = __builtin_fmaf(dy[e], u, dw[i][e]);
-        db[i][e] += dy[e];
+        if constexpr (kShared) {
+          f32x4_lds* at = kept + (i * (E / 4) + e / 4) * 64 * kWaves + threadIdx.x;
+          if (e % 4 == 0) sums[0] = at[0], sums[1] = at[kQuads * 64 * kWaves];
+          sums[0][e % 4] = __builtin_fmaf(dy[e], u, sums[0][e % 4]);
+          sums[1][e % 4] += dy[e];
+          if (e % 4 == 3) at[0] = sums[0], at[kQuads * 64 * kWaves] = sums[1];
+        } else {
+          dw[i][e] = __builtin_fmaf(dy[e], u, dw[i][e]);
+          db[i][e] += dy[e];
+        }
         o[e] = __builtin_fmaf(kKeep ? g[kKeep ? i : 0][e] : dy[e] * w[e], r.s, __builtin_fmaf(u, along, flat));
       }
       if (dx) {
@@ -525,6 +548,12 @@ __global__ __launch_bounds__(C == 4 && sizeof(T) == 2 ? 512 : 1024) void layer_n
 #pragma unroll
       for (int q = 0; q < 2 * C * (E / 4); ++q) *quad(q) += own[slot(g, q)];
   }
+  if constexpr (kShared)
+#pragma unroll
+    for (int q = 0; q < kQuads; ++q) {
+      *reinterpret_cast<f32x4_lds*>(&dw[q / (E / 4)][4 * (q % (E / 4))]) = kept[q * 64 * kWaves + threadIdx.x];
+      *reinterpret_cast<f32x4_lds*>(&db[q / (E / 4)][4 * (q % (E / 4))]) = kept[(kQuads + q) * 64 * kWaves + threadIdx.x];
+    }
   auto leave = [&](float* parts, const float (&v)[C][E]) __attribute__((always_inline)) {
     float* part = parts + (int64_t)blockIdx.x * a.part_pitch;
 #pragma unroll
@@ -585,7 +614,7 @@ __global__ __launch_bounds__(1024) void layer_norm_grad_long_kernel(LayerNormGra
     squares = row_sum(squares, scratch[2], wave, kWaves);
     g_sum = row_sum(g_sum, scratch[3], wave, kWaves);
     gd_sum = row_sum(gd_sum, scratch[4], wave, kWaves);
-    const float n = (float)a.cols, rest = left / n, s = 1.0f / sqrtf((squares - left * rest) / n + a.eps);
+    const float n = (float)a.cols, rest = left / n, s = 1.0f / sqrtf(variance(squares, left, rest, 1.0f / n) + a.eps);
     const float g_mean = g_sum / n, along = s * (s * ((gd_sum - rest * g_sum) / n));
     for (int64_t c = first; c < cols; c += kStep) {
       read(c);
@@ -736,17 +765,18 @@ int32_t norm_grad_by_shape(dc_hip_ctx* ctx, const LayerNormGradArgs& a, const Gr
   const int groups = grid.groups;
   const unsigned g = (unsigned)grid.workgroups, threads = 64 * waves * groups;
   const size_t lds = (size_t)(groups - 1) * waves * 64 * 2 * c * kElems<T> * sizeof(float);
-  if (c == 1) layer_norm_grad_kernel<T, 1, true><<<g, threads, lds, ctx->stream>>>(a, waves, groups);
-  else if (sizeof(T) == 4 && c == 2) layer_norm_grad_kernel<float, 2, false><<<g, threads, lds, ctx->stream>>>(a, waves, groups);
-  else if (c == 4) layer_norm_grad_kernel<T, 4, false><<<g, threads, lds, ctx->stream>>>(a, waves, groups);
+  if (c == 1) layer_norm_grad_kernel<T, 1, true, false><<<g, threads, lds, ctx->stream>>>(a, waves, groups);
+  else if (c == 2) layer_norm_grad_kernel<T, 2, sizeof(T) == 2, sizeof(T) == 2><<<g, threads, lds, ctx->stream>>>(a, waves, groups);
+  else if (sizeof(T) == 4 && c == 4) layer_norm_grad_kernel<float, 4, false, true><<<g, threads, lds, ctx->stream>>>(a, waves, groups);
   else layer_norm_grad_long_kernel<T><<<g, 64 * kWaves, 0, ctx->stream>>>(a);
   return last_launch_status();
 }
 
-// 16-byte chunks of a row that a lane of the gradient's kernel holds (0: the long kernel). bf16's four leave 8 waves of 256 registers.
+// 16-byte chunks of a row that a lane of the gradient's kernel holds (0: the long kernel). us, with the call, for those of more than 1024 chunks (bf16) and 2048 with
+// their parts of dweight and dbias in registers (bf16: 8 waves of four chunks) / in LDS: bf16 2000×12000 74.4 / 58.5, 4096×16384 147 / 125; float32 2000×12000 145 / 94.
 int norm_grad_chunks(bool f32, int64_t chunks) {
   if (f32) return chunks <= 64 * kWaves ? 1 : chunks <= 128 * kWaves ? 2 : chunks <= 256 * kWaves ? 4 : 0;
-  return chunks <= 64 * kWaves ? 1 : chunks <= 128 * kWaves ? 4 : 0;
+  return chunks <= 64 * kWaves ? 1 : chunks <= 128 * kWaves ? 2 : 0;
 }
 
 }  // namespace
@@ -806,8 +836,9 @@ DC_HIP_API int32_t dc_hip_layer_norm_backward(dc_hip_ctx* ctx, const dc_layer_no
   const GradGrid grid = norm_grad_grid(p.dtype == DC_DTYPE_F32, p.rows, c, waves, std::max(1, ctx->cu_count));
   const int outs = (p.dweight ? 1 : 0) + (p.dbias ? 1 : 0);
   const int64_t pitch = (p.cols + 3) / 4 * 4;
-  float *weight_parts = nullptr, *bias_parts = nullptr;
-  if (outs > 0) {
+  float *weight_parts = p.dweight, *bias_parts = p.dbias;  // (one workgroup's parts are the sums)
+  const bool join = outs > 0 && grid.workgroups > 1;
+  if (join) {
     DC_RETURN_IF(ensure_partials(ctx, (size_t)(grid.workgroups * outs * pitch) * sizeof(float)));
     float* parts = static_cast<float*>(ctx->partials);
     if (p.dweight) weight_parts = parts;
@@ -816,7 +847,7 @@ DC_HIP_API int32_t dc_hip_layer_norm_backward(dc_hip_ctx* ctx, const dc_layer_no
   const LayerNormGradArgs a{p.dy,        p.h,         p.weight,    p.dh,         p.dx,            weight_parts, bias_parts, p.rows,
                             p.dy_stride, p.h_stride, p.dh_stride, p.dx_stride, outs * pitch, (int32_t)p.cols, p.eps};
   DC_RETURN_IF(p.dtype == DC_DTYPE_F32 ? norm_grad_by_shape<float>(ctx, a, grid, c, waves) : norm_grad_by_shape<bf16>(ctx, a, grid, c, waves));
-  if (outs == 0) return DC_OK;
+  if (!join) return DC_OK;
   return launch_column_sums_of(ctx, static_cast<const float*>(ctx->partials), outs * pitch, pitch, p.dweight ? p.dweight : p.dbias,
                                outs > 1 ? p.dbias : nullptr, grid.workgroups, p.cols);
 }
