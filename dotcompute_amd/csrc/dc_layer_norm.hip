@@ -48,12 +48,14 @@ struct Span {
     typedef std::conditional_t<std::is_const_v<P>, const char, char> Byte;
     return reinterpret_cast<P*>(reinterpret_cast<Byte*>(p) + elements * (uint32_t)sizeof(P));
   }
+  template <bool kOnce = false>
   __device__ inline void load(const T* p, u32x4 (&raw)[C]) const {
     if (kInside > 0 || cols >= E) {
 #pragma unroll
       for (int i = 0; i < C; ++i) {
         const uint32_t c = at(i);
-        raw[i] = load_raw(past(p, inside(i) || c < cols - E ? c : cols - E));
+        const T* from = past(p, inside(i) || c < cols - E ? c : cols - E);
+        raw[i] = kOnce ? load_raw_once(from) : load_raw(from);
       }
     } else {
 #pragma unroll
@@ -184,7 +186,7 @@ typedef float f32x4_lds __attribute__((ext_vector_type(4)));
 
 // A workgroup walks over rows, one at a time, or, where a wave holds a row, four; the weights stay in registers, and the next row's operands are asked for before
 // this one's sums. (`sum` and y may lie over x or the residual: a workgroup writes a row after it has read it, and reads no other's.) 8 bits: a scale a row, or (kBlocks) one for each 128.
-template <typename T, typename Y, int C, bool kBlocks>
+template <typename T, typename Y, int C, bool kBlocks, bool kOnce>
 __global__ __launch_bounds__(1024) void layer_norm_kernel(LayerNormArgs a, int waves) {
   constexpr int E = kElems<T>;
   constexpr bool kFp8 = sizeof(Y) == 1;
@@ -201,8 +203,8 @@ __global__ __launch_bounds__(1024) void layer_norm_kernel(LayerNormArgs a, int w
   const int64_t step = (int64_t)gridDim.x * per;
   u32x4 xr[C], rr[C], wr[C], br[C];
   auto load = [&](int64_t row) __attribute__((always_inline)) {
-    R.load(static_cast<const T*>(a.x) + row * a.x_stride, xr);
-    if (a.residual) R.load(static_cast<const T*>(a.residual) + row * a.residual_stride, rr);
+    R.template load<kOnce>(static_cast<const T*>(a.x) + row * a.x_stride, xr);
+    if (a.residual) R.template load<kOnce>(static_cast<const T*>(a.residual) + row * a.residual_stride, rr);
   };
   const int64_t first = (int64_t)blockIdx.x * per + (waves == 1 ? group : 0);
   if (first < a.rows) load(first);
@@ -402,7 +404,7 @@ struct LayerNormGradArgs {
 // `groups` rows at a time to a workgroup, `waves` waves to each, at most 16 in all; their parts of dweight and dbias meet in LDS at the end, so that a
 // workgroup leaves one of each. With kAhead the next rows' operands are asked for before these ones' sums. With kShared (one row at a time) the parts
 // lie in LDS all along, up to 128 KiB, each lane's where it alone reads them: beside the rest of rows that long registers do not hold them.
-template <typename T, int C, bool kAhead, bool kShared>
+template <typename T, int C, bool kAhead, bool kShared, bool kOnce>
 __global__ __launch_bounds__(1024) void layer_norm_grad_kernel(LayerNormGradArgs a, int waves, int groups) {
   constexpr int E = kElems<T>, kQuads = C * (E / 4);  // of dweight's parts to a lane
   constexpr bool kKeep = C == 1;  // g over the barrier (of two chunks a lane it does not fit beside the rest, and is formed again)
@@ -427,9 +429,9 @@ __global__ __launch_bounds__(1024) void layer_norm_grad_kernel(LayerNormGradArgs
     for (int q = 0; q < 2 * kQuads; ++q) kept[q * 64 * kWaves + threadIdx.x] = f32x4_lds{0.0f, 0.0f, 0.0f, 0.0f};
   u32x4 wr[C], hr[C], dr[C], ur[C];
   auto load = [&](int64_t row) __attribute__((always_inline)) {
-    R.load(static_cast<const T*>(a.h) + row * a.h_stride, hr);
-    R.load(static_cast<const T*>(a.dy) + row * a.dy_stride, dr);
-    if (a.dh && a.dx) R.load(static_cast<const T*>(a.dh) + row * a.dh_stride, ur);
+    R.template load<kOnce>(static_cast<const T*>(a.h) + row * a.h_stride, hr);
+    R.template load<kOnce>(static_cast<const T*>(a.dy) + row * a.dy_stride, dr);
+    if (a.dh && a.dx) R.template load<kOnce>(static_cast<const T*>(a.dh) + row * a.dh_stride, ur);
   };
   R.load(static_cast<const T*>(a.weight), wr);
   const int64_t step = (int64_t)gridDim.x * groups;
@@ -650,13 +652,13 @@ __global__ __launch_bounds__(1024) void layer_norm_grad_long_kernel(LayerNormGra
 // ---- rows in 8 bits with a scale for each 128 elements -----------------------------------------------------
 // Memory-bound: 3 bytes an element of bf16, 5 of float32. A wave takes 64 chunks of 16 bytes (512 elements of bf16, 256 of float32) of kRows rows below each
 // other, all asked for at once; a block's maximum is found among 16 or 32 lanes, without LDS, and its first lane writes the rows' scales, which
-// lie beside each other, in one piece.
+// lie beside each other, in one piece. bf16 8192×8192 34.7 us (5.8 TB/s), 8191×8190, whose rows end inside lines, 40.4; with eight rows to a wave 34.1 and 41.7.
 struct QuantizeArgs {
   const void* x;
   uint8_t *q, *scales;
   int64_t rows, cols, x_stride, q_stride, scales_stride, across, total;  // across: pieces to a row; total: pieces
 };
-template <typename T, int kRows>
+template <typename T, int kRows, bool kOnce>
 __global__ __launch_bounds__(256) void quantize_blocks_kernel(QuantizeArgs a) {
   constexpr int E = kElems<T>;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -669,7 +671,10 @@ __global__ __launch_bounds__(256) void quantize_blocks_kernel(QuantizeArgs a) {
     if (a.cols >= E) {  // (a chunk at the row's end is cut out of its last 16 bytes, one past it is zeros; no branch between the loads)
       const int64_t from = at < left - E ? at : left - E;
 #pragma unroll
-      for (int i = 0; i < kRows; ++i) raw[i] = load_raw(x + (i < rows ? i : rows - 1) * a.x_stride + from);
+      for (int i = 0; i < kRows; ++i) {
+        const T* p = x + (i < rows ? i : rows - 1) * a.x_stride + from;
+        raw[i] = kOnce ? load_raw_once(p) : load_raw(p);
+      }
       if (left < 64 * E)
 #pragma unroll
         for (int i = 0; i < kRows; ++i) raw[i] = shift_down(raw[i], (at - from) * (int64_t)sizeof(T));
@@ -684,7 +689,7 @@ __global__ __launch_bounds__(256) void quantize_blocks_kernel(QuantizeArgs a) {
           for (int e = 0; e < 4; ++e) raw[i][e] = pack_bf16(v[2 * e], v[2 * e + 1]);
       }
     }
-    uint32_t scales[(kRows + 3) / 4] = {};
+    uint32_t scales = 0;
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
       float v[E];
@@ -696,17 +701,17 @@ __global__ __launch_bounds__(256) void quantize_blocks_kernel(QuantizeArgs a) {
       const float factor = block_factor(scale);
 #pragma unroll
       for (int e = 0; e < E; ++e) v[e] *= factor;
-      scales[i / 4] |= scale << (8 * (i % 4));
+      scales |= scale << (8 * i);
       if (i < rows && at < left) store_some(a.q + (row0 + i) * a.q_stride + c0 + at, left - at, v);
     }
     if (at % kScaleBlock == 0 && at < left) {
       uint8_t* to = a.scales + (c0 + at) / kScaleBlock * a.scales_stride + row0;
-      if (kRows == 8 && rows == 8) {
-        *reinterpret_cast<u32x2_at1*>(to) = u32x2{scales[0], scales[(kRows + 3) / 4 - 1]};
+      if (kRows == 4 && rows == 4) {
+        *reinterpret_cast<u32_at1*>(to) = scales;
       } else {
 #pragma unroll
         for (int i = 0; i < kRows; ++i)
-          if (i < rows) to[i] = (uint8_t)(scales[i / 4] >> (8 * (i % 4)));
+          if (i < rows) to[i] = (uint8_t)(scales >> (8 * i));
       }
     }
   }
@@ -717,13 +722,15 @@ template <typename T, typename Y, int C, bool kBlocks>
 int32_t launch_norm(dc_hip_ctx* ctx, const LayerNormArgs& a, int64_t chunks) {
   const int waves = waves_for(chunks, C), group = waves == 1 ? 4 : waves;  // (16 waves to a CU)
   const int64_t groups = waves == 1 ? (a.rows + 3) / 4 : a.rows, held = (int64_t)std::max(1, ctx->cu_count) * std::max(1, kWaves / group);
-  layer_norm_kernel<T, Y, C, kBlocks><<<(unsigned)std::min(groups, held), 64 * group, 0, ctx->stream>>>(a, waves);
+  const int64_t size = sizeof(T), bytes = size * (1 + (a.residual != nullptr) + (a.sum != nullptr)) + (int64_t)sizeof(Y);
+  auto* kernel = read_once(a.rows, a.cols, bytes) ? layer_norm_kernel<T, Y, C, kBlocks, true> : layer_norm_kernel<T, Y, C, kBlocks, false>;
+  kernel<<<(unsigned)std::min(groups, held), 64 * group, 0, ctx->stream>>>(a, waves);
   return last_launch_status();
 }
 
 // Chunks that a lane holds: one of bf16, over up to 16 waves; two where they let a wave hold a row by itself (but not where it is read and written in float32),
 // and in longer rows. us, with the call, for a workgroup to each row with one to two chunks / workgroups that walk with two / with one, bf16: 16384×4096 95.6 /
-// 103 / 96.0, to 8 bits 98.7 / 93.1 / 94.0; 8191×2050 34.8 / 29.8 / 28.0; 4096×8192 55.7 / 48.5 / 48.6; 2000×12000 53 / 38; 1000×4096 8.6 / 8.5 / 7.6; float32
+// 103 / 96.0, to 8 bits 98.7 / 93.1 / 94.0; 8191×2050 34.8 / 29.8 / 28.0 (25.5 with loads as read once); 4096×8192 55.7 / 48.5 / 48.6; 2000×12000 53 / 38 (35); 1000×4096 8.6 / 8.5 / 7.6; float32
 // 8192×2048 48.3 / 48.5 / 50.3. With 24 waves a CU 16384×4096 takes 101, with 32 108. Four chunks, for rows of more than 16 waves of two, spill: 2048×24576
 // 222, read again by the long kernel 124.
 template <typename T, typename Y, bool kBlocks>
@@ -765,9 +772,13 @@ int32_t norm_grad_by_shape(dc_hip_ctx* ctx, const LayerNormGradArgs& a, const Gr
   const int groups = grid.groups;
   const unsigned g = (unsigned)grid.workgroups, threads = 64 * waves * groups;
   const size_t lds = (size_t)(groups - 1) * waves * 64 * 2 * c * kElems<T> * sizeof(float);
-  if (c == 1) layer_norm_grad_kernel<T, 1, true, false><<<g, threads, lds, ctx->stream>>>(a, waves, groups);
-  else if (c == 2) layer_norm_grad_kernel<T, 2, sizeof(T) == 2, sizeof(T) == 2><<<g, threads, lds, ctx->stream>>>(a, waves, groups);
-  else if (sizeof(T) == 4 && c == 4) layer_norm_grad_kernel<float, 4, false, true><<<g, threads, lds, ctx->stream>>>(a, waves, groups);
+  auto launch = [&](auto* often, auto* once) {
+    const int64_t bytes = (int64_t)sizeof(T) * (2 + (a.dx ? 1 + (a.dh != nullptr) : 0));
+    (read_once(a.rows, a.cols, bytes) ? once : often)<<<g, threads, lds, ctx->stream>>>(a, waves, groups);
+  };
+  if (c == 1) launch(layer_norm_grad_kernel<T, 1, true, false, false>, layer_norm_grad_kernel<T, 1, true, false, true>);
+  else if (c == 2) launch(layer_norm_grad_kernel<T, 2, sizeof(T) == 2, sizeof(T) == 2, false>, layer_norm_grad_kernel<T, 2, sizeof(T) == 2, sizeof(T) == 2, true>);
+  else if (sizeof(T) == 4 && c == 4) launch(layer_norm_grad_kernel<float, 4, false, true, false>, layer_norm_grad_kernel<float, 4, false, true, true>);
   else layer_norm_grad_long_kernel<T><<<g, 64 * kWaves, 0, ctx->stream>>>(a);
   return last_launch_status();
 }
@@ -870,10 +881,14 @@ DC_HIP_API int32_t dc_hip_quantize_fp8_blocks(dc_hip_ctx* ctx, const void* x, in
     const QuantizeArgs a{x, q, scales, rows, cols, x_stride, q_stride, scales_stride, across, total};
     kernel<<<(unsigned)std::min((total + 3) / 4, kMaxGrid), 256, 0, ctx->stream>>>(a);
   };
-  // (eight rows to a wave where that leaves every CU some waves, else a row to a wave)
-  const bool few = across * ((rows + 7) / 8) < 4 * (int64_t)ctx->cu_count;
-  if (dtype == DC_DTYPE_F32) few ? launch(quantize_blocks_kernel<float, 1>, 1) : launch(quantize_blocks_kernel<float, 8>, 8);
-  else few ? launch(quantize_blocks_kernel<bf16, 1>, 1) : launch(quantize_blocks_kernel<bf16, 8>, 8);
+  // (four rows to a wave where that leaves every CU some waves, else a row to a wave)
+  const bool few = across * ((rows + 3) / 4) < 4 * (int64_t)ctx->cu_count, once = read_once(rows, cols, size_of(dtype) + 1);
+  auto by_type = [&](auto zero) {
+    typedef decltype(zero) T;
+    if (few) launch(quantize_blocks_kernel<T, 1, false>, 1);
+    else once ? launch(quantize_blocks_kernel<T, 4, true>, 4) : launch(quantize_blocks_kernel<T, 4, false>, 4);
+  };
+  dtype == DC_DTYPE_F32 ? by_type(0.0f) : by_type(bf16{});
   return last_launch_status();
 }
 

@@ -386,12 +386,35 @@ __global__ __launch_bounds__(kSumCols * kSumGroups) void column_sums_kernel(cons
                                                                             int64_t count, int64_t cols) {
   add_columns(parts, cols, out, count, cols);
 }
-// Of two such arrays whose rows take turns: the second's are `second` floats further on.
-__global__ __launch_bounds__(kSumCols * kSumGroups) void column_sums_of_two_kernel(const float* __restrict__ parts, int64_t pitch, int64_t second,
-                                                                                   float* __restrict__ out, float* __restrict__ out2,
-                                                                                   int64_t count, int64_t cols) {
-  if (blockIdx.y == 0) add_columns(parts, pitch, out, count, cols);
-  else add_columns(parts + second, pitch, out2, count, cols);
+// Of two such arrays whose rows take turns: the second's are `second` floats further on. 16 columns a workgroup, or 32 or 64 of wide arrays, so that no two
+// read halves of the same lines.
+template <int kCols>
+__global__ __launch_bounds__(1024) void column_sums_of_two_kernel(const float* __restrict__ parts, int64_t pitch, int64_t second, float* __restrict__ out,
+                                                                  float* __restrict__ out2, int64_t count, int64_t cols) {
+  if (blockIdx.y > 0) parts += second, out = out2;
+  if constexpr (kCols == kSumCols) {
+    add_columns(parts, pitch, out, count, cols);
+  } else {
+    constexpr int kGroups = 1024 / kCols, kAhead = 16;
+    __shared__ float sums[kGroups][kCols];
+    const int lane = threadIdx.x % kCols, g = threadIdx.x / kCols;
+    const int64_t c = (int64_t)blockIdx.x * kCols + lane;
+    float v = 0.0f;
+    if (c < cols)
+      for (int64_t i = g; i < count; i += kAhead * kGroups) {
+        float u[kAhead];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) u[j] = parts[min(i + j * kGroups, count - 1) * pitch + c];
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) v += i + j * kGroups < count ? u[j] : 0.0f;
+      }
+    sums[g][lane] = v;
+    __syncthreads();
+    if (g > 0 || c >= cols) return;
+#pragma unroll
+    for (int i = 1; i < kGroups; ++i) v += sums[i][lane];
+    out[c] = v;
+  }
 }
 
 template <typename T, typename Y, int C, bool kNorm>
@@ -452,8 +475,15 @@ int32_t launch_column_sums(dc_hip_ctx* ctx, const float* parts, float* out, int6
 
 int32_t launch_column_sums_of(dc_hip_ctx* ctx, const float* parts, int64_t pitch, int64_t second, float* out, float* out2, int64_t count,
                               int64_t cols) {
-  column_sums_of_two_kernel<<<dim3((unsigned)((cols + kSumCols - 1) / kSumCols), out2 ? 2 : 1), kSumCols * kSumGroups, 0, ctx->stream>>>(
-      parts, pitch, second, out, out2, count, cols);
+  auto launch = [&](auto kernel, int64_t each) {
+    kernel<<<dim3((unsigned)((cols + each - 1) / each), out2 ? 2 : 1), 1024, 0, ctx->stream>>>(parts, pitch, second, out, out2, count, cols);
+  };
+  // (wider where that leaves every CU a workgroup of both arrays; the same for one of them, whose bits then do not hang on the other's being asked for. With a layer norm's gradients, us, for 16 / 32 / 64 columns: 8192×4096 50.8 / 49.8, 1000×6000 21.2 / 20.0,
+  // 2000×12000 58.9 / 53.3 / 52.5, 28×14912 15.8 / 16.5 / 14.0)
+  const int64_t both = 2 * cols, cus = std::max(1, ctx->cu_count);
+  if (both >= 64 * cus) launch(column_sums_of_two_kernel<64>, 64);
+  else if (both >= 32 * cus) launch(column_sums_of_two_kernel<32>, 32);
+  else launch(column_sums_of_two_kernel<kSumCols>, kSumCols);
   return last_launch_status();
 }
 

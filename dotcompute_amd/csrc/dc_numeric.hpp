@@ -103,6 +103,18 @@ __device__ inline u32x4 load_raw(const T* p) {
   if constexpr (sizeof(T) == 4) return __builtin_bit_cast(u32x4, *reinterpret_cast<const f32x4_at4*>(p));
   else return *reinterpret_cast<const u32x4_at2*>(p);
 }
+// The same of what no cache need keep.
+template <typename T>
+__device__ inline u32x4 load_raw_once(const T* p) {
+  if constexpr (sizeof(T) == 4) return __builtin_bit_cast(u32x4, __builtin_nontemporal_load(reinterpret_cast<const f32x4_at4*>(p)));
+  else return __builtin_nontemporal_load(reinterpret_cast<const u32x4_at2*>(p));
+}
+// Whether a call's operands, `bytes` for each element, are more than the last cache (256 MiB) keeps beside twice as much of others; then no cache need keep them.
+// us, kept / not, each call over one of three sets of operands in turn: layer norm bf16 2000×4096 (66 MB) 11.8 / 13.0, 3000×4096 18.3 / 18.2, 4000×4096
+// 25.2 / 23.1, 8191×2050 28.1 / 25.5, 2000×12000 37.7 / 35.0; gradients 16384×512 (67 MB) 16.5 / 18.0, 8192×4096 56 / 51, float32 2000×2048 (66 MB)
+// 17.2 / 19.6, 4000×2048 31.6 / 29.0, 8192×2048 56.5 / 49.2; rows in 8 bits 3000×8192 (74 MB) 14.0 / 15.6, 5000×8192 25.2 / 23.3, 8191×8190 43.5 / 40.4;
+// a gated layer's gradients 2000×2504×1000 (70 MB beside the products) 80.6 / 86.0, 7819×2048×64 (224 MB) 93.7 / 77.2, 8192×8192×2048 1069 / 1062.
+inline bool read_once(int64_t rows, int64_t cols, int64_t bytes) { return rows * cols > (int64_t(96) << 20) / bytes; }
 __device__ inline void unpack(u32x4 w, float (&v)[8]) { unpack_bf16(w, v); }
 __device__ inline void unpack(u32x4 w, float (&v)[4]) {
   const f32x4 f = __builtin_bit_cast(f32x4, w);
