@@ -1,11 +1,14 @@
 // dc_layer_norm.hip — layer norm with the residual's addition, its gradients, and rows in 8 bits with a scale for each 128 elements.
 //
 // Forward, a row at a time: h = x + r, y = (h - mean) s w + b with s = 1 / sqrt(var + eps). Memory-bound: 8 bytes an element in bf16 (x, r
-// in; h, y out), 7 with y in 8 bits. A row stays in registers between its one read and its write, as an RMS norm's.
+// in; h, y out), 7 with y in 8 bits. A row stays in registers between its one read and its write, as an RMS norm's. 16384×4096 93.3 us (5.8 TB/s),
+// 8191×2050, whose rows lie at 4-byte boundaries, 25.9 (5.2); 8×4096 to 8 bits 4.2, of which the call is 3.7.
 //
 // Backward: u = (h - mean) s, g = dy w: dx = s (g - mean(g) - u mean(g u)) + dh, dw = the sum over rows of dy u, db of dy. One read of each
 // operand; the statistics are formed again from h, which is read anyway. A workgroup walks over rows and keeps its parts of dw
-// and db in registers; a second kernel adds the parts in a fixed order (no atomics: the same bits from call to call).
+// and db in registers, or of long rows in LDS; a second kernel adds the parts in a fixed order (no atomics: the same bits from call to call).
+// Memory-bound: 8192×4096 50 us with that kernel (5.4 TB/s), 8191×2050 37.4 (3.6: five waves a row, the last with one lane's worth, so that a CU's 15
+// hold fewer bytes in flight, at 4-byte boundaries); 500×1024 in float32 7.9, two launches.
 //
 // Statistics. The difference of mean(h^2) and mean(h)^2 loses the variance's digits where the mean is large, and a second sum over a row that
 // several waves share would be a second barrier. So each wave takes a value k near its own part's mean, the mean of the first 32 elements (of 256 or
@@ -44,7 +47,8 @@ __device__ inline void store_chunk_once(bf16* p, const float (&v)[8]) {
 
 // The chunks c_i = ((i waves + wave) 64 + lane) E, i < C, of a row, as dc::Row has them; offsets in 32 bits (a row has at most 2^27 bytes), beside a
 // pointer that all lanes share, which saves registers and additions for each of a row's operands. The first kInside chunks are in the row for every wave: where
-// half of them would hold a row there are fewer waves. (The gradients use that: f32 2000×12000 94 us, else 110. Forward it moves the loads' order: 8192×2048 51.7, else 48.5.)
+// half of them would hold a row there are fewer waves. (The gradients use that: float32 2000×12000 94 us, else 110. Forward it moves the loads' order:
+// float32 8192×2048 51.7, else 48.5.)
 template <typename T, int C, int kInside = 0>
 struct Span {
   static constexpr int E = kElems<T>;
@@ -200,8 +204,9 @@ __device__ inline RowStats own_stats(const Moments& m, float per, float eps) {
 
 typedef float f32x4_lds __attribute__((ext_vector_type(4)));
 
-// A workgroup walks over rows, one at a time, or, where a wave holds a row, four; the weights stay in registers, and the next row's operands are asked for before
-// this one's sums. (`sum` and y may lie over x or the residual: a workgroup writes a row after it has read it, and reads no other's.) 8 bits: a scale a row, or (kBlocks) one for each 128.
+// A workgroup walks over rows, one at a time, or, where a wave holds a row, four; the weights stay in registers, and the next row's operands are asked
+// for before this one's sums. (`sum` and y may lie over x or the residual: each lane writes what it alone has read, and a load that reaches back over the
+// row's end drops what is not its own.) 8 bits: a scale a row, or (kBlocks) one for each 128.
 template <typename T, typename Y, int C, bool kBlocks, bool kOnce>
 __global__ __launch_bounds__(1024) void layer_norm_kernel(LayerNormArgs a, int waves) {
   constexpr int E = kElems<T>;
@@ -748,8 +753,8 @@ int32_t launch_norm(dc_hip_ctx* ctx, const LayerNormArgs& a, int64_t chunks) {
 
 // Chunks that a lane holds: one of bf16, over up to 16 waves; two where they let a wave hold a row by itself (but not where it is read and written in float32),
 // and in longer rows. us, with the call, for a workgroup to each row with one to two chunks / workgroups that walk with two / with one, bf16: 16384×4096 95.6 /
-// 103 / 96.0, to 8 bits 98.7 / 93.1 / 94.0; 8191×2050 34.8 / 29.8 / 28.0 (25.5 with loads as read once); 4096×8192 55.7 / 48.5 / 48.6; 2000×12000 53 / 38 (35); 1000×4096 8.6 / 8.5 / 7.6; float32
-// 8192×2048 48.3 / 48.5 / 50.3. With 24 waves a CU 16384×4096 takes 101, with 32 108. Four chunks, for rows of more than 16 waves of two, spill: 2048×24576
+// 103 / 96.0, to 8 bits 98.7 / 93.1 / 94.0; 8191×2050 34.8 / 29.8 / 28.0; 4096×8192 55.7 / 48.5 / 48.6; 2000×12000 53 / 38;
+// 1000×4096 8.6 / 8.5 / 7.6; float32 8192×2048 48.3 / 48.5 / 50.3 (all before large operands were loaded as read once). With 24 waves a CU 16384×4096 takes 101, with 32 108. Four chunks, for rows of more than 16 waves of two, spill: 2048×24576
 // 222, read again by the long kernel 124.
 template <typename T, typename Y, bool kBlocks>
 int32_t norm_by_shape(dc_hip_ctx* ctx, const LayerNormArgs& a) {
@@ -787,6 +792,7 @@ GradGrid norm_grad_grid(bool f32, int64_t rows, int c, int waves, int64_t cus) {
 
 template <typename T>
 int32_t norm_grad_by_shape(dc_hip_ctx* ctx, const LayerNormGradArgs& a, const GradGrid& grid, int c, int waves) {
+  constexpr bool kShort = sizeof(T) == 2;
   const int groups = grid.groups;
   const unsigned g = (unsigned)grid.workgroups, threads = 64 * waves * groups;
   const size_t lds = (size_t)(groups - 1) * waves * 64 * 2 * c * kElems<T> * sizeof(float);
@@ -795,14 +801,15 @@ int32_t norm_grad_by_shape(dc_hip_ctx* ctx, const LayerNormGradArgs& a, const Gr
     (read_once(a.rows, a.cols, bytes) ? once : often)<<<g, threads, lds, ctx->stream>>>(a, waves, groups);
   };
   if (c == 1) launch(layer_norm_grad_kernel<T, 1, true, false, false>, layer_norm_grad_kernel<T, 1, true, false, true>);
-  else if (c == 2) launch(layer_norm_grad_kernel<T, 2, sizeof(T) == 2, sizeof(T) == 2, false>, layer_norm_grad_kernel<T, 2, sizeof(T) == 2, sizeof(T) == 2, true>);
+  else if (c == 2) launch(layer_norm_grad_kernel<T, 2, kShort, kShort, false>, layer_norm_grad_kernel<T, 2, kShort, kShort, true>);
   else if (sizeof(T) == 4 && c == 4) launch(layer_norm_grad_kernel<float, 4, false, true, false>, layer_norm_grad_kernel<float, 4, false, true, true>);
   else layer_norm_grad_long_kernel<T><<<g, 64 * kWaves, 0, ctx->stream>>>(a);
   return last_launch_status();
 }
 
-// 16-byte chunks of a row that a lane of the gradient's kernel holds (0: the long kernel). us, with the call, for those of more than 1024 chunks (bf16) and 2048 with
-// their parts of dweight and dbias in registers (bf16: 8 waves of four chunks) / in LDS: bf16 2000×12000 74.4 / 58.5, 4096×16384 147 / 125; float32 2000×12000 145 / 94.
+// 16-byte chunks of a row that a lane of the gradient's kernel holds (0: the long kernel). us, with the call, for rows of more than 1024 chunks in bf16, 2048
+// in float32, with their parts of dweight and dbias in registers (bf16: 8 waves of four chunks) / in LDS / by the long kernel: bf16 2000×12000
+// 74.4 / 58.5 / 236, 4096×16384 147 / 125 / 582; float32 2000×12000 145 / 94 / 209.
 int norm_grad_chunks(bool f32, int64_t chunks) {
   if (f32) return chunks <= 64 * kWaves ? 1 : chunks <= 128 * kWaves ? 2 : chunks <= 256 * kWaves ? 4 : 0;
   return chunks <= 64 * kWaves ? 1 : chunks <= 128 * kWaves ? 2 : 0;

@@ -478,8 +478,9 @@ int32_t launch_column_sums_of(dc_hip_ctx* ctx, const float* parts, int64_t pitch
   auto launch = [&](auto kernel, int64_t each) {
     kernel<<<dim3((unsigned)((cols + each - 1) / each), out2 ? 2 : 1), 1024, 0, ctx->stream>>>(parts, pitch, second, out, out2, count, cols);
   };
-  // (wider where that leaves every CU a workgroup of both arrays; the same for one of them, whose bits then do not hang on the other's being asked for. With a layer norm's gradients, us, for 16 / 32 / 64 columns: 8192×4096 50.8 / 49.8, 1000×6000 21.2 / 20.0,
-  // 2000×12000 58.9 / 53.3 / 52.5, 28×14912 15.8 / 16.5 / 14.0)
+  // (wider where that leaves every CU a workgroup of both arrays; the same for one of them, whose bits then do not hang on the other's being asked for.
+  // With a layer norm's gradients, us, for 16 / 32 / 64 columns: 8192×4096 50.8 / 49.8, 1000×6000 21.2 / 20.0, 2000×12000 58.9 / 53.3 / 52.5,
+  // 28×14912 15.8 / 16.5 / 14.0)
   const int64_t both = 2 * cols, cus = std::max(1, ctx->cu_count);
   if (both >= 64 * cus) launch(column_sums_of_two_kernel<64>, 64);
   else if (both >= 32 * cus) launch(column_sums_of_two_kernel<32>, 32);

@@ -3,7 +3,8 @@ stride says nothing, tall and wide gradients' kernels.
 
 Tolerances: of rows of a value v the formula leaves the bias alone. What a lane holds is the row's distance from a mean whose sum has been rounded ten times at
 most (forty, where a thread adds twenty terms before that), so within that many half steps of v, and that distance is known to 8e-6 of itself; times
-s = 1 / sqrt(eps) at most. Sums of squares in 8 bits lose at most 2^-13 of the largest for each of 64 terms, 2^-7 of themselves. The others as in the operators' own tests.
+s = 1 / sqrt(eps) at most. Sums of squares in 8 bits lose at most 2^-13 of the largest for each of 64 terms, 2^-7 of themselves. The others as in the
+operators' own tests.
 """
 import numpy as np
 import pytest
