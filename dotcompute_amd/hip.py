@@ -131,6 +131,7 @@ class LinqChain(C.Structure):
         return ch
 
 
+_BYTE = np.dtype(np.uint8)
 _DTYPE_CODES = {np.dtype(np.float32): DTYPE_F32, np.dtype(np.uint16): DTYPE_BF16, np.dtype(np.uint8): DTYPE_FP8}
 
 
@@ -901,15 +902,21 @@ class Context:
         """Rows of x (float32 or bf16) in e4m3 (uint8 bytes) with block scales, uint8 [scale_blocks(cols), rows]. Row strides in
         elements, else dense."""
         rows, cols = _matrix(x, "x")
-        _expect(q, "q", (DTYPE_FP8,), (rows, cols))
-        _expect(scales, "scales", (DTYPE_FP8,), (scale_blocks(cols), rows))
-        for name, a, stride in (("x", x, x_stride), ("q", q, q_stride), ("scales", scales, scales_stride)):
-            if stride is not None:
-                _check_reach(a, name, stride)
-        x_stride, q_stride = (cols if s is None else s for s in (x_stride, q_stride))
-        check(load().dc_hip_quantize_fp8_blocks(self.handle, x.ptr, dtype_of(x), x_stride, q.ptr, q_stride, scales.ptr,
-                                                rows if scales_stride is None else scales_stride, rows, cols),
-              "dc_hip_quantize_fp8_blocks")
+        by_block = (-(-cols // SCALE_BLOCK), rows)
+        # (compared here before _expect is called, which names what is wrong: the call is as long as the kernel of a few rows)
+        if q.shape != (rows, cols) or q.dtype != _BYTE:
+            _expect(q, "q", (DTYPE_FP8,), (rows, cols))
+        if scales.shape != by_block or scales.dtype != _BYTE:
+            _expect(scales, "scales", (DTYPE_FP8,), by_block)
+        if x_stride is not None:
+            _check_reach(x, "x", x_stride)
+        if q_stride is not None:
+            _check_reach(q, "q", q_stride)
+        if scales_stride is not None:
+            _check_reach(scales, "scales", scales_stride)
+        check(load().dc_hip_quantize_fp8_blocks(self.handle, x.ptr, dtype_of(x), cols if x_stride is None else x_stride, q.ptr,
+                                                cols if q_stride is None else q_stride, scales.ptr,
+                                                rows if scales_stride is None else scales_stride, rows, cols), "dc_hip_quantize_fp8_blocks")
 
     def adamw_step(self, args: AdamW, tensors: AdamWTensors) -> None:
         args = AdamW.from_buffer_copy(args)  # (the caller's may be another step's at the same time)
