@@ -353,9 +353,10 @@ struct Frag<true> {
   i32x8 v;
 };
 
-// 16 bytes a lane to 1 KiB of LDS, from `voff` (the lane's, kPast for zeros) + `soff` bytes past `base`.
+// 16 bytes a lane to 1 KiB of LDS, from `voff` (the lane's, kPast for zeros) + `soff` bytes past `base`. kOnce: of what no cache need keep (nontemporal).
+template <bool kOnce = false>
 __device__ inline void load_block(const unsigned char* base, unsigned char* to, uint32_t voff, int soff) {
-  __builtin_amdgcn_raw_ptr_buffer_load_lds(dc::range_rsrc(base, kRange), (dc::lds_ptr_t)to, 16, voff, soff, 0, 0);
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(dc::range_rsrc(base, kRange), (dc::lds_ptr_t)to, 16, voff, soff, 0, kOnce ? 2 : 0);
 }
 
 // The products of one launch. Workgroups take the first's tiles, part of c by part, then the second's: the two
@@ -987,8 +988,9 @@ __device__ inline void wait_loads() {  // until at most N of the wave's loads ar
 }
 
 // kGated: the second half of the NB blocks of 16 rows of w are the other weight's, so that a workgroup has 8 NB outputs. kBlocks: the lanes of group g
-// hold the scales of every fourth of the wave's steps from its g-th on, a load for four steps; a step's are handed over within the wave.
-template <bool kFp8, int XB, int NB, int W, int D, bool kGated, bool kBlocks>
+// hold the scales of every fourth of the wave's steps from its g-th on, a load for four steps; a step's are handed over within the wave. kOnce: the weights
+// are more than the caches keep.
+template <bool kFp8, int XB, int NB, int W, int D, bool kGated, bool kBlocks, bool kOnce = false>
 __global__ __launch_bounds__(64 * W) void few_rows_kernel(typename ProductTypes<false, kGated, kBlocks>::O o,
                                                           typename ProductTypes<false, kGated, kBlocks>::E ep) {
   static_assert(!kGated || NB % 2 == 0, "as many blocks of both weights");
@@ -1022,7 +1024,7 @@ __global__ __launch_bounds__(64 * W) void few_rows_kernel(typename ProductTypes<
     const int left = o.c_bytes - s * kTileBytes;
 #pragma unroll
     for (int i = 0; i < 2 * NB; ++i)
-      load_block((kGated && i >= 2 * kOut ? w2base : wbase) + at, stage + i * 1024, (piece ^ (64 * (i & 1))) < left ? woff[i] : kPast, 0);
+      load_block<kOnce>((kGated && i >= 2 * kOut ? w2base : wbase) + at, stage + i * 1024, (piece ^ (64 * (i & 1))) < left ? woff[i] : kPast, 0);
 #pragma unroll
     for (int i = 0; i < XB; ++i)
       load_block(xbase + at, stage + (2 * NB + i) * 1024, (piece ^ (64 * (i & 1))) < left ? xoff[i] : kPast, 0);
