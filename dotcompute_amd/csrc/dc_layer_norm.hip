@@ -7,8 +7,8 @@
 // Backward: u = (h - mean) s, g = dy w: dx = s (g - mean(g) - u mean(g u)) + dh, dw = the sum over rows of dy u, db of dy. One read of each
 // operand; the statistics are formed again from h, which is read anyway. A workgroup walks over rows and keeps its parts of dw
 // and db in registers, or of long rows in LDS; a second kernel adds the parts in a fixed order (no atomics: the same bits from call to call).
-// Memory-bound: 8192×4096 50 us with that kernel (5.4 TB/s), 8191×2050 37.4 (3.6: five waves a row, the last with one lane's worth, so that a CU's 15
-// hold fewer bytes in flight, at 4-byte boundaries); 500×1024 in float32 7.9, two launches.
+// Memory-bound: 8192×4096 50 us with that kernel (5.4 TB/s), 8191×2050 36.0 (3.7: five waves a row, the last with one lane's worth, so that a CU's 15
+// do the work of twelve, at 4-byte boundaries); 500×1024 in float32 7.8, two launches.
 //
 // Statistics. The difference of mean(h^2) and mean(h)^2 loses the variance's digits where the mean is large, and a second sum over a row that
 // several waves share would be a second barrier. So each wave takes a value k near its own part's mean, the mean of the first 32 elements (of 256 or
@@ -431,8 +431,7 @@ template <typename T, int C, bool kAhead, bool kShared, bool kOnce>
 __global__ __launch_bounds__(1024) void layer_norm_grad_kernel(LayerNormGradArgs a, int waves, int groups) {
   constexpr int E = kElems<T>, kQuads = C * (E / 4);  // of dweight's parts to a lane
   constexpr bool kKeep = C == 1;  // g over the barrier (of two chunks a lane it does not fit beside the rest, and is formed again)
-  __shared__ __align__(16) f32x4_lds words[2][kWaves];
-  __shared__ float more[2][kWaves];
+  __shared__ __align__(16) float words[2][kWaves][8];  // (of a wave: sums of d, d^2, g, g d, and the value that d is of)
   __shared__ __align__(16) f32x4_lds kept[kShared ? 2 * kQuads * 64 * kWaves : 1];
   extern __shared__ __align__(16) float left_by[];  // (groups - 1) waves 64 2 C E floats
   const int lane = threadIdx.x & 63, place = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -493,31 +492,27 @@ __global__ __launch_bounds__(1024) void layer_norm_grad_kernel(LayerNormGradArgs
         gd_sum = __builtin_fmaf(gi[e], d[i][e], gd_sum);
       }
     }
-    m.left = wave_sum_f32(m.left);
-    m.squares = wave_sum_f32(m.squares);
-    g_sum = wave_sum_f32(g_sum);
-    gd_sum = wave_sum_f32(gd_sum);
+    const float sums_of_lanes = wave_sums_of_four(m.left, m.squares, g_sum, gd_sum, lane);
     RowStats r;
     if (waves == 1) {
-      r = own_stats(m, per_col, a.eps);
-      gd_sum -= m.left * per_col * g_sum;
+      m.left = lane_value(sums_of_lanes, 0);
+      r = own_stats(Moments{m.near, m.left, lane_value(sums_of_lanes, 1)}, per_col, a.eps);
+      g_sum = lane_value(sums_of_lanes, 2);
+      gd_sum = lane_value(sums_of_lanes, 3) - m.left * per_col * g_sum;
     } else {
-      if (lane == 0) {
-        words[flip][place] = f32x4_lds{m.near, m.left, m.squares, g_sum};
-        more[flip][place] = gd_sum;
-      }
+      if (lane < 5) words[flip][place][lane] = lane < 4 ? sums_of_lanes : m.near;
       __syncthreads();  // (two sets in turn: a wave writes a set again only past the barrier of the row between)
       f32x4_lds v = {0.0f, 0.0f, 0.0f, 0.0f};
-      float gd = 0.0f;
+      float near = 0.0f;
       if (other < waves) {
-        v = words[flip][first + other];
-        gd = more[flip][first + other];
+        v = *reinterpret_cast<const f32x4_lds*>(words[flip][first + other]);
+        near = words[flip][first + other][4];
       }
       flip ^= 1;
-      const Joined j = join_moments(Moments{v.x, v.y, v.z}, n_other, m.near, per_col, a.eps);
+      const Joined j = join_moments(Moments{near, v.x, v.y}, n_other, m.near, per_col, a.eps);
       r = j.row;
-      g_sum = row16_sum_f32(v.w);
-      gd_sum = row16_sum_f32(__builtin_fmaf(j.off, v.w, gd)) - j.rest * g_sum;
+      g_sum = row16_sum_f32(v.z);
+      gd_sum = row16_sum_f32(__builtin_fmaf(j.off, v.z, v.w)) - j.rest * g_sum;
     }
     if (row >= a.rows) continue;
     // dx = s g - u s mean(g u) - s mean(g) + dh (s^2 alone may be no float where eps is 0)

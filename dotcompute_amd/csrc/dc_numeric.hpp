@@ -167,6 +167,33 @@ __device__ inline uint32_t wave_max_u32(uint32_t v) {
   v = max(v, dpp_u32<0x143, 0xC>(v));
   return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
+// Sums over the 64 lanes of a wave of two values, or four: in every lane l that of the (l % 2)-th, or (l % 4)-th (fixed tree; all lanes
+// active). The first steps add one value's lanes and another's in one instruction, which is half the instructions of one sum after the other.
+template <int kCtrl>
+__device__ inline float dpp_add(float to, float v) {
+  return to + __builtin_bit_cast(float, dpp_u32<kCtrl, 0xF>(__builtin_bit_cast(uint32_t, v)));
+}
+// The sum over the four rows of 16 lanes of what lies in a lane's place: the instructions exchange rows 1 and 3 of one copy with 0 and 2 of another, then halves.
+__device__ inline float across_rows(float v) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto rows = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const uint32_t even = rows[0], odd = rows[1];  // (a bit cast of a vector's element itself reads the first)
+  const uint32_t w = __builtin_bit_cast(uint32_t, __builtin_bit_cast(float, even) + __builtin_bit_cast(float, odd));
+  const auto halves = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  const uint32_t low = halves[0], high = halves[1];
+  return __builtin_bit_cast(float, low) + __builtin_bit_cast(float, high);
+}
+__device__ inline float pair_sums(float a, float b, bool odd) { return dpp_add<0xB1>(odd ? b : a, odd ? a : b); }
+__device__ inline float wave_sums_of_four(float a, float b, float c, float d, int lane) {
+  const float low = pair_sums(a, b, lane & 1), high = pair_sums(c, d, lane & 1);
+  float v = dpp_add<0x4E>(lane & 2 ? high : low, lane & 2 ? low : high);
+  v = dpp_add<0x124>(v, v);
+  v = dpp_add<0x128>(v, v);
+  return across_rows(v);
+}
+__device__ inline float lane_value(float v, int lane) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
 // The sum over each 16 lanes, in all of them.
 __device__ inline float row16_sum_f32(float v) {
   v += __builtin_bit_cast(float, dpp_u32<0xB1, 0xF>(__builtin_bit_cast(uint32_t, v)));
