@@ -13,6 +13,7 @@ import ffn_reference as ref
 import gated_reference as gated
 from dotcompute_amd import hip
 from test_gpu_layer_norm import EPS, F32, HALF, unit, within, y_bound
+from test_gpu_layer_norm import test_layer_norm as layer_norm
 from test_gpu_rms_norm import values, wide
 
 pytestmark = pytest.mark.gpu
@@ -104,3 +105,10 @@ def test_single_rows_have_no_stride(ctx, cols, stride):
     assert abs(out.to_host()[0, 0] - z * z) <= 2.0 ** -5 * z * z
     for a in (dx, dw, y, q, codes, sums, out):
         ctx.free(a)
+
+
+@pytest.mark.parametrize("rows,cols", [(1, 8193), (300, 8193), (257, 9000), (3, 12289), (2, 16383), (2, 16385)])
+def test_layer_norm_of_long_rows(ctx, rows, cols):
+    """Rows on both sides of what a workgroup holds in two and in four pieces to a lane."""
+    layer_norm(ctx, rows, cols, "f32")
+    layer_norm(ctx, rows, 2 * cols, "bf16")

@@ -11,7 +11,7 @@ pytestmark = pytest.mark.gpu
 LARGE = 96 << 20
 
 
-@pytest.mark.parametrize("rows,cols,dtype", [(6200, 2051, "bf16"), (21000, 601, "bf16"), (1060, 12001, "bf16"), (3100, 2051, "f32"), (8300, 4100, "bf16")])
+@pytest.mark.parametrize("rows,cols,dtype", [(6200, 2051, "bf16"), (21000, 601, "bf16"), (1060, 12001, "bf16"), (3100, 2051, "f32"), (420, 15217, "f32"), (8300, 4100, "bf16")])
 def test_layer_norm(ctx, rows, cols, dtype):
     assert rows * cols * (8 if dtype == "bf16" else 16) > LARGE
     layer_norm(ctx, rows, cols, dtype)  # (the last shape in 8 bits too)
