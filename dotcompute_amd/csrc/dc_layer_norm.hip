@@ -749,7 +749,8 @@ int32_t launch_norm(dc_hip_ctx* ctx, const LayerNormArgs& a, int64_t chunks) {
 // Chunks that a lane holds: one of bf16, over up to 16 waves; two where they let a wave hold a row by itself (but not where it is read and written in float32),
 // and in longer rows. us, with the call, for a workgroup to each row with one to two chunks / workgroups that walk with two / with one, bf16: 16384×4096 95.6 /
 // 103 / 96.0, to 8 bits 98.7 / 93.1 / 94.0; 8191×2050 34.8 / 29.8 / 28.0; 4096×8192 55.7 / 48.5 / 48.6; 2000×12000 53 / 38;
-// 1000×4096 8.6 / 8.5 / 7.6; float32 8192×2048 48.3 / 48.5 / 50.3 (all before large operands were loaded as read once). With 24 waves a CU 16384×4096 takes 101, with 32 108. Four chunks for float32 rows of more than 16 waves of two, which spill 9 to 23 registers,
+// 1000×4096 8.6 / 8.5 / 7.6; float32 8192×2048 48.3 / 48.5 / 50.3 (all before large operands were loaded as read once). With 24 waves a CU 16384×4096
+// takes 101, with 32 108. Four chunks for float32 rows of more than 16 waves of two, which spill 9 to 23 registers,
 // or such rows read again by the long kernel: 2322×15219 119 / 155, 2000×9000 57 / 80, to 8 bits 2000×12000 78 / 117, 20×12000 7.3 / 7.7; of bf16, whose
 // rows' values take twice the registers, 2048×24576 222 / 124.
 template <typename T, typename Y, bool kBlocks>
