@@ -40,7 +40,7 @@ __global__ __launch_bounds__(256) void gated_join_kernel(GatedJoin a) {
 
 int32_t join_gated(dc_hip_ctx* ctx, const float* parts, const MoreOperands& o, int64_t pitch, int64_t count, const GatedEpilogue& ep) {
   const GatedJoin a{parts, o.m, o.n, pitch, (int32_t)count, ep};
-  gated_join_kernel<<<(unsigned)std::min<int64_t>((o.m * ((o.n + 7) / 8) + 255) / 256, 1 << 16), 256, 0, ctx->stream>>>(a);
+  gated_join_kernel<<<(unsigned)dc::linear_join_groups(o.m, o.n), 256, 0, ctx->stream>>>(a);
   return dc::last_launch_status();
 }
 

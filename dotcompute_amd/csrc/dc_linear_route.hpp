@@ -205,4 +205,11 @@ inline bool linear_few_rows_any(int64_t m, int64_t n, int64_t c_bytes) {
 // 8×4096×4096: 9.6, 7.4).
 inline bool linear_wide_few_rows(int64_t m, int64_t n, int64_t cus) { return m <= kLinearFewRows && (n + 15) / 16 > 2 * cus; }
 
+// Workgroups of the kernels that add the sums of parts of c: a lane takes eight neighbouring results, 256 a workgroup, which walk over what is left.
+// (m below 2^30 and n up to kLinearWidth are more results than 32 bits count.)
+inline int64_t linear_join_groups(int64_t m, int64_t n) {
+  const int64_t groups = (m * ((n + 7) / 8) + 255) / 256;
+  return groups < (1 << 16) ? groups : 1 << 16;
+}
+
 }  // namespace dc
