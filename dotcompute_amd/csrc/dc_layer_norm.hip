@@ -11,11 +11,13 @@
 // do the work of twelve, at 4-byte boundaries); 500×1024 in float32 7.8, two launches.
 //
 // Statistics. The difference of mean(h^2) and mean(h)^2 loses the variance's digits where the mean is large, and a second sum over a row that
-// several waves share would be a second barrier. So each wave takes a value k near its own part's mean, the mean of the first 32 elements (of 256 or
-// 512, or up to four times as many), and the sums of d = h - k and d^2, in registers; the waves' triples meet in LDS once, and every wave joins them: M is
+// several waves share would be a second barrier. So each wave takes a value k near its own part's mean, the mean of its lanes' first chunks, and the sums
+// of d = h - k and d^2, in registers; the waves' triples meet in LDS once, and every wave joins them: M is
 // the rounded mean, e what is left, and sum((h - M)^2) = the sum over waves of sum(d^2) + 2 c sum(d) + n c^2, c = k - M. An
-// element's u is d s + ((k - M) - e) s, whose terms are of u's size. (However a wave's values lie, (k - mean)^2 is at most n / 32 times their variance, so
-// that at worst 4 to 6 bits of its 24 are lost there, where one value stands out by itself among the first 32; none for others.)
+// element's u is d s + ((k - M) - e) s, whose terms are of u's size. However a row's values lie, a lane with C chunks has the sum of n c^2 at C times the row's
+// squares at most (one chunk of C is the sample): with one chunk nothing cancels, with four the sum of d^2 is at most (1 + sqrt 4)^2 = 9 times what is left
+// of it, three bits. (The mean of the first 32 elements, 16 of float32, as k, which is four additions less a row, lost up to six where those lie apart from the
+// rest. us, that / this: bf16 8191×2050 25.7 / 25.9, its gradients 36.2 / 36.7, 16384×512 11.8 / 11.9, 16384×4096 93.3 both.)
 #include <algorithm>
 #include <type_traits>
 
@@ -127,11 +129,11 @@ __device__ inline float wave_count(int64_t cols, int waves, int wave) {
 struct Moments {
   float near, left, squares;
 };
-// 1 / the number of elements that `near` is the mean of.
+// 1 / the number of elements that `near` is the mean of: those of the wave's first chunks.
 template <int E>
 __device__ inline float near_weight(int64_t cols, int wave) {
   const int64_t left = cols - (int64_t)wave * 64 * E;
-  return 1.0f / (float)(left < 4 * E ? left : 4 * E);
+  return 1.0f / (float)(left < 64 * E ? left : 64 * E);
 }
 template <typename T, int C>
 __device__ inline float value_near(const float (&h)[C][kElems<T>], float weight) {
@@ -139,9 +141,7 @@ __device__ inline float value_near(const float (&h)[C][kElems<T>], float weight)
   float v = 0.0f;
 #pragma unroll
   for (int e = 0; e < E; e += 4) v += (h[0][e] + h[0][e + 1]) + (h[0][e + 2] + h[0][e + 3]);
-  v += __builtin_bit_cast(float, dpp_u32<0xB1, 0xF>(__builtin_bit_cast(uint32_t, v)));
-  v += __builtin_bit_cast(float, dpp_u32<0x4E, 0xF>(__builtin_bit_cast(uint32_t, v)));
-  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v))) * weight;
+  return wave_sum_f32(v) * weight;
 }
 // h becomes d = h - near (zeros past the row's end); the lane's part of the sums.
 template <typename T, int C, int kInside>
