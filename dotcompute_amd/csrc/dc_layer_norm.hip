@@ -2,12 +2,14 @@
 //
 // Forward, a row at a time: h = x + r, y = (h - mean) s w + b with s = 1 / sqrt(var + eps). Memory-bound: 8 bytes an element in bf16 (x, r
 // in; h, y out), 7 with y in 8 bits. A row stays in registers between its one read and its write, as an RMS norm's. 16384×4096 93.3 us (5.8 TB/s),
-// 8191×2050, whose rows lie at 4-byte boundaries, 25.9 (5.2); 8×4096 to 8 bits 4.2, of which the call is 3.7.
+// 8191×2050, whose rows lie at 4-byte boundaries, 25.9 (5.2); 8×4096 to 8 bits 4.2, of which the call is 3.7. To 8 bits with block scales 16384×4096 79 (5.9), but
+// without a residual 67 (3.0), with a scale a row 77: bound by a row's way through its statistics and maxima there.
+// Most of the forms for 8 bits, and of those with more than one chunk a lane, spill scalar registers, up to 92, beside the vector ones that are named at norm_by_shape.
 //
 // Backward: u = (h - mean) s, g = dy w: dx = s (g - mean(g) - u mean(g u)) + dh, dw = the sum over rows of dy u, db of dy. One read of each
 // operand; the statistics are formed again from h, which is read anyway. A workgroup walks over rows and keeps its parts of dw
 // and db in registers, or of long rows in LDS; a second kernel adds the parts in a fixed order (no atomics: the same bits from call to call).
-// Memory-bound: 8192×4096 50 us with that kernel (5.4 TB/s), 8191×2050 36.0 (3.7: five waves a row, the last with one lane's worth, so that a CU's 15
+// Memory-bound: 8192×4096 50 us with that kernel (5.4 TB/s), 8191×2050 36.8 (3.7: five waves a row, the last with one lane's worth, so that a CU's 15
 // do the work of twelve, at 4-byte boundaries); 500×1024 in float32 7.8, two launches.
 //
 // Statistics. The difference of mean(h^2) and mean(h)^2 loses the variance's digits where the mean is large, and a second sum over a row that

@@ -3,7 +3,8 @@
 // The scales are powers of two held as exponents, which v_mfma_scale_f32_*_f8f6f4 takes beside the codes, a byte for each row and 32 of c: a tile's turn
 // is 128 bytes of c, one block, so that the scales cost a byte's load a row and turn, and no arithmetic. (A float32 scale would be a product and an
 // addition for each sum and block, beside the matrix cores: 128 of them a lane and turn in the largest tiles, whose sums take half of the registers.)
-// Everything else is a linear layer's (dc_linear.hip).
+// Everything else is a linear layer's (dc_linear.hip), what the 8-bit instructions cut products at (2^-13 of the largest that they add at once) among it: results in
+// bf16 differ from those of float32 products by 0.0002 of themselves, in the mean, beside their rounding's 0.0017.
 #include "dc_linear_device.hpp"
 
 namespace {
