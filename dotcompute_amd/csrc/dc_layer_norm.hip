@@ -143,7 +143,7 @@ __device__ inline float value_near(const float (&h)[C][kElems<T>], float weight)
   float v = 0.0f;
 #pragma unroll
   for (int e = 0; e < E; e += 4) v += (h[0][e] + h[0][e + 1]) + (h[0][e + 2] + h[0][e + 3]);
-  return wave_sum_f32(v) * weight;
+  return wave_sum_f32(v * weight);  // (weighted before the lanes meet: the sum of a wave's largest floats is none)
 }
 // h becomes d = h - near (zeros past the row's end); the lane's part of the sums.
 template <typename T, int C, int kInside>

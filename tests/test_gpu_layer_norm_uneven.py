@@ -76,3 +76,25 @@ def test_layer_norm_backward(ctx, dtype, cols, waves, ahead):
         within(dx.to_host(), x64, 20 * HALF * terms + (ref.BF16 * (1 + 20 * HALF) * np.abs(x64) if dtype == "bf16" else 0.0), "dx")
         for a in (ddy, dh, dw, dx, dweight, dbias):
             ctx.free(a)
+
+
+@pytest.mark.parametrize("dtype,cols", [("f32", 4), ("f32", 64), ("f32", 256), ("bf16", 8), ("bf16", 128), ("bf16", 512)])
+def test_rows_of_one_value_near_the_largest(ctx, dtype, cols):
+    """Rows that one wave holds, of lanes that are a power of two: every sum on the way to the value's mean is exact, and a float as long as a lane's is, so
+    that nothing is left of the row but the bias."""
+    to = ref.to_bf16 if dtype == "bf16" else (lambda v: v.astype(np.float32))
+    rng = np.random.default_rng(cols)
+    h = to(np.repeat(np.array([[1e37], [-3e37], [4e37], [1e-37], [7e5]]), cols, axis=1))
+    w, b, dy = to(rng.normal(size=cols)), to(rng.normal(size=cols)), to(rng.normal(size=h.shape))
+    dh, dw, db, ddy, y, dx = (ctx.to_device(a) for a in (h, w, b, dy, np.zeros_like(h), np.zeros_like(h)))
+    dweight = ctx.empty(cols, np.float32)
+    ctx.layer_norm(hip.LayerNorm.of(dh, dw, db, y, eps=EPS))
+    ctx.layer_norm_backward(hip.LayerNormGrad.of(ddy, dh, dw, dx, dweight, eps=EPS))
+    ctx.synchronize()
+    assert np.array_equal(y.to_host(), np.broadcast_to(b, h.shape)) and np.all(dweight.to_host() == 0)
+    g, s = wide(dy) * wide(w), EPS ** -0.5
+    want = s * (g - np.mean(g, axis=1, keepdims=True))
+    terms = s * (np.abs(g) + np.mean(np.abs(g), axis=1, keepdims=True))
+    within(dx.to_host(), want, 20 * HALF * terms + (ref.BF16 * (1 + 20 * HALF) * np.abs(want) if dtype == "bf16" else 0.0), "dx")
+    for a in (dh, dw, db, ddy, y, dx, dweight):
+        ctx.free(a)
